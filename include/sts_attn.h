@@ -220,6 +220,114 @@ int sts_prefill_attention_bf16kv(const float* q, const uint16_t* k16, const uint
                                  float scale, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Drafts, masks and kept attention weights over ring windows                */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * The calls of this section have no counterpart in the reference; they work on
+ * the same ring windows as sts_decode_ring, batched over streams:
+ *   k/v cache    [batch][kv_heads][max_len][head_dim], f32 or bf16 (row_type;
+ *                bf16 head dims are multiples of 8), 16-byte aligned
+ *   lens[b]      rows of stream b's window, 0..max_len    (device int32)
+ *   starts[b]    slot of its oldest row, 0..max_len-1      (device int32)
+ *   row r of stream b lives in slot (starts[b] + r) % max_len
+ * with values outside their ranges clamped on the device as there.  Query head
+ * h reads K/V head h / (heads / kv_heads); q and out are f32, and so is the
+ * arithmetic for either row type.  One head's rows take less than 2 GiB.  What
+ * a query does not see has no influence on it, whatever values are there.
+ * Splits use the per-(device, stream) workspace as sts_decode_ring does.
+ */
+enum sts_row_type {
+  STS_ROWS_F32 = 0,
+  STS_ROWS_BF16 = 1
+};
+
+/* The largest draft of sts_tree_attention, sts_tree_commit and sts_kv_tree_step. */
+#define STS_TREE_MAX_NODES 256u
+
+/*
+ * Attention of a draft: a tree of tokens proposed after the window's committed
+ * rows, all verified in one pass.  Stream b's nodes are the last counts[b] rows
+ * of its window (counts NULL: `nodes` of them; at most `nodes` and lens[b]),
+ * parents before children.  Node i sees the committed rows, its ancestors and
+ * itself: out_i = softmax(scale * q_i . k) v over those.
+ *   q, out       [batch][nodes][heads][head_dim]; rows of out from counts[b] on
+ *                are zeros
+ *   parents      [batch][nodes] (device int32): the parent's index below i, or
+ *                -1 for a child of the last committed row, as which any other
+ *                value is taken
+ */
+int sts_tree_attention(const float* q, const void* k_cache, const void* v_cache, float* out,
+                       const int32_t* parents, const int32_t* counts, const int32_t* lens,
+                       const int32_t* starts, uint32_t batch, uint32_t nodes, uint32_t heads,
+                       uint32_t kv_heads, uint32_t head_dim, uint32_t max_len, float scale,
+                       int row_type, void* stream);
+
+/*
+ * Keeps the accepted path of each stream's draft: row path[b][j] of the draft
+ * becomes its row j for j < accepted[b], in place (path [batch][nodes], accepted
+ * [batch], counts as above; device int32).  The caller then shortens the window
+ * by counts[b] - accepted[b] rows.  An entry below j or not below counts[b]
+ * moves nothing; the rows behind the accepted ones are left as they were.
+ */
+int sts_tree_commit(void* k_cache, void* v_cache, const int32_t* path, const int32_t* accepted,
+                    const int32_t* counts, const int32_t* lens, const int32_t* starts, uint32_t batch,
+                    uint32_t nodes, uint32_t kv_heads, uint32_t head_dim, uint32_t max_len,
+                    int row_type, void* stream);
+
+/*
+ * Attention under a row range per query, with capped scores and a distance
+ * bias, for chunks and single tokens.  Query i of stream b's counts[b] (NULL:
+ * `seq`) is window row w = lens[b] - counts[b] + i and sees the rows r with
+ * lo <= r < hi of lo, hi [batch][seq] (device int32, clamped to the window;
+ * lo NULL: 0, hi NULL: w + 1, i.e. causal):
+ *   documents        lo = the first row of the query's document
+ *   prefix           hi = max(w + 1, prefix rows)
+ *   sliding window   lo = w + 1 - width
+ * Its score of row r is x = scale * q . k; with softcap > 0
+ * x = softcap * tanh(x / softcap); with slopes [heads] (device, or NULL) then
+ * x -= slopes[head] * |w - r|.  A query that sees nothing gets zeros, and so do
+ * the rows of out [batch][seq][heads][head_dim] from counts[b] on.
+ */
+int sts_masked_attention(const float* q, const void* k_cache, const void* v_cache, float* out,
+                         const int32_t* lo, const int32_t* hi, const float* slopes,
+                         const int32_t* counts, const int32_t* lens, const int32_t* starts,
+                         uint32_t batch, uint32_t seq, uint32_t heads, uint32_t kv_heads,
+                         uint32_t head_dim, uint32_t max_len, float scale, float softcap, int row_type,
+                         void* stream);
+
+/*
+ * sts_decode_ring that also keeps account of where the attention went:
+ *   weights[b][j][slot of row r] += sum over the heads of K/V head j of the
+ *                                   softmax weight of row r
+ * for the rows of the window (weights [batch][kv_heads][max_len] f32; other
+ * slots are left as they were).  q, out [batch][heads][head_dim].  scratch:
+ * sts_decode_ring_weights_scratch floats of the caller's, 16-byte aligned, used
+ * until the call's work on `stream` is done.
+ */
+int sts_decode_ring_weights(const float* q, const void* k_cache, const void* v_cache, float* out,
+                            float* weights, float* scratch, const int32_t* lens,
+                            const int32_t* starts, uint32_t batch, uint32_t heads, uint32_t kv_heads,
+                            uint32_t head_dim, uint32_t max_len, float scale, int row_type,
+                            void* stream);
+uint64_t sts_decode_ring_weights_scratch(uint32_t batch, uint32_t heads, uint32_t max_len);
+
+/*
+ * Cuts each stream's window down to `keep` rows by weight, per K/V head: the
+ * `recent` newest rows stay, and of the others the keep - recent of largest
+ * weight (equal ones: the oldest first; NaN counts as the largest).  The kept
+ * rows, in their order and with their weights, become the last `keep` rows of
+ * the window; the slots before them are left as they are, so that the caller
+ * sets starts[b] += lens[b] - keep (modulo max_len), lens[b] = keep.  A stream
+ * of at most `keep` rows stays as it is.  Rows keep what they were rotated by.
+ * kept [batch][kv_heads][keep] (device int32, written): the window rows kept,
+ * ascending; -1 past the rows of a shorter window.
+ */
+int sts_evict_ring(void* k_cache, void* v_cache, float* weights, int32_t* kept, const int32_t* lens,
+                   const int32_t* starts, uint32_t batch, uint32_t kv_heads, uint32_t head_dim,
+                   uint32_t max_len, uint32_t keep, uint32_t recent, int row_type, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* RoPE (model.rs:38-122)                                                     */
 /* ------------------------------------------------------------------------ */
 
@@ -262,12 +370,14 @@ typedef struct sts_kv_state {
   uint64_t head_dim;
   uint64_t batch;     /* 0 until the buffers are allocated                 */
   int32_t allocated;  /* 1 when the K/V buffers exist                      */
-  int32_t flags;      /* the sts_kv_create_ex flags (STS_KV_BF16_MIRROR)   */
+  int32_t flags;      /* the sts_kv_create_ex flags                        */
   uint64_t q_heads;   /* query heads of q/out (sts_kv_set_query_heads)     */
 } sts_kv_state;
 
 /* sts_kv_create_ex flag: keep a bf16 copy of K and V (see sts_kv_create_ex). */
 #define STS_KV_BF16_MIRROR 1u
+/* sts_kv_create_ex flag: keep each row's share of the attention (see there). */
+#define STS_KV_WEIGHTS 2u
 
 /* KVCache::new (model.rs:207-219).  Allocates nothing on the device. */
 int sts_kv_create(uint64_t max_len, uint64_t heads, uint64_t head_dim, sts_kv_cache** out);
@@ -284,6 +394,13 @@ int sts_kv_create(uint64_t max_len, uint64_t heads, uint64_t head_dim, sts_kv_ca
  * into the f32 buffers by other means (sts_cache_write on the pointers of
  * sts_kv_ensure_allocated) reach the mirror only through sts_kv_sync_mirror.
  * A mirrored cache needs 16-byte aligned inputs in sts_kv_update.
+ * STS_KV_WEIGHTS: the handle keeps, for every slot and K/V head, the attention
+ * weight its row was given by sts_kv_attend and sts_kv_decode_step (summed over
+ * the heads of the group, as sts_decode_ring_weights does; these two then read
+ * the window with that call's kernel), for sts_kv_evict.  A row appended through
+ * the handle starts at zero; the attention of sts_kv_prefill and
+ * sts_kv_tree_step is not counted, and rows entered by sts_kv_advance keep what
+ * their slots had.  Query heads are set before the first use.
  */
 int sts_kv_create_ex(uint64_t max_len, uint64_t heads, uint64_t head_dim, uint32_t flags,
                      sts_kv_cache** out);
@@ -291,6 +408,10 @@ int sts_kv_create_ex(uint64_t max_len, uint64_t heads, uint64_t head_dim, uint32
 /* The bf16 mirror buffers [batch][heads][max_len][head_dim] (bf16 bits), or
  * NULL when the cache has none or is not allocated yet. */
 int sts_kv_mirror(const sts_kv_cache* cache, uint16_t** k16, uint16_t** v16);
+
+/* The kept attention weights [batch][heads][max_len] by slot, or NULL when the
+ * cache keeps none or is not allocated yet. */
+int sts_kv_weights(const sts_kv_cache* cache, float** weights);
 
 /* Rebuilds the bf16 mirror from the f32 caches (after direct writes). */
 int sts_kv_sync_mirror(sts_kv_cache* cache, void* stream);
@@ -390,6 +511,37 @@ int sts_kv_decode_step(sts_kv_cache* cache, const sts_rope* rope, const float* q
 int sts_kv_prefill(sts_kv_cache* cache, const sts_rope* rope, const float* q,
                    const float* k_new, const float* v_new, float* out, uint64_t seq,
                    float scale, int precision, void* stream);
+
+/*
+ * A draft on the handle (batch 1): appends the drafted rows k_new, v_new
+ * [nodes][heads][head_dim] in their order, advances by `nodes`, and attends as
+ * sts_tree_attention does, q, out [nodes][q_heads][head_dim], parents [nodes]
+ * (device int32).  With `rope`, q and k_new of a node are rotated at offset +
+ * its depth (0 for a child of the last committed row), offset + nodes within the
+ * table.  In a full ring the drafted rows replace the oldest ones, as appended
+ * rows do.  Every argument is checked before anything is written.
+ * sts_kv_tree_commit or sts_kv_rollback(nodes) has to follow before other rows
+ * are appended.
+ */
+int sts_kv_tree_step(sts_kv_cache* cache, const sts_rope* rope, const float* q, const float* k_new,
+                     const float* v_new, const int32_t* parents, float* out, uint64_t nodes,
+                     float scale, void* stream);
+
+/*
+ * Ends a draft of `nodes` rows: the accepted path (host array of `accepted` node
+ * indices, ascending, from a child of the last committed row down) stays as the
+ * window's last rows, at the positions it was rotated for; the others are rolled
+ * back.  accepted 0 drops the draft.
+ */
+int sts_kv_tree_commit(sts_kv_cache* cache, uint64_t nodes, const uint32_t* path, uint64_t accepted,
+                       void* stream);
+
+/*
+ * sts_evict_ring on a handle made with STS_KV_WEIGHTS, whose window becomes the
+ * kept rows; offset (and with it the position of the next row) does not change.
+ * kept [batch][heads][keep] (device int32) may be NULL.
+ */
+int sts_kv_evict(sts_kv_cache* cache, uint64_t keep, uint64_t recent, int32_t* kept, void* stream);
 
 /* ---- device error word ---------------------------------------------------- */
 

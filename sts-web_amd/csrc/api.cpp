@@ -15,121 +15,14 @@
 #include "decode.hpp"
 #include "depformer.hpp"
 #include "errors.hpp"
+#include "kv_cache.hpp"
 #include "prefill.hpp"
 #include "q4k.hpp"
+#include "window.hpp"
 
 using sts::fail;
 
-struct sts_rope {
-  uint32_t head_dim = 0;
-  uint32_t max_seq_len = 0;
-  float* cos_t = nullptr;  // device [max_seq_len][head_dim/2]
-  float* sin_t = nullptr;
-};
-
-struct sts_kv_cache {
-  uint64_t max_len = 0, heads = 0, head_dim = 0;
-  uint64_t q_heads = 0;  // query heads of q/out (a multiple of heads: GQA)
-  uint64_t offset = 0, len = 0, write_pos = 0;
-  uint64_t batch = 0;
-  uint32_t flags = 0;
-  float* k = nullptr;
-  float* v = nullptr;
-  uint16_t* k16 = nullptr;  // bf16 mirror (STS_KV_BF16_MIRROR)
-  uint16_t* v16 = nullptr;
-};
-
-namespace {
-
-hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// Any multiple of 4 up to 128 (shader_attention.wgsl:36 takes head_dim <= 128);
-// 64 and 128 have their own kernels, the others run padded ones.
-int check_head_dim(uint64_t d) {
-  if (d == 0 || d > 128 || d % 4 != 0)
-    return fail(STS_ERR_INVALID, "head_dim %llu not supported (a multiple of 4 up to 128)",
-                (unsigned long long)d);
-  return STS_OK;
-}
-
-// KVCache::advance (model.rs:293-298), n steps of the one-step update.
-void kv_advance(sts_kv_cache* c, uint64_t n) {
-  if (n >= c->max_len) {
-    // Whole-ring advance: the same end state as n single steps.
-    c->write_pos = (c->write_pos + n) % c->max_len;
-    c->offset += n;
-    c->len = c->max_len;
-    return;
-  }
-  c->write_pos = (c->write_pos + n) % c->max_len;
-  c->offset += n;
-  c->len = (c->len + n < c->max_len) ? c->len + n : c->max_len;
-}
-
-// Oldest valid slot of the logical window.
-uint64_t kv_start(const sts_kv_cache* c) {
-  return (c->write_pos + c->max_len - c->len) % c->max_len;
-}
-
-int kv_ensure(sts_kv_cache* c, uint64_t batch, hipStream_t stream) {
-  if (c->k) {
-    if (batch != c->batch)
-      return fail(STS_ERR_STATE, "cache allocated for batch %llu, called with batch %llu",
-                  (unsigned long long)c->batch, (unsigned long long)batch);
-    return STS_OK;
-  }
-  if (batch == 0) return fail(STS_ERR_INVALID, "batch must be >= 1");
-  // The lazy allocation must not be recorded into a HIP graph (its zero fill
-  // would be a memset node, and the graph would own nothing it addresses).
-  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-  STS_HIP(hipStreamIsCapturing(stream, &cap));
-  if (cap != hipStreamCaptureStatusNone)
-    return fail(STS_ERR_STATE,
-                "the cache's first use allocates its buffers, which cannot happen while the "
-                "stream is being captured; allocate it first (sts_kv_ensure_allocated)");
-  const uint64_t n = batch * c->heads * c->max_len * c->head_dim;
-  if (hipMalloc(&c->k, n * sizeof(float)) != hipSuccess) {
-    c->k = nullptr;
-    return fail(STS_ERR_NOMEM, "K cache allocation of %llu bytes failed",
-                (unsigned long long)(n * sizeof(float)));
-  }
-  if (hipMalloc(&c->v, n * sizeof(float)) != hipSuccess) {
-    (void)hipFree(c->k);
-    c->k = nullptr;
-    c->v = nullptr;
-    return fail(STS_ERR_NOMEM, "V cache allocation of %llu bytes failed",
-                (unsigned long long)(n * sizeof(float)));
-  }
-  if (c->flags & STS_KV_BF16_MIRROR) {
-    if (hipMalloc(&c->k16, n * sizeof(uint16_t)) != hipSuccess ||
-        hipMalloc(&c->v16, n * sizeof(uint16_t)) != hipSuccess) {
-      for (void* ptr : {(void*)c->k, (void*)c->v, (void*)c->k16, (void*)c->v16})
-        if (ptr) (void)hipFree(ptr);
-      c->k = c->v = nullptr;
-      c->k16 = c->v16 = nullptr;
-      return fail(STS_ERR_NOMEM, "bf16 mirror allocation of %llu bytes failed",
-                  (unsigned long long)(2 * n * sizeof(uint16_t)));
-    }
-    STS_HIP(hipMemsetAsync(c->k16, 0, n * sizeof(uint16_t), stream));
-    STS_HIP(hipMemsetAsync(c->v16, 0, n * sizeof(uint16_t), stream));
-  }
-  // Zero-filled like Tensor::zeros (model.rs:272-279).
-  STS_HIP(hipMemsetAsync(c->k, 0, n * sizeof(float), stream));
-  STS_HIP(hipMemsetAsync(c->v, 0, n * sizeof(float), stream));
-  c->batch = batch;
-  return STS_OK;
-}
-
-void kv_free(sts_kv_cache* c) {
-  for (void* ptr : {(void*)c->k, (void*)c->v, (void*)c->k16, (void*)c->v16})
-    if (ptr) (void)hipFree(ptr);
-  c->k = c->v = nullptr;
-  c->k16 = c->v16 = nullptr;
-}
-
-}  // namespace
+using namespace sts::kv;
 
 extern "C" {
 
@@ -403,7 +296,7 @@ int sts_kv_create(uint64_t max_len, uint64_t heads, uint64_t head_dim, sts_kv_ca
 int sts_kv_create_ex(uint64_t max_len, uint64_t heads, uint64_t head_dim, uint32_t flags,
                      sts_kv_cache** out) {
   sts::clear_error();
-  STS_CHECK((flags & ~(uint32_t)STS_KV_BF16_MIRROR) == 0, "unknown flags 0x%x", flags);
+  STS_CHECK((flags & ~(uint32_t)(STS_KV_BF16_MIRROR | STS_KV_WEIGHTS)) == 0, "unknown flags 0x%x", flags);
   STS_CHECK(out, "null out pointer");
   *out = nullptr;
   STS_CHECK(max_len >= 1 && max_len <= 0x7fffffffull, "max_len must be in 1..2^31-1");
@@ -426,6 +319,9 @@ int sts_kv_set_query_heads(sts_kv_cache* cache, uint64_t q_heads) {
   STS_CHECK(q_heads >= cache->heads && q_heads <= 65535 && q_heads % cache->heads == 0,
             "query heads %llu must be a multiple of the %llu K/V heads, at most 65535",
             (unsigned long long)q_heads, (unsigned long long)cache->heads);
+  if (cache->scores && q_heads > cache->q_heads)
+    return fail(STS_ERR_STATE, "a cache that keeps attention weights takes its query heads before "
+                "its first use");
   cache->q_heads = q_heads;
   return STS_OK;
 }
@@ -528,6 +424,11 @@ int sts_kv_update(sts_kv_cache* cache, const float* k_new, const float* v_new, u
                                          (uint32_t)cache->max_len, s))
       return rc;
   }
+  if (cache->weights) {
+    if (int rc = sts::launch_clear_weights(cache->weights, batch * cache->heads,
+                                           (uint32_t)cache->max_len, pos, (uint32_t)seq, s))
+      return rc;
+  }
   kv_advance(cache, seq);
   return STS_OK;
 }
@@ -551,6 +452,12 @@ int sts_kv_reset_keep_buffers(sts_kv_cache* cache, void* stream) {
     if (cache->k16) {
       STS_HIP(hipMemsetAsync(cache->k16, 0, n * sizeof(uint16_t), as_stream(stream)));
       STS_HIP(hipMemsetAsync(cache->v16, 0, n * sizeof(uint16_t), as_stream(stream)));
+    }
+    if (cache->weights) {
+      if (int rc = sts::launch_clear_weights(cache->weights, cache->batch * cache->heads,
+                                             (uint32_t)cache->max_len, 0, (uint32_t)cache->max_len,
+                                             as_stream(stream)))
+        return rc;
     }
   }
   cache->offset = cache->len = cache->write_pos = 0;
@@ -594,6 +501,9 @@ int sts_kv_attend(sts_kv_cache* cache, const float* q, float* out, float scale, 
   STS_CHECK(cache->len >= 1, "cache window is empty");
   STS_CHECK(aligned16(q) && aligned16(out), "q and out must be 16-byte aligned");
   STS_CHECK(std::isfinite(scale), "scale must be finite");
+  if (cache->weights)
+    return decode_keeping_weights(cache, cache, nullptr, q, nullptr, nullptr, out, scale,
+                                  as_stream(stream));
   sts::DecodeParams p;
   fill_cache_decode(cache, p);
   p.q = q;
@@ -625,6 +535,11 @@ int sts_kv_decode_step(sts_kv_cache* cache, const sts_rope* rope, const float* q
   const uint64_t pos = cache->offset;
   sts_kv_cache next = *cache;
   kv_advance(&next, 1);
+  if (cache->weights) {
+    if (int rc = decode_keeping_weights(cache, &next, rope, q, k_new, v_new, out, scale, s)) return rc;
+    *cache = next;
+    return STS_OK;
+  }
   sts::DecodeParams p;
   fill_cache_decode(cache, p);
   p.q = q;
@@ -691,6 +606,8 @@ int sts_kv_prefill(sts_kv_cache* cache, const sts_rope* rope, const float* q,
   next.v = cache->v;
   next.k16 = cache->k16;
   next.v16 = cache->v16;
+  next.weights = cache->weights;
+  next.scores = cache->scores;
   next.batch = cache->batch;
   const uint32_t pos = (uint32_t)(cache->offset % cache->max_len);
   // RoPE of k (at offset + s) fused into one append launch of K and V.
@@ -700,6 +617,11 @@ int sts_kv_prefill(sts_kv_cache* cache, const sts_rope* rope, const float* q,
                                      rope ? rope->sin_t : nullptr, (uint32_t)cache->offset,
                                      cache->k16, cache->v16, s))
     return rc;
+  if (cache->weights) {
+    if (int rc = sts::launch_clear_weights(cache->weights, cache->heads, (uint32_t)cache->max_len,
+                                           pos, (uint32_t)seq, s))
+      return rc;
+  }
   const uint64_t q_pos0 = cache->offset;
   *cache = next;
   sts::PrefillParams p;

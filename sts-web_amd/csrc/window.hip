@@ -1,0 +1,132 @@
+// window.hip -- launch plans of the window attention kernels, and the account of
+// the attention weights that sts_decode_ring_weights keeps.
+#include <algorithm>
+
+#include "window_kernel.hpp"
+
+namespace sts {
+
+namespace {
+
+using window::exp2_hw;
+
+// One thread per window row and K/V head: the row's weight under every query
+// head of the group, from its kept scores, added to the row's account.
+__global__ __launch_bounds__(256) void account_kernel(const WindowParams p, float* __restrict__ weights,
+                                                      bool fresh) {
+  const uint32_t r = blockIdx.x * 256 + threadIdx.x;
+  const uint32_t b = blockIdx.z;
+  uint32_t len = p.len, start = p.start;
+  if (p.lens) {
+    const int32_t L = p.lens[b];
+    len = L <= 0 ? 0u : min((uint32_t)L, p.M);
+    const int32_t st = p.starts[b] % (int32_t)p.M;
+    start = (uint32_t)(st < 0 ? st + (int32_t)p.M : st);
+  }
+  if (r >= len) return;
+  const size_t h0 = (size_t)b * p.H + blockIdx.y * p.group;
+  float sum = 0.f;
+  for (uint32_t h = 0; h < p.group; ++h) {
+    const float m = p.stats[(h0 + h) * 2], l = p.stats[(h0 + h) * 2 + 1];
+    sum += exp2_hw(p.scores[(h0 + h) * p.score_stride + r] - m) / l;
+  }
+  uint32_t slot = start + r;
+  slot = slot >= p.M ? slot - p.M : slot;
+  float* w = weights + ((size_t)b * p.KH + blockIdx.y) * p.M + slot;
+  *w = fresh && r == len - 1 ? sum : *w + sum;
+}
+
+__global__ __launch_bounds__(256) void clear_weights_kernel(float* weights, uint64_t units, uint32_t M,
+                                                            uint32_t pos, uint32_t n) {
+  const uint32_t s = blockIdx.x * 256 + threadIdx.x;
+  if (s >= n) return;
+  const uint32_t slot = (uint32_t)(((uint64_t)pos + s) % M);
+  for (uint64_t u = blockIdx.y; u < units; u += gridDim.y) weights[u * M + slot] = 0.f;
+}
+
+struct WindowPlan {
+  int row_tiles = 1;
+  uint32_t rblocks = 1, nsplit = 1;
+  size_t record = 0;  // floats of a split's record
+};
+
+WindowPlan plan_window(const WindowParams& p, uint32_t batch, uint32_t max_rows) {
+  WindowPlan pl;
+  const uint32_t rows = p.T * p.group;
+  pl.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const uint32_t per = 16u * pl.row_tiles;
+  pl.rblocks = (rows + per - 1) / per;
+  const uint64_t units = (uint64_t)batch * p.KH * pl.rblocks;
+  const uint64_t target = (uint64_t)device_cu_count();
+  const uint64_t want = std::max<uint64_t>(1, (target + units - 1) / units);
+  // A split is worth its record from a tile for each of its waves on.
+  const uint64_t most = (max_rows + window::kTile * window::kWaves - 1) / (window::kTile * window::kWaves);
+  pl.nsplit = (uint32_t)std::max<uint64_t>(1, std::min({want, most, (uint64_t)window::kMaxSplits}));
+  pl.record = (size_t)per * ((p.dh <= 64 ? 64 : 128) + 2);
+  return pl;
+}
+
+int window_workspace(const WindowParams& p, const WindowPlan& pl, uint32_t batch, hipStream_t stream,
+                     Workspace** out) {
+  *out = nullptr;
+  if (pl.nsplit <= 1) return STS_OK;
+  const size_t units = (size_t)batch * p.KH * pl.rblocks;
+  return get_workspace(stream, units * pl.nsplit * pl.record, units, out);
+}
+
+}  // namespace
+
+int check_window(const WindowParams& p, uint32_t batch, bool bf16) {
+  STS_CHECK(batch >= 1 && p.T >= 1 && p.H >= 1 && p.KH >= 1 && p.M >= 1, "empty shape");
+  STS_CHECK(p.dh >= 4 && p.dh <= 128 && p.dh % 4 == 0,
+            "head_dim %u not supported (a multiple of 4 up to 128)", p.dh);
+  STS_CHECK(!bf16 || p.dh % 8 == 0, "bf16 K/V rows need a head_dim that is a multiple of 8 (got %u)", p.dh);
+  STS_CHECK(p.H % p.KH == 0, "query heads %u not a multiple of the %u K/V heads", p.H, p.KH);
+  STS_CHECK((uint64_t)p.M * p.dh * (bf16 ? 2 : 4) <= 0x7FFFFFF0ull,
+            "max_len %u too large for one head's buffer resource", p.M);
+  STS_CHECK(batch <= 65535 && p.KH <= 65535, "batch (%u) and kv_heads (%u) must be <= 65535", batch, p.KH);
+  STS_CHECK((uint64_t)p.T * p.H <= 0x7FFFFFFull, "too many query rows (%u x %u)", p.T, p.H);
+  return STS_OK;
+}
+
+int reserve_window(const WindowParams& p, uint32_t batch, uint32_t max_rows, hipStream_t stream) {
+  Workspace* ws = nullptr;
+  return window_workspace(p, plan_window(p, batch, max_rows), batch, stream, &ws);
+}
+
+int launch_window(WindowParams p, WindowMode mode, uint32_t batch, bool bf16, uint32_t max_rows,
+                  hipStream_t stream) {
+  if (int rc = check_window(p, batch, bf16)) return rc;
+  const WindowPlan pl = plan_window(p, batch, max_rows);
+  Workspace* ws = nullptr;
+  if (int rc = window_workspace(p, pl, batch, stream, &ws)) return rc;
+  p.rblocks = pl.rblocks;
+  p.nsplit = pl.nsplit;
+  if (ws) {
+    p.part = ws->part;
+    p.counters = ws->counters;
+  }
+  const dim3 grid(pl.nsplit * pl.rblocks, p.KH, batch);
+  if (mode == kWindowTree) return launch_window_tree(p, pl.row_tiles, bf16, grid, stream);
+  if (mode == kWindowMasked) return launch_window_masked(p, pl.row_tiles, bf16, grid, stream);
+  return launch_window_weights(p, pl.row_tiles, bf16, grid, stream);
+}
+
+int launch_account(const WindowParams& p, float* weights, uint32_t batch, uint32_t max_rows,
+                   bool fresh, hipStream_t stream) {
+  const dim3 grid((max_rows + 255) / 256, p.KH, batch);
+  hipLaunchKernelGGL(account_kernel, grid, dim3(256), 0, stream, p, weights, fresh);
+  STS_HIP(hipGetLastError());
+  return STS_OK;
+}
+
+int launch_clear_weights(float* weights, uint64_t units, uint32_t M, uint32_t pos, uint32_t n,
+                         hipStream_t stream) {
+  if (n == 0) return STS_OK;
+  const dim3 grid((n + 255) / 256, (uint32_t)std::min<uint64_t>(units, 4096));
+  hipLaunchKernelGGL(clear_weights_kernel, grid, dim3(256), 0, stream, weights, units, M, pos, n);
+  STS_HIP(hipGetLastError());
+  return STS_OK;
+}
+
+}  // namespace sts

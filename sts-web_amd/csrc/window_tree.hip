@@ -1,0 +1,12 @@
+// window_tree.hip -- the instances of window_kernel.hpp's kernel behind
+// sts_tree_attention.
+#include "window_kernel.hpp"
+
+namespace sts {
+
+int launch_window_tree(const WindowParams& p, int row_tiles, bool bf16, dim3 grid,
+                       hipStream_t stream) {
+  return window::launch_mode<kWindowTree>(p, row_tiles, bf16, grid, stream);
+}
+
+}  // namespace sts

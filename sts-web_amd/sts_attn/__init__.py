@@ -38,6 +38,10 @@ PREC_F32 = 0
 PREC_BF16_MFMA = 1
 PREC_F32_SPLIT_BF16 = 2
 KV_BF16_MIRROR = 1
+KV_WEIGHTS = 2
+ROWS_F32 = 0
+ROWS_BF16 = 1
+TREE_MAX_NODES = 256
 
 _vp = ctypes.c_void_p
 _u32 = ctypes.c_uint32
@@ -71,6 +75,12 @@ SIGNATURES = {
                                   _u32, _f32, _vp]),
     "sts_prefill_attention": (_int, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _f32,
                                      _int, _vp]),
+    "sts_tree_attention": (_int, [_vp] * 8 + [_u32] * 6 + [_f32, _int, _vp]),
+    "sts_tree_commit": (_int, [_vp] * 7 + [_u32] * 5 + [_int, _vp]),
+    "sts_masked_attention": (_int, [_vp] * 10 + [_u32] * 6 + [_f32, _f32, _int, _vp]),
+    "sts_decode_ring_weights": (_int, [_vp] * 8 + [_u32] * 5 + [_f32, _int, _vp]),
+    "sts_decode_ring_weights_scratch": (_u64, [_u32, _u32, _u32]),
+    "sts_evict_ring": (_int, [_vp] * 6 + [_u32] * 6 + [_int, _vp]),
     "sts_rope_create": (_int, [_u32, _u32, _f32, ctypes.POINTER(_vp)]),
     "sts_rope_destroy": (_int, [_vp]),
     "sts_rope_apply": (_int, [_vp, _vp, _u32, _u32, _u32, _u32, _vp]),
@@ -94,6 +104,10 @@ SIGNATURES = {
     "sts_kv_attend": (_int, [_vp, _vp, _vp, _f32, _vp]),
     "sts_kv_decode_step": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _u64, _f32, _vp]),
     "sts_kv_prefill": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _u64, _f32, _int, _vp]),
+    "sts_kv_weights": (_int, [_vp, ctypes.POINTER(_vp)]),
+    "sts_kv_tree_step": (_int, [_vp] * 7 + [_u64, _f32, _vp]),
+    "sts_kv_tree_commit": (_int, [_vp, _u64, ctypes.POINTER(_u32), _u64, _vp]),
+    "sts_kv_evict": (_int, [_vp, _u64, _u64, _vp, _vp]),
     "sts_device_errors": (_int, [_vp, ctypes.POINTER(_u32)]),
     "sts_debug_set_wait_limit": (_int, [_u32]),
     "sts_q4k_matvec": (_int, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp]),
@@ -263,6 +277,178 @@ def prefill_attention_bf16kv(q: torch.Tensor, k16: torch.Tensor, v16: torch.Tens
 
 
 # ---------------------------------------------------------------------------
+# Drafts, masks and kept attention weights over ring windows
+# ---------------------------------------------------------------------------
+
+_ROW_TYPES = {torch.float32: ROWS_F32, torch.bfloat16: ROWS_BF16}
+
+
+def _rows(k_cache: torch.Tensor, v_cache: torch.Tensor):
+    """(B, KVH, M, D, row type, device) of K/V caches, after their checks."""
+    shape, dtype, device = k_cache.shape, k_cache.dtype, k_cache.device
+    if dtype not in _ROW_TYPES or v_cache.dtype != dtype:
+        raise TypeError(f"K/V caches must both be float32 or bfloat16, got {dtype}, {v_cache.dtype}")
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError(f"K/V caches must both be [B, KVH, M, D], got {tuple(shape)}, "
+                         f"{tuple(v_cache.shape)}")
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise ValueError(f"K/V caches must be on the current GPU, got {device}")
+    _arg(v_cache, "v_cache", dtype, shape, device)
+    if not k_cache.is_contiguous():
+        raise ValueError("k_cache must be contiguous")
+    return (*shape, _ROW_TYPES[dtype], device)
+
+
+def _arg(t: Optional[torch.Tensor], name: str, dtype, shape, device) -> Optional[int]:
+    """The address of a contiguous tensor of this type, shape and device (None: none)."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _made_for(stream, *tensors) -> None:
+    """Tensors allocated here on the current stream and used on `stream`: their
+    memory is not reused before that stream is done with them."""
+    if stream is None:
+        return
+    handle = _stream(stream)
+    if handle != _stream(None):
+        s = torch.cuda.ExternalStream(handle) if isinstance(stream, int) else stream
+        for t in tensors:
+            t.record_stream(s)
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   parents: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor, scale: float,
+                   counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                   stream=None) -> torch.Tensor:
+    """Attention of each stream's draft, its window's last counts[b] rows (default
+    all T), over the committed rows and each node's ancestors: q [B,T,H,D] float32,
+    caches [B,KVH,M,D] float32 or bfloat16, parents [B,T] int32 (-1: a child of the
+    last committed row), lens/starts/counts [B] int32."""
+    B, KH, M, D, rows, dev = _rows(k_cache, v_cache)
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:
+        raise ValueError(f"q must be [{B}, T, H, {D}], got {tuple(q.shape)}")
+    T, H = q.shape[1], q.shape[2]
+    qp = _arg(q, "q", torch.float32, q.shape, dev)
+    if out is None:
+        out = torch.empty_like(q)
+        _made_for(stream, out)
+    i32 = torch.int32
+    _check(load().sts_tree_attention(
+        qp, k_cache.data_ptr(), v_cache.data_ptr(), _arg(out, "out", torch.float32, q.shape, dev),
+        _arg(parents, "parents", i32, (B, T), dev), _arg(counts, "counts", i32, (B,), dev),
+        _arg(lens, "lens", i32, (B,), dev), _arg(starts, "starts", i32, (B,), dev), B, T, H, KH, D, M,
+        scale, rows, _stream(stream)))
+    return out
+
+
+def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, path: torch.Tensor,
+                accepted: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor,
+                counts: Optional[torch.Tensor] = None, stream=None) -> None:
+    """Keeps the accepted path of each stream's draft in place: draft row path[b][j]
+    becomes draft row j for j < accepted[b].  path [B,T], the others [B], int32; the
+    caller then shortens the window by counts[b] - accepted[b]."""
+    B, KH, M, D, rows, dev = _rows(k_cache, v_cache)
+    i32 = torch.int32
+    if path.dim() != 2:
+        raise ValueError(f"path must be [{B}, T], got {tuple(path.shape)}")
+    T = path.shape[1]
+    _check(load().sts_tree_commit(
+        k_cache.data_ptr(), v_cache.data_ptr(), _arg(path, "path", i32, (B, T), dev),
+        _arg(accepted, "accepted", i32, (B,), dev), _arg(counts, "counts", i32, (B,), dev),
+        _arg(lens, "lens", i32, (B,), dev), _arg(starts, "starts", i32, (B,), dev), B, T, KH, D, M,
+        rows, _stream(stream)))
+
+
+def masked_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     lens: torch.Tensor, starts: torch.Tensor, scale: float,
+                     lo: Optional[torch.Tensor] = None, hi: Optional[torch.Tensor] = None,
+                     counts: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None,
+                     softcap: float = 0.0, out: Optional[torch.Tensor] = None,
+                     stream=None) -> torch.Tensor:
+    """Attention of each stream's last counts[b] rows (default all S) over the window
+    rows lo..hi-1 of each query (defaults 0 and its own row + 1): q [B,S,H,D] float32,
+    caches [B,KVH,M,D] float32 or bfloat16, lo/hi [B,S] int32, lens/starts/counts [B]
+    int32.  softcap > 0 caps the scores at softcap * tanh(x / softcap); slopes [H]
+    float32 takes slopes[h] * distance off them.  A query that sees nothing gets 0."""
+    B, KH, M, D, rows, dev = _rows(k_cache, v_cache)
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:
+        raise ValueError(f"q must be [{B}, S, H, {D}], got {tuple(q.shape)}")
+    S, H = q.shape[1], q.shape[2]
+    qp = _arg(q, "q", torch.float32, q.shape, dev)
+    if out is None:
+        out = torch.empty_like(q)
+        _made_for(stream, out)
+    i32 = torch.int32
+    _check(load().sts_masked_attention(
+        qp, k_cache.data_ptr(), v_cache.data_ptr(), _arg(out, "out", torch.float32, q.shape, dev),
+        _arg(lo, "lo", i32, (B, S), dev), _arg(hi, "hi", i32, (B, S), dev),
+        _arg(slopes, "slopes", torch.float32, (H,), dev), _arg(counts, "counts", i32, (B,), dev),
+        _arg(lens, "lens", i32, (B,), dev), _arg(starts, "starts", i32, (B,), dev), B, S, H, KH, D, M,
+        scale, softcap, rows, _stream(stream)))
+    return out
+
+
+def decode_ring_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                        weights: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor,
+                        scale: float, out: Optional[torch.Tensor] = None,
+                        stream=None) -> torch.Tensor:
+    """decode_ring that adds every window row's attention weight (summed over the
+    heads of its K/V head) to weights [B,KVH,M] float32 at the row's slot: q [B,H,D]
+    float32, caches [B,KVH,M,D] float32 or bfloat16, lens/starts [B] int32."""
+    B, KH, M, D, rows, dev = _rows(k_cache, v_cache)
+    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D:
+        raise ValueError(f"q must be [{B}, H, {D}], got {tuple(q.shape)}")
+    H = q.shape[1]
+    qp = _arg(q, "q", torch.float32, q.shape, dev)
+    lib = load()
+    scratch = torch.empty(lib.sts_decode_ring_weights_scratch(B, H, M), dtype=torch.float32, device=dev)
+    if out is None:
+        out = torch.empty_like(q)
+        _made_for(stream, out)
+    _made_for(stream, scratch)
+    i32 = torch.int32
+    _check(lib.sts_decode_ring_weights(
+        qp, k_cache.data_ptr(), v_cache.data_ptr(), _arg(out, "out", torch.float32, q.shape, dev),
+        _arg(weights, "weights", torch.float32, (B, KH, M), dev), scratch.data_ptr(),
+        _arg(lens, "lens", i32, (B,), dev), _arg(starts, "starts", i32, (B,), dev), B, H, KH, D, M,
+        scale, rows, _stream(stream)))
+    return out
+
+
+def evict_ring(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor,
+               lens: torch.Tensor, starts: torch.Tensor, keep: int, recent: int,
+               kept: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """Cuts each stream's window to `keep` rows per K/V head, in place: the `recent`
+    newest and those of the others with the largest weight (the oldest first among
+    equals) become its last `keep` rows, weights with them.  Returns the window rows
+    kept, [B,KVH,keep] int32 (-1 past a shorter window, which stays as it is); the
+    caller then sets starts += lens - keep (modulo M) and lens = keep where lens > keep."""
+    B, KH, M, D, rows, dev = _rows(k_cache, v_cache)
+    if keep < 1 or keep > M or recent < 0 or recent > keep:
+        raise StsError(STS_ERR_INVALID, f"need 1 <= keep ({keep}) <= max_len ({M}) and "
+                       f"0 <= recent ({recent}) <= keep")
+    if kept is None:
+        kept = torch.empty((B, KH, keep), dtype=torch.int32, device=dev)
+        _made_for(stream, kept)
+    i32 = torch.int32
+    _check(load().sts_evict_ring(
+        k_cache.data_ptr(), v_cache.data_ptr(), _arg(weights, "weights", torch.float32, (B, KH, M), dev),
+        _arg(kept, "kept", i32, (B, KH, keep), dev), _arg(lens, "lens", i32, (B,), dev),
+        _arg(starts, "starts", i32, (B,), dev), B, KH, D, M, keep, recent, rows, _stream(stream)))
+    return kept
+
+
+# ---------------------------------------------------------------------------
 # RoPE
 # ---------------------------------------------------------------------------
 
@@ -345,13 +531,15 @@ class KVCache:
     """Ring-buffer KV cache in HBM, KVCache (model.rs:195-363)."""
 
     def __init__(self, max_len: int, n_kv_heads: int, head_dim: int, bf16_mirror: bool = False,
-                 n_heads: Optional[int] = None):
+                 n_heads: Optional[int] = None, keep_weights: bool = False):
         """n_heads: query heads when they outnumber the K/V heads (grouped-query
-        attention, model.rs:766-783); q and out then have n_heads heads."""
+        attention, model.rs:766-783); q and out then have n_heads heads.
+        keep_weights: attend and decode_step keep each row's share of the attention,
+        by which evict chooses."""
         _drain_deferred()
         h = _vp()
-        _check(load().sts_kv_create_ex(max_len, n_kv_heads, head_dim,
-                                       KV_BF16_MIRROR if bf16_mirror else 0, ctypes.byref(h)))
+        flags = (KV_BF16_MIRROR if bf16_mirror else 0) | (KV_WEIGHTS if keep_weights else 0)
+        _check(load().sts_kv_create_ex(max_len, n_kv_heads, head_dim, flags, ctypes.byref(h)))
         self._h = h
         self.n_kv_heads = n_kv_heads
         self.n_heads = n_heads or n_kv_heads
@@ -413,6 +601,13 @@ class KVCache:
         return (copy_device(kp.value, shape, torch.int16),
                 copy_device(vp.value, shape, torch.int16))
 
+    def read_weights(self):
+        """A copy of the kept attention weights [B, H, max_len] by slot, or None."""
+        s = self.state()
+        wp = _vp()
+        _check(load().sts_kv_weights(self._h, ctypes.byref(wp)))
+        return copy_device(wp.value, (s.batch, s.heads, s.max_len)) if wp.value else None
+
     def sync_mirror(self, stream=None) -> None:
         _check(load().sts_kv_sync_mirror(self._h, _stream(stream)))
 
@@ -468,6 +663,47 @@ class KVCache:
                                      _ptr(k_new), _ptr(v_new), _ptr(out), S, scale, precision,
                                      _stream(stream)))
         return out
+
+    def tree_step(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
+                  parents: torch.Tensor, scale: float, rope: Optional[RoPE] = None,
+                  out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """Appends a draft's T rows k_new, v_new [T, KVH, D] and attends with q [T, H, D]
+        over the committed rows and each node's ancestors; parents [T] int32 (-1: a child
+        of the last committed row).  With `rope`, node rows are rotated at offset + depth.
+        tree_commit (or rollback(T)) has to follow."""
+        T, dev = q.shape[0], q.device
+        if dev.type != "cuda" or dev.index != torch.cuda.current_device():
+            raise ValueError(f"q must be on the current GPU, got {dev}")
+        qs, ks = (T, self.n_heads, self.head_dim), (T, self.n_kv_heads, self.head_dim)
+        qp = _arg(q, "q", torch.float32, qs, dev)
+        if out is None:
+            out = torch.empty_like(q)
+            _made_for(stream, out)
+        _check(load().sts_kv_tree_step(
+            self._h, rope.handle if rope is not None else None, qp,
+            _arg(k_new, "k_new", torch.float32, ks, dev), _arg(v_new, "v_new", torch.float32, ks, dev),
+            _arg(parents, "parents", torch.int32, (T,), dev), _arg(out, "out", torch.float32, qs, dev),
+            T, scale, _stream(stream)))
+        return out
+
+    def tree_commit(self, nodes: int, path: Sequence[int], stream=None) -> None:
+        """Ends a draft of `nodes` rows: the rows of the accepted path (node indices,
+        ascending) stay as the window's last ones, the others are rolled back."""
+        host = (_u32 * max(len(path), 1))(*path)
+        _check(load().sts_kv_tree_commit(self._h, nodes, host, len(path), _stream(stream)))
+
+    def evict(self, keep: int, recent: int, kept: Optional[torch.Tensor] = None,
+              stream=None) -> None:
+        """Cuts the window to `keep` rows per K/V head: the `recent` newest and those of
+        the others that got most of the attention (keep_weights).  kept [B, KVH, keep]
+        int32 receives the window rows kept."""
+        s = self.state()
+        kp = None
+        if kept is not None:
+            kp = _arg(kept, "kept", torch.int32, (s.batch, s.heads, keep), kept.device)
+            if kept.device.type != "cuda":
+                raise ValueError("kept must be on the GPU")
+        _check(load().sts_kv_evict(self._h, keep, recent, kp, _stream(stream)))
 
     def close(self):
         if self._h:

@@ -1,0 +1,126 @@
+"""Ring windows for the tests of drafts, masks and kept weights, and their 64-bit forms.
+
+A Window holds ragged streams' caches with every slot outside the windows set to
+NaN, so that a kernel that lets one through shows it.  attend64 is attention from
+its definition in 64 bits on one stream's ordered rows; its bound is an upper bound
+of the rounding of an f32 evaluation.
+"""
+import numpy as np
+import torch
+
+U = 2.0 ** -24  # half a step of f32, relative
+
+
+class Window:
+    def __init__(self, seed, B, KH, M, D, lens, dtype=torch.float32, starts=None):
+        rng = np.random.default_rng(seed)
+        self.rng, self.B, self.KH, self.M, self.D = rng, B, KH, M, D
+        self.lens = np.asarray(lens, np.int32)
+        self.starts = rng.integers(0, M, B).astype(np.int32) if starts is None else np.asarray(starts, np.int32)
+        self.dtype = dtype
+        k = torch.full((B, KH, M, D), float("nan"), dtype=dtype)
+        v = torch.full((B, KH, M, D), float("nan"), dtype=dtype)
+        for b in range(B):
+            s = torch.from_numpy(self.slots(b))
+            k[b, :, s] = torch.from_numpy(rng.standard_normal((KH, len(s), D))).to(dtype)
+            v[b, :, s] = torch.from_numpy(rng.standard_normal((KH, len(s), D))).to(dtype)
+        self.k, self.v = k, v
+
+    def slots(self, b):
+        return (int(self.starts[b]) + np.arange(int(self.lens[b]))) % self.M
+
+    def rows(self, b, t):
+        """Stream b's ordered rows of a cache, [KH, L, D] in 64 bits."""
+        return t[b][:, torch.from_numpy(self.slots(b))].double().numpy()
+
+    def dev(self, *names):
+        out = []
+        for n in names:
+            x = getattr(self, n)
+            out.append((torch.from_numpy(x) if isinstance(x, np.ndarray) else x).cuda())
+        return out
+
+
+def queries(rng, *shape):
+    """f32 queries, some heads broad and some sharp."""
+    return (rng.standard_normal(shape) * rng.uniform(0.5, 3.0, (shape[-2], 1))).astype(np.float32)
+
+
+def attend64(q, k, v, seen, scale, softcap=0.0, slopes=None, w=None):
+    """q [n,H,D], k/v [KH,L,D], seen [n,L] -> (out [n,H,D], p [n,H,L], bound [n,H]).
+
+    bound: each score is a sum of D products and two scalings, off by at most
+    (D + 4) u sum |q k| scale; the cap's tanh, within 3 u relative, and the bias add
+    8 u of their size.  A score off by e turns its weight by the factor 1 +- (e + 3u)
+    (the base-2 exponential of the hardware within 2 u), the normalised sum by twice
+    that, and adding up L weighted rows by (L + 8) u, all of the largest |v|."""
+    n, H, D = q.shape
+    g = H // k.shape[0]
+    L = k.shape[1]
+    out, p, bound = np.zeros((n, H, D)), np.zeros((n, H, L)), np.zeros((n, H))
+    for h in range(H):
+        kk, vv = k[h // g], v[h // g]
+        x = np.full((n, L), -np.inf)
+        size = np.zeros((n, L))
+        for i in range(n):
+            at = np.flatnonzero(seen[i])
+            if not len(at):
+                continue
+            qi = q[i, h].astype(np.float64)
+            s = kk[at] @ qi * scale
+            big = np.abs(kk[at]) @ np.abs(qi) * abs(scale) * (D + 4) * U
+            if softcap > 0:
+                s = softcap * np.tanh(s / softcap)
+                big = big + 8 * U * np.abs(s)
+            if slopes is not None:
+                away = slopes[h] * np.abs(w[i] - at)
+                s = s - away
+                big = big + 8 * U * (np.abs(away) + np.abs(s))
+            # The exponent's own scaling by log2 e and the subtraction of the maximum.
+            big = big + 4 * U * np.abs(s).max()
+            e = np.exp(s - s.max())
+            p[i, h, at] = e / e.sum()
+            out[i, h] = p[i, h, at] @ vv[at]
+            bound[i, h] = (2 * (big.max() + 3 * U) + (L + 8) * U) * np.abs(vv[at]).max()
+    return out, p, bound
+
+
+def ancestors(parents, n):
+    """[n, n] truth: j is i or above it; a parent outside 0..i-1 is the committed row."""
+    a = np.eye(n, dtype=bool)
+    for i in range(n):
+        if 0 <= parents[i] < i:
+            a[i] |= a[parents[i]]
+    return a
+
+
+def depths(parents, n):
+    d = np.zeros(n, np.int64)
+    for i in range(n):
+        if 0 <= parents[i] < i:
+            d[i] = d[parents[i]] + 1
+    return d
+
+
+def tree_seen(parents, n, L):
+    seen = np.ones((n, L), bool)
+    seen[:, L - n:] = ancestors(parents, n)
+    return seen
+
+
+def random_tree(rng, n, T):
+    p = np.full(T, -1, np.int32)
+    for i in range(1, n):
+        p[i] = rng.integers(-1, i)
+    return p
+
+
+def evict64(w, keep, recent):
+    """The rows kept of one head's ordered weights, by sorting."""
+    L = len(w)
+    if L <= keep:
+        return np.arange(L)
+    old = np.where(np.isnan(w[:L - recent]), np.inf, w[:L - recent])  # NaN: the largest
+    nan = np.isnan(w[:L - recent])
+    order = np.lexsort((np.arange(len(old)), -old, ~nan))
+    return np.concatenate([np.sort(order[:keep - recent]), np.arange(L - recent, L)])
