@@ -50,18 +50,27 @@ struct WindowPlan {
   size_t record = 0;  // floats of a split's record
 };
 
-WindowPlan plan_window(const WindowParams& p, uint32_t batch, uint32_t max_rows) {
+WindowPlan plan_window(const WindowParams& p, uint32_t batch, bool bf16, uint32_t max_rows) {
   WindowPlan pl;
   const uint32_t rows = p.T * p.group;
-  pl.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  pl.row_tiles = rows <= 16 ? 1 : 2;
   const uint32_t per = 16u * pl.row_tiles;
   pl.rblocks = (rows + per - 1) / per;
   const uint64_t units = (uint64_t)batch * p.KH * pl.rblocks;
-  const uint64_t target = (uint64_t)device_cu_count();
+  // One row tile is bound by the reads: as many workgroups as keep 64 KB of rows
+  // requested on each CU (f32 rows of 128 one, bf16 rows of 64 four; at 7 streams of
+  // 20011 such rows 52 us against 102 with one).  Two are bound by their products:
+  // two workgroups, what a CU holds at once (a draft of 60 over 3000 rows 34 us, with
+  // four 49).
+  const uint32_t tile = 16 * pl.row_tiles;
+  const uint32_t wide = p.dh <= 64 ? 64 : 128;
+  const uint32_t tile_bytes = 2 * tile * wide * (bf16 ? 2 : 4) * window::kWaves;
+  const uint32_t per_cu = pl.row_tiles > 1 ? 2 : std::min(4u, std::max(1u, 65536 / tile_bytes));
+  const uint64_t target = (uint64_t)device_cu_count() * per_cu;
   const uint64_t want = std::max<uint64_t>(1, (target + units - 1) / units);
   // A split is worth its record from a tile for each of its waves on.
-  const uint64_t most = (max_rows + window::kTile * window::kWaves - 1) / (window::kTile * window::kWaves);
-  pl.nsplit = (uint32_t)std::max<uint64_t>(1, std::min({want, most, (uint64_t)window::kMaxSplits}));
+  const uint64_t most = (max_rows + tile * window::kWaves - 1) / (tile * window::kWaves);
+  pl.nsplit = (uint32_t)std::max<uint64_t>(1, std::min({want, most, (uint64_t)window::max_splits(pl.row_tiles)}));
   pl.record = (size_t)per * ((p.dh <= 64 ? 64 : 128) + 2);
   return pl;
 }
@@ -89,15 +98,16 @@ int check_window(const WindowParams& p, uint32_t batch, bool bf16) {
   return STS_OK;
 }
 
-int reserve_window(const WindowParams& p, uint32_t batch, uint32_t max_rows, hipStream_t stream) {
+int reserve_window(const WindowParams& p, uint32_t batch, bool bf16, uint32_t max_rows,
+                   hipStream_t stream) {
   Workspace* ws = nullptr;
-  return window_workspace(p, plan_window(p, batch, max_rows), batch, stream, &ws);
+  return window_workspace(p, plan_window(p, batch, bf16, max_rows), batch, stream, &ws);
 }
 
 int launch_window(WindowParams p, WindowMode mode, uint32_t batch, bool bf16, uint32_t max_rows,
                   hipStream_t stream) {
   if (int rc = check_window(p, batch, bf16)) return rc;
-  const WindowPlan pl = plan_window(p, batch, max_rows);
+  const WindowPlan pl = plan_window(p, batch, bf16, max_rows);
   Workspace* ws = nullptr;
   if (int rc = window_workspace(p, pl, batch, stream, &ws)) return rc;
   p.rblocks = pl.rblocks;
@@ -106,7 +116,8 @@ int launch_window(WindowParams p, WindowMode mode, uint32_t batch, bool bf16, ui
     p.part = ws->part;
     p.counters = ws->counters;
   }
-  const dim3 grid(pl.nsplit * pl.rblocks, p.KH, batch);
+  p.shares = batch * p.KH * pl.nsplit;
+  const dim3 grid((p.shares + window::kXcds - 1) / window::kXcds * window::kXcds * pl.rblocks);
   if (mode == kWindowTree) return launch_window_tree(p, pl.row_tiles, bf16, grid, stream);
   if (mode == kWindowMasked) return launch_window_masked(p, pl.row_tiles, bf16, grid, stream);
   return launch_window_weights(p, pl.row_tiles, bf16, grid, stream);

@@ -46,6 +46,7 @@ struct WindowParams {
   uint32_t score_stride = 0;
   // Set by launch_window.
   uint32_t rblocks = 1, nsplit = 1;
+  uint32_t shares = 0;  // streams x K/V heads x splits
   float* part = nullptr;
   uint32_t* counters = nullptr;
 };
@@ -59,7 +60,8 @@ int launch_window(WindowParams p, WindowMode mode, uint32_t batch, bool bf16, ui
 
 // Makes sure the split workspace launch_window needs for these sizes exists, so
 // that a caller can fail before it changes any state.
-int reserve_window(const WindowParams& p, uint32_t batch, uint32_t max_rows, hipStream_t stream);
+int reserve_window(const WindowParams& p, uint32_t batch, bool bf16, uint32_t max_rows,
+                   hipStream_t stream);
 
 // weights[b][j][slot of row r] += sum over the group's heads of
 // 2^(score - max) / sum, for the rows of each window; with `fresh` the newest

@@ -1,4 +1,4 @@
-// window_kernel.hpp -- attention of up to 64 query rows per K/V head over a
+// window_kernel.hpp -- attention of up to 32 query rows per K/V head over a
 // ring window on the f32 matrix cores (gfx950): the kernel behind
 // sts_tree_attention, sts_masked_attention and sts_decode_ring_weights.
 //
@@ -10,17 +10,25 @@
 // A workgroup takes 16*R query rows of one (stream, K/V head) -- the nodes or
 // queries times the heads of the group, so that a K/V row is read once for all
 // of them -- and one split of the window.  Its four waves share the query rows
-// and deal the split's 16-row tiles among themselves; nothing goes through LDS
-// until the end:
+// and deal the split's tiles among themselves; neither K, V nor the weights go
+// through LDS, the outputs only at the end:
 //   S^T = K Q^T    A = K tile: lane (m, g) = (lane & 15, lane >> 4) holds row m,
 //                  dims (4c + g)*CW + e; B = Q in the same dims.  The lane then
 //                  has the scores of query m for rows 4g .. 4g+3
-//   O^T += V^T P^T A = V^T: step i of 4 takes rows 4g + i, and the lane holds of
-//                  row 4g + i the dims (16 tc + m)*VW + e; B = the scores'
-//                  exponentials as they stand, register i
+//   O^T += V^T P^T A = V^T: the lane holds of rows 4g + i the dims
+//                  (16 tc + m)*VW + e; B = the scores' exponentials as they stand
 // Both tiles are 16-byte loads straight from the cache, and the exponentials
 // never leave their registers.  The waves' (m, l, O) are merged through LDS, the
 // splits' through records in the stream's workspace by the last to arrive.
+//
+// One row tile (R = 1) multiplies in f32 (16x16x4): its 64 products of a 16 KB tile
+// take a quarter of the time that HBM takes to deliver it.  Two (R = 2) would be
+// bound by those products and multiply parts instead (16x16x32): f32 rows as two
+// f16 values each, three products for one; bf16 rows as they are against three
+// bf16 parts of Q and of the weights.  Either is as close to the exact result as f32
+// products are.  At 1000 queries of 32 heads over 2600 bf16 rows of 8 K/V heads
+// that is 111 us against 488 in f32; at 24 drafts of 40 nodes over f32 rows 189
+// against 513.
 #pragma once
 
 #include <cfloat>
@@ -36,8 +44,10 @@ namespace window {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWaves = 4;
-constexpr int kTile = 16;             // window rows a wave takes at once
-constexpr int kMaxSplits = 64;
+constexpr uint32_t kXcds = 8;
+// Splits of a block of 16 * row_tiles query rows at most: the merge holds two
+// numbers for each split and row in LDS.
+constexpr int max_splits(int row_tiles) { return 128 / row_tiles; }
 constexpr uint32_t kOutside = 0x80000000u;  // past every buffer resource: loads zeros
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -88,6 +98,12 @@ struct Piece {
       w[1] = x[1];
     }
   }
+  __device__ __forceinline__ void times(float f) {
+    if constexpr (!BF) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * f);
+    }
+  }
   __device__ __forceinline__ float operator[](int e) const {
     if constexpr (BF) {
       const uint32_t x = w[e >> 1];
@@ -102,18 +118,128 @@ __device__ __forceinline__ bool not_finite(float x) {
   return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
 }
 
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// The matrix operands that stand for f32 values x[8].  Against f32 rows: two f16
+// values, each the nearest, off by at most 2^-22 of x, and by 2^-25 where the second
+// falls below f16's normal range; the products of the two second parts are left
+// out.  Against bf16 rows, which are operands as they are: three bf16 values whose
+// sum is x.
+template <bool BF>
+struct Parts {
+  typedef half8 V;
+  static constexpr int N = 2;
+  static __device__ __forceinline__ void split(const float* x, V (&y)[N]) {
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    u32x4 w[N];  // pairs put together as words: no half moves on its own
+    // A one that the compiler does not know: x * one - h is a single mixed-precision
+    // instruction, x - h a conversion and a subtraction.
+    float one = 1.f;
+    asm("" : "+s"(one));
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const half2v h = __builtin_convertvector((f2){x[e], x[e + 1]}, half2v);
+      const half2v r = __builtin_convertvector((f2){fmaf(x[e], one, -(float)h[0]), fmaf(x[e + 1], one, -(float)h[1])}, half2v);
+      w[0][e / 2] = __builtin_bit_cast(uint32_t, h);
+      w[1][e / 2] = __builtin_bit_cast(uint32_t, r);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) y[n] = __builtin_bit_cast(V, w[n]);
+  }
+  static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Parts<true> {
+  typedef bf16x8 V;
+  static constexpr int N = 3;
+  static __device__ __forceinline__ void split(const float* x, V (&y)[N]) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    u32x4 w[N];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      float a = x[e], z = x[e + 1];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        w[n][e / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, z}, b2));
+        a -= __uint_as_float(w[n][e / 2] << 16);
+        z -= __uint_as_float(w[n][e / 2] & 0xffff0000u);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) y[n] = __builtin_bit_cast(V, w[n]);
+  }
+  static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+// The power of two that takes x (positive, finite) to 64..128, within 2^+-60.
+__device__ __forceinline__ float scale_to_64(float x) {
+  const int e = 127 + 6 - ((int)(__float_as_uint(x) >> 23) - 127);
+  return __uint_as_float((uint32_t)min(max(e, 127 - 60), 127 + 60) << 23);
+}
+
+// What the f32 rows are multiplied by before they are split: 1 where the wave's
+// first tile that holds anything reaches between 1/2 and 2^12, else the power of
+// two that takes its largest value to 64..128.
+struct TileScale {
+  float scale = 1.f, inverse = 1.f;
+  bool set = false;
+  __device__ __forceinline__ void choose(float top) {
+    const float all = wave_max(top);
+    if (all > 0.f && all < INFINITY) {  // (outputs of tiles of zeros need no rescaling)
+      const float x = all >= 0.5f && all <= 4096.f ? 1.f : scale_to_64(all);
+      scale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
+      inverse = 1.f / scale;
+      set = true;
+    }
+  }
+  // Whether a tile that reaches `top` in magnitude in this lane (NaN and infinity
+  // kept) is held well: all finite, below f16's range, and not so small that its
+  // steps would show.
+  __device__ __forceinline__ bool holds(float top) {
+    if (!set) choose(top);
+    const float t = top * scale;
+    return __all(t < 60000.f) && (__any(t >= 0.25f) || __all(t == 0.f));
+  }
+};
+
 template <int D, int R, bool BF, WindowMode MODE, bool PAD>
-__global__ __launch_bounds__(kWaves * 64) void window_kernel(const WindowParams p) {
+__global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowParams p) {
   constexpr int CW = BF ? 8 : 4;                    // dims of K a lane loads at once
   constexpr int NC = D / (4 * CW);                  // loads per K row tile
   constexpr int VW = CW < D / 16 ? CW : D / 16;     // dims of V a lane loads at once
   constexpr int NV = D / (16 * VW);                 // loads per V row
   constexpr int ES = BF ? 2 : 4;                    // bytes per element
+  constexpr bool PARTS = R > 1;                     // products of f16 parts
+  constexpr int KT = PARTS ? 2 : 1;                 // 16-row tiles a wave takes at once
+  constexpr int TILE = 16 * KT;
+  constexpr int NP = NC * CW / 8;                   // 32-dim steps of K Q^T in f16
+  constexpr int NX = NV * VW;                       // 16-dim tiles of the output
   constexpr int ROWS = 16 * R;
   constexpr int LDO = D + 4;                        // LDS row of a partial output
   constexpr int C4 = D / 4;
 
-  __shared__ __align__(16) float s_o[kWaves][16][LDO];
+  // The queries' f16 parts while the tiles are read, partial outputs after that.
+  typedef Parts<BF> P;
+  typedef typename P::V Frag;
+  constexpr int kPartBytes = PARTS ? R * NP * P::N * 64 * 16 : 0;
+  constexpr int kOutBytes = kWaves * ROWS * LDO * 4;
+  __shared__ __align__(16) char s_mem[kPartBytes > kOutBytes ? kPartBytes : kOutBytes];
+  auto& s_q = *reinterpret_cast<Frag(*)[PARTS ? R : 1][NP][P::N][64]>(s_mem);
+  auto& s_o = *reinterpret_cast<float(*)[kWaves][ROWS][LDO]>(s_mem);
+  __shared__ float s_qs[PARTS ? ROWS : 1];  // what the rows' scores are multiplied by
+  struct Row {
+    uint32_t lo, hi;
+    int at;       // window row of the query
+    float slope;  // in units of log2(e)
+  };
+  __shared__ Row s_row[MODE == kWindowMasked ? ROWS : 1];
   __shared__ float s_ml[kWaves][ROWS][2];
   __shared__ uint32_t s_last;
   __shared__ uint32_t s_anc[MODE == kWindowTree ? kMaxTreeNodes : 1][kMaxTreeNodes / 32];
@@ -122,9 +248,35 @@ __global__ __launch_bounds__(kWaves * 64) void window_kernel(const WindowParams 
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int m16 = lane & 15, g = lane >> 4;
-  const uint32_t split = blockIdx.x % p.nsplit, rb = blockIdx.x / p.nsplit;
-  const uint32_t kvh = blockIdx.y, b = blockIdx.z;
+  // Workgroups go round the XCDs: the row blocks of one (stream, K/V head, split),
+  // which read the same rows, take turns on one of them, next to one another, so that
+  // its L2 serves all but the first.
+  const uint32_t turn = blockIdx.x / kXcds, rb = turn % p.rblocks;
+  const uint32_t share = turn / p.rblocks * kXcds + blockIdx.x % kXcds;
+  if (share >= p.shares) return;
+  const uint32_t split = share % p.nsplit, kvh = share / p.nsplit % p.KH, b = share / p.nsplit / p.KH;
   const uint32_t dh = PAD ? p.dh : (uint32_t)D;
+
+  // What does not depend on the window's length is requested first: the queries of
+  // the wave's row tile (dims (4c + g)*CW + e of row m16 in this lane), the draft.
+  const uint32_t all = p.T * p.group;
+  const uint32_t qrow = rb * ROWS + (PARTS ? wave % R * 16 : 0) + m16;
+  float4 qraw[NC * CW / 4];
+  {
+    const float* src = p.q + (((size_t)b * p.T + qrow / p.group) * p.H + kvh * p.group + qrow % p.group) * dh;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < CW; e += 4) {
+        const uint32_t d = (c * 4 + g) * CW + e;
+        qraw[(c * CW + e) / 4] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (qrow < all && (!PAD || d < dh)) qraw[(c * CW + e) / 4] = *reinterpret_cast<const float4*>(src + d);
+      }
+  }
+  const bool narrow = MODE == kWindowTree && p.T <= 64;
+  const int me = narrow ? lane : tid;  // the node that this lane looks after
+  int up = -1;
+  if (MODE == kWindowTree && me < (int)p.T) up = p.parents[(size_t)b * p.T + me];
 
   uint32_t len = p.len, start = p.start;
   if (p.lens) {
@@ -141,7 +293,7 @@ __global__ __launch_bounds__(kWaves * 64) void window_kernel(const WindowParams 
   const uint32_t base = len - n;  // window row of query 0
 
   // Row rr of the block is query rr / group, head kvh*group + rr % group.
-  const uint32_t row0 = rb * ROWS, nrows = n * p.group, all = p.T * p.group;
+  const uint32_t row0 = rb * ROWS, nrows = n * p.group;
   auto out_row = [&](uint32_t rr) {
     return p.out + (((size_t)b * p.T + rr / p.group) * p.H + kvh * p.group + rr % p.group) * dh;
   };
@@ -155,52 +307,53 @@ __global__ __launch_bounds__(kWaves * 64) void window_kernel(const WindowParams 
   if (split == 0 && live < end) zero_rows(live, end);
   if (live == row0) return;
 
-  // The rows that each query sees, and their union over the block.  Rows of the
-  // block past the queries see everything, so that they never make a tile
-  // partly seen; their results go nowhere.
-  uint32_t lo[R], hi[R], ulo = 0, uhi = len;
-  bool real[R];
+  // The rows that each query sees, their union over the block, and the rows that
+  // all of its queries see.  Rows of the block past the queries see everything, so
+  // that they never make a tile partly seen; their results go nowhere.
+  uint32_t ulo = 0, uhi = len, alo = 0, ahi = MODE == kWindowTree ? base : len;
   if constexpr (MODE == kWindowMasked) {
     ulo = len;
     uhi = 0;
-  }
-#pragma unroll
-  for (int rt = 0; rt < R; ++rt) {
-    const uint32_t rr = row0 + rt * 16 + m16;
-    real[rt] = rr < nrows;
-    lo[rt] = 0;
-    hi[rt] = len;
-    if constexpr (MODE == kWindowMasked) {
-      if (real[rt]) {
-        const uint32_t i = rr / p.group;
+    if (tid < ROWS) {
+      const uint32_t rr = row0 + tid, i = rr / p.group;
+      uint32_t lo = 0, hi = len;
+      if (rr < nrows) {
         const size_t at = (size_t)b * p.T + i;
-        hi[rt] = base + i + 1;
-        if (p.lo) lo[rt] = (uint32_t)max(p.lo[at], 0);
-        if (p.hi) hi[rt] = min((uint32_t)max(p.hi[at], 0), len);
-        if (lo[rt] < hi[rt]) {
-          ulo = min(ulo, lo[rt]);
-          uhi = max(uhi, hi[rt]);
-        }
+        hi = base + i + 1;
+        if (p.lo) lo = (uint32_t)max(p.lo[at], 0);
+        if (p.hi) hi = min((uint32_t)max(p.hi[at], 0), len);
       }
+      s_row[tid] = Row{lo, hi, (int)(base + i), rr < nrows && p.slopes ? p.slopes[kvh * p.group + rr % p.group] * kLog2e : 0.f};
     }
-  }
-  if constexpr (MODE == kWindowMasked) {
+    __syncthreads();
+    const int last = (int)(live - row0);  // (the last rows of a block may be missing)
+    const Row mine = s_row[min(lane, last - 1)];
+    if (mine.lo < mine.hi) {
+      ulo = mine.lo;
+      uhi = mine.hi;
+    }
+    alo = mine.lo;
+    ahi = mine.lo < mine.hi ? mine.hi : 0;
 #pragma unroll
-    for (int x = 1; x < 16; x *= 2) {  // the four lane groups hold the same rows
+    for (int x = 1; x < 64; x *= 2) {
       ulo = min(ulo, (uint32_t)__shfl_xor((int)ulo, x, 64));
       uhi = max(uhi, (uint32_t)__shfl_xor((int)uhi, x, 64));
+      alo = max(alo, (uint32_t)__shfl_xor((int)alo, x, 64));
+      ahi = min(ahi, (uint32_t)__shfl_xor((int)ahi, x, 64));
     }
     ulo = __builtin_amdgcn_readfirstlane(ulo);
     uhi = __builtin_amdgcn_readfirstlane(uhi);
+    alo = __builtin_amdgcn_readfirstlane(alo);
+    ahi = __builtin_amdgcn_readfirstlane(ahi);
     if (ulo >= uhi) {  // no query of the block sees anything
       if (split == 0) zero_rows(row0, live);
       return;
     }
   }
 
-  // Tiles of 16 window rows, dealt to the splits and waves in turn; a split gets
+  // Tiles of TILE window rows, dealt to the splits and waves in turn; a split gets
   // at least a tile for each wave.
-  const uint32_t t0 = ulo / kTile, t1 = (uhi + kTile - 1) / kTile;
+  const uint32_t t0 = ulo / TILE, t1 = (uhi + TILE - 1) / TILE;
   const uint32_t nsplit = min(p.nsplit, (t1 - t0 + kWaves - 1) / kWaves);
   if (split >= nsplit) return;
 
@@ -212,210 +365,276 @@ __global__ __launch_bounds__(kWaves * 64) void window_kernel(const WindowParams 
     slot = slot >= p.M ? slot - p.M : slot;
     return r < uhi ? slot * (dh * ES) : kOutside;
   };
-  Piece<BF, CW> kk[NC];
-  Piece<BF, VW> vv[4][NV];
-  auto load_k = [&](uint32_t r0) {
+  typedef Piece<BF, CW> KRow[NC];  // a lane's part of 16 rows of K, and of V
+  typedef Piece<BF, VW> VRow[4][NV];
+  auto load_k = [&](uint32_t r0, KRow& k) {
     const uint32_t off = row_off(r0 + m16) + g * (CW * ES);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
-      kk[c].load(krs, !PAD || (uint32_t)(c * 4 + g) * CW < dh ? off + c * (4 * CW * ES) : kOutside);
+      k[c].load(krs, !PAD || (uint32_t)(c * 4 + g) * CW < dh ? off + c * (4 * CW * ES) : kOutside);
   };
-  auto load_v = [&](uint32_t r0) {
+  auto load_v = [&](uint32_t r0, VRow& v) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t off = row_off(r0 + 4 * g + i) + m16 * (VW * ES);
 #pragma unroll
       for (int c = 0; c < NV; ++c)
-        vv[i][c].load(vrs, !PAD || (uint32_t)(c * 16 + m16) * VW < dh ? off + c * (16 * VW * ES) : kOutside);
+        v[i][c].load(vrs, !PAD || (uint32_t)(c * 16 + m16) * VW < dh ? off + c * (16 * VW * ES) : kOutside);
     }
   };
+  KRow kk[KT];
+  VRow vv[KT];
   const uint32_t tstep = nsplit * kWaves;
   uint32_t t = t0 + split + nsplit * wave;
-  load_k(t * kTile);
-  load_v(t * kTile);
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) load_k(t * TILE + kt * 16, kk[kt]);
+  if constexpr (!PARTS) load_v(t * TILE, vv[0]);
 
-  // The draft's relation "is above or is", a bit per node, and the nodes'
-  // depths: each node takes over what its jump target knows and jumps twice as
-  // far, log2 of the nodes' number times.
+  // The draft's relation "is above or is", a bit per node, and the nodes' depths:
+  // each node takes over what its jump target knows and jumps as far as that one
+  // does, until none has anywhere left to go.  Up to 64 nodes every wave does it for
+  // itself, in registers; larger drafts go through LDS.
   if constexpr (MODE == kWindowTree) {
-    const uint32_t words = (n + 31) / 32;
-    if (tid < (int)n) {
-      int up = p.parents[(size_t)b * p.T + tid];
-      up = up < 0 || up >= tid ? -1 : up;
+    up = me < (int)n && up >= 0 && up < me ? up : -1;
+    if (narrow) {
+      uint32_t a0 = lane < 32 ? 1u << lane : 0u, a1 = lane < 32 ? 0u : 1u << (lane - 32);
+      int depth = up >= 0;
+      while (__any(up >= 0)) {
+        const int from = up >= 0 ? up : lane;
+        const uint32_t b0 = __shfl((int)a0, from, 64), b1 = __shfl((int)a1, from, 64);
+        const int deeper = __shfl(depth, from, 64), next = __shfl(up, from, 64);
+        if (up >= 0) {
+          a0 |= b0;
+          a1 |= b1;
+          depth += deeper;
+          up = next;
+        }
+      }
+      s_anc[lane][0] = a0;  // (the waves write the same)
+      s_anc[lane][1] = a1;
+      s_depth[lane] = depth;
+    } else {
+      const uint32_t words = (n + 31) / 32;
 #pragma unroll
       for (int w = 0; w < (int)kMaxTreeNodes / 32; ++w) s_anc[tid][w] = 0;
       s_anc[tid][tid >> 5] = 1u << (tid & 31);
-      s_jump[tid] = up;
       s_depth[tid] = up >= 0;
-    }
-    __syncthreads();
-    for (uint32_t reach = 1; reach < n; reach *= 2) {
-      const int to = tid < (int)n ? s_jump[tid] : -1;
-      uint32_t above[kMaxTreeNodes / 32];
-      int next = -1, deeper = 0;
-      if (to >= 0) {
-        for (uint32_t w = 0; w < kMaxTreeNodes / 32; ++w) above[w] = w < words ? s_anc[to][w] : 0;
-        next = s_jump[to];
-        deeper = s_depth[to];
-      }
-      __syncthreads();
-      if (to >= 0) {
-        for (uint32_t w = 0; w < kMaxTreeNodes / 32; ++w)
-          if (w < words) s_anc[tid][w] |= above[w];
-        s_jump[tid] = next;
-        s_depth[tid] += deeper;
+      s_jump[tid] = up;
+      for (uint32_t reach = 1; reach < n; reach *= 2) {
+        __syncthreads();
+        uint32_t above[kMaxTreeNodes / 32];
+        int next = -1, deeper = 0;
+        if (up >= 0) {
+#pragma unroll
+          for (int w = 0; w < (int)kMaxTreeNodes / 32; ++w) above[w] = w < (int)words ? s_anc[up][w] : 0;
+          next = s_jump[up];
+          deeper = s_depth[up];
+        }
+        __syncthreads();
+        if (up >= 0) {
+#pragma unroll
+          for (int w = 0; w < (int)kMaxTreeNodes / 32; ++w)
+            if (w < (int)words) s_anc[tid][w] |= above[w];
+          s_depth[tid] += deeper;
+          s_jump[tid] = up = next;
+        }
       }
       __syncthreads();
     }
   }
 
-  // The query rows: rotated, scaled, in the matrix operand's layout.
-  float qf[R][NC][CW];
-  uint32_t node[R];
-#pragma unroll
-  for (int rt = 0; rt < R; ++rt) {
-    const uint32_t rr = row0 + rt * 16 + m16;
-    node[rt] = real[rt] ? rr / p.group : 0;
-    const float* src = p.q + (((size_t)b * p.T + node[rt]) * p.H + kvh * p.group + rr % p.group) * dh;
+  // The query rows, rotated.
+  auto turn_q = [&](float (&x)[NC][CW]) {
     uint32_t pos = p.rope_pos;
-    if constexpr (MODE == kWindowTree) pos += s_depth[node[rt]];
+    if constexpr (MODE == kWindowTree) pos += s_depth[qrow < nrows ? qrow / p.group : 0];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < CW; e += 4) {
         const uint32_t d = (c * 4 + g) * CW + e;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (real[rt] && (!PAD || d < dh)) {
-          x = *reinterpret_cast<const float4*>(src + d);
-          if (p.rope_cos) {
-            const size_t ro = (size_t)pos * (dh / 2) + d / 2;
-            x = rope4(x, *reinterpret_cast<const float2*>(p.rope_cos + ro),
-                      *reinterpret_cast<const float2*>(p.rope_sin + ro));
-          }
+        float4 y = qraw[(c * CW + e) / 4];
+        if (p.rope_cos && (!PAD || d < dh)) {
+          const size_t ro = (size_t)pos * (dh / 2) + d / 2;
+          y = rope4(y, *reinterpret_cast<const float2*>(p.rope_cos + ro),
+                    *reinterpret_cast<const float2*>(p.rope_sin + ro));
         }
-        qf[rt][c][e] = x.x * p.qscale;
-        qf[rt][c][e + 1] = x.y * p.qscale;
-        qf[rt][c][e + 2] = x.z * p.qscale;
-        qf[rt][c][e + 3] = x.w * p.qscale;
+        const bool on = qrow < nrows;
+        x[c][e] = on ? y.x : 0.f;
+        x[c][e + 1] = on ? y.y : 0.f;
+        x[c][e + 2] = on ? y.z : 0.f;
+        x[c][e + 3] = on ? y.w : 0.f;
       }
-  }
-  float slope[R];
-  if constexpr (MODE == kWindowMasked) {
+  };
+  float qf[PARTS ? 1 : NC][CW];  // one row tile: in registers, scaled
+  if constexpr (PARTS) {
+    // In LDS as operand parts; f16 ones of each row scaled to its largest value.
+    if (wave < R) {
+      float x[NC][CW];
+      turn_q(x);
+      float sc = 1.f;
+      if constexpr (!BF) {
+        float top = 0.f;
 #pragma unroll
-    for (int rt = 0; rt < R; ++rt)
-      slope[rt] = p.slopes && real[rt]
-                      ? p.slopes[kvh * p.group + (row0 + rt * 16 + m16) % p.group] * kLog2e
-                      : 0.f;
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < CW; ++e) top = fmaxf(top, fabsf(x[c][e]));
+        top = max_xor32(max_xor16(top));
+        sc = top > 0.f && top < INFINITY ? scale_to_64(top) : 1.f;
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < CW; ++e) x[c][e] *= BF ? p.qscale : sc;
+#pragma unroll
+      for (int c = 0; c < NP; ++c) {
+        Frag y[P::N];
+        P::split(&x[0][0] + 8 * c, y);
+#pragma unroll
+        for (int n = 0; n < P::N; ++n) s_q[wave][c][n][lane] = y[n];
+      }
+      if (g == 0) s_qs[wave * 16 + m16] = BF ? 1.f : p.qscale / sc;
+    }
+    __syncthreads();
+  } else {
+    turn_q(qf);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < CW; ++e) qf[c][e] *= p.qscale;
   }
 
+  // The weights are taken relative to m, which follows the scores' maximum only
+  // when they pass it by 2^kSlack, and then to 2^kHead below it: the outputs are
+  // seldom rescaled, and the weights use the range of f16.
+  constexpr float kSlack = 15.f, kHead = 7.f;
+  TileScale ks, vs;
   float m[R], l[R];
-  f32x4 o[R][NV * VW];
+  f32x4 o[R][NX];
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     m[rt] = -FLT_MAX;
     l[rt] = 0.f;
 #pragma unroll
-    for (int x = 0; x < NV * VW; ++x) o[rt][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int x = 0; x < NX; ++x) o[rt][x] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  // Whether some query does not see all of n rows from r0, or the window ends there.
+  auto partly_seen = [&](uint32_t r0, uint32_t n) { return r0 < alo || r0 + n > ahi; };
 
-  for (; t < t1; t += tstep) {
-    const uint32_t r0 = t * kTile;
-    f32x4 s[R];
-#pragma unroll
-    for (int rt = 0; rt < R; ++rt) s[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < CW; ++e)
+  // What follows the scores of rows r0 .. (16 for each of s's tiles): cap, bias,
+  // mask, and the weights they turn into, relative to m.
+  auto weigh = [&](uint32_t r0, auto& s, bool partly) __attribute__((always_inline)) {
+    constexpr int K = sizeof(s[0]) / sizeof(f32x4);
+    if constexpr (MODE == kWindowMasked) {
+      if (p.cap_log2 > 0.f) {
 #pragma unroll
         for (int rt = 0; rt < R; ++rt)
-          s[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[c][e], qf[rt][c][e], s[rt], 0, 0, 0);
-    load_k((t + tstep) * kTile);
-
-    // A tile that some query does not see, or that the window's end cuts.
-    bool partly = false;
-    if constexpr (MODE == kWindowMasked) {
+#pragma unroll
+          for (int kt = 0; kt < K; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[rt][kt][i] = p.cap_log2 * tanh_rel(s[rt][kt][i]);
+      }
+      if (p.slopes) {
+#pragma unroll
+        for (int rt = 0; rt < R; ++rt) {
+          const int away = s_row[rt * 16 + m16].at - (int)(r0 + 4 * g);
+          const float slope = s_row[rt * 16 + m16].slope;
+#pragma unroll
+          for (int kt = 0; kt < K; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[rt][kt][i] -= slope * fabsf((float)(away - kt * 16 - i));
+        }
+      }
+    }
+    if constexpr (MODE == kWindowWeights) {
 #pragma unroll
       for (int rt = 0; rt < R; ++rt)
-        partly |= real[rt] && (lo[rt] > r0 || hi[rt] < r0 + kTile);
-      partly = __any(partly);
-    } else {
-      partly = r0 + kTile > (MODE == kWindowTree ? base : len);
+        if (row0 + rt * 16 + m16 < nrows) {
+          float* to = p.scores + ((size_t)b * p.H + kvh * p.group + row0 + rt * 16 + m16) * p.score_stride + r0 + 4 * g;
+          // The stride covers whole tiles of 16 rows.
+#pragma unroll
+          for (int kt = 0; kt < K; ++kt)
+            if (kt == 0 || r0 + kt * 16 < len) *reinterpret_cast<f32x4*>(to + kt * 16) = s[rt][kt];
+        }
     }
+    if (partly) {
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) {
+        const uint32_t rr = row0 + rt * 16 + m16;
+        uint32_t lo = 0, hi = len, node = 0;
+        if constexpr (MODE == kWindowMasked) {
+          lo = s_row[rt * 16 + m16].lo;
+          hi = s_row[rt * 16 + m16].hi;
+        }
+        if constexpr (MODE == kWindowTree) node = rr < nrows ? rr / p.group : 0;
+#pragma unroll
+        for (int kt = 0; kt < K; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t r = r0 + kt * 16 + 4 * g + i;
+            bool seen = r >= lo && r < hi;
+            if constexpr (MODE == kWindowTree) {
+              if (seen && r >= base && rr < nrows) {
+                const uint32_t j = r - base;
+                seen = (s_anc[node][j >> 5] >> (j & 31)) & 1u;
+              }
+            }
+            s[rt][kt][i] = seen ? s[rt][kt][i] : -INFINITY;
+          }
+      }
+    }
+    float top[R];
+    bool passed = false;
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) {
-      if constexpr (MODE == kWindowMasked) {
-        if (p.cap_log2 > 0.f) {
+      float x = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[rt][i] = p.cap_log2 * tanh_rel(s[rt][i]);
-        }
-        if (p.slopes) {
-          const int away = (int)(base + node[rt]) - (int)(r0 + 4 * g);
+      for (int kt = 0; kt < K; ++kt)
+        x = fmaxf(x, fmaxf(fmaxf(s[rt][kt][0], s[rt][kt][1]), fmaxf(s[rt][kt][2], s[rt][kt][3])));
+      top[rt] = max_xor32(max_xor16(x));
+      passed |= top[rt] > m[rt] + kSlack;
+    }
+    if (__any(passed)) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[rt][i] -= slope[rt] * fabsf((float)(away - i));
-        }
-      }
-      if constexpr (MODE == kWindowWeights) {
-        if (real[rt]) {
-          float* to = p.scores + ((size_t)b * p.H + kvh * p.group + row0 + rt * 16 + m16) * p.score_stride + r0 + 4 * g;
-          *reinterpret_cast<f32x4*>(to) = s[rt];  // the stride covers whole tiles
-        }
-      }
-      if (partly) {
+      for (int rt = 0; rt < R; ++rt) {
+        const float now = fmaxf(m[rt], top[rt] - kHead), alpha = exp2_hw(m[rt] - now);
+        m[rt] = now;
+        l[rt] *= alpha;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t r = r0 + 4 * g + i;
-          bool seen = r >= lo[rt] && r < hi[rt];
-          if constexpr (MODE == kWindowTree) {
-            if (seen && r >= base && real[rt]) {
-              const uint32_t j = r - base;
-              seen = (s_anc[node[rt]][j >> 5] >> (j & 31)) & 1u;
-            }
-          }
-          s[rt][i] = seen ? s[rt][i] : -INFINITY;
-        }
-      }
-      float top = fmaxf(fmaxf(s[rt][0], s[rt][1]), fmaxf(s[rt][2], s[rt][3]));
-      top = fmaxf(m[rt], max_xor32(max_xor16(top)));
-      const float alpha = exp2_hw(m[rt] - top);
-      m[rt] = top;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[rt][i] = exp2_hw(s[rt][i] - top);
-      l[rt] = l[rt] * alpha + ((s[rt][0] + s[rt][1]) + (s[rt][2] + s[rt][3]));
-      if (__any(alpha != 1.f)) {
-#pragma unroll
-        for (int x = 0; x < NV * VW; ++x) o[rt][x] *= alpha;
+        for (int x = 0; x < NX; ++x) o[rt][x] *= alpha;
       }
     }
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+      for (int kt = 0; kt < K; ++kt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[rt][kt][i] = exp2_hw(s[rt][kt][i] - m[rt]);
+        l[rt] += (s[rt][kt][0] + s[rt][kt][1]) + (s[rt][kt][2] + s[rt][kt][3]);
+      }
+  };
 
-    float vf[4][NV * VW];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int c = 0; c < NV; ++c)
-#pragma unroll
-        for (int e = 0; e < VW; ++e) vf[i][c * VW + e] = vv[i][c][e];
-    // A value that is not finite, in a row that some query does not see: the
-    // product would carry it to that query as 0 * inf.  It is taken out of the
-    // operand and added by hand to the queries that see its row.
+  // The products of 16 rows of V in f32, with the weights w(rt) of the lane's four
+  // rows.  A value that is not finite, in a row that some query does not see, would
+  // be carried to that query as 0 * inf: it is taken out of the operand and added by
+  // hand to the queries that see its row.
+  auto add_values = [&](uint32_t r0, const VRow& v, auto w, float oscale, bool partly)
+      __attribute__((always_inline)) {
     if (partly) {
       bool bad = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int x = 0; x < NV * VW; ++x) {
-          bad |= not_finite(vf[i][x]);
-          vf[i][x] = not_finite(vf[i][x]) ? 0.f : vf[i][x];
-        }
+        for (int x = 0; x < NX; ++x) bad |= not_finite(v[i][x / VW][x % VW] * oscale);
       if (__any(bad)) {
-        for (int key = 0; key < kTile; ++key) {
+        for (int key = 0; key < 16; ++key) {
           const uint32_t off = row_off(r0 + key);
           const int from = (key >> 2) * 16 + m16;
-          float w[R];
+          float u[R];
 #pragma unroll
           for (int rt = 0; rt < R; ++rt) {
-            const float a = (key & 1) ? s[rt][1] : s[rt][0], z = (key & 1) ? s[rt][3] : s[rt][2];
-            w[rt] = __shfl((key & 2) ? z : a, from, 64);
+            const f32x4 y = w(rt);
+            const float a = (key & 1) ? y[1] : y[0], z = (key & 1) ? y[3] : y[2];
+            u[rt] = __shfl((key & 2) ? z : a, from, 64);
           }
 #pragma unroll
           for (int c = 0; c < NV; ++c)
@@ -425,10 +644,13 @@ __global__ __launch_bounds__(kWaves * 64) void window_kernel(const WindowParams 
               Piece<BF, VW> x;
               x.load(vrs, !PAD || d < dh ? off + d * ES : kOutside);
 #pragma unroll
-              for (int e = 0; e < VW; ++e)
+              for (int e = 0; e < VW; ++e) {
+                const float y = x[e] * oscale;
 #pragma unroll
                 for (int rt = 0; rt < R; ++rt)
-                  if (not_finite(x[e]) && !(w[rt] == 0.f)) o[rt][c * VW + e][i] += w[rt] * x[e];
+                  if (not_finite(y) && !(u[rt] == 0.f)) o[rt][c * VW + e][i] += u[rt] * y;
+              }
+              __builtin_amdgcn_sched_barrier(0);
             }
         }
       }
@@ -436,14 +658,230 @@ __global__ __launch_bounds__(kWaves * 64) void window_kernel(const WindowParams 
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int x = 0; x < NV * VW; ++x)
+      for (int x = 0; x < NX; ++x) {
+        float y = v[i][x / VW][x % VW] * oscale;
+        y = partly && not_finite(y) ? 0.f : y;
 #pragma unroll
         for (int rt = 0; rt < R; ++rt)
-          o[rt][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[i][x], s[rt][i], o[rt][x], 0, 0, 0);
-    load_v((t + tstep) * kTile);
+          o[rt][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(y, w(rt)[i], o[rt][x], 0, 0, 0);
+      }
+  };
+
+  // Products of parts, as long as the tiles are held well by them: f32 rows within
+  // f16's range, and for either type no value that is not finite in a row that some
+  // query does not see.  From the first tile that is not, the wave goes on in f32.
+  // V is requested while K is consumed and the next tile's K while V is: a tile and
+  // a half in registers in all, so that two waves fit a SIMD, which measured faster
+  // than one wave with 64 query rows and both tiles ahead.
+  if constexpr (PARTS) {
+    bool weighed = false;
+    f32x4 s[R][KT];
+    for (; t < t1; t += tstep) {
+      const uint32_t r0 = t * TILE;
+      const bool partly = partly_seen(r0, TILE);
+      if constexpr (!BF) {
+        float top = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < CW; ++e) top = __builtin_elementwise_maximum(top, fabsf(kk[kt][c][e]));
+        if (!ks.holds(top)) break;
+        if (ks.scale != 1.f) {
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) kk[kt][c].times(ks.scale);
+        }
+      }
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      // The queries' parts are read anew for every tile: kept in registers (the
+      // compiler lifts the loads out of the loop) they would push others out.
+      int at = lane;
+      asm volatile("" : "+v"(at));
+#pragma unroll
+      for (int c = 0; c < NP; ++c) {
+        Frag kf[KT][P::N];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          if constexpr (BF) {
+            kf[kt][0] = __builtin_bit_cast(Frag, kk[kt][c]);
+          } else {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = kk[kt][(c * 8 + e) / CW][(c * 8 + e) % CW];
+            P::split(x, kf[kt]);
+          }
+        }
+#pragma unroll
+        for (int rt = 0; rt < R; ++rt) {
+          Frag qq[P::N];
+#pragma unroll
+          for (int n = 0; n < P::N; ++n) qq[n] = s_q[rt][c][n][at];
+          // The smaller products first.
+          if constexpr (!BF) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) s[rt][kt] = P::mfma(kf[kt][1], qq[0], s[rt][kt]);
+          }
+#pragma unroll
+          for (int n = P::N - 1; n >= 0; --n)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) s[rt][kt] = P::mfma(kf[kt][0], qq[n], s[rt][kt]);
+        }
+        if (c == NP / 2 - 1) load_v(r0, vv[0]);
+      }
+      load_v(r0 + 16, vv[1]);
+      if constexpr (!BF) {
+#pragma unroll
+        for (int rt = 0; rt < R; ++rt) {
+          const float f = s_qs[rt * 16 + m16] * ks.inverse;
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) s[rt][kt] *= f;
+        }
+      }
+      weigh(r0, s, partly);
+      if constexpr (!BF) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4 * KT; ++i)
+#pragma unroll
+          for (int c = 0; c < NV; ++c)
+#pragma unroll
+            for (int e = 0; e < VW; ++e) top = __builtin_elementwise_maximum(top, fabsf(vv[i / 4][i % 4][c][e]));
+        weighed = !vs.holds(top);
+      } else if (partly) {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 4 * KT; ++i)
+#pragma unroll
+          for (int x = 0; x < NX; ++x) bad |= not_finite(vv[i / 4][i % 4][x / VW][x % VW]);
+        weighed = __any(bad);
+      }
+      if (weighed) break;
+      if constexpr (!BF) {
+        if (vs.scale != 1.f) {
+#pragma unroll
+          for (int i = 0; i < 4 * KT; ++i)
+#pragma unroll
+            for (int c = 0; c < NV; ++c) vv[i / 4][i % 4][c].times(vs.scale);
+        }
+      }
+      Frag pp[R][P::N];
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = s[rt][e >> 2][e & 3];
+        P::split(x, pp[rt]);
+      }
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        Frag vf[P::N];
+        if constexpr (BF) {
+          // The halves of the rows' words, paired along the rows.
+          u32x4 y;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            y[k] = __builtin_amdgcn_perm(vv[k / 2][k % 2 * 2 + 1][x / VW].w[x % VW / 2],
+                                         vv[k / 2][k % 2 * 2][x / VW].w[x % VW / 2], x & 1 ? 0x07060302 : 0x05040100);
+          vf[0] = __builtin_bit_cast(Frag, y);
+        } else {
+          float y[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] = vv[k / 4][k % 4][x / VW][x % VW];
+          P::split(y, vf);
+#pragma unroll
+          for (int rt = 0; rt < R; ++rt) o[rt][x] = P::mfma(vf[1], pp[rt][0], o[rt][x]);
+        }
+#pragma unroll
+        for (int n = P::N - 1; n >= 0; --n)
+#pragma unroll
+          for (int rt = 0; rt < R; ++rt) o[rt][x] = P::mfma(vf[0], pp[rt][n], o[rt][x]);
+        if (x == NX / 2 - 1) load_k((t + tstep) * TILE, kk[0]);
+      }
+      load_k((t + tstep) * TILE + 16, kk[1]);
+    }
+    if (weighed) {
+      const float oscale = vs.scale;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        const uint32_t r0 = t * TILE + kt * 16;
+        load_v(r0, vv[0]);
+        add_values(r0, vv[0], [&](int rt) { return s[rt][kt]; }, oscale, partly_seen(r0, 16));
+      }
+      t += tstep;
+    }
   }
 
-  // The waves' states merged through LDS, a row tile at a time.
+  // In f32, 16 rows at a time: one row tile from the start, more from the tile on
+  // that the parts did not hold (which is read again).
+  const float oscale = PARTS ? vs.scale : 1.f;  // carried by the outputs
+  for (uint32_t half = 0; t < t1;) {
+    const uint32_t r0 = t * TILE + half * 16;
+    const bool partly = partly_seen(r0, 16);
+    if constexpr (PARTS) {
+      load_k(r0, kk[0]);
+      load_v(r0, vv[0]);
+    }
+    f32x4 s[R][1];
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt) s[rt][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int at = lane;
+    asm volatile("" : "+v"(at));
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+      for (int c = 0; c < NP; ++c) {
+        float x[8];
+        if constexpr (PARTS) {
+          Frag qq[P::N];
+#pragma unroll
+          for (int n = 0; n < P::N; ++n) qq[n] = s_q[rt][c][n][at];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = (float)qq[0][e] + (float)qq[1][e];
+            if constexpr (BF) x[e] += (float)qq[P::N - 1][e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = qf[(c * 8 + e) / CW][(c * 8 + e) % CW];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          s[rt][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[0][(c * 8 + e) / CW][(c * 8 + e) % CW], x[e], s[rt][0],
+                                                          0, 0, 0);
+        if constexpr (PARTS) __builtin_amdgcn_sched_barrier(0);
+      }
+    if constexpr (PARTS) {
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) s[rt][0] *= s_qs[rt * 16 + m16];
+    } else {
+      load_k((t + tstep) * TILE, kk[0]);
+    }
+    weigh(r0, s, partly);
+    add_values(r0, vv[0], [&](int rt) { return s[rt][0]; }, oscale, partly);
+    if constexpr (PARTS) {
+      half ^= 1;
+      if (half == 0) t += tstep;
+    } else {
+      t += tstep;
+      load_v(t * TILE, vv[0]);
+    }
+  }
+  if constexpr (PARTS) {
+    const float f = vs.inverse;
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+      for (int x = 0; x < NX; ++x) o[rt][x] *= f;
+    __syncthreads();  // every wave is done with the queries' parts
+  }
+
+  // The waves' states merged through LDS.
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     l[rt] = sum_xor32(sum_xor16(l[rt]));
@@ -451,7 +889,16 @@ __global__ __launch_bounds__(kWaves * 64) void window_kernel(const WindowParams 
       s_ml[wave][rt * 16 + m16][0] = m[rt];
       s_ml[wave][rt * 16 + m16][1] = l[rt];
     }
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < VW; e += 4)
+          *reinterpret_cast<f32x4*>(&s_o[wave][rt * 16 + m16][(c * 16 + 4 * g + i) * VW + e]) =
+              f32x4{o[rt][c * VW + e][i], o[rt][c * VW + e + 1][i], o[rt][c * VW + e + 2][i], o[rt][c * VW + e + 3][i]};
   }
+  __syncthreads();
   constexpr uint32_t REC = ROWS * (D + 2);  // floats of a split's record: O, then (m, l)
   const size_t unit = ((size_t)b * p.KH + kvh) * p.rblocks + rb;
   const __amdgpu_buffer_rsrc_t prs =
@@ -468,43 +915,32 @@ __global__ __launch_bounds__(kWaves * 64) void window_kernel(const WindowParams 
       st[1] = lt;
     }
   };
+  constexpr int NXT = ROWS * C4 / (kWaves * 64);  // float4 columns of a thread
 #pragma unroll
-  for (int rt = 0; rt < R; ++rt) {
-    if (rt > 0) __syncthreads();
+  for (int k = 0; k < NXT; ++k) {
+    const int x = tid + k * kWaves * 64, row = x / C4, col = x % C4;
+    float mt = s_ml[0][row][0];
 #pragma unroll
-    for (int c = 0; c < NV; ++c)
+    for (int w = 1; w < kWaves; ++w) mt = fmaxf(mt, s_ml[w][row][0]);
+    float lt = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < VW; ++e) s_o[wave][m16][(c * 16 + 4 * g + i) * VW + e] = o[rt][c * VW + e][i];
-    __syncthreads();
-    for (int x = tid; x < 16 * C4; x += kWaves * 64) {
-      const int row = x / C4, col = x % C4;
-      float mt = s_ml[0][rt * 16 + row][0];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) mt = fmaxf(mt, s_ml[w][rt * 16 + row][0]);
-      float lt = 0.f;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = exp2_hw(s_ml[w][rt * 16 + row][0] - mt);
-        lt += f * s_ml[w][rt * 16 + row][1];
-        const float4 y = *reinterpret_cast<const float4*>(&s_o[w][row][col * 4]);
-        a.x += f * y.x;
-        a.y += f * y.y;
-        a.z += f * y.z;
-        a.w += f * y.w;
-      }
-      if (nsplit == 1) {
-        finish(rt * 16 + row, col, a, mt, lt);
-      } else {
-        const uint32_t rec = split * REC * 4;
-        st_coherent4(prs, rec + ((rt * 16 + row) * D + col * 4) * 4, coh_f4{a.x, a.y, a.z, a.w});
-        if (col == 0) {
-          st_coherent(prs, rec + (ROWS * D + (rt * 16 + row) * 2) * 4, mt);
-          st_coherent(prs, rec + (ROWS * D + (rt * 16 + row) * 2 + 1) * 4, lt);
-        }
-      }
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = exp2_hw(s_ml[w][row][0] - mt);
+      lt += f * s_ml[w][row][1];
+      const float4 y = *reinterpret_cast<const float4*>(&s_o[w][row][col * 4]);
+      a.x += f * y.x;
+      a.y += f * y.y;
+      a.z += f * y.z;
+      a.w += f * y.w;
+    }
+    if (nsplit == 1) {
+      finish(row, col, a, mt, lt);
+    } else {
+      const uint32_t rec = split * REC * 4;
+      st_coherent4(prs, rec + x * 16, coh_f4{a.x, a.y, a.z, a.w});
+      if (col == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(mt), __float_as_uint(lt)}, prs,
+                                                          rec + (ROWS * D + row * 2) * 4, 0, kSc1);
     }
   }
   if (nsplit == 1) return;
@@ -522,48 +958,68 @@ __global__ __launch_bounds__(kWaves * 64) void window_kernel(const WindowParams 
   __syncthreads();
   if (!s_last) return;
   __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
-  // Each split's factor 2^(m_s - m) and the rows' (m, l), in the LDS of the
-  // partial outputs, which every thread is done with.
-  float* s_f = &s_o[0][0][0];  // [split][ROWS]
-  static_assert(kMaxSplits * ROWS <= kWaves * 16 * LDO, "the factors fit");
-  if (tid < ROWS) {
-    float mt = -FLT_MAX;
-    for (uint32_t sp = 0; sp < nsplit; ++sp) {
-      const float x = ld_coherent(prs, (sp * REC + ROWS * D + tid * 2) * 4);
-      s_f[sp * ROWS + tid] = x;
-      mt = fmaxf(mt, x);
+  // The splits' (m, l) of every row, all requested at once, in the LDS of the
+  // partial outputs, which every thread is done with; m then gives way to the
+  // split's factor 2^(m_s - m).
+  constexpr int MS = max_splits(R);
+  auto& s_f = *reinterpret_cast<float(*)[MS][ROWS]>(s_mem);
+  auto& s_l = *reinterpret_cast<float(*)[MS][ROWS]>(s_mem + MS * ROWS * 4);
+  static_assert(2 * MS * ROWS * 4 <= kOutBytes, "the splits' numbers fit");
+  constexpr int NML = MS * ROWS / (kWaves * 64);
+  u32x2 ml[NML];
+#pragma unroll
+  for (int k = 0; k < NML; ++k) {
+    const uint32_t x = tid + k * kWaves * 64;
+    if (x < nsplit * ROWS)
+      ml[k] = __builtin_amdgcn_raw_buffer_load_b64(prs, (x / ROWS * REC + ROWS * D + x % ROWS * 2) * 4, 0, kSc1);
+  }
+#pragma unroll
+  for (int k = 0; k < NML; ++k) {
+    const uint32_t x = tid + k * kWaves * 64;
+    if (x < nsplit * ROWS) {
+      s_f[x / ROWS][x % ROWS] = __uint_as_float(ml[k][0]);
+      s_l[x / ROWS][x % ROWS] = __uint_as_float(ml[k][1]);
     }
-    float lt = 0.f;
+  }
+  __syncthreads();
+  if (tid < ROWS) {
+    float mt = -FLT_MAX, lt = 0.f;
+    for (uint32_t sp = 0; sp < nsplit; ++sp) mt = fmaxf(mt, s_f[sp][tid]);
     for (uint32_t sp = 0; sp < nsplit; ++sp) {
-      const float f = exp2_hw(s_f[sp * ROWS + tid] - mt);
-      s_f[sp * ROWS + tid] = f;
-      lt += f * ld_coherent(prs, (sp * REC + ROWS * D + tid * 2 + 1) * 4);
+      const float f = exp2_hw(s_f[sp][tid] - mt);
+      s_f[sp][tid] = f;
+      lt += f * s_l[sp][tid];
     }
     s_ml[0][tid][0] = mt;
     s_ml[0][tid][1] = lt;
   }
   __syncthreads();
-  for (int x = tid; x < ROWS * C4; x += kWaves * 64) {
-    const int row = x / C4, col = x % C4;
-    if (row0 + row >= nrows) break;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t sp = 0; sp < nsplit; sp += 4) {
-      coh_f4 y[4];
+  // Each thread's columns of four splits at a time, requested together.
+  float4 a[NXT];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        y[k] = coh_f4{0.f, 0.f, 0.f, 0.f};
-        if (sp + k < nsplit) y[k] = ld_coherent4(prs, ((sp + k) * REC + row * D + col * 4) * 4);
-      }
+  for (int k = 0; k < NXT; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (uint32_t sp = 0; sp < nsplit; sp += 4) {
+    coh_f4 y[4][NXT];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float f = sp + k < nsplit ? s_f[(sp + k) * ROWS + row] : 0.f;
-        a.x += f * y[k].x;
-        a.y += f * y[k].y;
-        a.z += f * y[k].z;
-        a.w += f * y[k].w;
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int k = 0; k < NXT; ++k)  // (past the record: zeros)
+        y[u][k] = ld_coherent4(prs, sp + u < nsplit ? (sp + u) * REC * 4 + (tid + k * kWaves * 64) * 16 : kOutside);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int k = 0; k < NXT; ++k) {
+        const float f = sp + u < nsplit ? s_f[sp + u][(tid + k * kWaves * 64) / C4] : 0.f;
+        a[k].x += f * y[u][k].x;
+        a[k].y += f * y[u][k].y;
+        a[k].z += f * y[u][k].z;
+        a[k].w += f * y[u][k].w;
       }
-    }
-    finish(row, col, a, s_ml[0][row][0], s_ml[0][row][1]);
+  }
+#pragma unroll
+  for (int k = 0; k < NXT; ++k) {
+    const int row = (tid + k * kWaves * 64) / C4;
+    finish(row, (tid + k * kWaves * 64) % C4, a[k], s_ml[0][row][0], s_ml[0][row][1]);
   }
 }
 
@@ -585,10 +1041,8 @@ template <WindowMode MODE>
 int launch_mode(const WindowParams& p, int row_tiles, bool bf16, dim3 grid, hipStream_t stream) {
   if (row_tiles == 1)
     bf16 ? launch_rows<MODE, 1, true>(p, grid, stream) : launch_rows<MODE, 1, false>(p, grid, stream);
-  else if (row_tiles == 2)
-    bf16 ? launch_rows<MODE, 2, true>(p, grid, stream) : launch_rows<MODE, 2, false>(p, grid, stream);
   else
-    bf16 ? launch_rows<MODE, 4, true>(p, grid, stream) : launch_rows<MODE, 4, false>(p, grid, stream);
+    bf16 ? launch_rows<MODE, 2, true>(p, grid, stream) : launch_rows<MODE, 2, false>(p, grid, stream);
   STS_HIP(hipGetLastError());
   return STS_OK;
 }

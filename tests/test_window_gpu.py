@@ -22,6 +22,13 @@ def close(got, want, bound, what):
     assert worst <= 0, f"{what}: off by {err.max():.3e}, bound {bound.max():.3e}"
 
 
+def same(got, clean, bound, what):
+    """Two evaluations of one value, each within its bound of it (the values that a
+    query does not see may decide how its tile is multiplied, not what comes out)."""
+    assert np.isfinite(got).all(), what
+    assert (np.abs(got - clean) <= 2 * bound[..., None]).all(), what
+
+
 def i32(x):
     return torch.as_tensor(np.asarray(x, np.int32)).cuda()
 
@@ -115,14 +122,39 @@ def test_tree_hidden_values(gpu, poison, D, dtype):
     parents = random_tree(w.rng, T, T)
     parents[4] = -1
     clean = run_tree(w, q, parents[None], None, scale_for(D))
+    bound = attend64(q[0], w.rows(0, w.k), w.rows(0, w.v), tree_seen(parents, T, L), scale_for(D))[2]
     slot = int(w.slots(0)[L - T + 4])
     w.k[0, :, slot] = poison
     w.v[0, :, slot, ::3] = poison
     got = run_tree(w, q, parents[None], None, scale_for(D))
     below = ancestors(parents, T)[:, 4]
     assert 1 <= below.sum() < T
-    np.testing.assert_array_equal(got[0, ~below], clean[0, ~below])
+    same(got[0, ~below], clean[0, ~below], bound[~below], "nodes that do not see it")
     assert (got[0, below] != clean[0, below]).any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["tiny", "huge", "steps", "zeros first", "one row", "zeros"])
+@pytest.mark.parametrize("T", [8, 30, 64])
+def test_tree_magnitudes(gpu, T, kind, dtype):
+    """Rows of any size: all tiny or huge, from step to step, zeros before others,
+    one row far above the rest."""
+    L, D = 500, 128
+    w = Window(7, 1, 1, 600, D, [L], dtype)
+    size = {"tiny": np.full(L, 1e-20), "huge": np.full(L, 1e20), "steps": 10.0 ** (np.arange(L) // 40 - 6),
+            "zeros first": np.where(np.arange(L) < 300, 0, 1e-3), "one row": np.where(np.arange(L) == 137, 1e6, 1.0),
+            "zeros": np.zeros(L)}[kind]
+    f = torch.from_numpy(size).to(F32)[None, :, None]
+    slots = torch.from_numpy(w.slots(0))
+    w.v[0][:, slots] = (w.v[0][:, slots].float() * f).to(dtype)
+    for which in ("values", "rows"):
+        if which == "rows":  # keys too, with queries that keep the scores moderate
+            w.k[0][:, slots] = (w.k[0][:, slots].float() * f).to(dtype)
+        q = queries(w.rng, 1, T, 2, D) / (np.float32(size.max() or 1) if which == "rows" else np.float32(1))
+        parents = random_tree(w.rng, T, T)
+        got = run_tree(w, q, parents[None], None, scale_for(D))
+        want, _, bound = attend64(q[0], w.rows(0, w.k), w.rows(0, w.v), tree_seen(parents, T, L), scale_for(D))
+        close(got[0], want, bound, which)
 
 
 def test_tree_visible_infinite_value(gpu):
@@ -133,13 +165,13 @@ def test_tree_visible_infinite_value(gpu):
     parents = random_tree(w.rng, T, T)
     parents[2] = -1
     clean = run_tree(w, q, parents[None], None, scale_for(D))
+    bound = attend64(q[0], w.rows(0, w.k), w.rows(0, w.v), tree_seen(parents, T, L), scale_for(D))[2]
     w.v[0, 0, int(w.slots(0)[L - T + 2]), 7] = float("inf")
     got = run_tree(w, q, parents[None], None, scale_for(D))
     below = ancestors(parents, T)[:, 2]
     assert (got[0, below][..., 7] == np.inf).all()
-    clean[0, below, :, 7] = np.inf
-    np.testing.assert_array_equal(np.delete(got[0, below], 7, -1), np.delete(clean[0, below], 7, -1))
-    np.testing.assert_array_equal(got[0, ~below], clean[0, ~below])
+    same(np.delete(got[0, below], 7, -1), np.delete(clean[0, below], 7, -1), bound[below], "its other dims")
+    same(got[0, ~below], clean[0, ~below], bound[~below], "nodes that do not see it")
 
 
 def test_tree_of_the_whole_batch_range(gpu):
@@ -299,18 +331,21 @@ def test_masked_hidden_values(gpu, poison):
     at = np.arange(L - S, L)
     lo = np.where(at >= 101, 101, 0)[None]
     clean = run_masked(w, q, 0.09, lo)
+    rows = np.arange(L)
+    seen = (rows >= lo[0][:, None]) & (rows <= at[:, None])
+    bound = attend64(q[0], w.rows(0, w.k), w.rows(0, w.v), seen, 0.09)[2]
     hidden = torch.from_numpy(w.slots(0)[:101])
     w.k[0][:, hidden] = poison
     w.v[0][:, hidden[::2]] = poison
     got = run_masked(w, q, 0.09, lo)
-    np.testing.assert_array_equal(got[0, at >= 101], clean[0, at >= 101])
+    same(got[0, at >= 101], clean[0, at >= 101], bound[at >= 101], "the other document")
     # And a poisoned row of the same document, for the queries before it.
     clean = got
     w.v[0][:, int(w.slots(0)[133])] = poison
     w.k[0][:, int(w.slots(0)[133])] = poison
     got = run_masked(w, q, 0.09, lo)
     early = (at >= 101) & (at < 133)
-    np.testing.assert_array_equal(got[0, early], clean[0, early])
+    same(got[0, early], clean[0, early], bound[early], "the queries before it")
 
 
 def test_masked_large_scores(gpu):

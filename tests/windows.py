@@ -49,11 +49,16 @@ def queries(rng, *shape):
 def attend64(q, k, v, seen, scale, softcap=0.0, slopes=None, w=None):
     """q [n,H,D], k/v [KH,L,D], seen [n,L] -> (out [n,H,D], p [n,H,L], bound [n,H]).
 
-    bound: each score is a sum of D products and two scalings, off by at most
-    (D + 4) u sum |q k| scale; the cap's tanh, within 3 u relative, and the bias add
-    8 u of their size.  A score off by e turns its weight by the factor 1 +- (e + 3u)
-    (the base-2 exponential of the hardware within 2 u), the normalised sum by twice
-    that, and adding up L weighted rows by (L + 8) u, all of the largest |v|."""
+    bound: of an evaluation whose products are f32's or those of two f16 parts (off
+    by 4 u of the element each, by 4 u of the product for the parts left out, and by
+    2 u of the largest element of the tile where the second part is below f16's
+    normal range).  A score, a sum of D products with two scalings, is then off by
+    at most scale ((D + 16) u sum |q k| + 2 u sum |q| max |k| + 2 u sum |k| max |q|).
+    The cap's tanh, within 3 u relative, and the bias add 8 u of their size.  A score
+    off by e turns its weight by the factor 1 +- (e + 3u) (the base-2 exponential of
+    the hardware within 2 u), the normalised sum by twice that; the weights' and
+    values' own parts add 16 u, and adding up L weighted rows (L + 8) u, all of the
+    largest |v|."""
     n, H, D = q.shape
     g = H // k.shape[0]
     L = k.shape[1]
@@ -68,7 +73,8 @@ def attend64(q, k, v, seen, scale, softcap=0.0, slopes=None, w=None):
                 continue
             qi = q[i, h].astype(np.float64)
             s = kk[at] @ qi * scale
-            big = np.abs(kk[at]) @ np.abs(qi) * abs(scale) * (D + 4) * U
+            ka, qa = np.abs(kk[at]), np.abs(qi)
+            big = (ka @ qa * (D + 16) + 2 * qa.sum() * ka.max() + 2 * ka.sum(1) * qa.max()) * abs(scale) * U
             if softcap > 0:
                 s = softcap * np.tanh(s / softcap)
                 big = big + 8 * U * np.abs(s)
@@ -81,7 +87,7 @@ def attend64(q, k, v, seen, scale, softcap=0.0, slopes=None, w=None):
             e = np.exp(s - s.max())
             p[i, h, at] = e / e.sum()
             out[i, h] = p[i, h, at] @ vv[at]
-            bound[i, h] = (2 * (big.max() + 3 * U) + (L + 8) * U) * np.abs(vv[at]).max()
+            bound[i, h] = (2 * (big.max() + 3 * U) + (L + 24) * U) * np.abs(vv[at]).max()
     return out, p, bound
 
 
