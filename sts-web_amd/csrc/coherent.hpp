@@ -18,6 +18,7 @@ namespace sts {
 
 typedef float coh_f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t coh_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t coh_u2 __attribute__((ext_vector_type(2)));
 
 constexpr int kSc1 = 16;                  // cache-policy bit of sc1
 constexpr int kBufferWord3 = 0x00020000;  // raw 32-bit buffer, no swizzle

@@ -4,6 +4,7 @@
 // a radix selection per (stream, K/V head).
 #include <algorithm>
 
+#include "coherent.hpp"
 #include "common.hpp"
 #include "rope.hpp"
 #include "window.hpp"
@@ -134,30 +135,42 @@ __device__ __forceinline__ uint32_t order_key(float w) {
   return x & 0x80000000u ? ~x : x | 0x80000000u;
 }
 
-// Sum over the workgroup's lower threads of `flag` (0/1), and over all of them.
-__device__ __forceinline__ uint32_t scan_flags(bool flag, uint32_t* s_wave, uint32_t& total) {
+// Sum of `x` over the workgroup's lower threads, and over all of them.
+__device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t* s_wave, uint32_t& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint64_t mask = __ballot(flag);
-  if (lane == 0) s_wave[wave] = __popcll(mask);
+  uint32_t upto = x;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t y = __shfl_up(upto, d, 64);
+    upto += lane >= d ? y : 0;
+  }
+  if (lane == 63) s_wave[wave] = upto;
   __syncthreads();
   uint32_t before = 0;
   total = 0;
+#pragma unroll
   for (int w = 0; w < kSelThreads / 64; ++w) {
     const uint32_t c = s_wave[w];
     before += w < wave ? c : 0;
     total += c;
   }
   __syncthreads();
-  return before + __popcll(mask & ((1ull << lane) - 1));
+  return before + upto - x;
 }
 
 // Which window rows stay, for one (stream, K/V head): the `recent` newest, and of
 // the others the `keep - recent` of largest weight, the oldest first among equals.
-// The least key that stays is found a byte at a time from the top.
+// The least key that stays is found a byte at a time from the top.  A thread looks
+// after kPer rows in a row of each run of kSelThreads * kPer; windows of one run
+// (SMALL: max_len 4096 or less) keep their keys in registers, and their weights are
+// moved here, all of them having been read: at 3000 rows of 32 heads that and the
+// scans over runs instead of single rows take 9 us, reading them for every byte 11.
+template <bool SMALL>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const Evict p) {
-  __shared__ uint32_t s_hist[256];
+  constexpr int kPer = 4, kRun = kSelThreads * kPer;
+  __shared__ uint32_t s_hist[4][256];  // one for each byte
+  __shared__ uint32_t s_pick[4][2];    // the byte taken, and how many of it are wanted
   __shared__ uint32_t s_wave[kSelThreads / 64];
-  __shared__ uint32_t s_pick[2];  // the byte taken, and how many of it are wanted
   const uint32_t h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const Span s = span_of(p.lens, p.starts, p.len, p.start, p.M, b);
   int32_t* kept = p.kept + ((size_t)b * p.KH + h) * p.keep;
@@ -167,25 +180,40 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const Evict p
   }
   const uint32_t old = s.len - p.recent;
   uint32_t want = p.keep - p.recent;  // < old
+  const uint32_t total_want = want;
   for (uint32_t j = tid; j < p.recent; j += kSelThreads) kept[want + j] = (int32_t)(old + j);
   if (want == 0) return;
-  const float* w = p.weights + ((size_t)b * p.KH + h) * p.M;
-  const uint32_t total_want = want;
+  float* w = p.weights + ((size_t)b * p.KH + h) * p.M;
+  float mine[kPer];  // the weights of rows r0 + kPer*tid .. of a run
+  auto read_run = [&](uint32_t r0) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const uint32_t r = r0 + tid * kPer + k;
+      mine[k] = r < old ? w[slot_of(s, r, p.M)] : 0.f;
+    }
+  };
+  if (SMALL) read_run(0);
+  s_hist[tid >> 8][tid & 255] = 0;
+  __syncthreads();
   uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) s_hist[tid] = 0;
-    __syncthreads();
+#pragma unroll
+  for (int byte = 0; byte < 4; ++byte) {
+    const int shift = 24 - 8 * byte;
     const uint32_t above = shift == 24 ? 0 : 0xffffffffu << (shift + 8);
-    for (uint32_t r = tid; r < old; r += kSelThreads) {
-      const uint32_t key = order_key(w[slot_of(s, r, p.M)]);
-      if ((key & above) == prefix) atomicAdd(&s_hist[key >> shift & 255], 1u);
+    for (uint32_t r0 = 0; r0 < (SMALL ? 1 : old); r0 += kRun) {
+      if (!SMALL) read_run(r0);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const uint32_t key = order_key(mine[k]);
+        if (r0 + tid * kPer + k < old && (key & above) == prefix) atomicAdd(&s_hist[byte][key >> shift & 255], 1u);
+      }
     }
     __syncthreads();
     if (tid < 64) {
       // Lane x holds the bins 255-4x .. 252-4x, largest first; the bin in which
       // the running count reaches `want` is taken.
       uint32_t c[4], sum = 0;
-      for (int k = 0; k < 4; ++k) sum += c[k] = s_hist[255 - 4 * tid - k];
+      for (int k = 0; k < 4; ++k) sum += c[k] = s_hist[byte][255 - 4 * tid - k];
       uint32_t upto = sum;
       for (int x = 1; x < 64; x *= 2) {
         const uint32_t y = __shfl_up(upto, x, 64);
@@ -194,95 +222,144 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const Evict p
       uint32_t run = upto - sum;
       for (int k = 0; k < 4; ++k) {
         if (run < want && run + c[k] >= want) {
-          s_pick[0] = 255 - 4 * tid - k;
-          s_pick[1] = want - run;
+          s_pick[byte][0] = 255 - 4 * tid - k;
+          s_pick[byte][1] = want - run;
         }
         run += c[k];
       }
     }
     __syncthreads();
-    prefix |= s_pick[0] << shift;
-    want = s_pick[1];
-    __syncthreads();
+    prefix |= s_pick[byte][0] << shift;
+    want = s_pick[byte][1];
   }
   // Rows above the least key stay, and the oldest `want` rows that equal it.
   uint32_t placed = 0, equal = 0;
-  for (uint32_t r0 = 0; r0 < old && placed < total_want; r0 += kSelThreads) {
-    const uint32_t r = r0 + tid;
-    const uint32_t key = r < old ? order_key(w[slot_of(s, r, p.M)]) : 0;
-    uint32_t total;
-    const bool same = r < old && key == prefix;
-    const uint32_t rank = equal + scan_flags(same, s_wave, total);
+  for (uint32_t r0 = 0; r0 < old && placed < total_want; r0 += kRun) {
+    if (!SMALL) read_run(r0);
+    uint32_t total, same = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) same += r0 + tid * kPer + k < old && order_key(mine[k]) == prefix;
+    uint32_t rank = equal + scan(same, s_wave, total);
     equal += total;
-    const bool stays = r < old && (key > prefix || (same && rank < want));
-    const uint32_t at = placed + scan_flags(stays, s_wave, total);
+    bool stays[kPer];
+    uint32_t count = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const bool in = r0 + tid * kPer + k < old;
+      const uint32_t key = order_key(mine[k]);
+      stays[k] = in && (key > prefix || (key == prefix && rank < want));
+      rank += in && key == prefix;
+      count += stays[k];
+    }
+    uint32_t at = placed + scan(count, s_wave, total);
     placed += total;
-    if (stays) kept[at] = (int32_t)r;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (!stays[k]) continue;
+      kept[at] = (int32_t)(r0 + tid * kPer + k);
+      if (SMALL) w[slot_of(s, s.len - p.keep + at, p.M)] = mine[k];
+      ++at;
+    }
   }
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kMoveDeep = 8;  // rows a thread has in flight
+constexpr int kMoveDeep = 8;  // loads of a wave in a batch, two batches in flight (16: 33 us for 29)
 
-// The kept rows moved to the window's end, the last ones first: row kept[j] to
-// row len - keep + j.  A workgroup moves a slice of the row (LANES lanes of 8 or
-// 16 bytes) for one (stream, head, buffer), 256 / LANES * 8 rows at a time: all of
-// them are read before any is written, and rows still to be read lie below the
-// rows written, so that nothing is read after it was overwritten.
+// The kept rows moved to the window's end, the last ones first: row kept[j] to row
+// len - keep + j, for one slice of the rows (LANES lanes of T), by one wave.  A load
+// instruction takes 64 / LANES rows from the highest j down, the stores follow in
+// the loads' order.  Nothing is read after it was overwritten: a row lies at or
+// below the place it goes to, so the rows that a store overwrites are those of the
+// same or of earlier loads, which have returned.  Waves need nothing of one another.
 template <typename T>
-__device__ __forceinline__ void move_rows(T* rows, uint32_t cols, uint32_t lanes, uint32_t c0, Span s,
+__device__ __forceinline__ void move_rows(char* head, uint32_t row_bytes, uint32_t lanes, uint32_t slice, Span s,
                                           const int32_t* kept, uint32_t keep, uint32_t moved, uint32_t M) {
-  const uint32_t tid = threadIdx.x;
-  const uint32_t c = c0 + tid % lanes, sub = tid / lanes, per = kMoveThreads / lanes;
-  const bool on = sub < per && c < cols;
+  constexpr uint32_t kNone = 0x80000000u;  // past the buffer: loads zeros, stores nothing
+  const uint32_t lane = threadIdx.x & 63, per = 64 / lanes;
+  const uint32_t col = (slice * lanes + lane % lanes) * sizeof(T), sub = lane / lanes;
+  const bool on = col < row_bytes;
   const uint32_t gone = s.len - keep;
-  for (uint32_t done = 0; done < moved; done += per * kMoveDeep) {
+  const __amdgpu_buffer_rsrc_t rs = coherent_rsrc(head, M * row_bytes);
+  struct Batch {
     T x[kMoveDeep];
     uint32_t to[kMoveDeep];
-    bool move[kMoveDeep];
+  } one, two;
+  int from[kMoveDeep];
+  auto indices = [&](uint32_t done) {
 #pragma unroll
     for (int k = 0; k < kMoveDeep; ++k) {
       const uint32_t back = done + k * per + sub;  // counted from the last row that moves
-      move[k] = false;
-      if (on && back < moved) {
-        const uint32_t j = moved - 1 - back;
-        const uint32_t from = (uint32_t)kept[j];
-        to[k] = gone + j;
-        move[k] = from != to[k];
-        if (move[k]) x[k] = rows[(size_t)slot_of(s, from, M) * cols + c];
-      }
+      from[k] = back < moved ? kept[moved - 1 - back] : -1;
     }
-    // The loads have returned, not only been issued, before any wave stores.
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
+  };
+  auto load = [&](Batch& b, uint32_t done) {
 #pragma unroll
-    for (int k = 0; k < kMoveDeep; ++k)
-      if (move[k]) rows[(size_t)slot_of(s, to[k], M) * cols + c] = x[k];
+    for (int k = 0; k < kMoveDeep; ++k) {
+      const uint32_t back = done + k * per + sub;
+      const bool move = on && from[k] >= 0;
+      const uint32_t off = move ? slot_of(s, (uint32_t)from[k], M) * row_bytes + col : kNone;
+      b.to[k] = move ? slot_of(s, gone + moved - 1 - back, M) * row_bytes + col : kNone;
+      if constexpr (sizeof(T) == 16)
+        b.x[k] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
+      else if constexpr (sizeof(T) == 8)
+        b.x[k] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, 0));
+      else
+        b.x[k] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
+    }
+  };
+  auto store = [&](const Batch& b) {
+#pragma unroll
+    for (int k = 0; k < kMoveDeep; ++k) {
+      if constexpr (sizeof(T) == 16)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(coh_u4, b.x[k]), rs, b.to[k], 0, 0);
+      else if constexpr (sizeof(T) == 8)
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(coh_u2, b.x[k]), rs, b.to[k], 0, 0);
+      else
+        __builtin_amdgcn_raw_buffer_store_b32(b.x[k], rs, b.to[k], 0, 0);
+    }
+  };
+  const uint32_t step = per * kMoveDeep;
+  indices(0);
+  load(one, 0);
+  indices(step);
+  for (uint32_t done = 0; done < moved; done += 2 * step) {
+    load(two, done + step);
+    indices(done + 2 * step);
+    __builtin_amdgcn_sched_barrier(0);
+    store(one);
+    __builtin_amdgcn_sched_barrier(0);
+    load(one, done + 2 * step);
+    indices(done + 3 * step);
+    __builtin_amdgcn_sched_barrier(0);
+    store(two);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(const Evict p, uint32_t slices, uint32_t lanes) {
-  const uint32_t which = blockIdx.x / slices, slice = blockIdx.x % slices;
+// A wave per slice of a (stream, K/V head, buffer), and one for the head's weights
+// where the selection left them (with_weights).
+__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(const Evict p, uint32_t slices, uint32_t lanes,
+                                                                  bool with_weights) {
+  const uint32_t job = blockIdx.x * (kMoveThreads / 64) + threadIdx.x / 64;
+  const uint32_t which = job / slices, slice = job % slices;
   const uint32_t h = blockIdx.y, b = blockIdx.z;
   const Span s = span_of(p.lens, p.starts, p.len, p.start, p.M, b);
   if (s.len <= p.keep) return;
   const uint32_t moved = p.keep - p.recent;  // the newest rows are in place
   const size_t unit = (size_t)b * p.KH + h;
   const int32_t* kept = p.kept + unit * p.keep;
-  if (which == p.nbuf) {
-    if (slice == 0) move_rows(p.weights + unit * p.M, 1, 1, 0, s, kept, p.keep, moved, p.M);
+  if (which >= p.nbuf) {
+    if (which == p.nbuf && slice == 0 && with_weights)
+      move_rows<uint32_t>(reinterpret_cast<char*>(p.weights + unit * p.M), 4, 1, 0, s, kept, p.keep, moved, p.M);
     return;
   }
   const uint32_t bytes = p.dh * p.size[which];
   char* head = static_cast<char*>(p.buf[which]) + unit * p.M * bytes;
-  if (bytes % 16 == 0) {
-    for (uint32_t c0 = slice * lanes; c0 < bytes / 16; c0 += slices * lanes)
-      move_rows(reinterpret_cast<uint4*>(head), bytes / 16, lanes, c0, s, kept, p.keep, moved, p.M);
-  } else {
-    for (uint32_t c0 = slice * lanes; c0 < bytes / 8; c0 += slices * lanes)
-      move_rows(reinterpret_cast<uint2*>(head), bytes / 8, lanes, c0, s, kept, p.keep, moved, p.M);
-  }
+  if (bytes % 16 == 0)
+    move_rows<uint4>(head, bytes, lanes, slice, s, kept, p.keep, moved, p.M);
+  else  // (the bf16 copy of an odd head dim: twice the lanes, at most 32)
+    move_rows<uint2>(head, bytes, 2 * lanes, slice, s, kept, p.keep, moved, p.M);
 }
 
 }  // namespace
@@ -312,21 +389,25 @@ int launch_tree_commit(const TreeCommit& p, uint32_t batch, hipStream_t stream) 
 }
 
 int launch_evict(const Evict& p, uint32_t batch, hipStream_t stream) {
-  hipLaunchKernelGGL(evict_select_kernel, dim3(p.KH, batch), dim3(kSelThreads), 0, stream, p);
+  const bool small = p.M <= 4 * kSelThreads;
+  if (small)
+    hipLaunchKernelGGL(evict_select_kernel<true>, dim3(p.KH, batch), dim3(kSelThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL(evict_select_kernel<false>, dim3(p.KH, batch), dim3(kSelThreads), 0, stream, p);
   STS_HIP(hipGetLastError());
   if (p.keep == p.recent) return STS_OK;  // only the newest rows stay, and they are in place
-  // Slices of a row, at least 64 bytes each, until the chip is full.
-  const uint64_t units = (uint64_t)batch * p.KH * p.nbuf;
+  // Slices of a row of 64 (4 lanes of 16 bytes) to 256 bytes, the wider while there
+  // are two waves for every CU (20 streams of 8 heads 83 us, with eight 94; one of 32
+  // takes 64 bytes either way, 29 us, with 128 41).
   uint32_t bytes = 0;
   for (uint32_t i = 0; i < p.nbuf; ++i) bytes = std::max(bytes, p.dh * p.size[i]);
-  const uint32_t unit_bytes = bytes % 16 == 0 ? 16 : 8;
-  uint32_t lanes = 32, slices = (bytes / unit_bytes + lanes - 1) / lanes;
-  while (lanes * unit_bytes > 64 && units * slices < 2 * (uint64_t)device_cu_count()) {
-    lanes /= 2;
-    slices = (bytes / unit_bytes + lanes - 1) / lanes;
-  }
-  hipLaunchKernelGGL(evict_move_kernel, dim3((p.nbuf + 1) * slices, p.KH, batch), dim3(kMoveThreads), 0, stream,
-                     p, slices, lanes);
+  const uint64_t units = (uint64_t)batch * p.KH * p.nbuf;
+  uint32_t lanes = 16;
+  auto slices_of = [&](uint32_t l) { return (bytes + 16 * l - 1) / (16 * l); };
+  while (lanes > 4 && units * slices_of(lanes) < 2 * (uint64_t)device_cu_count()) lanes /= 2;
+  const uint32_t slices = slices_of(lanes), jobs = p.nbuf * slices + !small;
+  hipLaunchKernelGGL(evict_move_kernel, dim3((jobs + 3) / 4, p.KH, batch), dim3(kMoveThreads), 0, stream, p, slices,
+                     lanes, !small);
   STS_HIP(hipGetLastError());
   return STS_OK;
 }
