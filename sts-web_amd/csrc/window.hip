@@ -48,9 +48,11 @@ struct WindowPlan {
   int row_tiles = 1;
   uint32_t rblocks = 1, nsplit = 1;
   size_t record = 0;  // floats of a split's record
+  uint32_t shares = 0;
+  float rows_factor = 0.f;
 };
 
-WindowPlan plan_window(const WindowParams& p, uint32_t batch, bool bf16, uint32_t max_rows) {
+WindowPlan plan_window(const WindowParams& p, WindowMode mode, uint32_t batch, bool bf16, uint32_t max_rows) {
   WindowPlan pl;
   const uint32_t rows = p.T * p.group;
   pl.row_tiles = rows <= 16 ? 1 : 2;
@@ -62,15 +64,28 @@ WindowPlan plan_window(const WindowParams& p, uint32_t batch, bool bf16, uint32_
   // 20011 such rows 52 us against 102 with one).  Two are bound by their products:
   // two workgroups, what a CU holds at once (a draft of 60 over 3000 rows 34 us, with
   // four 49).
-  const uint32_t tile = 16 * pl.row_tiles;
+  const uint32_t tile = pl.row_tiles > 1 || bf16 ? 32 : 16;
   const uint32_t wide = p.dh <= 64 ? 64 : 128;
   const uint32_t tile_bytes = 2 * tile * wide * (bf16 ? 2 : 4) * window::kWaves;
   const uint32_t per_cu = pl.row_tiles > 1 ? 2 : std::min(4u, std::max(1u, 65536 / tile_bytes));
   const uint64_t target = (uint64_t)device_cu_count() * per_cu;
-  const uint64_t want = std::max<uint64_t>(1, (target + units - 1) / units);
   // A split is worth its record from a tile for each of its waves on.
-  const uint64_t most = (max_rows + tile * window::kWaves - 1) / (tile * window::kWaves);
-  pl.nsplit = (uint32_t)std::max<uint64_t>(1, std::min({want, most, (uint64_t)window::max_splits(pl.row_tiles)}));
+  const uint64_t most = std::min<uint64_t>((max_rows + tile * window::kWaves - 1) / (tile * window::kWaves),
+                                           window::max_splits(pl.row_tiles));
+  if (mode != kWindowMasked && batch > 1 && batch <= 64) {
+    // Streams of different ages: splits of about equal length whatever their stream,
+    // not more than fit at once where one round can hold them (rounding up gives each
+    // window half a split more), else in two rounds or more, of half the length.
+    const uint64_t fit = 2 * units <= target ? target - units / 2 : 2 * target;
+    const uint64_t heads = (uint64_t)p.KH * pl.rblocks;
+    pl.rows_factor = (float)heads / (float)fit;
+    pl.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(fit / heads + 1, most));
+    pl.shares = (uint32_t)(p.KH * (fit / heads + batch + 1));
+  } else {
+    const uint64_t want = std::max<uint64_t>(1, (target + units - 1) / units);
+    pl.nsplit = (uint32_t)std::max<uint64_t>(1, std::min(want, most));
+    pl.shares = batch * p.KH * pl.nsplit;
+  }
   pl.record = (size_t)per * ((p.dh <= 64 ? 64 : 128) + 2);
   return pl;
 }
@@ -98,16 +113,16 @@ int check_window(const WindowParams& p, uint32_t batch, bool bf16) {
   return STS_OK;
 }
 
-int reserve_window(const WindowParams& p, uint32_t batch, bool bf16, uint32_t max_rows,
-                   hipStream_t stream) {
+int reserve_window(const WindowParams& p, WindowMode mode, uint32_t batch, bool bf16,
+                   uint32_t max_rows, hipStream_t stream) {
   Workspace* ws = nullptr;
-  return window_workspace(p, plan_window(p, batch, bf16, max_rows), batch, stream, &ws);
+  return window_workspace(p, plan_window(p, mode, batch, bf16, max_rows), batch, stream, &ws);
 }
 
 int launch_window(WindowParams p, WindowMode mode, uint32_t batch, bool bf16, uint32_t max_rows,
                   hipStream_t stream) {
   if (int rc = check_window(p, batch, bf16)) return rc;
-  const WindowPlan pl = plan_window(p, batch, bf16, max_rows);
+  const WindowPlan pl = plan_window(p, mode, batch, bf16, max_rows);
   Workspace* ws = nullptr;
   if (int rc = window_workspace(p, pl, batch, stream, &ws)) return rc;
   p.rblocks = pl.rblocks;
@@ -116,7 +131,9 @@ int launch_window(WindowParams p, WindowMode mode, uint32_t batch, bool bf16, ui
     p.part = ws->part;
     p.counters = ws->counters;
   }
-  p.shares = batch * p.KH * pl.nsplit;
+  p.shares = pl.shares;
+  p.batch = batch;
+  p.rows_factor = pl.rows_factor;
   const dim3 grid((p.shares + window::kXcds - 1) / window::kXcds * window::kXcds * pl.rblocks);
   if (mode == kWindowTree) return launch_window_tree(p, pl.row_tiles, bf16, grid, stream);
   if (mode == kWindowMasked) return launch_window_masked(p, pl.row_tiles, bf16, grid, stream);

@@ -47,6 +47,8 @@ struct WindowParams {
   // Set by launch_window.
   uint32_t rblocks = 1, nsplit = 1;
   uint32_t shares = 0;  // streams x K/V heads x splits
+  uint32_t batch = 0;
+  float rows_factor = 0.f;  // rows of a split for each row there is; 0: nsplit for every stream
   float* part = nullptr;
   uint32_t* counters = nullptr;
 };
@@ -60,8 +62,8 @@ int launch_window(WindowParams p, WindowMode mode, uint32_t batch, bool bf16, ui
 
 // Makes sure the split workspace launch_window needs for these sizes exists, so
 // that a caller can fail before it changes any state.
-int reserve_window(const WindowParams& p, uint32_t batch, bool bf16, uint32_t max_rows,
-                   hipStream_t stream);
+int reserve_window(const WindowParams& p, WindowMode mode, uint32_t batch, bool bf16,
+                   uint32_t max_rows, hipStream_t stream);
 
 // weights[b][j][slot of row r] += sum over the group's heads of
 // 2^(score - max) / sum, for the rows of each window; with `fresh` the newest

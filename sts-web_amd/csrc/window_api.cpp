@@ -68,7 +68,7 @@ int decode_keeping_weights(const sts_kv_cache* c, const sts_kv_cache* next, cons
   WindowParams p = handle_params(next, q, out, 1);
   const uint32_t batch = (uint32_t)c->batch, max_len = (uint32_t)c->max_len;
   if (int rc = check_window(p, batch, false)) return rc;
-  if (int rc = reserve_window(p, batch, false, p.len, stream)) return rc;
+  if (int rc = reserve_window(p, kWindowWeights, batch, false, p.len, stream)) return rc;
   if (k_new) {
     const uint32_t pos = (uint32_t)(c->offset % c->max_len);
     if (int rc = launch_kv_append(k_new, v_new, c->k, c->v, pos, batch, 1, p.KH, p.dh, max_len,
@@ -270,7 +270,8 @@ int sts_kv_tree_step(sts_kv_cache* cache, const sts_rope* rope, const float* q, 
   kv_advance(&next, nodes);
   const uint32_t n = (uint32_t)nodes;
   if (int rc = sts::check_window(handle_params(&next, q, out, n), 1, false)) return rc;
-  if (int rc = sts::reserve_window(handle_params(&next, q, out, n), 1, false, (uint32_t)next.len, s)) return rc;
+  if (int rc = sts::reserve_window(handle_params(&next, q, out, n), sts::kWindowTree, 1, false,
+                                (uint32_t)next.len, s)) return rc;
   if (int rc = kv_ensure(cache, 1, s)) return rc;
   const uint64_t offset = cache->offset;
   const uint32_t pos = (uint32_t)(offset % cache->max_len);

@@ -21,11 +21,11 @@
 // never leave their registers.  The waves' (m, l, O) are merged through LDS, the
 // splits' through records in the stream's workspace by the last to arrive.
 //
-// One row tile (R = 1) multiplies in f32 (16x16x4): its 64 products of a 16 KB tile
-// take a quarter of the time that HBM takes to deliver it.  Two (R = 2) would be
-// bound by those products and multiply parts instead (16x16x32): f32 rows as two
-// f16 values each, three products for one; bf16 rows as they are against three
-// bf16 parts of Q and of the weights.  Either is as close to the exact result as f32
+// One row tile (R = 1) over f32 rows multiplies in f32 (16x16x4): its 64 products of
+// a 16 KB tile take a quarter of the time that HBM takes to deliver it.  Two (R = 2),
+// or bf16 rows, would be bound by those products and multiply parts instead
+// (16x16x32): f32 rows as two f16 values each, three products for one; bf16 rows as
+// they are against three bf16 parts of Q and of the weights.  Either is as close to the exact result as f32
 // products are.  At 1000 queries of 32 heads over 2600 bf16 rows of 8 K/V heads
 // that is 111 us against 488 in f32; at 24 drafts of 40 nodes over f32 rows 189
 // against 513.
@@ -45,6 +45,7 @@ namespace window {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWaves = 4;
 constexpr uint32_t kXcds = 8;
+constexpr int kNt = 2;                // cache policy: nontemporal
 // Splits of a block of 16 * row_tiles query rows at most: the merge holds two
 // numbers for each split and row in LDS.
 constexpr int max_splits(int row_tiles) { return 128 / row_tiles; }
@@ -82,18 +83,19 @@ __device__ __forceinline__ float wave_max(float x) {
 }
 
 // W elements loaded at a byte offset of a cache head, as f32 (bf16 is widened).
-template <bool BF, int W>
+// AUX: the cache policy of the load.
+template <bool BF, int W, int AUX>
 struct Piece {
   static constexpr int kWords = BF ? W / 2 : W;
   uint32_t w[kWords];
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t off) {
     if constexpr (kWords == 4) {
-      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0);
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, AUX);
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = x[i];
     } else {
       static_assert(kWords == 2, "8 or 16 bytes a lane");
-      const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, 0);
+      const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, AUX);
       w[0] = x[0];
       w[1] = x[1];
     }
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   constexpr int VW = CW < D / 16 ? CW : D / 16;     // dims of V a lane loads at once
   constexpr int NV = D / (16 * VW);                 // loads per V row
   constexpr int ES = BF ? 2 : 4;                    // bytes per element
-  constexpr bool PARTS = R > 1;                     // products of f16 parts
+  constexpr bool PARTS = R > 1 || BF;               // products of parts
   constexpr int KT = PARTS ? 2 : 1;                 // 16-row tiles a wave takes at once
   constexpr int TILE = 16 * KT;
   constexpr int NP = NC * CW / 8;                   // 32-dim steps of K Q^T in f16
@@ -253,8 +255,37 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   // its L2 serves all but the first.
   const uint32_t turn = blockIdx.x / kXcds, rb = turn % p.rblocks;
   const uint32_t share = turn / p.rblocks * kXcds + blockIdx.x % kXcds;
-  if (share >= p.shares) return;
-  const uint32_t split = share % p.nsplit, kvh = share / p.nsplit % p.KH, b = share / p.nsplit / p.KH;
+  uint32_t b, kvh, split, splits;
+  if (MODE != kWindowMasked && p.rows_factor > 0.f) {
+    // Windows of different lengths are cut into splits of about the same length:
+    // lane x looks at stream x, and the share's stream is the last whose streams
+    // before take no more shares.
+    const uint32_t rows = lane < (int)p.batch ? (p.lens ? (uint32_t)min(max(p.lens[lane], 0), (int32_t)p.M) : p.len) : 0;
+    uint32_t total = rows;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) total += (uint32_t)__shfl_xor((int)total, x, 64);
+    const uint32_t chunk = max((uint32_t)((float)total * p.rows_factor) + 1, (uint32_t)(kWaves * TILE));
+    const uint32_t mine = lane < (int)p.batch ? min(max((rows + chunk - 1) / chunk, 1u), p.nsplit) : 0;
+    uint32_t before = mine;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) {
+      const uint32_t y = (uint32_t)__shfl_up((int)before, x, 64);
+      before += lane >= x ? y : 0;
+    }
+    if (share >= (uint32_t)__builtin_amdgcn_readlane((int)before, 63) * p.KH) return;
+    before -= mine;
+    b = 63 - __builtin_clzll(__ballot(lane < (int)p.batch && before * p.KH <= share));
+    splits = (uint32_t)__builtin_amdgcn_readlane((int)mine, b);
+    const uint32_t at = share - (uint32_t)__builtin_amdgcn_readlane((int)before, b) * p.KH;
+    kvh = at % p.KH;
+    split = at / p.KH;
+  } else {
+    if (share >= p.shares) return;
+    splits = p.nsplit;
+    split = share % splits;
+    kvh = share / splits % p.KH;
+    b = share / splits / p.KH;
+  }
   const uint32_t dh = PAD ? p.dh : (uint32_t)D;
 
   // What does not depend on the window's length is requested first: the queries of
@@ -354,7 +385,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   // Tiles of TILE window rows, dealt to the splits and waves in turn; a split gets
   // at least a tile for each wave.
   const uint32_t t0 = ulo / TILE, t1 = (uhi + TILE - 1) / TILE;
-  const uint32_t nsplit = min(p.nsplit, (t1 - t0 + kWaves - 1) / kWaves);
+  const uint32_t nsplit = min(splits, (t1 - t0 + kWaves - 1) / kWaves);
   if (split >= nsplit) return;
 
   const size_t head = ((size_t)b * p.KH + kvh) * p.M * dh * ES;
@@ -365,8 +396,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
     slot = slot >= p.M ? slot - p.M : slot;
     return r < uhi ? slot * (dh * ES) : kOutside;
   };
-  typedef Piece<BF, CW> KRow[NC];  // a lane's part of 16 rows of K, and of V
-  typedef Piece<BF, VW> VRow[4][NV];
+  // One row tile is all the query rows there are: nothing is read twice.
+  constexpr int AUX = R > 1 ? 0 : kNt;
+  typedef Piece<BF, CW, AUX> KRow[NC];  // a lane's part of 16 rows of K, and of V
+  typedef Piece<BF, VW, AUX> VRow[4][NV];
   auto load_k = [&](uint32_t r0, KRow& k) {
     const uint32_t off = row_off(r0 + m16) + g * (CW * ES);
 #pragma unroll
@@ -641,7 +674,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t d = (c * 16 + 4 * g + i) * VW;
-              Piece<BF, VW> x;
+              Piece<BF, VW, AUX> x;
               x.load(vrs, !PAD || d < dh ? off + d * ES : kOutside);
 #pragma unroll
               for (int e = 0; e < VW; ++e) {
