@@ -211,6 +211,14 @@ struct TileScale {
   }
 };
 
+// The lane's number, found anew: kept through the loops it, and what is derived from
+// it, would cost registers that the tiles need.
+__device__ __forceinline__ int fresh_lane() {
+  int x = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 template <int D, int R, bool BF, WindowMode MODE, bool PAD>
 __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowParams p) {
   constexpr int CW = BF ? 8 : 4;                    // dims of K a lane loads at once
@@ -248,7 +256,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   __shared__ int s_jump[MODE == kWindowTree ? kMaxTreeNodes : 1];
   __shared__ int s_depth[MODE == kWindowTree ? kMaxTreeNodes : 1];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m16 = lane & 15, g = lane >> 4;
   // Workgroups go round the XCDs: the row blocks of one (stream, K/V head, split),
   // which read the same rows, take turns on one of them, next to one another, so that
@@ -256,11 +264,25 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   const uint32_t turn = blockIdx.x / kXcds, rb = turn % p.rblocks;
   const uint32_t share = turn / p.rblocks * kXcds + blockIdx.x % kXcds;
   uint32_t b, kvh, split, splits;
-  if (MODE != kWindowMasked && p.rows_factor > 0.f) {
+  int32_t len_at = (int32_t)p.len, start_at = (int32_t)p.start, count_at = (int32_t)p.T;  // the stream's
+  if (p.rows_factor > 0.f) {
     // Windows of different lengths are cut into splits of about the same length:
     // lane x looks at stream x, and the share's stream is the last whose streams
     // before take no more shares.
-    const uint32_t rows = lane < (int)p.batch ? (p.lens ? (uint32_t)min(max(p.lens[lane], 0), (int32_t)p.M) : p.len) : 0;
+    uint32_t rows = 0;
+    if (lane < (int)p.batch) {
+      if (p.lens) {
+        len_at = p.lens[lane];
+        start_at = p.starts[lane];
+      }
+      if (p.counts) count_at = p.counts[lane];
+      rows = (uint32_t)min(max(len_at, 0), (int32_t)p.M);
+      if constexpr (MODE == kWindowMasked) {  // (one query a stream: the rows that it sees)
+        const uint32_t hi = p.hi ? min((uint32_t)max(p.hi[lane], 0), rows) : rows;
+        const uint32_t lo = p.lo ? (uint32_t)max(p.lo[lane], 0) : 0;
+        rows = lo < hi ? hi - lo : 0;
+      }
+    }
     uint32_t total = rows;
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) total += (uint32_t)__shfl_xor((int)total, x, 64);
@@ -279,12 +301,20 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
     const uint32_t at = share - (uint32_t)__builtin_amdgcn_readlane((int)before, b) * p.KH;
     kvh = at % p.KH;
     split = at / p.KH;
+    len_at = __builtin_amdgcn_readlane(len_at, b);
+    start_at = __builtin_amdgcn_readlane(start_at, b);
+    count_at = __builtin_amdgcn_readlane(count_at, b);
   } else {
     if (share >= p.shares) return;
     splits = p.nsplit;
     split = share % splits;
     kvh = share / splits % p.KH;
     b = share / splits / p.KH;
+    if (p.lens) {
+      len_at = p.lens[b];
+      start_at = p.starts[b];
+    }
+    if (p.counts) count_at = p.counts[b];
   }
   const uint32_t dh = PAD ? p.dh : (uint32_t)D;
 
@@ -309,18 +339,21 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   int up = -1;
   if (MODE == kWindowTree && me < (int)p.T) up = p.parents[(size_t)b * p.T + me];
 
-  uint32_t len = p.len, start = p.start;
-  if (p.lens) {
-    const int32_t L = p.lens[b];
-    len = L <= 0 ? 0u : min((uint32_t)L, p.M);
-    const int32_t st = p.starts[b] % (int32_t)p.M;
-    start = (uint32_t)(st < 0 ? st + (int32_t)p.M : st);
+  int32_t lo_at = 0, hi_at = 0;  // of the block's row tid
+  float slope_at = 0.f;
+  if (MODE == kWindowMasked && tid < ROWS && rb * ROWS + tid < all) {
+    const uint32_t rr = rb * ROWS + tid;
+    const size_t at = (size_t)b * p.T + rr / p.group;
+    if (p.lo) lo_at = p.lo[at];
+    if (p.hi) hi_at = p.hi[at];
+    if (p.slopes) slope_at = p.slopes[kvh * p.group + rr % p.group];
   }
-  uint32_t n = min(p.T, len);
-  if (p.counts) {
-    const int32_t c = p.counts[b];
-    n = c <= 0 ? 0u : min((uint32_t)c, n);
-  }
+
+  const uint32_t len = __builtin_amdgcn_readfirstlane(len_at <= 0 ? 0u : min((uint32_t)len_at, p.M));
+  start_at %= (int32_t)p.M;
+  const uint32_t start =
+      __builtin_amdgcn_readfirstlane((uint32_t)(start_at < 0 ? start_at + (int32_t)p.M : start_at));
+  const uint32_t n = __builtin_amdgcn_readfirstlane(count_at <= 0 ? 0u : min(min((uint32_t)count_at, p.T), len));
   const uint32_t base = len - n;  // window row of query 0
 
   // Row rr of the block is query rr / group, head kvh*group + rr % group.
@@ -349,12 +382,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
       const uint32_t rr = row0 + tid, i = rr / p.group;
       uint32_t lo = 0, hi = len;
       if (rr < nrows) {
-        const size_t at = (size_t)b * p.T + i;
-        hi = base + i + 1;
-        if (p.lo) lo = (uint32_t)max(p.lo[at], 0);
-        if (p.hi) hi = min((uint32_t)max(p.hi[at], 0), len);
+        lo = (uint32_t)max(lo_at, 0);
+        hi = p.hi ? min((uint32_t)max(hi_at, 0), len) : base + i + 1;
       }
-      s_row[tid] = Row{lo, hi, (int)(base + i), rr < nrows && p.slopes ? p.slopes[kvh * p.group + rr % p.group] * kLog2e : 0.f};
+      s_row[tid] = Row{lo, hi, (int)(base + i), slope_at * kLog2e};
     }
     __syncthreads();
     const int last = (int)(live - row0);  // (the last rows of a block may be missing)
@@ -400,13 +431,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   constexpr int AUX = R > 1 ? 0 : kNt;
   typedef Piece<BF, CW, AUX> KRow[NC];  // a lane's part of 16 rows of K, and of V
   typedef Piece<BF, VW, AUX> VRow[4][NV];
-  auto load_k = [&](uint32_t r0, KRow& k) {
+  auto load_k = [&](uint32_t r0, KRow& k, int lane) {
+    const int m16 = lane & 15, g = lane >> 4;
     const uint32_t off = row_off(r0 + m16) + g * (CW * ES);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
       k[c].load(krs, !PAD || (uint32_t)(c * 4 + g) * CW < dh ? off + c * (4 * CW * ES) : kOutside);
   };
-  auto load_v = [&](uint32_t r0, VRow& v) {
+  auto load_v = [&](uint32_t r0, VRow& v, int lane) {
+    const int m16 = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t off = row_off(r0 + 4 * g + i) + m16 * (VW * ES);
@@ -420,8 +453,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   const uint32_t tstep = nsplit * kWaves;
   uint32_t t = t0 + split + nsplit * wave;
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) load_k(t * TILE + kt * 16, kk[kt]);
-  if constexpr (!PARTS) load_v(t * TILE, vv[0]);
+  for (int kt = 0; kt < KT; ++kt) load_k(t * TILE + kt * 16, kk[kt], lane);
+  if constexpr (!PARTS) load_v(t * TILE, vv[0], lane);
 
   // The draft's relation "is above or is", a bit per node, and the nodes' depths:
   // each node takes over what its jump target knows and jumps as far as that one
@@ -555,7 +588,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
 
   // What follows the scores of rows r0 .. (16 for each of s's tiles): cap, bias,
   // mask, and the weights they turn into, relative to m.
-  auto weigh = [&](uint32_t r0, auto& s, bool partly) __attribute__((always_inline)) {
+  auto weigh = [&](uint32_t r0, auto& s, bool partly, int lane) __attribute__((always_inline)) {
+    const int m16 = lane & 15, g = lane >> 4;
     constexpr int K = sizeof(s[0]) / sizeof(f32x4);
     if constexpr (MODE == kWindowMasked) {
       if (p.cap_log2 > 0.f) {
@@ -650,8 +684,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   // rows.  A value that is not finite, in a row that some query does not see, would
   // be carried to that query as 0 * inf: it is taken out of the operand and added by
   // hand to the queries that see its row.
-  auto add_values = [&](uint32_t r0, const VRow& v, auto w, float oscale, bool partly)
+  auto add_values = [&](uint32_t r0, const VRow& v, auto w, float oscale, bool partly, int lane)
       __attribute__((always_inline)) {
+    const int m16 = lane & 15, g = lane >> 4;
     if (partly) {
       bool bad = false;
 #pragma unroll
@@ -712,6 +747,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
     for (; t < t1; t += tstep) {
       const uint32_t r0 = t * TILE;
       const bool partly = partly_seen(r0, TILE);
+      const int at = fresh_lane();
       if constexpr (!BF) {
         float top = 0.f;
 #pragma unroll
@@ -734,8 +770,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
         for (int kt = 0; kt < KT; ++kt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
       // The queries' parts are read anew for every tile: kept in registers (the
       // compiler lifts the loads out of the loop) they would push others out.
-      int at = lane;
-      asm volatile("" : "+v"(at));
 #pragma unroll
       for (int c = 0; c < NP; ++c) {
         Frag kf[KT][P::N];
@@ -765,18 +799,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) s[rt][kt] = P::mfma(kf[kt][0], qq[n], s[rt][kt]);
         }
-        if (c == NP / 2 - 1) load_v(r0, vv[0]);
+        if (c == NP / 2 - 1) load_v(r0, vv[0], at);
       }
-      load_v(r0 + 16, vv[1]);
+      load_v(r0 + 16, vv[1], at);
       if constexpr (!BF) {
 #pragma unroll
         for (int rt = 0; rt < R; ++rt) {
-          const float f = s_qs[rt * 16 + m16] * ks.inverse;
+          const float f = s_qs[rt * 16 + (at & 15)] * ks.inverse;
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt) s[rt][kt] *= f;
         }
       }
-      weigh(r0, s, partly);
+      weigh(r0, s, partly, at);
       if constexpr (!BF) {
         float top = 0.f;
 #pragma unroll
@@ -834,17 +868,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
         for (int n = P::N - 1; n >= 0; --n)
 #pragma unroll
           for (int rt = 0; rt < R; ++rt) o[rt][x] = P::mfma(vf[0], pp[rt][n], o[rt][x]);
-        if (x == NX / 2 - 1) load_k((t + tstep) * TILE, kk[0]);
+        if (x == NX / 2 - 1) load_k((t + tstep) * TILE, kk[0], at);
       }
-      load_k((t + tstep) * TILE + 16, kk[1]);
+      load_k((t + tstep) * TILE + 16, kk[1], at);
     }
     if (weighed) {
       const float oscale = vs.scale;
+      const int at = fresh_lane();
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
         const uint32_t r0 = t * TILE + kt * 16;
-        load_v(r0, vv[0]);
-        add_values(r0, vv[0], [&](int rt) { return s[rt][kt]; }, oscale, partly_seen(r0, 16));
+        load_v(r0, vv[0], at);
+        add_values(r0, vv[0], [&](int rt) { return s[rt][kt]; }, oscale, partly_seen(r0, 16), at);
       }
       t += tstep;
     }
@@ -856,15 +891,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   for (uint32_t half = 0; t < t1;) {
     const uint32_t r0 = t * TILE + half * 16;
     const bool partly = partly_seen(r0, 16);
+    const int at = fresh_lane();
     if constexpr (PARTS) {
-      load_k(r0, kk[0]);
-      load_v(r0, vv[0]);
+      load_k(r0, kk[0], at);
+      load_v(r0, vv[0], at);
     }
     f32x4 s[R][1];
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) s[rt][0] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int at = lane;
-    asm volatile("" : "+v"(at));
 #pragma unroll
     for (int rt = 0; rt < R; ++rt)
 #pragma unroll
@@ -891,18 +925,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
       }
     if constexpr (PARTS) {
 #pragma unroll
-      for (int rt = 0; rt < R; ++rt) s[rt][0] *= s_qs[rt * 16 + m16];
+      for (int rt = 0; rt < R; ++rt) s[rt][0] *= s_qs[rt * 16 + (at & 15)];
     } else {
-      load_k((t + tstep) * TILE, kk[0]);
+      load_k((t + tstep) * TILE, kk[0], at);
     }
-    weigh(r0, s, partly);
-    add_values(r0, vv[0], [&](int rt) { return s[rt][0]; }, oscale, partly);
+    weigh(r0, s, partly, at);
+    add_values(r0, vv[0], [&](int rt) { return s[rt][0]; }, oscale, partly, at);
     if constexpr (PARTS) {
       half ^= 1;
       if (half == 0) t += tstep;
     } else {
       t += tstep;
-      load_v(t * TILE, vv[0]);
+      load_v(t * TILE, vv[0], at);
     }
   }
   if constexpr (PARTS) {
@@ -915,12 +949,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   }
 
   // The waves' states merged through LDS.
+  const int lane1 = fresh_lane(), tid1 = wave * 64 + lane1;
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     l[rt] = sum_xor32(sum_xor16(l[rt]));
-    if (g == 0) {
-      s_ml[wave][rt * 16 + m16][0] = m[rt];
-      s_ml[wave][rt * 16 + m16][1] = l[rt];
+    if ((lane1 >> 4) == 0) {
+      s_ml[wave][rt * 16 + (lane1 & 15)][0] = m[rt];
+      s_ml[wave][rt * 16 + (lane1 & 15)][1] = l[rt];
     }
 #pragma unroll
     for (int c = 0; c < NV; ++c)
@@ -928,7 +963,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < VW; e += 4)
-          *reinterpret_cast<f32x4*>(&s_o[wave][rt * 16 + m16][(c * 16 + 4 * g + i) * VW + e]) =
+          *reinterpret_cast<f32x4*>(&s_o[wave][rt * 16 + (lane1 & 15)][(c * 16 + 4 * (lane1 >> 4) + i) * VW + e]) =
               f32x4{o[rt][c * VW + e][i], o[rt][c * VW + e + 1][i], o[rt][c * VW + e + 2][i], o[rt][c * VW + e + 3][i]};
   }
   __syncthreads();
@@ -951,7 +986,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   constexpr int NXT = ROWS * C4 / (kWaves * 64);  // float4 columns of a thread
 #pragma unroll
   for (int k = 0; k < NXT; ++k) {
-    const int x = tid + k * kWaves * 64, row = x / C4, col = x % C4;
+    const int x = tid1 + k * kWaves * 64, row = x / C4, col = x % C4;
     float mt = s_ml[0][row][0];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) mt = fmaxf(mt, s_ml[w][row][0]);
@@ -983,7 +1018,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   __builtin_amdgcn_s_waitcnt(0);
   __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
   __syncthreads();
-  if (tid == 0) {
+  if (tid1 == 0) {
     const uint32_t ticket = atomicAdd(p.counters + unit, 1u);
     s_last = ticket == nsplit - 1;
     if (ticket == nsplit - 1) atomicExch(p.counters + unit, 0u);
@@ -991,6 +1026,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   __syncthreads();
   if (!s_last) return;
   __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+  // Each thread's columns of the first four splits, requested before anything else.
+  coh_f4 y[4][NXT];
+  auto request = [&](uint32_t sp) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int k = 0; k < NXT; ++k)  // (past the record: zeros)
+        y[u][k] = ld_coherent4(prs, sp + u < nsplit ? (sp + u) * REC * 4 + (tid1 + k * kWaves * 64) * 16 : kOutside);
+  };
   // The splits' (m, l) of every row, all requested at once, in the LDS of the
   // partial outputs, which every thread is done with; m then gives way to the
   // split's factor 2^(m_s - m).
@@ -1000,49 +1044,44 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   static_assert(2 * MS * ROWS * 4 <= kOutBytes, "the splits' numbers fit");
   constexpr int NML = MS * ROWS / (kWaves * 64);
   u32x2 ml[NML];
+  request(0);
 #pragma unroll
   for (int k = 0; k < NML; ++k) {
-    const uint32_t x = tid + k * kWaves * 64;
+    const uint32_t x = tid1 + k * kWaves * 64;
     if (x < nsplit * ROWS)
       ml[k] = __builtin_amdgcn_raw_buffer_load_b64(prs, (x / ROWS * REC + ROWS * D + x % ROWS * 2) * 4, 0, kSc1);
   }
 #pragma unroll
   for (int k = 0; k < NML; ++k) {
-    const uint32_t x = tid + k * kWaves * 64;
+    const uint32_t x = tid1 + k * kWaves * 64;
     if (x < nsplit * ROWS) {
       s_f[x / ROWS][x % ROWS] = __uint_as_float(ml[k][0]);
       s_l[x / ROWS][x % ROWS] = __uint_as_float(ml[k][1]);
     }
   }
   __syncthreads();
-  if (tid < ROWS) {
+  if (tid1 < ROWS) {
     float mt = -FLT_MAX, lt = 0.f;
-    for (uint32_t sp = 0; sp < nsplit; ++sp) mt = fmaxf(mt, s_f[sp][tid]);
+    for (uint32_t sp = 0; sp < nsplit; ++sp) mt = fmaxf(mt, s_f[sp][tid1]);
     for (uint32_t sp = 0; sp < nsplit; ++sp) {
-      const float f = exp2_hw(s_f[sp][tid] - mt);
-      s_f[sp][tid] = f;
-      lt += f * s_l[sp][tid];
+      const float f = exp2_hw(s_f[sp][tid1] - mt);
+      s_f[sp][tid1] = f;
+      lt += f * s_l[sp][tid1];
     }
-    s_ml[0][tid][0] = mt;
-    s_ml[0][tid][1] = lt;
+    s_ml[0][tid1][0] = mt;
+    s_ml[0][tid1][1] = lt;
   }
   __syncthreads();
-  // Each thread's columns of four splits at a time, requested together.
   float4 a[NXT];
 #pragma unroll
   for (int k = 0; k < NXT; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (uint32_t sp = 0; sp < nsplit; sp += 4) {
-    coh_f4 y[4][NXT];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int k = 0; k < NXT; ++k)  // (past the record: zeros)
-        y[u][k] = ld_coherent4(prs, sp + u < nsplit ? (sp + u) * REC * 4 + (tid + k * kWaves * 64) * 16 : kOutside);
+    if (sp > 0) request(sp);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int k = 0; k < NXT; ++k) {
-        const float f = sp + u < nsplit ? s_f[sp + u][(tid + k * kWaves * 64) / C4] : 0.f;
+        const float f = sp + u < nsplit ? s_f[sp + u][(tid1 + k * kWaves * 64) / C4] : 0.f;
         a[k].x += f * y[u][k].x;
         a[k].y += f * y[u][k].y;
         a[k].z += f * y[u][k].z;
@@ -1051,8 +1090,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   }
 #pragma unroll
   for (int k = 0; k < NXT; ++k) {
-    const int row = (tid + k * kWaves * 64) / C4;
-    finish(row, (tid + k * kWaves * 64) % C4, a[k], s_ml[0][row][0], s_ml[0][row][1]);
+    const int row = (tid1 + k * kWaves * 64) / C4;
+    finish(row, (tid1 + k * kWaves * 64) % C4, a[k], s_ml[0][row][0], s_ml[0][row][1]);
   }
 }
 
