@@ -10,11 +10,14 @@ namespace {
 
 using window::exp2_hw;
 
-// One thread per window row and K/V head: the row's weight under every query
-// head of the group, from its kept scores, added to the row's account.
+// The rows' weights under every query head of a K/V head's group, from their kept
+// scores, added to their accounts: a thread takes kAccountRows rows, 256 apart, so
+// that its requests go out together (64 streams of 32 heads over 128 to 3000 rows: one
+// row a thread 23 us, four 10).
+constexpr int kAccountRows = 4;
 __global__ __launch_bounds__(256) void account_kernel(const WindowParams p, float* __restrict__ weights,
                                                       bool fresh) {
-  const uint32_t r = blockIdx.x * 256 + threadIdx.x;
+  const uint32_t r0 = blockIdx.x * (256 * kAccountRows) + threadIdx.x;
   const uint32_t b = blockIdx.z;
   uint32_t len = p.len, start = p.start;
   if (p.lens) {
@@ -23,17 +26,32 @@ __global__ __launch_bounds__(256) void account_kernel(const WindowParams p, floa
     const int32_t st = p.starts[b] % (int32_t)p.M;
     start = (uint32_t)(st < 0 ? st + (int32_t)p.M : st);
   }
-  if (r >= len) return;
+  if (r0 >= len) return;
   const size_t h0 = (size_t)b * p.H + blockIdx.y * p.group;
-  float sum = 0.f;
+  float* w = weights + ((size_t)b * p.KH + blockIdx.y) * p.M;
+  uint32_t slot[kAccountRows];
+  float had[kAccountRows], sum[kAccountRows];
+#pragma unroll
+  for (int k = 0; k < kAccountRows; ++k) {
+    const uint32_t r = r0 + 256 * k;
+    slot[k] = start + r;
+    slot[k] = slot[k] >= p.M ? slot[k] - p.M : slot[k];
+    had[k] = r < len ? w[slot[k]] : 0.f;
+    sum[k] = 0.f;
+  }
   for (uint32_t h = 0; h < p.group; ++h) {
     const float m = p.stats[(h0 + h) * 2], l = p.stats[(h0 + h) * 2 + 1];
-    sum += exp2_hw(p.scores[(h0 + h) * p.score_stride + r] - m) / l;
+#pragma unroll
+    for (int k = 0; k < kAccountRows; ++k) {
+      const uint32_t r = r0 + 256 * k;
+      if (r < len) sum[k] += exp2_hw(p.scores[(h0 + h) * p.score_stride + r] - m) / l;
+    }
   }
-  uint32_t slot = start + r;
-  slot = slot >= p.M ? slot - p.M : slot;
-  float* w = weights + ((size_t)b * p.KH + blockIdx.y) * p.M + slot;
-  *w = fresh && r == len - 1 ? sum : *w + sum;
+#pragma unroll
+  for (int k = 0; k < kAccountRows; ++k) {
+    const uint32_t r = r0 + 256 * k;
+    if (r < len) w[slot[k]] = fresh && r == len - 1 ? sum[k] : had[k] + sum[k];
+  }
 }
 
 __global__ __launch_bounds__(256) void clear_weights_kernel(float* weights, uint64_t units, uint32_t M,
@@ -145,7 +163,7 @@ int launch_window(WindowParams p, WindowMode mode, uint32_t batch, bool bf16, ui
 
 int launch_account(const WindowParams& p, float* weights, uint32_t batch, uint32_t max_rows,
                    bool fresh, hipStream_t stream) {
-  const dim3 grid((max_rows + 255) / 256, p.KH, batch);
+  const dim3 grid((max_rows + 256 * kAccountRows - 1) / (256 * kAccountRows), p.KH, batch);
   hipLaunchKernelGGL(account_kernel, grid, dim3(256), 0, stream, p, weights, fresh);
   STS_HIP(hipGetLastError());
   return STS_OK;

@@ -458,27 +458,31 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
 
   // The draft's relation "is above or is", a bit per node, and the nodes' depths:
   // each node takes over what its jump target knows and jumps as far as that one
-  // does, until none has anywhere left to go.  Up to 64 nodes every wave does it for
-  // itself, in registers; larger drafts go through LDS.
+  // does, until none has anywhere left to go.  Up to 64 nodes a wave does it for
+  // itself, in registers, if it comes to any of the draft's rows; larger drafts go
+  // through LDS.
+  auto narrow_tree = [&]() __attribute__((always_inline)) {
+    uint32_t a0 = lane < 32 ? 1u << lane : 0u, a1 = lane < 32 ? 0u : 1u << (lane - 32);
+    int depth = up >= 0;
+    while (__any(up >= 0)) {
+      const int from = up >= 0 ? up : lane;
+      const uint32_t b0 = __shfl((int)a0, from, 64), b1 = __shfl((int)a1, from, 64);
+      const int deeper = __shfl(depth, from, 64), next = __shfl(up, from, 64);
+      if (up >= 0) {
+        a0 |= b0;
+        a1 |= b1;
+        depth += deeper;
+        up = next;
+      }
+    }
+    s_anc[lane][0] = a0;  // (the waves write the same)
+    s_anc[lane][1] = a1;
+    s_depth[lane] = depth;
+  };
   if constexpr (MODE == kWindowTree) {
     up = me < (int)n && up >= 0 && up < me ? up : -1;
     if (narrow) {
-      uint32_t a0 = lane < 32 ? 1u << lane : 0u, a1 = lane < 32 ? 0u : 1u << (lane - 32);
-      int depth = up >= 0;
-      while (__any(up >= 0)) {
-        const int from = up >= 0 ? up : lane;
-        const uint32_t b0 = __shfl((int)a0, from, 64), b1 = __shfl((int)a1, from, 64);
-        const int deeper = __shfl(depth, from, 64), next = __shfl(up, from, 64);
-        if (up >= 0) {
-          a0 |= b0;
-          a1 |= b1;
-          depth += deeper;
-          up = next;
-        }
-      }
-      s_anc[lane][0] = a0;  // (the waves write the same)
-      s_anc[lane][1] = a1;
-      s_depth[lane] = depth;
+      if (p.rope_cos) narrow_tree();  // (for the depths)
     } else {
       const uint32_t words = (n + 31) / 32;
 #pragma unroll
@@ -567,6 +571,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < CW; ++e) qf[c][e] *= p.qscale;
+  }
+
+  if constexpr (MODE == kWindowTree) {
+    if (narrow && !p.rope_cos && t < t1 && (t + (t1 - 1 - t) / tstep * tstep + 1) * TILE > base) narrow_tree();
   }
 
   // The weights are taken relative to m, which follows the scores' maximum only
@@ -1026,11 +1034,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   __syncthreads();
   if (!s_last) return;
   __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
-  // Each thread's columns of the first four splits, requested before anything else.
-  coh_f4 y[4][NXT];
+  // Each thread's columns of the first splits, requested before anything else.
+  constexpr int AT = R == 1 ? 8 : 4;
+  coh_f4 y[AT][NXT];
   auto request = [&](uint32_t sp) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < AT; ++u)
 #pragma unroll
       for (int k = 0; k < NXT; ++k)  // (past the record: zeros)
         y[u][k] = ld_coherent4(prs, sp + u < nsplit ? (sp + u) * REC * 4 + (tid1 + k * kWaves * 64) * 16 : kOutside);
@@ -1075,10 +1084,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   float4 a[NXT];
 #pragma unroll
   for (int k = 0; k < NXT; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (uint32_t sp = 0; sp < nsplit; sp += 4) {
+  for (uint32_t sp = 0; sp < nsplit; sp += AT) {
     if (sp > 0) request(sp);
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < AT; ++u)
 #pragma unroll
       for (int k = 0; k < NXT; ++k) {
         const float f = sp + u < nsplit ? s_f[sp + u][(tid1 + k * kWaves * 64) / C4] : 0.f;
