@@ -116,7 +116,7 @@ int window_workspace(const WindowParams& p, const WindowPlan& pl, uint32_t batch
   *out = nullptr;
   if (pl.nsplit <= 1) return STS_OK;
   const size_t units = (size_t)batch * p.KH * pl.rblocks;
-  return get_workspace(stream, units * pl.nsplit * pl.record, units, out);
+  return get_workspace(stream, (size_t)pl.shares * pl.rblocks * pl.record, units, out);
 }
 
 }  // namespace
@@ -130,7 +130,11 @@ int check_window(const WindowParams& p, uint32_t batch, bool bf16) {
   STS_CHECK((uint64_t)p.M * p.dh * (bf16 ? 2 : 4) <= 0x7FFFFFF0ull,
             "max_len %u too large for one head's buffer resource", p.M);
   STS_CHECK(batch <= 65535 && p.KH <= 65535, "batch (%u) and kv_heads (%u) must be <= 65535", batch, p.KH);
-  STS_CHECK((uint64_t)p.T * p.H <= 0x7FFFFFFull, "too many query rows (%u x %u)", p.T, p.H);
+  // (The launch counts its threads in 32 bits: 16 rows of a K/V head and up to 128
+  // splits make a workgroup of 256.)
+  STS_CHECK((uint64_t)p.T * p.H <= 0x7FFFFFFull &&
+                ((uint64_t)p.T * (p.H / p.KH) / 16 + 1) * batch * p.KH <= (1u << 23),
+            "too many query rows (%u streams x %u x %u heads)", batch, p.T, p.H);
   return STS_OK;
 }
 
@@ -155,7 +159,9 @@ int launch_window(WindowParams p, WindowMode mode, uint32_t batch, bool bf16, ui
   p.shares = pl.shares;
   p.batch = batch;
   p.rows_factor = pl.rows_factor;
-  const dim3 grid((p.shares + window::kXcds - 1) / window::kXcds * window::kXcds * pl.rblocks);
+  const uint64_t blocks =
+      ((uint64_t)p.shares + window::kXcds - 1) / window::kXcds * window::kXcds * (uint64_t)pl.rblocks;
+  const dim3 grid((uint32_t)blocks);
   if (mode == kWindowTree) return launch_window_tree(p, pl.row_tiles, bf16, grid, stream);
   if (mode == kWindowMasked) return launch_window_masked(p, pl.row_tiles, bf16, grid, stream);
   return launch_window_weights(p, pl.row_tiles, bf16, grid, stream);

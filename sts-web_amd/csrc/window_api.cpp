@@ -352,6 +352,8 @@ int sts_kv_evict(sts_kv_cache* cache, uint64_t keep, uint64_t recent, int32_t* k
   STS_CHECK(recent <= keep, "recent %llu must be at most keep %llu", (unsigned long long)recent,
             (unsigned long long)keep);
   if (!cache->k) return fail(STS_ERR_STATE, "cache has no buffers yet (nothing appended)");
+  if (int rc = sts::check_window(handle_params(cache, nullptr, nullptr, 1), (uint32_t)cache->batch, false))
+    return rc;
   if (cache->len <= keep && !kept) return STS_OK;
   sts::Evict e;
   e.buf[0] = cache->k;

@@ -100,12 +100,6 @@ struct Piece {
       w[1] = x[1];
     }
   }
-  __device__ __forceinline__ void times(float f) {
-    if constexpr (!BF) {
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * f);
-    }
-  }
   __device__ __forceinline__ float operator[](int e) const {
     if constexpr (BF) {
       const uint32_t x = w[e >> 1];
@@ -124,26 +118,23 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // The matrix operands that stand for f32 values x[8].  Against f32 rows: two f16
-// values, each the nearest, off by at most 2^-22 of x, and by 2^-25 where the second
-// falls below f16's normal range; the products of the two second parts are left
-// out.  Against bf16 rows, which are operands as they are: three bf16 values whose
-// sum is x.
+// values of x * scale, each the nearest, off by at most 2^-22 of it, and by 2^-25
+// where the second falls below f16's normal range; the products of the two second
+// parts are left out.  Against bf16 rows, which are operands as they are: three bf16
+// values whose sum is x (scale is not used).
 template <bool BF>
 struct Parts {
   typedef half8 V;
   static constexpr int N = 2;
-  static __device__ __forceinline__ void split(const float* x, V (&y)[N]) {
+  static __device__ __forceinline__ void split(const float* x, float scale, V (&y)[N]) {
     typedef _Float16 half2v __attribute__((ext_vector_type(2)));
     typedef float f2 __attribute__((ext_vector_type(2)));
     u32x4 w[N];  // pairs put together as words: no half moves on its own
-    // A one that the compiler does not know: x * one - h is a single mixed-precision
-    // instruction, x - h a conversion and a subtraction.
-    float one = 1.f;
-    asm("" : "+s"(one));
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const half2v h = __builtin_convertvector((f2){x[e], x[e + 1]}, half2v);
-      const half2v r = __builtin_convertvector((f2){fmaf(x[e], one, -(float)h[0]), fmaf(x[e + 1], one, -(float)h[1])}, half2v);
+      const half2v h = __builtin_convertvector((f2){x[e] * scale, x[e + 1] * scale}, half2v);
+      const half2v r = __builtin_convertvector(
+          (f2){fmaf(x[e], scale, -(float)h[0]), fmaf(x[e + 1], scale, -(float)h[1])}, half2v);
       w[0][e / 2] = __builtin_bit_cast(uint32_t, h);
       w[1][e / 2] = __builtin_bit_cast(uint32_t, r);
     }
@@ -158,7 +149,7 @@ template <>
 struct Parts<true> {
   typedef bf16x8 V;
   static constexpr int N = 3;
-  static __device__ __forceinline__ void split(const float* x, V (&y)[N]) {
+  static __device__ __forceinline__ void split(const float* x, float, V (&y)[N]) {
     typedef __bf16 b2 __attribute__((ext_vector_type(2)));
     typedef float f2 __attribute__((ext_vector_type(2)));
     u32x4 w[N];
@@ -180,34 +171,51 @@ struct Parts<true> {
   }
 };
 
-// The power of two that takes x (positive, finite) to 64..128, within 2^+-60.
-__device__ __forceinline__ float scale_to_64(float x) {
-  const int e = 127 + 6 - ((int)(__float_as_uint(x) >> 23) - 127);
-  return __uint_as_float((uint32_t)min(max(e, 127 - 60), 127 + 60) << 23);
+// The power of two that takes x (positive, finite) to 2^11..2^12, from 2^-117 to 2^110.
+__device__ __forceinline__ float scale_up(float x) {
+  const int e = 127 + 11 - ((int)(__float_as_uint(x) >> 23) - 127);
+  return __uint_as_float((uint32_t)min(max(e, 127 - 117), 127 + 110) << 23);
 }
 
-// What the f32 rows are multiplied by before they are split: 1 where the wave's
-// first tile that holds anything reaches between 1/2 and 2^12, else the power of
-// two that takes its largest value to 64..128.
+// What the f32 rows are multiplied by before they are split: the power of two that
+// takes the largest value of the wave's first tile that holds anything to 2^11..2^12.
 struct TileScale {
   float scale = 1.f, inverse = 1.f;
   bool set = false;
-  __device__ __forceinline__ void choose(float top) {
-    const float all = wave_max(top);
-    if (all > 0.f && all < INFINITY) {  // (outputs of tiles of zeros need no rescaling)
-      const float x = all >= 0.5f && all <= 4096.f ? 1.f : scale_to_64(all);
-      scale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
-      inverse = 1.f / scale;
-      set = true;
+  // Whether N rows, of which this lane holds a part that reaches top[] in magnitude
+  // (NaN and infinity kept; ROW is the lane exchange over the parts of a row), are
+  // held well: all below f16's range, and each with a value of 2^-3 or more, so that
+  // a step of f16's smallest is no more than 2^-22 of it.  A row's parts are put
+  // together only where some part is smaller than that.
+  template <int N, typename ROW>
+  __device__ __forceinline__ bool holds(const float (&top)[N], ROW row) {
+    if (!set) {
+      float all = top[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) all = fmaxf(all, top[i]);
+      all = wave_max(all);
+      if (all > 0.f && all < INFINITY) {  // (outputs of tiles of zeros need no rescaling)
+        scale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(scale_up(all))));
+        inverse = 1.f / scale;
+        set = true;
+      }
     }
-  }
-  // Whether a tile that reaches `top` in magnitude in this lane (NaN and infinity
-  // kept) is held well: all finite, below f16's range, and not so small that its
-  // steps would show.
-  __device__ __forceinline__ bool holds(float top) {
-    if (!set) choose(top);
-    const float t = top * scale;
-    return __all(t < 60000.f) && (__any(t >= 0.25f) || __all(t == 0.f));
+    const float most = 60000.f * inverse, least = 0.125f * inverse;
+    bool fits = true, small = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      fits &= top[i] < most;
+      small |= top[i] < least && top[i] > 0.f;
+    }
+    if (!__all(fits)) return false;
+    if (!__any(small)) return true;
+    small = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float x = row(top[i]);
+      small |= x < least && x > 0.f;
+    }
+    return !__any(small);
   }
 };
 
@@ -264,6 +272,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   const uint32_t turn = blockIdx.x / kXcds, rb = turn % p.rblocks;
   const uint32_t share = turn / p.rblocks * kXcds + blockIdx.x % kXcds;
   uint32_t b, kvh, split, splits;
+  uint32_t first;  // splits of the streams before, each counted once for all heads
   int32_t len_at = (int32_t)p.len, start_at = (int32_t)p.start, count_at = (int32_t)p.T;  // the stream's
   if (p.rows_factor > 0.f) {
     // Windows of different lengths are cut into splits of about the same length:
@@ -298,7 +307,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
     before -= mine;
     b = 63 - __builtin_clzll(__ballot(lane < (int)p.batch && before * p.KH <= share));
     splits = (uint32_t)__builtin_amdgcn_readlane((int)mine, b);
-    const uint32_t at = share - (uint32_t)__builtin_amdgcn_readlane((int)before, b) * p.KH;
+    first = (uint32_t)__builtin_amdgcn_readlane((int)before, b);
+    const uint32_t at = share - first * p.KH;
     kvh = at % p.KH;
     split = at / p.KH;
     len_at = __builtin_amdgcn_readlane(len_at, b);
@@ -310,6 +320,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
     split = share % splits;
     kvh = share / splits % p.KH;
     b = share / splits / p.KH;
+    first = b * splits;
     if (p.lens) {
       len_at = p.lens[b];
       start_at = p.starts[b];
@@ -549,16 +560,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
 #pragma unroll
           for (int e = 0; e < CW; ++e) top = fmaxf(top, fabsf(x[c][e]));
         top = max_xor32(max_xor16(top));
-        sc = top > 0.f && top < INFINITY ? scale_to_64(top) : 1.f;
+        sc = top > 0.f && top < INFINITY ? scale_up(top) : 1.f;
       }
+      if constexpr (BF) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int e = 0; e < CW; ++e) x[c][e] *= BF ? p.qscale : sc;
+          for (int e = 0; e < CW; ++e) x[c][e] *= p.qscale;
+      }
 #pragma unroll
       for (int c = 0; c < NP; ++c) {
         Frag y[P::N];
-        P::split(&x[0][0] + 8 * c, y);
+        P::split(&x[0][0] + 8 * c, sc, y);
 #pragma unroll
         for (int n = 0; n < P::N; ++n) s_q[wave][c][n][lane] = y[n];
       }
@@ -743,34 +756,71 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
       }
   };
 
+  // 16 rows in f32, of which K and V stand in kk[0] and vv[0]; `next` runs when K is
+  // no longer needed.
+  auto in_f32 = [&](uint32_t r0, float oscale, int at, auto next) __attribute__((always_inline)) {
+    const bool partly = partly_seen(r0, 16);
+    f32x4 s[R][1];
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt) s[rt][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+      for (int c = 0; c < NP; ++c) {
+        float x[8];
+        if constexpr (PARTS) {
+          Frag qq[P::N];
+#pragma unroll
+          for (int n = 0; n < P::N; ++n) qq[n] = s_q[rt][c][n][at];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = (float)qq[0][e] + (float)qq[1][e];
+            if constexpr (BF) x[e] += (float)qq[P::N - 1][e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = qf[(c * 8 + e) / CW][(c * 8 + e) % CW];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          s[rt][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[0][(c * 8 + e) / CW][(c * 8 + e) % CW], x[e], s[rt][0],
+                                                          0, 0, 0);
+        if constexpr (PARTS) __builtin_amdgcn_sched_barrier(0);
+      }
+    next();
+    if constexpr (PARTS) {
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) s[rt][0] *= s_qs[rt * 16 + (at & 15)];
+    }
+    weigh(r0, s, partly, at);
+    add_values(r0, vv[0], [&](int rt) { return s[rt][0]; }, oscale, partly, at);
+  };
+
   // Products of parts, as long as the tiles are held well by them: f32 rows within
   // f16's range, and for either type no value that is not finite in a row that some
-  // query does not see.  From the first tile that is not, the wave goes on in f32.
+  // query does not see.  A tile that is not is multiplied in f32.
   // V is requested while K is consumed and the next tile's K while V is: a tile and
   // a half in registers in all, so that two waves fit a SIMD, which measured faster
   // than one wave with 64 query rows and both tiles ahead.
   if constexpr (PARTS) {
-    bool weighed = false;
     f32x4 s[R][KT];
+    for (;;) {
+    bool weighed = false;  // the tile's weights stand in s
     for (; t < t1; t += tstep) {
       const uint32_t r0 = t * TILE;
       const bool partly = partly_seen(r0, TILE);
       const int at = fresh_lane();
       if constexpr (!BF) {
-        float top = 0.f;
+        float top[KT];
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+        for (int kt = 0; kt < KT; ++kt) {
+          top[kt] = 0.f;
 #pragma unroll
           for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int e = 0; e < CW; ++e) top = __builtin_elementwise_maximum(top, fabsf(kk[kt][c][e]));
-        if (!ks.holds(top)) break;
-        if (ks.scale != 1.f) {
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) kk[kt][c].times(ks.scale);
+            for (int e = 0; e < CW; ++e) top[kt] = __builtin_elementwise_maximum(top[kt], fabsf(kk[kt][c][e]));
         }
+        if (!ks.holds(top, [](float x) { return max_xor32(max_xor16(x)); })) break;
       }
 #pragma unroll
       for (int rt = 0; rt < R; ++rt)
@@ -789,7 +839,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = kk[kt][(c * 8 + e) / CW][(c * 8 + e) % CW];
-            P::split(x, kf[kt]);
+            P::split(x, ks.scale, kf[kt]);
           }
         }
 #pragma unroll
@@ -820,14 +870,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
       }
       weigh(r0, s, partly, at);
       if constexpr (!BF) {
-        float top = 0.f;
+        float top[4 * KT];
 #pragma unroll
-        for (int i = 0; i < 4 * KT; ++i)
+        for (int i = 0; i < 4 * KT; ++i) {
+          top[i] = 0.f;
 #pragma unroll
           for (int c = 0; c < NV; ++c)
 #pragma unroll
-            for (int e = 0; e < VW; ++e) top = __builtin_elementwise_maximum(top, fabsf(vv[i / 4][i % 4][c][e]));
-        weighed = !vs.holds(top);
+            for (int e = 0; e < VW; ++e)
+              top[i] = __builtin_elementwise_maximum(top[i], fabsf(vv[i / 4][i % 4][c][e]));
+        }
+        weighed = !vs.holds(top, [](float x) {
+          x = fmaxf(x, xchg<0>(x));
+          x = fmaxf(x, xchg<1>(x));
+          x = fmaxf(x, xchg<2>(x));
+          return fmaxf(x, xchg<3>(x));
+        });
       } else if (partly) {
         bool bad = false;
 #pragma unroll
@@ -837,21 +895,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
         weighed = __any(bad);
       }
       if (weighed) break;
-      if constexpr (!BF) {
-        if (vs.scale != 1.f) {
-#pragma unroll
-          for (int i = 0; i < 4 * KT; ++i)
-#pragma unroll
-            for (int c = 0; c < NV; ++c) vv[i / 4][i % 4][c].times(vs.scale);
-        }
-      }
       Frag pp[R][P::N];
 #pragma unroll
       for (int rt = 0; rt < R; ++rt) {
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = s[rt][e >> 2][e & 3];
-        P::split(x, pp[rt]);
+        P::split(x, 1.f, pp[rt]);
       }
 #pragma unroll
       for (int x = 0; x < NX; ++x) {
@@ -868,7 +918,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
           float y[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) y[k] = vv[k / 4][k % 4][x / VW][x % VW];
-          P::split(y, vf);
+          P::split(y, vs.scale, vf);
 #pragma unroll
           for (int rt = 0; rt < R; ++rt) o[rt][x] = P::mfma(vf[1], pp[rt][0], o[rt][x]);
         }
@@ -880,71 +930,32 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
       }
       load_k((t + tstep) * TILE + 16, kk[1], at);
     }
+    if (t >= t1) break;
+    vs.set = true;  // the outputs' scale stays from here on
+    const int at = fresh_lane();
     if (weighed) {
-      const float oscale = vs.scale;
-      const int at = fresh_lane();
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
         const uint32_t r0 = t * TILE + kt * 16;
         load_v(r0, vv[0], at);
-        add_values(r0, vv[0], [&](int rt) { return s[rt][kt]; }, oscale, partly_seen(r0, 16), at);
+        add_values(r0, vv[0], [&](int rt) { return s[rt][kt]; }, vs.scale, partly_seen(r0, 16), at);
       }
-      t += tstep;
-    }
-  }
-
-  // In f32, 16 rows at a time: one row tile from the start, more from the tile on
-  // that the parts did not hold (which is read again).
-  const float oscale = PARTS ? vs.scale : 1.f;  // carried by the outputs
-  for (uint32_t half = 0; t < t1;) {
-    const uint32_t r0 = t * TILE + half * 16;
-    const bool partly = partly_seen(r0, 16);
-    const int at = fresh_lane();
-    if constexpr (PARTS) {
-      load_k(r0, kk[0], at);
-      load_v(r0, vv[0], at);
-    }
-    f32x4 s[R][1];
-#pragma unroll
-    for (int rt = 0; rt < R; ++rt) s[rt][0] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int rt = 0; rt < R; ++rt)
-#pragma unroll
-      for (int c = 0; c < NP; ++c) {
-        float x[8];
-        if constexpr (PARTS) {
-          Frag qq[P::N];
-#pragma unroll
-          for (int n = 0; n < P::N; ++n) qq[n] = s_q[rt][c][n][at];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] = (float)qq[0][e] + (float)qq[1][e];
-            if constexpr (BF) x[e] += (float)qq[P::N - 1][e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = qf[(c * 8 + e) / CW][(c * 8 + e) % CW];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          s[rt][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[0][(c * 8 + e) / CW][(c * 8 + e) % CW], x[e], s[rt][0],
-                                                          0, 0, 0);
-        if constexpr (PARTS) __builtin_amdgcn_sched_barrier(0);
+    } else {
+      for (uint32_t r0 = t * TILE; r0 < (t + 1) * TILE; r0 += 16) {
+        load_k(r0, kk[0], at);
+        load_v(r0, vv[0], at);
+        in_f32(r0, vs.scale, at, [] {});
       }
-    if constexpr (PARTS) {
-#pragma unroll
-      for (int rt = 0; rt < R; ++rt) s[rt][0] *= s_qs[rt * 16 + (at & 15)];
-    } else {
-      load_k((t + tstep) * TILE, kk[0], at);
     }
-    weigh(r0, s, partly, at);
-    add_values(r0, vv[0], [&](int rt) { return s[rt][0]; }, oscale, partly, at);
-    if constexpr (PARTS) {
-      half ^= 1;
-      if (half == 0) t += tstep;
-    } else {
-      t += tstep;
-      load_v(t * TILE, vv[0], at);
+    t += tstep;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) load_k(t * TILE + kt * 16, kk[kt], at);
+    }
+  } else {
+    for (; t < t1; t += tstep) {
+      const int at = fresh_lane();
+      in_f32(t * TILE, 1.f, at, [&] { load_k((t + tstep) * TILE, kk[0], at); });
+      load_v((t + tstep) * TILE, vv[0], at);
     }
   }
   if constexpr (PARTS) {
@@ -978,7 +989,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   constexpr uint32_t REC = ROWS * (D + 2);  // floats of a split's record: O, then (m, l)
   const size_t unit = ((size_t)b * p.KH + kvh) * p.rblocks + rb;
   const __amdgpu_buffer_rsrc_t prs =
-      coherent_rsrc(p.part + unit * p.nsplit * REC, nsplit > 1 ? p.nsplit * REC * 4 : 0);
+      coherent_rsrc(p.part + (((size_t)first * p.KH + kvh * splits) * p.rblocks + rb * splits) * REC,
+                    nsplit > 1 ? splits * REC * 4 : 0);
   auto finish = [&](uint32_t row, int col, float4 a, float mt, float lt) {
     const uint32_t rr = row0 + row;
     if (rr >= nrows) return;

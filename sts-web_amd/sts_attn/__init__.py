@@ -281,37 +281,38 @@ def prefill_attention_bf16kv(q: torch.Tensor, k16: torch.Tensor, v16: torch.Tens
 # ---------------------------------------------------------------------------
 
 _ROW_TYPES = {torch.float32: ROWS_F32, torch.bfloat16: ROWS_BF16}
+_i32, _f32t = torch.int32, torch.float32
 
 
-def _rows(k_cache: torch.Tensor, v_cache: torch.Tensor):
+def _rows(k: torch.Tensor, v: torch.Tensor):
     """(B, KVH, M, D, row type, device) of K/V caches, after their checks."""
-    shape, dtype, device = k_cache.shape, k_cache.dtype, k_cache.device
-    if dtype not in _ROW_TYPES or v_cache.dtype != dtype:
-        raise TypeError(f"K/V caches must both be float32 or bfloat16, got {dtype}, {v_cache.dtype}")
-    if len(shape) != 4 or v_cache.shape != shape:
+    shape, dtype, device = k.shape, k.dtype, k.device
+    if dtype not in _ROW_TYPES or v.dtype is not dtype:
+        raise TypeError(f"K/V caches must both be float32 or bfloat16, got {dtype}, {v.dtype}")
+    if len(shape) != 4 or v.shape != shape:
         raise ValueError(f"K/V caches must both be [B, KVH, M, D], got {tuple(shape)}, "
-                         f"{tuple(v_cache.shape)}")
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
+                         f"{tuple(v.shape)}")
+    if device.type != "cuda" or device.index != torch._C._cuda_getDevice():
         raise ValueError(f"K/V caches must be on the current GPU, got {device}")
-    _arg(v_cache, "v_cache", dtype, shape, device)
-    if not k_cache.is_contiguous():
-        raise ValueError("k_cache must be contiguous")
-    return (*shape, _ROW_TYPES[dtype], device)
+    if v.device != device or not k.is_contiguous() or not v.is_contiguous():
+        raise ValueError("K/V caches must be contiguous and on one GPU")
+    B, KH, M, D = shape
+    return B, KH, M, D, _ROW_TYPES[dtype], device
 
 
 def _arg(t: Optional[torch.Tensor], name: str, dtype, shape, device) -> Optional[int]:
     """The address of a contiguous tensor of this type, shape and device (None: none)."""
     if t is None:
         return None
-    if t.dtype != dtype:
+    if t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous():
+        return t.data_ptr()
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
+    raise ValueError(f"{name} must be contiguous")
 
 
 def _made_for(stream, *tensors) -> None:
@@ -335,19 +336,22 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     caches [B,KVH,M,D] float32 or bfloat16, parents [B,T] int32 (-1: a child of the
     last committed row), lens/starts/counts [B] int32."""
     B, KH, M, D, rows, dev = _rows(k_cache, v_cache)
-    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:
-        raise ValueError(f"q must be [{B}, T, H, {D}], got {tuple(q.shape)}")
-    T, H = q.shape[1], q.shape[2]
-    qp = _arg(q, "q", torch.float32, q.shape, dev)
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != B or shape[3] != D:
+        raise ValueError(f"q must be [{B}, T, H, {D}], got {tuple(shape)}")
+    T, H = shape[1], shape[2]
+    qp = _arg(q, "q", _f32t, shape, dev)
     if out is None:
         out = torch.empty_like(q)
         _made_for(stream, out)
-    i32 = torch.int32
+        op = out.data_ptr()
+    else:
+        op = _arg(out, "out", _f32t, shape, dev)
+    one = (B,)
     _check(load().sts_tree_attention(
-        qp, k_cache.data_ptr(), v_cache.data_ptr(), _arg(out, "out", torch.float32, q.shape, dev),
-        _arg(parents, "parents", i32, (B, T), dev), _arg(counts, "counts", i32, (B,), dev),
-        _arg(lens, "lens", i32, (B,), dev), _arg(starts, "starts", i32, (B,), dev), B, T, H, KH, D, M,
-        scale, rows, _stream(stream)))
+        qp, k_cache.data_ptr(), v_cache.data_ptr(), op, _arg(parents, "parents", _i32, (B, T), dev),
+        _arg(counts, "counts", _i32, one, dev), _arg(lens, "lens", _i32, one, dev),
+        _arg(starts, "starts", _i32, one, dev), B, T, H, KH, D, M, scale, rows, _stream(stream)))
     return out
 
 
@@ -381,20 +385,24 @@ def masked_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     int32.  softcap > 0 caps the scores at softcap * tanh(x / softcap); slopes [H]
     float32 takes slopes[h] * distance off them.  A query that sees nothing gets 0."""
     B, KH, M, D, rows, dev = _rows(k_cache, v_cache)
-    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:
-        raise ValueError(f"q must be [{B}, S, H, {D}], got {tuple(q.shape)}")
-    S, H = q.shape[1], q.shape[2]
-    qp = _arg(q, "q", torch.float32, q.shape, dev)
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != B or shape[3] != D:
+        raise ValueError(f"q must be [{B}, S, H, {D}], got {tuple(shape)}")
+    S, H = shape[1], shape[2]
+    qp = _arg(q, "q", _f32t, shape, dev)
     if out is None:
         out = torch.empty_like(q)
         _made_for(stream, out)
-    i32 = torch.int32
+        op = out.data_ptr()
+    else:
+        op = _arg(out, "out", _f32t, shape, dev)
+    one, each = (B,), (B, S)
     _check(load().sts_masked_attention(
-        qp, k_cache.data_ptr(), v_cache.data_ptr(), _arg(out, "out", torch.float32, q.shape, dev),
-        _arg(lo, "lo", i32, (B, S), dev), _arg(hi, "hi", i32, (B, S), dev),
-        _arg(slopes, "slopes", torch.float32, (H,), dev), _arg(counts, "counts", i32, (B,), dev),
-        _arg(lens, "lens", i32, (B,), dev), _arg(starts, "starts", i32, (B,), dev), B, S, H, KH, D, M,
-        scale, softcap, rows, _stream(stream)))
+        qp, k_cache.data_ptr(), v_cache.data_ptr(), op, _arg(lo, "lo", _i32, each, dev),
+        _arg(hi, "hi", _i32, each, dev), _arg(slopes, "slopes", _f32t, (H,), dev),
+        _arg(counts, "counts", _i32, one, dev), _arg(lens, "lens", _i32, one, dev),
+        _arg(starts, "starts", _i32, one, dev), B, S, H, KH, D, M, scale, softcap, rows,
+        _stream(stream)))
     return out
 
 
@@ -406,22 +414,26 @@ def decode_ring_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     heads of its K/V head) to weights [B,KVH,M] float32 at the row's slot: q [B,H,D]
     float32, caches [B,KVH,M,D] float32 or bfloat16, lens/starts [B] int32."""
     B, KH, M, D, rows, dev = _rows(k_cache, v_cache)
-    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D:
-        raise ValueError(f"q must be [{B}, H, {D}], got {tuple(q.shape)}")
-    H = q.shape[1]
-    qp = _arg(q, "q", torch.float32, q.shape, dev)
-    lib = load()
-    scratch = torch.empty(lib.sts_decode_ring_weights_scratch(B, H, M), dtype=torch.float32, device=dev)
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != B or shape[2] != D:
+        raise ValueError(f"q must be [{B}, H, {D}], got {tuple(shape)}")
+    H = shape[1]
+    qp = _arg(q, "q", _f32t, shape, dev)
+    # sts_decode_ring_weights_scratch floats: whole tiles of 16 scores and two
+    # statistics for each head of each stream.
+    scratch = torch.empty(B * H * ((M + 15) // 16 * 16 + 2), dtype=_f32t, device=dev)
     if out is None:
         out = torch.empty_like(q)
         _made_for(stream, out)
+        op = out.data_ptr()
+    else:
+        op = _arg(out, "out", _f32t, shape, dev)
     _made_for(stream, scratch)
-    i32 = torch.int32
-    _check(lib.sts_decode_ring_weights(
-        qp, k_cache.data_ptr(), v_cache.data_ptr(), _arg(out, "out", torch.float32, q.shape, dev),
-        _arg(weights, "weights", torch.float32, (B, KH, M), dev), scratch.data_ptr(),
-        _arg(lens, "lens", i32, (B,), dev), _arg(starts, "starts", i32, (B,), dev), B, H, KH, D, M,
-        scale, rows, _stream(stream)))
+    one = (B,)
+    _check(load().sts_decode_ring_weights(
+        qp, k_cache.data_ptr(), v_cache.data_ptr(), op, _arg(weights, "weights", _f32t, (B, KH, M), dev),
+        scratch.data_ptr(), _arg(lens, "lens", _i32, one, dev), _arg(starts, "starts", _i32, one, dev),
+        B, H, KH, D, M, scale, rows, _stream(stream)))
     return out
 
 

@@ -157,6 +157,54 @@ def test_tree_magnitudes(gpu, T, kind, dtype):
         close(got[0], want, bound, which)
 
 
+@pytest.mark.parametrize("size", [1e30, 1e22, 1e-30])
+@pytest.mark.parametrize("T", [8, 30])
+def test_tree_query_magnitudes(gpu, T, size):
+    """Queries of any size against keys that keep the scores moderate."""
+    L, D = 200, 64
+    w = Window(17, 1, 1, 200, D, [L])
+    w.k = w.k / np.float32(size)
+    q = queries(w.rng, 1, T, 2, D) * np.float32(size)
+    parents = random_tree(w.rng, T, T)
+    got = run_tree(w, q, parents[None], None, scale_for(D))
+    want, _, bound = attend64(q[0], w.rows(0, w.k), w.rows(0, w.v), tree_seen(parents, T, L), scale_for(D))
+    close(got[0], want, bound, "queries")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,H,KH,T", [(64, 4, 2, 3), (65, 4, 2, 3), (2, 12, 1, 6), (130, 2, 2, 1)])
+def test_streams_of_very_different_lengths(gpu, B, H, KH, T, dtype):
+    """One long window among short and empty ones: splits by the rows of all of them
+    (up to 64 streams) or the same for each; drafts, kept weights, single tokens."""
+    M, D = 3000, 64
+    rng = np.random.default_rng(B)
+    lens = rng.integers(0, 40, B)
+    lens[B // 2], lens[0] = M, 0
+    w = Window(B, B, KH, M, D, lens, dtype)
+    q = queries(w.rng, B, T, H, D)
+    n = np.minimum(lens, T)
+    parents = np.stack([random_tree(w.rng, c, T) for c in n])
+    got = run_tree(w, q, parents, None, 0.125)
+    one = run_masked(w, q[:, :1].copy(), 0.125, lo=np.maximum(lens - 1500, 0)[:, None])
+    k, v, dl, ds = w.dev("k", "v", "lens", "starts")
+    acc = torch.zeros((B, KH, M), device="cuda")
+    dec = sts_attn.decode_ring_weights(torch.from_numpy(q[:, 0].copy()).cuda(), k, v, acc, dl, ds, 0.125)
+    dec, acc = dec.cpu().numpy(), acc.cpu().numpy()
+    for b in range(B):
+        L = int(lens[b])
+        if L == 0:
+            assert not got[b].any() and not one[b].any() and not dec[b].any() and not acc[b].any()
+            continue
+        kk, vv = w.rows(b, w.k), w.rows(b, w.v)
+        want, _, bound = attend64(q[b, :n[b]], kk, vv, tree_seen(parents[b], n[b], L), 0.125)
+        close(got[b, :n[b]], want, bound, f"draft {b}")
+        want, p, bound = attend64(q[b, :1], kk, vv, np.ones((1, L), bool), 0.125)
+        close(dec[b], want[0], bound[0], f"decode {b}")
+        assert np.allclose(acc[b].sum(-1), H // KH, rtol=1e-4)
+        want, _, bound = attend64(q[b, :1], kk, vv, (np.arange(L) >= L - 1500)[None], 0.125)
+        close(one[b], want, bound, f"window {b}")
+
+
 def test_tree_visible_infinite_value(gpu):
     """An infinite V element reaches exactly the nodes and dims that see it."""
     T, L, D = 10, 40, 64

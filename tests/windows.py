@@ -50,15 +50,15 @@ def attend64(q, k, v, seen, scale, softcap=0.0, slopes=None, w=None):
     """q [n,H,D], k/v [KH,L,D], seen [n,L] -> (out [n,H,D], p [n,H,L], bound [n,H]).
 
     bound: of an evaluation whose products are f32's or those of two f16 parts (off
-    by 4 u of the element each, by 4 u of the product for the parts left out, and by
-    2 u of the largest element of the tile where the second part is below f16's
-    normal range).  A score, a sum of D products with two scalings, is then off by
-    at most scale ((D + 16) u sum |q k| + 2 u sum |q| max |k| + 2 u sum |k| max |q|).
-    The cap's tanh, within 3 u relative, and the bias add 8 u of their size.  A score
-    off by e turns its weight by the factor 1 +- (e + 3u) (the base-2 exponential of
-    the hardware within 2 u), the normalised sum by twice that; the weights' and
-    values' own parts add 16 u, and adding up L weighted rows (L + 8) u, all of the
-    largest |v|."""
+    by 4 u of the element, or of its row's largest where the second part is below
+    f16's normal range, and by 4 u of the product for the parts left out).  A score, a
+    sum of D products with two scalings, is then off by at most
+    scale ((D + 16) u sum |q k| + 4 u sum |q| max |k| + 4 u sum |k| max |q|) with the
+    maxima of its own rows.  The cap's tanh, within 3 u relative, and the bias add 8 u
+    of their size.  A score off by e turns its weight by the factor 1 +- (e + 3u) (the
+    base-2 exponential of the hardware within 2 u), the normalised sum by twice that;
+    the weights' and values' own parts add 16 u, and adding up L weighted rows (L + 8)
+    u, all of the largest |v|."""
     n, H, D = q.shape
     g = H // k.shape[0]
     L = k.shape[1]
@@ -74,7 +74,7 @@ def attend64(q, k, v, seen, scale, softcap=0.0, slopes=None, w=None):
             qi = q[i, h].astype(np.float64)
             s = kk[at] @ qi * scale
             ka, qa = np.abs(kk[at]), np.abs(qi)
-            big = (ka @ qa * (D + 16) + 2 * qa.sum() * ka.max() + 2 * ka.sum(1) * qa.max()) * abs(scale) * U
+            big = (ka @ qa * (D + 16) + 4 * qa.sum() * ka.max(1) + 4 * ka.sum(1) * qa.max()) * abs(scale) * U
             if softcap > 0:
                 s = softcap * np.tanh(s / softcap)
                 big = big + 8 * U * np.abs(s)
