@@ -99,7 +99,9 @@ __device__ __forceinline__ float wave_sum(float x) {
 // PAD: a head dim below D (a multiple of 4, p.head_dim) on the D-wide lane
 // layout: the lanes past it load zeros, so they add nothing to the scores or
 // the weighted sums, and store nothing.
-template <int D, int WAVES, bool PAD = false>
+// KEEP: the rows' scores and the heads' maximum and sum also go to p.scores and
+// p.stats.
+template <int D, int WAVES, bool PAD = false, bool KEEP = false>
 __global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p) {
   constexpr int G = D / 4;
   constexpr int NG = 64 / G;
@@ -249,6 +251,9 @@ __global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p
       s[j] = q4.x * kk[j].x + q4.y * kk[j].y + q4.z * kk[j].z + q4.w * kk[j].w;
     float sc = reduce_rows<G>(s, c);
     const uint32_t my_row = r0 + jj * NG + g;
+    if constexpr (KEEP) {
+      if ((c & 3) == 0 && my_row < len) p.scores[((size_t)b * p.H + h) * p.score_stride + my_row] = sc;
+    }
     sc = my_row < len ? sc : -INFINITY;
     const float mn = fmaxf(m, group_max<G>(sc));
     const float alpha = fast_exp2(m - mn);
@@ -401,7 +406,17 @@ __global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p
     a4.w += fw[w] * x.w;
   }
 
+  // The maximum and sum of the head, from the lane that knows them.
+  auto keep_stats = [&](float m_all, float l_all) {
+    if constexpr (KEEP) {
+      if (lane == 0) {
+        p.stats[((size_t)b * p.H + h) * 2] = m_all;
+        p.stats[((size_t)b * p.H + h) * 2 + 1] = l_all;
+      }
+    }
+  };
   if (nsplit == 1) {
+    keep_stats(m_t, l_t);
     if (lane < C4 && (!PAD || (uint32_t)col * 4 < dh))
       st4(outp + col * 4, make_float4(a4.x / l_t, a4.y / l_t, a4.z / l_t, a4.w / l_t));
     return;
@@ -478,6 +493,7 @@ __global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p
       fl[t] = fast_exp2(mu[t] - mg);  // 0 for the lanes past nsplit (m = -FLT_MAX)
       l += fl[t] * lu[t];
     }
+    keep_stats(mg, l);
     float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < kPass; ++i) {
@@ -512,6 +528,7 @@ __global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p
   mg = fmaxf(mg, xor32(mg));
   const float fl = fast_exp2(ms - mg);
   const float l = wave_sum(lane < (int)nsplit ? fl * ls : 0.f);
+  keep_stats(mg, l);
   float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
   for (uint32_t s0 = 0; s0 < nsplit; s0 += NG2 * kPass) {
     if (s0 > 0) fetch(s0);
@@ -608,35 +625,44 @@ int check_decode(const DecodeParams& p, uint32_t batch, uint32_t head_dim) {
   return STS_OK;
 }
 
+template <bool KEEP>
+void launch_instance(const DecodeParams& p, const DecodePlan& pl, dim3 grid, uint32_t head_dim,
+                     hipStream_t stream) {
+  const bool one = pl.waves == 1;
+  const dim3 block(one ? 64 : 256);
+  if (head_dim == 128) {
+    if (one)
+      hipLaunchKernelGGL((decode_kernel<128, 1, false, KEEP>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((decode_kernel<128, 4, false, KEEP>), grid, block, 0, stream, p);
+  } else if (head_dim == 64) {
+    if (one)
+      hipLaunchKernelGGL((decode_kernel<64, 1, false, KEEP>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((decode_kernel<64, 4, false, KEEP>), grid, block, 0, stream, p);
+  } else if (head_dim < 64) {
+    if (one)
+      hipLaunchKernelGGL((decode_kernel<64, 1, true, KEEP>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((decode_kernel<64, 4, true, KEEP>), grid, block, 0, stream, p);
+  } else {
+    if (one)
+      hipLaunchKernelGGL((decode_kernel<128, 1, true, KEEP>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((decode_kernel<128, 4, true, KEEP>), grid, block, 0, stream, p);
+  }
+}
+
 int launch_planned(DecodeParams p, const DecodePlan& pl, uint32_t batch, uint32_t head_dim,
                    hipStream_t stream) {
   p.chunk = pl.chunk;
   p.nsplit_max = pl.nsplit;
   p.head_dim = head_dim;
   const dim3 grid(pl.nsplit, p.H, batch);
-  const bool one = pl.waves == 1;
-  const dim3 block(one ? 64 : 256);
-  if (head_dim == 128) {
-    if (one)
-      hipLaunchKernelGGL((decode_kernel<128, 1>), grid, block, 0, stream, p);
-    else
-      hipLaunchKernelGGL((decode_kernel<128, 4>), grid, block, 0, stream, p);
-  } else if (head_dim == 64) {
-    if (one)
-      hipLaunchKernelGGL((decode_kernel<64, 1>), grid, block, 0, stream, p);
-    else
-      hipLaunchKernelGGL((decode_kernel<64, 4>), grid, block, 0, stream, p);
-  } else if (head_dim < 64) {
-    if (one)
-      hipLaunchKernelGGL((decode_kernel<64, 1, true>), grid, block, 0, stream, p);
-    else
-      hipLaunchKernelGGL((decode_kernel<64, 4, true>), grid, block, 0, stream, p);
-  } else {
-    if (one)
-      hipLaunchKernelGGL((decode_kernel<128, 1, true>), grid, block, 0, stream, p);
-    else
-      hipLaunchKernelGGL((decode_kernel<128, 4, true>), grid, block, 0, stream, p);
-  }
+  if (p.scores)
+    launch_instance<true>(p, pl, grid, head_dim, stream);
+  else
+    launch_instance<false>(p, pl, grid, head_dim, stream);
   STS_HIP(hipGetLastError());
   return STS_OK;
 }

@@ -50,6 +50,12 @@ struct DecodeParams {
   // len + b * len_step rows and its RoPE position is rope_pos + b * len_step
   // (the queries of a causal chunk as streams over one cache: kv_bstride 0).
   uint32_t len_step = 0;
+  // With scores set, the scores of the window's rows in units of log2(e),
+  // [B][H][score_stride], and each head's maximum and sum of 2^(score - maximum),
+  // [B][H][2], are kept (heads with a window only).
+  float* scores = nullptr;
+  float* stats = nullptr;
+  uint32_t score_stride = 0;
 };
 
 // scale * log2(e), the factor the decode and prefill kernels fold into q.

@@ -62,20 +62,44 @@ int check_rope(const sts_rope* rope, const sts_kv_cache* c, uint64_t rows) {
 namespace sts {
 namespace kv {
 
+// One token a stream with the scores kept: where every head has K and V rows of its
+// own, in f32, the decode kernel, which has no matrix tile to leave 15/16 empty (32 heads
+// of 3000 rows 17.5 us against 22, 64 such streams 550 against 577; on a handle it
+// also rotates and appends the token's rows, a launch less); else the window kernel,
+// which reads the rows of a group of heads, or bf16 rows, once.
+static bool by_decode(const WindowParams& p, bool bf16) { return p.group == 1 && !bf16; }
+
+static DecodeParams decode_params(const WindowParams& p) {
+  DecodeParams d;
+  d.q = p.q;
+  d.k = static_cast<const float*>(p.k);
+  d.v = static_cast<const float*>(p.v);
+  d.out = p.out;
+  d.rope_cos = p.rope_cos;
+  d.rope_sin = p.rope_sin;
+  d.rope_pos = p.rope_pos;
+  d.lens = p.lens;
+  d.starts = p.starts;
+  d.len = p.len;
+  d.start = p.start;
+  d.H = p.H;
+  d.M = p.M;
+  d.q_bstride = d.out_bstride = d.kn_bstride = (uint64_t)p.H * p.dh;
+  d.kv_hstride = (uint64_t)p.M * p.dh;
+  d.kv_bstride = (uint64_t)p.H * p.M * p.dh;
+  d.scale_log2 = p.qscale;
+  d.scores = p.scores;
+  d.stats = p.stats;
+  d.score_stride = p.score_stride;
+  return d;
+}
+
 int decode_keeping_weights(const sts_kv_cache* c, const sts_kv_cache* next, const sts_rope* rope,
                            const float* q, const float* k_new, const float* v_new, float* out,
                            float scale, hipStream_t stream) {
   WindowParams p = handle_params(next, q, out, 1);
   const uint32_t batch = (uint32_t)c->batch, max_len = (uint32_t)c->max_len;
   if (int rc = check_window(p, batch, false)) return rc;
-  if (int rc = reserve_window(p, kWindowWeights, batch, false, p.len, stream)) return rc;
-  if (k_new) {
-    const uint32_t pos = (uint32_t)(c->offset % c->max_len);
-    if (int rc = launch_kv_append(k_new, v_new, c->k, c->v, pos, batch, 1, p.KH, p.dh, max_len,
-                                  rope ? rope->cos_t : nullptr, rope ? rope->sin_t : nullptr,
-                                  (uint32_t)c->offset, c->k16, c->v16, stream))
-      return rc;
-  }
   if (rope) {
     p.rope_cos = rope->cos_t;
     p.rope_sin = rope->sin_t;
@@ -85,7 +109,28 @@ int decode_keeping_weights(const sts_kv_cache* c, const sts_kv_cache* next, cons
   p.score_stride = (uint32_t)score_stride(max_len);
   p.scores = c->scores;
   p.stats = c->scores + (uint64_t)batch * p.H * p.score_stride;
-  if (int rc = launch_window(p, kWindowWeights, batch, false, p.len, stream)) return rc;
+  if (by_decode(p, false)) {
+    DecodeParams d = decode_params(p);
+    if (k_new) {
+      d.k_new = k_new;
+      d.v_new = v_new;
+      d.k_wr = c->k;
+      d.v_wr = c->v;
+      d.k16_wr = c->k16;
+      d.v16_wr = c->v16;
+    }
+    if (int rc = launch_decode(d, batch, p.dh, p.len, stream)) return rc;
+  } else {
+    if (int rc = reserve_window(p, kWindowWeights, batch, false, p.len, stream)) return rc;
+    if (k_new) {
+      const uint32_t pos = (uint32_t)(c->offset % c->max_len);
+      if (int rc = launch_kv_append(k_new, v_new, c->k, c->v, pos, batch, 1, p.KH, p.dh, max_len,
+                                    rope ? rope->cos_t : nullptr, rope ? rope->sin_t : nullptr,
+                                    (uint32_t)c->offset, c->k16, c->v16, stream))
+        return rc;
+    }
+    if (int rc = launch_window(p, kWindowWeights, batch, false, p.len, stream)) return rc;
+  }
   return launch_account(p, c->weights, batch, p.len, k_new != nullptr, stream);
 }
 
@@ -201,9 +246,14 @@ int sts_decode_ring_weights(const float* q, const void* k_cache, const void* v_c
   p.score_stride = (uint32_t)score_stride(max_len);
   p.scores = scratch;
   p.stats = scratch + (uint64_t)batch * heads * p.score_stride;
-  if (int rc = sts::launch_window(p, sts::kWindowWeights, batch, row_type == STS_ROWS_BF16, max_len,
-                                  as_stream(stream)))
+  const bool bf16 = row_type == STS_ROWS_BF16;
+  if (int rc = sts::check_window(p, batch, bf16)) return rc;
+  if (sts::kv::by_decode(p, bf16)) {
+    if (int rc = sts::launch_decode(sts::kv::decode_params(p), batch, head_dim, max_len, as_stream(stream)))
+      return rc;
+  } else if (int rc = sts::launch_window(p, sts::kWindowWeights, batch, bf16, max_len, as_stream(stream))) {
     return rc;
+  }
   return sts::launch_account(p, weights, batch, max_len, false, as_stream(stream));
 }
 

@@ -432,6 +432,12 @@ WEIGHTS = [
     (1, 72, 1, 128, 150, [149], F32),     # more heads than a block's rows
     (2, 20, 1, 80, 333, [332, 16], BF16),
     (1, 6, 3, 12, 77, [70], F32),
+    # every head its own rows: head dims between, long windows in many parts
+    (3, 5, 5, 40, 700, [700, 1, 33], F32),
+    (1, 2, 2, 100, 4100, [4099], F32),
+    (1, 1, 1, 128, 20001, [20000], F32),
+    (2, 2, 2, 64, 9000, [8999, 17], F32),
+    (70, 1, 1, 4, 65, [(7 * i) % 66 for i in range(70)], F32),
 ]
 
 
