@@ -234,7 +234,10 @@ int sts_prefill_attention_bf16kv(const float* q, const uint16_t* k16, const uint
  * with values outside their ranges clamped on the device as there.  Query head
  * h reads K/V head h / (heads / kv_heads); q and out are f32, and so is the
  * arithmetic for either row type.  One head's rows take less than 2 GiB.  What
- * a query does not see has no influence on it, whatever values are there.
+ * a query does not see has no influence on it beyond the rounding of f32, whatever
+ * values are there.  Queries, K and V of up to 1e30 in magnitude are served; where
+ * a query sees an infinity or NaN its outputs follow f32 arithmetic over f32 rows and
+ * are undefined over bf16 rows.
  * Splits use the per-(device, stream) workspace as sts_decode_ring does.
  */
 enum sts_row_type {
@@ -285,7 +288,7 @@ int sts_tree_commit(void* k_cache, void* v_cache, const int32_t* path, const int
  *   prefix           hi = max(w + 1, prefix rows)
  *   sliding window   lo = w + 1 - width
  * Its score of row r is x = scale * q . k; with softcap > 0
- * x = softcap * tanh(x / softcap); with slopes [heads] (device, or NULL) then
+ * x = softcap * tanh(x / softcap) (softcap at most 2^100 |scale|); with slopes [heads] (device, or NULL) then
  * x -= slopes[head] * |w - r|.  A query that sees nothing gets zeros, and so do
  * the rows of out [batch][seq][heads][head_dim] from counts[b] on.
  */

@@ -90,7 +90,8 @@ WindowPlan plan_window(const WindowParams& p, WindowMode mode, uint32_t batch, b
   // A split is worth its record from a tile for each of its waves on.
   const uint64_t most = std::min<uint64_t>((max_rows + tile * window::kWaves - 1) / (tile * window::kWaves),
                                            window::max_splits(pl.row_tiles));
-  if ((mode != kWindowMasked || p.T == 1) && batch > 1 && batch <= 64) {
+  // (The kernel adds up the streams' rows in 32 bits.)
+  if ((mode != kWindowMasked || p.T == 1) && batch > 1 && batch <= 64 && (uint64_t)batch * p.M >> 32 == 0) {
     // Streams of different ages: splits of about equal length whatever their stream,
     // not more than fit at once where one round can hold them (rounding up gives each
     // window half a split more).  Products in several rounds end more evenly with

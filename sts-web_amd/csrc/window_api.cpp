@@ -218,6 +218,9 @@ int sts_masked_attention(const float* q, const void* k_cache, const void* v_cach
     p.cap_log2 = sts::softmax_scale_log2(softcap);
     STS_CHECK(std::isfinite(p.qscale) && std::isfinite(p.cap_log2) && p.cap_log2 > 0.f,
               "scale / softcap out of range");
+    // Below, terms of q . k in units of the cap would fall under f32's range.
+    STS_CHECK(scale == 0.f || std::fabs(p.qscale) >= 0x1p-100f,
+              "softcap %g too large for the scale %g (2^100 times at most)", softcap, scale);
   }
   return sts::launch_window(p, sts::kWindowMasked, batch, row_type == STS_ROWS_BF16, max_len,
                             as_stream(stream));

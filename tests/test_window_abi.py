@@ -76,6 +76,8 @@ def test_masked_refusals():
     assert "softcap" in _err(masked(cap=float("nan")))
     assert "softcap" in _err(masked(cap=float("inf")))
     assert "softcap" in _err(masked(cap=1e-44, scale=1.0))  # scale / softcap is not finite
+    assert "softcap" in _err(masked(cap=2e30, scale=1.0))  # scale / softcap below 2^-100
+    assert "softcap" in _err(masked(cap=-1.0, scale=0.0))
     assert "empty" in _err(masked(seq=0))
     assert "too many" in _err(masked(seq=1 << 28, heads=8, kv_heads=8))
 

@@ -655,3 +655,25 @@ def test_binding_refuses_on_the_gpu(gpu):
             sts_attn.evict_ring(k, v, torch.zeros((2, 2, 50), device="cuda"), dl, ds, keep, recent)
     with pytest.raises(sts_attn.StsError, match="aligned"):
         sts_attn.tree_attention(torch.zeros(2 * 4 * 2 * 64 + 1, device="cuda")[1:].view(2, 4, 2, 64), k, v, p, dl, ds, 0.1)
+
+
+def test_rows_of_all_streams_past_32_bits(gpu):
+    """33 streams whose windows hold more than 2^32 rows together, 4 dims each: the
+    splits cover every row (69 GB, K and V the same, of ones: the mean is one)."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GB")
+    B, M = 33, 0x7FFFFFF0 // 16
+    lens = torch.full((B,), M, dtype=torch.int32, device="cuda")
+    starts = torch.arange(B, dtype=torch.int32, device="cuda") * 1000
+    assert B * M > 2 ** 32
+    k = torch.ones((B, 1, M, 4), device="cuda")
+    q = torch.randn((B, 1, 1, 4), device="cuda")
+    parents = torch.full((B, 1), -1, dtype=torch.int32, device="cuda")
+    for run in (lambda out: sts_attn.tree_attention(q, k, k, parents, lens, starts, 0.5, out=out),
+                lambda out: sts_attn.masked_attention(q, k, k, lens, starts, 0.5, out=out)):
+        out = torch.full((B, 1, 1, 4), float("nan"), device="cuda")
+        run(out)
+        # Every weight is the same: sums of equal terms, in chains of at most 2^17.
+        assert (out - 1).abs().max().item() <= 2.0 ** 17 * 2.0 ** -24
+    del k
+    torch.cuda.empty_cache()
