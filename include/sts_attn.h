@@ -399,8 +399,7 @@ int sts_kv_create(uint64_t max_len, uint64_t heads, uint64_t head_dim, sts_kv_ca
  * A mirrored cache needs 16-byte aligned inputs in sts_kv_update.
  * STS_KV_WEIGHTS: the handle keeps, for every slot and K/V head, the attention
  * weight its row was given by sts_kv_attend and sts_kv_decode_step (summed over
- * the heads of the group, as sts_decode_ring_weights does; these two then read
- * the window with that call's kernel), for sts_kv_evict.  A row appended through
+ * the heads of the group, as sts_decode_ring_weights does), for sts_kv_evict.  A row appended through
  * the handle starts at zero; the attention of sts_kv_prefill and
  * sts_kv_tree_step is not counted, and rows entered by sts_kv_advance keep what
  * their slots had.  Query heads are set before the first use.
