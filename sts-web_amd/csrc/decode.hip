@@ -26,12 +26,12 @@
 #include "decode.hpp"
 #include "lane.hpp"
 #include "rope.hpp"
+#include "score.hpp"
 
 namespace sts {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxSplits = 64;  // splits per (stream, head), bounded by the merge's LDS
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -99,9 +99,11 @@ __device__ __forceinline__ float wave_sum(float x) {
 // PAD: a head dim below D (a multiple of 4, p.head_dim) on the D-wide lane
 // layout: the lanes past it load zeros, so they add nothing to the scores or
 // the weighted sums, and store nothing.
-// KEEP: the rows' scores and the heads' maximum and sum also go to p.scores and
-// p.stats.
-template <int D, int WAVES, bool PAD = false, bool KEEP = false>
+// MODE kDecodeKeep: the rows' scores and the heads' maximum and sum also go to
+// p.scores and p.stats.  kDecodeMasked: the window is cut to the rows p.lo..p.hi,
+// and the scores are capped and biased.
+enum DecodeMode { kDecodePlain, kDecodeKeep, kDecodeMasked };
+template <int D, int WAVES, bool PAD = false, DecodeMode MODE = kDecodePlain>
 __global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p) {
   constexpr int G = D / 4;
   constexpr int NG = 64 / G;
@@ -120,6 +122,15 @@ __global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p
   const int c = lane % G;
   const uint32_t split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
 
+  // (Requested before the first of them is used.)
+  int32_t count_at = 1, lo_at = 0, hi_at = INT32_MAX;
+  float slope = 0.f;
+  if constexpr (MODE == kDecodeMasked) {
+    if (p.counts) count_at = p.counts[b];
+    if (p.lo) lo_at = p.lo[b];
+    if (p.hi) hi_at = p.hi[b];
+    if (p.slopes) slope = p.slopes[h] * kLog2e;
+  }
   uint32_t len, start;
   if (p.lens) {
     const int32_t L = p.lens[b];
@@ -129,6 +140,15 @@ __global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p
   } else {
     len = p.len + (PAD ? b * p.len_step : 0u);
     start = p.start;
+  }
+  uint32_t newest = 0;  // the query's distance to the first row that it may see
+  if constexpr (MODE == kDecodeMasked) {
+    if (count_at <= 0) len = 0;
+    const uint32_t hi = min((uint32_t)max(hi_at, 0), len), lo = (uint32_t)max(lo_at, 0);
+    newest = len - 1 - lo;
+    len = lo < hi ? hi - lo : 0u;
+    start += len ? lo : 0u;  // both below M, which is below 2^29
+    start = start >= p.M ? start - p.M : start;
   }
 
   const uint32_t dh = PAD ? p.head_dim : (uint32_t)D;  // the head dim in memory
@@ -251,7 +271,11 @@ __global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p
       s[j] = q4.x * kk[j].x + q4.y * kk[j].y + q4.z * kk[j].z + q4.w * kk[j].w;
     float sc = reduce_rows<G>(s, c);
     const uint32_t my_row = r0 + jj * NG + g;
-    if constexpr (KEEP) {
+    if constexpr (MODE == kDecodeMasked) {
+      if (p.cap_log2 > 0.f) sc = p.cap_log2 * tanh_rel(sc);
+      if (p.slopes) sc -= slope * (float)(int)(newest - my_row);
+    }
+    if constexpr (MODE == kDecodeKeep) {
       if ((c & 3) == 0 && my_row < len) p.scores[((size_t)b * p.H + h) * p.score_stride + my_row] = sc;
     }
     sc = my_row < len ? sc : -INFINITY;
@@ -408,7 +432,7 @@ __global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p
 
   // The maximum and sum of the head, from the lane that knows them.
   auto keep_stats = [&](float m_all, float l_all) {
-    if constexpr (KEEP) {
+    if constexpr (MODE == kDecodeKeep) {
       if (lane == 0) {
         p.stats[((size_t)b * p.H + h) * 2] = m_all;
         p.stats[((size_t)b * p.H + h) * 2 + 1] = l_all;
@@ -625,31 +649,31 @@ int check_decode(const DecodeParams& p, uint32_t batch, uint32_t head_dim) {
   return STS_OK;
 }
 
-template <bool KEEP>
+template <DecodeMode MODE>
 void launch_instance(const DecodeParams& p, const DecodePlan& pl, dim3 grid, uint32_t head_dim,
                      hipStream_t stream) {
   const bool one = pl.waves == 1;
   const dim3 block(one ? 64 : 256);
   if (head_dim == 128) {
     if (one)
-      hipLaunchKernelGGL((decode_kernel<128, 1, false, KEEP>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((decode_kernel<128, 1, false, MODE>), grid, block, 0, stream, p);
     else
-      hipLaunchKernelGGL((decode_kernel<128, 4, false, KEEP>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((decode_kernel<128, 4, false, MODE>), grid, block, 0, stream, p);
   } else if (head_dim == 64) {
     if (one)
-      hipLaunchKernelGGL((decode_kernel<64, 1, false, KEEP>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((decode_kernel<64, 1, false, MODE>), grid, block, 0, stream, p);
     else
-      hipLaunchKernelGGL((decode_kernel<64, 4, false, KEEP>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((decode_kernel<64, 4, false, MODE>), grid, block, 0, stream, p);
   } else if (head_dim < 64) {
     if (one)
-      hipLaunchKernelGGL((decode_kernel<64, 1, true, KEEP>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((decode_kernel<64, 1, true, MODE>), grid, block, 0, stream, p);
     else
-      hipLaunchKernelGGL((decode_kernel<64, 4, true, KEEP>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((decode_kernel<64, 4, true, MODE>), grid, block, 0, stream, p);
   } else {
     if (one)
-      hipLaunchKernelGGL((decode_kernel<128, 1, true, KEEP>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((decode_kernel<128, 1, true, MODE>), grid, block, 0, stream, p);
     else
-      hipLaunchKernelGGL((decode_kernel<128, 4, true, KEEP>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((decode_kernel<128, 4, true, MODE>), grid, block, 0, stream, p);
   }
 }
 
@@ -660,9 +684,11 @@ int launch_planned(DecodeParams p, const DecodePlan& pl, uint32_t batch, uint32_
   p.head_dim = head_dim;
   const dim3 grid(pl.nsplit, p.H, batch);
   if (p.scores)
-    launch_instance<true>(p, pl, grid, head_dim, stream);
+    launch_instance<kDecodeKeep>(p, pl, grid, head_dim, stream);
+  else if (p.masked)
+    launch_instance<kDecodeMasked>(p, pl, grid, head_dim, stream);
   else
-    launch_instance<false>(p, pl, grid, head_dim, stream);
+    launch_instance<kDecodePlain>(p, pl, grid, head_dim, stream);
   STS_HIP(hipGetLastError());
   return STS_OK;
 }
@@ -735,7 +761,15 @@ int launch_decode(DecodeParams p, uint32_t batch, uint32_t head_dim, uint32_t ma
   const uint64_t units = (uint64_t)batch * p.H;
   if (units == 0) return STS_OK;
   if (int rc = check_decode(p, batch, head_dim)) return rc;
-  const DecodePlan pl = plan_decode(units, max_rows);
+  DecodePlan pl = plan_decode(units, max_rows);
+  // Ranges are often far shorter than max_rows, and splits without rows cost their
+  // launch: with a workgroup for each CU without splitting, splits twice as long (64
+  // tokens of 32 heads over 300 rows of 3000 95 us for 121; 9 tokens over 700 rows 35
+  // for 40, over up to 2777 rows 78 for 74).
+  if (p.masked && units >= (uint64_t)device_cu_count()) {
+    pl.chunk *= 2;
+    pl.nsplit = (max_rows + pl.chunk - 1) / pl.chunk;
+  }
   Workspace* ws = nullptr;
   if (int rc = decode_workspace(units, head_dim, pl, stream, &ws)) return rc;
   if (ws) {

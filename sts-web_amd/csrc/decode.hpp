@@ -56,6 +56,16 @@ struct DecodeParams {
   float* scores = nullptr;
   float* stats = nullptr;
   uint32_t score_stride = 0;
+  // With `masked` (no new row, no len_step), stream b's query, the window's newest
+  // row, sees its rows lo[b] <= r < hi[b] (null: all) and nothing where counts[b]
+  // is 0; cap_log2 > 0: scale_log2 gives the scores in units of the cap, which is
+  // cap_log2 / log2(e); slopes [H]: the bias by distance.
+  bool masked = false;
+  const int32_t* lo = nullptr;
+  const int32_t* hi = nullptr;
+  const int32_t* counts = nullptr;
+  const float* slopes = nullptr;
+  float cap_log2 = 0.f;
 };
 
 // scale * log2(e), the factor the decode and prefill kernels fold into q.

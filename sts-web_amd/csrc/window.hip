@@ -8,7 +8,6 @@ namespace sts {
 
 namespace {
 
-using window::exp2_hw;
 
 // The rows' weights under every query head of a K/V head's group, from their kept
 // scores, added to their accounts: a thread takes kAccountRows rows, 256 apart, so

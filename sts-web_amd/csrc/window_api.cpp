@@ -62,11 +62,13 @@ int check_rope(const sts_rope* rope, const sts_kv_cache* c, uint64_t rows) {
 namespace sts {
 namespace kv {
 
-// One token a stream with the scores kept: where every head has K and V rows of its
-// own, in f32, the decode kernel, which has no matrix tile to leave 15/16 empty (32 heads
-// of 3000 rows 17.5 us against 22, 64 such streams 550 against 577; on a handle it
-// also rotates and appends the token's rows, a launch less); else the window kernel,
-// which reads the rows of a group of heads, or bf16 rows, once.
+// One token a stream, with the scores kept or under a range: where every head has K
+// and V rows of its own, in f32, the decode kernel, which has no matrix tile to leave
+// 15/16 empty (kept, 32 heads of 3000 rows 17.5 us against 22, 64 such streams 550
+// against 577, and on a handle it also rotates and appends the token's rows, a launch
+// less; under a range, 2777 rows 18 us against 24, 64 streams over 300 rows each 93
+// against 113); else the window kernel, which reads the rows of a group of heads, or
+// bf16 rows, once.
 static bool by_decode(const WindowParams& p, bool bf16) { return p.group == 1 && !bf16; }
 
 static DecodeParams decode_params(const WindowParams& p) {
@@ -91,6 +93,11 @@ static DecodeParams decode_params(const WindowParams& p) {
   d.scores = p.scores;
   d.stats = p.stats;
   d.score_stride = p.score_stride;
+  d.lo = p.lo;
+  d.hi = p.hi;
+  d.counts = p.counts;
+  d.slopes = p.slopes;
+  d.cap_log2 = p.cap_log2;
   return d;
 }
 
@@ -222,8 +229,14 @@ int sts_masked_attention(const float* q, const void* k_cache, const void* v_cach
     STS_CHECK(scale == 0.f || std::fabs(p.qscale) >= 0x1p-100f,
               "softcap %g too large for the scale %g (2^100 times at most)", softcap, scale);
   }
-  return sts::launch_window(p, sts::kWindowMasked, batch, row_type == STS_ROWS_BF16, max_len,
-                            as_stream(stream));
+  const bool bf16 = row_type == STS_ROWS_BF16;
+  if (int rc = sts::check_window(p, batch, bf16)) return rc;
+  if (seq == 1 && sts::kv::by_decode(p, bf16)) {
+    sts::DecodeParams d = sts::kv::decode_params(p);
+    d.masked = true;
+    return sts::launch_decode(d, batch, head_dim, max_len, as_stream(stream));
+  }
+  return sts::launch_window(p, sts::kWindowMasked, batch, bf16, max_len, as_stream(stream));
 }
 
 uint64_t sts_decode_ring_weights_scratch(uint32_t batch, uint32_t heads, uint32_t max_len) {

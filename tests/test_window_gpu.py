@@ -359,6 +359,40 @@ def test_masked_ranges(gpu, case, mask):
     check_masked(w, q, scale_for(D), lo, hi, counts)
 
 
+SINGLE = [
+    # B, H, D, M, lens (f32 rows, every head its own)
+    (4, 3, 128, 64, [64, 1, 0, 33]),                        # one wave a head
+    (3, 2, 40, 50, [50, 20, 7]),
+    (5, 2, 64, 1500, [1500, 1, 700, 1499, 0]),              # several splits
+    (2, 3, 100, 9001, [9000, 513]),
+    (1, 1, 4, 20000, [20000]),
+    (37, 8, 128, 1100, [(97 * i) % 1101 for i in range(37)]),  # more heads than CUs: longer splits
+    (70, 4, 12, 2100, [(331 * i) % 2101 for i in range(70)]),
+]
+
+
+@pytest.mark.parametrize("feature", ["plain", "cap", "bias", "both"])
+@pytest.mark.parametrize("case", SINGLE, ids=lambda c: "-".join(str(x) for x in c[:4]))
+def test_masked_single_tokens(gpu, case, feature):
+    """A token a stream under any range: none, one row, the ring's seam, past both ends,
+    a stream without a token."""
+    B, H, D, M, lens = case
+    w = Window(sum(case[:4]), B, H, M, D, lens, F32)
+    q = queries(w.rng, B, 1, H, D)
+    slopes = (2.0 ** -w.rng.uniform(0, 8, H)).astype(np.float32) if feature in ("bias", "both") else None
+    cap = 5.0 if feature in ("cap", "both") else 0.0
+    lo = np.stack([w.rng.integers(-3, max(L, 1), 1) for L in lens])
+    hi = np.stack([w.rng.integers(-1, L + 3, 1) for L in lens])
+    hi[::3] = lo[::3] + 1
+    hi[1::3] = 2 ** 31 - 1
+    lo[3::7] = 2 ** 31 - 1
+    counts = np.ones(B, np.int64)
+    counts[2::9] = 0
+    check_masked(w, q, scale_for(D), lo, hi, counts, slopes, cap)
+    check_masked(w, q, scale_for(D), lo, None, None, slopes, cap)
+    check_masked(w, q, scale_for(D), None, hi, None, slopes, cap)
+
+
 def test_masked_nothing_seen(gpu):
     """All ranges empty, of a block or of the whole call: zeros."""
     w = Window(4, 2, 2, 200, 64, [200, 150])
