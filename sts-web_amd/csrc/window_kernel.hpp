@@ -27,7 +27,7 @@
 // (16x16x32): f32 rows as two f16 values each, three products for one; bf16 rows as
 // they are against three bf16 parts of Q and of the weights.  Either is as close to the exact result as f32
 // products are.  At 1000 queries of 32 heads over 2600 bf16 rows of 8 K/V heads
-// that is 111 us against 488 in f32; at 24 drafts of 40 nodes over f32 rows 189
+// that is 110 us against 488 in f32; at 24 drafts of 40 nodes over f32 rows 178
 // against 513.
 #pragma once
 
@@ -229,6 +229,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   typedef typename P::V Frag;
   constexpr int kPartBytes = PARTS ? R * NP * P::N * 64 * 16 : 0;
   constexpr int kOutBytes = kWaves * ROWS * LDO * 4;
+  // f32 rows in parts: the first 16 rows of the wave's next tile, each lane's pieces.
+  constexpr bool AHEAD = PARTS && !BF;
+  static_assert(!AHEAD || kPartBytes + kWaves * NC * 1024 <= kOutBytes, "the next rows fit behind the queries");
   __shared__ __align__(16) char s_mem[kPartBytes > kOutBytes ? kPartBytes : kOutBytes];
   auto& s_q = *reinterpret_cast<Frag(*)[PARTS ? R : 1][NP][P::N][64]>(s_mem);
   auto& s_o = *reinterpret_cast<float(*)[kWaves][ROWS][LDO]>(s_mem);
@@ -429,6 +432,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
 #pragma unroll
     for (int c = 0; c < NC; ++c)
       k[c].load(krs, !PAD || (uint32_t)(c * 4 + g) * CW < dh ? off + c * (4 * CW * ES) : kOutside);
+  };
+  // The same pieces as load_k's, by way of LDS: each lane's where it takes them.
+  auto request_ahead = [&](uint32_t r0, int lane) {
+    const int m16 = lane & 15, g = lane >> 4;
+    const uint32_t off = row_off(r0 + m16) + g * (CW * ES);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          krs, (__attribute__((address_space(3))) void*)(s_mem + kPartBytes + (wave * NC + c) * 1024), 16,
+          !PAD || (uint32_t)(c * 4 + g) * CW < dh ? off + c * (4 * CW * ES) : kOutside, 0, 0, AUX);
+  };
+  auto take_ahead = [&](KRow& k, int lane) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      k[c] = __builtin_bit_cast(Piece<BF, CW, AUX>,
+                                *reinterpret_cast<const u32x4*>(s_mem + kPartBytes + (wave * NC + c) * 1024 + lane * 16));
   };
   auto load_v = [&](uint32_t r0, VRow& v, int lane) {
     const int m16 = lane & 15, g = lane >> 4;
@@ -782,7 +801,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   // query does not see.  A tile that is not is multiplied in f32.
   // V is requested while K is consumed and the next tile's K while V is: a tile and
   // a half in registers in all, so that two waves fit a SIMD, which measured faster
-  // than one wave with 64 query rows and both tiles ahead.
+  // than one wave with 64 query rows and both tiles ahead.  The first 16 f32 rows of
+  // the next K go straight to the LDS that the outputs will need, as soon as the
+  // last of this tile's operands has been read from LDS (a read of LDS waits for what
+  // is on its way there), the other 16 are needed only after those: 24 drafts of 40
+  // nodes 184 -> 178 us.
   if constexpr (PARTS) {
     f32x4 s[R][KT];
     for (;;) {
@@ -791,56 +814,62 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
       const uint32_t r0 = t * TILE;
       const bool partly = partly_seen(r0, TILE);
       const int at = fresh_lane();
-      if constexpr (!BF) {
-        float top[KT];
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          top[kt] = 0.f;
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int e = 0; e < CW; ++e) top[kt] = __builtin_elementwise_maximum(top[kt], fabsf(kk[kt][c][e]));
-        }
-        if (!ks.holds(top, [](float x) { return max_xor32(max_xor16(x)); })) break;
-      }
 #pragma unroll
       for (int rt = 0; rt < R; ++rt)
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      // The queries' parts are read anew for every tile: kept in registers (the
-      // compiler lifts the loads out of the loop) they would push others out.
+      // f32 rows 16 at a time: the second 16 arrive while the first are multiplied.
+      constexpr int KS = BF ? KT : 1;
+      bool held = true;
 #pragma unroll
-      for (int c = 0; c < NP; ++c) {
-        Frag kf[KT][P::N];
+      for (int k0 = 0; k0 < KT; k0 += KS) {
+        if constexpr (!BF) {
+          float top[1] = {0.f};
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          if constexpr (BF) {
-            kf[kt][0] = __builtin_bit_cast(Frag, kk[kt][c]);
-          } else {
-            float x[8];
+          for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = kk[kt][(c * 8 + e) / CW][(c * 8 + e) % CW];
-            P::split(x, ks.scale, kf[kt]);
-          }
+            for (int e = 0; e < CW; ++e) top[0] = __builtin_elementwise_maximum(top[0], fabsf(kk[k0][c][e]));
+          held = ks.holds(top, [](float x) { return max_xor32(max_xor16(x)); });
+          if (!held) break;
         }
+        // The queries' parts are read anew for every tile: kept in registers (the
+        // compiler lifts the loads out of the loop) they would push others out.
 #pragma unroll
-        for (int rt = 0; rt < R; ++rt) {
-          Frag qq[P::N];
+        for (int c = 0; c < NP; ++c) {
+          Frag kf[KS][P::N];
 #pragma unroll
-          for (int n = 0; n < P::N; ++n) qq[n] = s_q[rt][c][n][at];
-          // The smaller products first.
-          if constexpr (!BF) {
+          for (int kt = 0; kt < KS; ++kt) {
+            if constexpr (BF) {
+              kf[kt][0] = __builtin_bit_cast(Frag, kk[k0 + kt][c]);
+            } else {
+              float x[8];
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) s[rt][kt] = P::mfma(kf[kt][1], qq[0], s[rt][kt]);
+              for (int e = 0; e < 8; ++e) x[e] = kk[k0 + kt][(c * 8 + e) / CW][(c * 8 + e) % CW];
+              P::split(x, ks.scale, kf[kt]);
+            }
           }
 #pragma unroll
-          for (int n = P::N - 1; n >= 0; --n)
+          for (int rt = 0; rt < R; ++rt) {
+            Frag qq[P::N];
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) s[rt][kt] = P::mfma(kf[kt][0], qq[n], s[rt][kt]);
+            for (int n = 0; n < P::N; ++n) qq[n] = s_q[rt][c][n][at];
+            // The smaller products first.
+            if constexpr (!BF) {
+#pragma unroll
+              for (int kt = 0; kt < KS; ++kt) s[rt][k0 + kt] = P::mfma(kf[kt][1], qq[0], s[rt][k0 + kt]);
+            }
+#pragma unroll
+            for (int n = P::N - 1; n >= 0; --n)
+#pragma unroll
+              for (int kt = 0; kt < KS; ++kt) s[rt][k0 + kt] = P::mfma(kf[kt][0], qq[n], s[rt][k0 + kt]);
+          }
+          if (BF && c == NP / 2 - 1) load_v(r0, vv[0], at);
         }
-        if (c == NP / 2 - 1) load_v(r0, vv[0], at);
+        if (!BF && k0 == 0) load_v(r0, vv[0], at);
       }
+      if (!held) break;
       load_v(r0 + 16, vv[1], at);
+      if constexpr (AHEAD) request_ahead((t + tstep) * TILE, at);
       if constexpr (!BF) {
 #pragma unroll
         for (int rt = 0; rt < R; ++rt) {
@@ -907,9 +936,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
         for (int n = P::N - 1; n >= 0; --n)
 #pragma unroll
           for (int rt = 0; rt < R; ++rt) o[rt][x] = P::mfma(vf[0], pp[rt][n], o[rt][x]);
-        if (x == NX / 2 - 1) load_k((t + tstep) * TILE, kk[0], at);
+        if (x == NX / 2 - 1) load_k((t + tstep) * TILE + (AHEAD ? 16 : 0), kk[AHEAD ? 1 : 0], at);
       }
-      load_k((t + tstep) * TILE + 16, kk[1], at);
+      if constexpr (AHEAD)
+        take_ahead(kk[0], at);
+      else
+        load_k((t + tstep) * TILE + 16, kk[1], at);
     }
     if (t >= t1) break;
     vs.set = true;  // the outputs' scale stays from here on
@@ -945,6 +977,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
     for (int rt = 0; rt < R; ++rt)
 #pragma unroll
       for (int x = 0; x < NX; ++x) o[rt][x] *= f;
+    if constexpr (AHEAD) __builtin_amdgcn_s_waitcnt(0);  // no row is on its way into this LDS any more
     __syncthreads();  // every wave is done with the queries' parts
   }
 
