@@ -1,5 +1,5 @@
 // window_kernel.hpp -- attention of up to 32 query rows per K/V head over a
-// ring window on the f32 matrix cores (gfx950): the kernel behind
+// ring window on the matrix cores (gfx950): the kernel behind
 // sts_tree_attention, sts_masked_attention and sts_decode_ring_weights.
 //
 // For query row i and window row r
@@ -10,25 +10,29 @@
 // A workgroup takes 16*R query rows of one (stream, K/V head) -- the nodes or
 // queries times the heads of the group, so that a K/V row is read once for all
 // of them -- and one split of the window.  Its four waves share the query rows
-// and deal the split's tiles among themselves; neither K, V nor the weights go
-// through LDS, the outputs only at the end:
+// and deal the split's tiles among themselves:
 //   S^T = K Q^T    A = K tile: lane (m, g) = (lane & 15, lane >> 4) holds row m,
 //                  dims (4c + g)*CW + e; B = Q in the same dims.  The lane then
 //                  has the scores of query m for rows 4g .. 4g+3
 //   O^T += V^T P^T A = V^T: the lane holds of rows 4g + i the dims
 //                  (16 tc + m)*VW + e; B = the scores' exponentials as they stand
 // Both tiles are 16-byte loads straight from the cache, and the exponentials
-// never leave their registers.  The waves' (m, l, O) are merged through LDS, the
-// splits' through records in the stream's workspace by the last to arrive.
+// never leave their registers; in LDS stand the queries' operands and, at the end,
+// the waves' (m, l, O), which are merged there.  The splits are merged through
+// records in the stream's workspace by the last to arrive.
 //
 // One row tile (R = 1) over f32 rows multiplies in f32 (16x16x4): its 64 products of
 // a 16 KB tile take a quarter of the time that HBM takes to deliver it.  Two (R = 2),
-// or bf16 rows, would be bound by those products and multiply parts instead
-// (16x16x32): f32 rows as two f16 values each, three products for one; bf16 rows as
-// they are against three bf16 parts of Q and of the weights.  Either is as close to the exact result as f32
-// products are.  At 1000 queries of 32 heads over 2600 bf16 rows of 8 K/V heads
-// that is 110 us against 488 in f32; at 24 drafts of 40 nodes over f32 rows 178
-// against 513.
+// or bf16 rows, would be bound by those products and multiply bf16 parts instead
+// (16x16x32): an f32 value is the exact sum of three, so that f32 rows take six
+// products for one (those of parts below 2^-26 of the whole are left out), and bf16
+// rows, as they are against the parts of Q and of the weights, three.  Parts have
+// f32's exponents: every element is held to f32's grade by itself, whatever stands in
+// its row, tile or channel.  (Two f16 parts of each value under a common scale take
+// half the products, but hold small elements only relative to the largest; 24 drafts
+// of 40 nodes took 174 us with them.)  At 1000 queries of 32 heads over 2600 bf16 rows
+// of 8 K/V heads that is 110 us against 488 in f32; at 24 drafts of 40 nodes over f32
+// rows 203 against 513.
 #pragma once
 
 #include <cfloat>
@@ -54,14 +58,6 @@ constexpr uint32_t kOutside = 0x80000000u;  // past every buffer resource: loads
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ float wave_max(float x) {
-  x = fmaxf(x, xchg<0>(x));
-  x = fmaxf(x, xchg<1>(x));
-  x = fmaxf(x, xchg<2>(x));
-  x = fmaxf(x, xchg<3>(x));
-  return max_xor32(max_xor16(x));
-}
 
 // W elements loaded at a byte offset of a cache head, as f32 (bf16 is widened).
 // AUX: the cache policy of the load.
@@ -95,110 +91,35 @@ __device__ __forceinline__ bool not_finite(float x) {
   return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
 }
 
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// The matrix operands that stand for f32 values x[8].  Against f32 rows: two f16
-// values of x * scale, each the nearest, off by at most 2^-22 of it, and by 2^-25
-// where the second falls below f16's normal range; the products of the two second
-// parts are left out.  Against bf16 rows, which are operands as they are: three bf16
-// values whose sum is x (scale is not used).
-template <bool BF>
-struct Parts {
-  typedef half8 V;
-  static constexpr int N = 2;
-  static __device__ __forceinline__ void split(const float* x, float scale, V (&y)[N]) {
-    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    u32x4 w[N];  // pairs put together as words: no half moves on its own
+// x[8] as matrix operands: three bf16 values each, the nearest to what is left, whose
+// sum is x exactly (24 bits; bf16 has f32's exponents, and subnormals from 2^-133 on).
+// x is finite and at most kMostParts in magnitude, above which the first would be rounded
+// to infinity.
+constexpr int kParts = 3;
+constexpr float kMostParts = 0x1.FEp127f;
+__device__ __forceinline__ void split_parts(const float* x, bf16x8 (&y)[kParts]) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  u32x4 w[kParts];  // pairs put together as words: no half moves on its own
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const half2v h = __builtin_convertvector((f2){x[e] * scale, x[e + 1] * scale}, half2v);
-      const half2v r = __builtin_convertvector(
-          (f2){fmaf(x[e], scale, -(float)h[0]), fmaf(x[e + 1], scale, -(float)h[1])}, half2v);
-      w[0][e / 2] = __builtin_bit_cast(uint32_t, h);
-      w[1][e / 2] = __builtin_bit_cast(uint32_t, r);
+  for (int e = 0; e < 8; e += 2) {
+    float a = x[e], z = x[e + 1];
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) {
+      w[n][e / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, z}, b2));
+      a -= __uint_as_float(w[n][e / 2] << 16);
+      z -= __uint_as_float(w[n][e / 2] & 0xffff0000u);
     }
-#pragma unroll
-    for (int n = 0; n < N; ++n) y[n] = __builtin_bit_cast(V, w[n]);
   }
-  static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-  }
-};
-template <>
-struct Parts<true> {
-  typedef bf16x8 V;
-  static constexpr int N = 3;
-  static __device__ __forceinline__ void split(const float* x, float, V (&y)[N]) {
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    u32x4 w[N];
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      float a = x[e], z = x[e + 1];
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        w[n][e / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, z}, b2));
-        a -= __uint_as_float(w[n][e / 2] << 16);
-        z -= __uint_as_float(w[n][e / 2] & 0xffff0000u);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < N; ++n) y[n] = __builtin_bit_cast(V, w[n]);
-  }
-  static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  }
-};
-
-// The power of two that takes x (positive, finite) to 2^11..2^12, from 2^-117 to 2^110.
-__device__ __forceinline__ float scale_up(float x) {
-  const int e = 127 + 11 - ((int)(__float_as_uint(x) >> 23) - 127);
-  return __uint_as_float((uint32_t)min(max(e, 127 - 117), 127 + 110) << 23);
+  for (int n = 0; n < kParts; ++n) y[n] = __builtin_bit_cast(bf16x8, w[n]);
 }
 
-// What the f32 rows are multiplied by before they are split: the power of two that
-// takes the largest value of the wave's first tile that holds anything to 2^11..2^12.
-struct TileScale {
-  float scale = 1.f, inverse = 1.f;
-  bool set = false;
-  // Whether N rows, of which this lane holds a part that reaches top[] in magnitude
-  // (NaN and infinity kept; ROW is the lane exchange over the parts of a row), are
-  // held well: all below f16's range, and each with a value of 2^-3 or more, so that
-  // a step of f16's smallest is no more than 2^-22 of it.  A row's parts are put
-  // together only where some part is smaller than that.
-  template <int N, typename ROW>
-  __device__ __forceinline__ bool holds(const float (&top)[N], ROW row) {
-    if (!set) {
-      float all = top[0];
-#pragma unroll
-      for (int i = 1; i < N; ++i) all = fmaxf(all, top[i]);
-      all = wave_max(all);
-      if (all > 0.f && all < INFINITY) {  // (outputs of tiles of zeros need no rescaling)
-        scale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(scale_up(all))));
-        inverse = 1.f / scale;
-        set = true;
-      }
-    }
-    const float most = 60000.f * inverse, least = 0.125f * inverse;
-    bool fits = true, small = false;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      fits &= top[i] < most;
-      small |= top[i] < least && top[i] > 0.f;
-    }
-    if (!__all(fits)) return false;
-    if (!__any(small)) return true;
-    small = false;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float x = row(top[i]);
-      small |= x < least && x > 0.f;
-    }
-    return !__any(small);
-  }
-};
+__device__ __forceinline__ f32x4 multiply(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
 
 // The lane's number, found anew: kept through the loops it, and what is derived from
 // it, would cost registers that the tiles need.
@@ -218,24 +139,19 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   constexpr bool PARTS = R > 1 || BF;               // products of parts
   constexpr int KT = PARTS ? 2 : 1;                 // 16-row tiles a wave takes at once
   constexpr int TILE = 16 * KT;
-  constexpr int NP = NC * CW / 8;                   // 32-dim steps of K Q^T in f16
+  constexpr int NP = NC * CW / 8;                   // 32-dim steps of K Q^T in parts
   constexpr int NX = NV * VW;                       // 16-dim tiles of the output
   constexpr int ROWS = 16 * R;
   constexpr int LDO = D + 4;                        // LDS row of a partial output
   constexpr int C4 = D / 4;
 
-  // The queries' f16 parts while the tiles are read, partial outputs after that.
-  typedef Parts<BF> P;
-  typedef typename P::V Frag;
-  constexpr int kPartBytes = PARTS ? R * NP * P::N * 64 * 16 : 0;
+  // The queries' parts while the tiles are read, partial outputs after that.
+  typedef bf16x8 Frag;
+  constexpr int kPartBytes = PARTS ? R * NP * kParts * 64 * 16 : 0;
   constexpr int kOutBytes = kWaves * ROWS * LDO * 4;
-  // f32 rows in parts: the first 16 rows of the wave's next tile, each lane's pieces.
-  constexpr bool AHEAD = PARTS && !BF;
-  static_assert(!AHEAD || kPartBytes + kWaves * NC * 1024 <= kOutBytes, "the next rows fit behind the queries");
   __shared__ __align__(16) char s_mem[kPartBytes > kOutBytes ? kPartBytes : kOutBytes];
-  auto& s_q = *reinterpret_cast<Frag(*)[PARTS ? R : 1][NP][P::N][64]>(s_mem);
+  auto& s_q = *reinterpret_cast<Frag(*)[PARTS ? R : 1][NP][kParts][64]>(s_mem);
   auto& s_o = *reinterpret_cast<float(*)[kWaves][ROWS][LDO]>(s_mem);
-  __shared__ float s_qs[PARTS ? ROWS : 1];  // what the rows' scores are multiplied by
   struct Row {
     uint32_t lo, hi;
     int at;       // window row of the query
@@ -433,22 +349,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
     for (int c = 0; c < NC; ++c)
       k[c].load(krs, !PAD || (uint32_t)(c * 4 + g) * CW < dh ? off + c * (4 * CW * ES) : kOutside);
   };
-  // The same pieces as load_k's, by way of LDS: each lane's where it takes them.
-  auto request_ahead = [&](uint32_t r0, int lane) {
-    const int m16 = lane & 15, g = lane >> 4;
-    const uint32_t off = row_off(r0 + m16) + g * (CW * ES);
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          krs, (__attribute__((address_space(3))) void*)(s_mem + kPartBytes + (wave * NC + c) * 1024), 16,
-          !PAD || (uint32_t)(c * 4 + g) * CW < dh ? off + c * (4 * CW * ES) : kOutside, 0, 0, AUX);
-  };
-  auto take_ahead = [&](KRow& k, int lane) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-      k[c] = __builtin_bit_cast(Piece<BF, CW, AUX>,
-                                *reinterpret_cast<const u32x4*>(s_mem + kPartBytes + (wave * NC + c) * 1024 + lane * 16));
-  };
   auto load_v = [&](uint32_t r0, VRow& v, int lane) {
     const int m16 = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -548,34 +448,21 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   };
   float qf[PARTS ? 1 : NC][CW];  // one row tile: in registers, scaled
   if constexpr (PARTS) {
-    // In LDS as operand parts; f16 ones of each row scaled to its largest value.
+    // In LDS as operand parts, scaled.
     if (wave < R) {
       float x[NC][CW];
       turn_q(x);
-      float sc = 1.f;
-      if constexpr (!BF) {
-        float top = 0.f;
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int e = 0; e < CW; ++e) top = fmaxf(top, fabsf(x[c][e]));
-        top = max_xor32(max_xor16(top));
-        sc = top > 0.f && top < INFINITY ? scale_up(top) : 1.f;
-      }
-      if constexpr (BF) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int e = 0; e < CW; ++e) x[c][e] *= p.qscale;
-      }
+        for (int e = 0; e < CW; ++e) x[c][e] *= p.qscale;
 #pragma unroll
       for (int c = 0; c < NP; ++c) {
-        Frag y[P::N];
-        P::split(&x[0][0] + 8 * c, sc, y);
+        Frag y[kParts];
+        split_parts(&x[0][0] + 8 * c, y);
 #pragma unroll
-        for (int n = 0; n < P::N; ++n) s_q[wave][c][n][lane] = y[n];
+        for (int n = 0; n < kParts; ++n) s_q[wave][c][n][lane] = y[n];
       }
-      if (g == 0) s_qs[wave * 16 + m16] = BF ? 1.f : p.qscale / sc;
     }
     __syncthreads();
   } else {
@@ -592,9 +479,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
 
   // The weights are taken relative to m, which follows the scores' maximum only
   // when they pass it by 2^kSlack, and then to 2^kHead below it: the outputs are
-  // seldom rescaled, and the weights use the range of f16.
+  // seldom rescaled.
   constexpr float kSlack = 15.f, kHead = 7.f;
-  TileScale ks, vs;
   float m[R], l[R];
   f32x4 o[R][NX];
 #pragma unroll
@@ -705,7 +591,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   // rows.  A value that is not finite, in a row that some query does not see, would
   // be carried to that query as 0 * inf: it is taken out of the operand and added by
   // hand to the queries that see its row.
-  auto add_values = [&](uint32_t r0, const VRow& v, auto w, float oscale, bool partly, int lane)
+  auto add_values = [&](uint32_t r0, const VRow& v, auto w, bool partly, int lane)
       __attribute__((always_inline)) {
     const int m16 = lane & 15, g = lane >> 4;
     if (partly) {
@@ -713,7 +599,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int x = 0; x < NX; ++x) bad |= not_finite(v[i][x / VW][x % VW] * oscale);
+        for (int x = 0; x < NX; ++x) bad |= not_finite(v[i][x / VW][x % VW]);
       if (__any(bad)) {
         for (int key = 0; key < 16; ++key) {
           const uint32_t off = row_off(r0 + key);
@@ -734,7 +620,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
               x.load(vrs, !PAD || d < dh ? off + d * ES : kOutside);
 #pragma unroll
               for (int e = 0; e < VW; ++e) {
-                const float y = x[e] * oscale;
+                const float y = x[e];
 #pragma unroll
                 for (int rt = 0; rt < R; ++rt)
                   if (not_finite(y) && !(u[rt] == 0.f)) o[rt][c * VW + e][i] += u[rt] * y;
@@ -748,7 +634,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int x = 0; x < NX; ++x) {
-        float y = v[i][x / VW][x % VW] * oscale;
+        float y = v[i][x / VW][x % VW];
         y = partly && not_finite(y) ? 0.f : y;
 #pragma unroll
         for (int rt = 0; rt < R; ++rt)
@@ -758,7 +644,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
 
   // 16 rows in f32, of which K and V stand in kk[0] and vv[0]; `next` runs when K is
   // no longer needed.
-  auto in_f32 = [&](uint32_t r0, float oscale, int at, auto next) __attribute__((always_inline)) {
+  auto in_f32 = [&](uint32_t r0, int at, auto next) __attribute__((always_inline)) {
     const bool partly = partly_seen(r0, 16);
     f32x4 s[R][1];
 #pragma unroll
@@ -769,14 +655,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
       for (int c = 0; c < NP; ++c) {
         float x[8];
         if constexpr (PARTS) {
-          Frag qq[P::N];
+          Frag qq[kParts];
 #pragma unroll
-          for (int n = 0; n < P::N; ++n) qq[n] = s_q[rt][c][n][at];
+          for (int n = 0; n < kParts; ++n) qq[n] = s_q[rt][c][n][at];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] = (float)qq[0][e] + (float)qq[1][e];
-            if constexpr (BF) x[e] += (float)qq[P::N - 1][e];
-          }
+          for (int e = 0; e < 8; ++e) x[e] = (float)qq[0][e] + ((float)qq[1][e] + (float)qq[2][e]);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = qf[(c * 8 + e) / CW][(c * 8 + e) % CW];
@@ -788,24 +671,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
         if constexpr (PARTS) __builtin_amdgcn_sched_barrier(0);
       }
     next();
-    if constexpr (PARTS) {
-#pragma unroll
-      for (int rt = 0; rt < R; ++rt) s[rt][0] *= s_qs[rt * 16 + (at & 15)];
-    }
     weigh(r0, s, partly, at);
-    add_values(r0, vv[0], [&](int rt) { return s[rt][0]; }, oscale, partly, at);
+    add_values(r0, vv[0], [&](int rt) { return s[rt][0]; }, partly, at);
   };
 
-  // Products of parts, as long as the tiles are held well by them: f32 rows within
-  // f16's range, and for either type no value that is not finite in a row that some
-  // query does not see.  A tile that is not is multiplied in f32.
+  // Products of parts.  A tile of f32 rows with a value that is not finite, or too
+  // near the end of f32's range to be split, is multiplied in f32, so that what sees
+  // it follows f32; so are V rows of either type that hold such a value where some
+  // query does not see them (0 * inf).
   // V is requested while K is consumed and the next tile's K while V is: a tile and
   // a half in registers in all, so that two waves fit a SIMD, which measured faster
-  // than one wave with 64 query rows and both tiles ahead.  The first 16 f32 rows of
-  // the next K go straight to the LDS that the outputs will need, as soon as the
-  // last of this tile's operands has been read from LDS (a read of LDS waits for what
-  // is on its way there), the other 16 are needed only after those: 24 drafts of 40
-  // nodes 184 -> 178 us.
+  // than one wave with 64 query rows and both tiles ahead.  f32 rows 16 at a time,
+  // which takes fewer registers, measured 222 us where 24 drafts of 40 nodes take 203.
   if constexpr (PARTS) {
     f32x4 s[R][KT];
     for (;;) {
@@ -814,88 +691,57 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
       const uint32_t r0 = t * TILE;
       const bool partly = partly_seen(r0, TILE);
       const int at = fresh_lane();
+      float top = 0.f;  // K's largest (NaN stays)
 #pragma unroll
       for (int rt = 0; rt < R; ++rt)
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      // f32 rows 16 at a time: the second 16 arrive while the first are multiplied.
-      constexpr int KS = BF ? KT : 1;
-      bool held = true;
+      // The queries' parts are read anew for every tile: kept in registers (the
+      // compiler lifts the loads out of the loop) they would push others out.
 #pragma unroll
-      for (int k0 = 0; k0 < KT; k0 += KS) {
-        if constexpr (!BF) {
-          float top[1] = {0.f};
+      for (int c = 0; c < NP; ++c) {
+        Frag kf[KT][BF ? 1 : kParts];
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+        for (int kt = 0; kt < KT; ++kt) {
+          if constexpr (BF) {
+            kf[kt][0] = __builtin_bit_cast(Frag, kk[kt][c]);
+          } else {
+            float x[8];
 #pragma unroll
-            for (int e = 0; e < CW; ++e) top[0] = __builtin_elementwise_maximum(top[0], fabsf(kk[k0][c][e]));
-          held = ks.holds(top, [](float x) { return max_xor32(max_xor16(x)); });
-          if (!held) break;
-        }
-        // The queries' parts are read anew for every tile: kept in registers (the
-        // compiler lifts the loads out of the loop) they would push others out.
-#pragma unroll
-        for (int c = 0; c < NP; ++c) {
-          Frag kf[KS][P::N];
-#pragma unroll
-          for (int kt = 0; kt < KS; ++kt) {
-            if constexpr (BF) {
-              kf[kt][0] = __builtin_bit_cast(Frag, kk[k0 + kt][c]);
-            } else {
-              float x[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = kk[k0 + kt][(c * 8 + e) / CW][(c * 8 + e) % CW];
-              P::split(x, ks.scale, kf[kt]);
+            for (int e = 0; e < 8; ++e) {
+              x[e] = kk[kt][(c * 8 + e) / CW][(c * 8 + e) % CW];
+              top = __builtin_elementwise_maximum(top, fabsf(x[e]));
             }
+            split_parts(x, kf[kt]);
           }
-#pragma unroll
-          for (int rt = 0; rt < R; ++rt) {
-            Frag qq[P::N];
-#pragma unroll
-            for (int n = 0; n < P::N; ++n) qq[n] = s_q[rt][c][n][at];
-            // The smaller products first.
-            if constexpr (!BF) {
-#pragma unroll
-              for (int kt = 0; kt < KS; ++kt) s[rt][k0 + kt] = P::mfma(kf[kt][1], qq[0], s[rt][k0 + kt]);
-            }
-#pragma unroll
-            for (int n = P::N - 1; n >= 0; --n)
-#pragma unroll
-              for (int kt = 0; kt < KS; ++kt) s[rt][k0 + kt] = P::mfma(kf[kt][0], qq[n], s[rt][k0 + kt]);
-          }
-          if (BF && c == NP / 2 - 1) load_v(r0, vv[0], at);
         }
-        if (!BF && k0 == 0) load_v(r0, vv[0], at);
+        // The products below 2^-26 of the whole are left out.
+#pragma unroll
+        for (int n = kParts - 1; n >= 0; --n) {
+          Frag qq[R];
+#pragma unroll
+          for (int rt = 0; rt < R; ++rt) qq[rt] = s_q[rt][c][n][at];
+#pragma unroll
+          for (int j = BF ? 0 : kParts - 1 - n; j >= 0; --j)
+#pragma unroll
+            for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+              for (int kt = 0; kt < KT; ++kt) s[rt][kt] = multiply(kf[kt][j], qq[rt], s[rt][kt]);
+        }
+        if (c == NP / 2 - 1) load_v(r0, vv[0], at);
       }
-      if (!held) break;
+      if (!BF && !__all(top <= kMostParts)) break;
       load_v(r0 + 16, vv[1], at);
-      if constexpr (AHEAD) request_ahead((t + tstep) * TILE, at);
-      if constexpr (!BF) {
-#pragma unroll
-        for (int rt = 0; rt < R; ++rt) {
-          const float f = s_qs[rt * 16 + (at & 15)] * ks.inverse;
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt) s[rt][kt] *= f;
-        }
-      }
       weigh(r0, s, partly, at);
       if constexpr (!BF) {
-        float top[4 * KT];
+        top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4 * KT; ++i) {
-          top[i] = 0.f;
+        for (int i = 0; i < 4 * KT; ++i)
 #pragma unroll
           for (int c = 0; c < NV; ++c)
 #pragma unroll
-            for (int e = 0; e < VW; ++e)
-              top[i] = __builtin_elementwise_maximum(top[i], fabsf(vv[i / 4][i % 4][c][e]));
-        }
-        weighed = !vs.holds(top, [](float x) {
-          x = fmaxf(x, xchg<0>(x));
-          x = fmaxf(x, xchg<1>(x));
-          x = fmaxf(x, xchg<2>(x));
-          return fmaxf(x, xchg<3>(x));
-        });
+            for (int e = 0; e < VW; ++e) top = __builtin_elementwise_maximum(top, fabsf(vv[i / 4][i % 4][c][e]));
+        weighed = !__all(top <= kMostParts);
       } else if (partly) {
         bool bad = false;
 #pragma unroll
@@ -905,17 +751,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
         weighed = __any(bad);
       }
       if (weighed) break;
-      Frag pp[R][P::N];
+      Frag pp[R][kParts];
 #pragma unroll
       for (int rt = 0; rt < R; ++rt) {
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = s[rt][e >> 2][e & 3];
-        P::split(x, 1.f, pp[rt]);
+        split_parts(x, pp[rt]);
       }
 #pragma unroll
       for (int x = 0; x < NX; ++x) {
-        Frag vf[P::N];
+        Frag vf[BF ? 1 : kParts];
         if constexpr (BF) {
           // The halves of the rows' words, paired along the rows.
           u32x4 y;
@@ -928,36 +774,32 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
           float y[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) y[k] = vv[k / 4][k % 4][x / VW][x % VW];
-          P::split(y, vs.scale, vf);
-#pragma unroll
-          for (int rt = 0; rt < R; ++rt) o[rt][x] = P::mfma(vf[1], pp[rt][0], o[rt][x]);
+          split_parts(y, vf);
         }
 #pragma unroll
-        for (int n = P::N - 1; n >= 0; --n)
+        for (int n = kParts - 1; n >= 0; --n)
 #pragma unroll
-          for (int rt = 0; rt < R; ++rt) o[rt][x] = P::mfma(vf[0], pp[rt][n], o[rt][x]);
-        if (x == NX / 2 - 1) load_k((t + tstep) * TILE + (AHEAD ? 16 : 0), kk[AHEAD ? 1 : 0], at);
+          for (int j = BF ? 0 : n; j >= 0; --j)
+#pragma unroll
+            for (int rt = 0; rt < R; ++rt) o[rt][x] = multiply(vf[j], pp[rt][n - j], o[rt][x]);
+        if (x == NX / 2 - 1) load_k((t + tstep) * TILE, kk[0], at);
       }
-      if constexpr (AHEAD)
-        take_ahead(kk[0], at);
-      else
-        load_k((t + tstep) * TILE + 16, kk[1], at);
+      load_k((t + tstep) * TILE + 16, kk[1], at);
     }
     if (t >= t1) break;
-    vs.set = true;  // the outputs' scale stays from here on
     const int at = fresh_lane();
     if (weighed) {
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
         const uint32_t r0 = t * TILE + kt * 16;
         load_v(r0, vv[0], at);
-        add_values(r0, vv[0], [&](int rt) { return s[rt][kt]; }, vs.scale, partly_seen(r0, 16), at);
+        add_values(r0, vv[0], [&](int rt) { return s[rt][kt]; }, partly_seen(r0, 16), at);
       }
     } else {
       for (uint32_t r0 = t * TILE; r0 < (t + 1) * TILE; r0 += 16) {
         load_k(r0, kk[0], at);
         load_v(r0, vv[0], at);
-        in_f32(r0, vs.scale, at, [] {});
+        in_f32(r0, at, [] {});
       }
     }
     t += tstep;
@@ -967,19 +809,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
   } else {
     for (; t < t1; t += tstep) {
       const int at = fresh_lane();
-      in_f32(t * TILE, 1.f, at, [&] { load_k((t + tstep) * TILE, kk[0], at); });
+      in_f32(t * TILE, at, [&] { load_k((t + tstep) * TILE, kk[0], at); });
       load_v((t + tstep) * TILE, vv[0], at);
     }
   }
-  if constexpr (PARTS) {
-    const float f = vs.inverse;
-#pragma unroll
-    for (int rt = 0; rt < R; ++rt)
-#pragma unroll
-      for (int x = 0; x < NX; ++x) o[rt][x] *= f;
-    if constexpr (AHEAD) __builtin_amdgcn_s_waitcnt(0);  // no row is on its way into this LDS any more
-    __syncthreads();  // every wave is done with the queries' parts
-  }
+  if constexpr (PARTS) __syncthreads();  // every wave is done with the queries' parts
 
   // The waves' states merged through LDS.
   const int lane1 = fresh_lane(), tid1 = wave * 64 + lane1;

@@ -130,3 +130,45 @@ def evict64(w, keep, recent):
     nan = np.isnan(w[:L - recent])
     order = np.lexsort((np.arange(len(old)), -old, ~nan))
     return np.concatenate([np.sort(order[:keep - recent]), np.arange(L - recent, L)])
+
+
+def attend64_channels(q, k, v, seen, scale, softcap=0.0, slopes=None, w=None):
+    """attend64 with a bound for every output channel: (out [n,H,D], bound [n,H,D]).
+
+    The bound of an evaluation whose every operand keeps f32's 24 bits at any size:
+    f32 products, or the six larger products of three bf16 parts each.  (Parts rounded
+    to nearest stand for the value exactly; the three products left out are below
+    2^-26 of it together, u/4.)  A score adds up 6 D products of |q k| at most and is
+    scaled twice: off by e = scale (6 D + 16) u sum |q k|, and 8 u of its size for cap
+    and bias each, 4 u of the largest for the exponent.  A weight is off by the factor
+    e of its own row, the sum of the weights by their mean e, 3 u each for the
+    exponentials.  A channel adds up 6 L terms p |v| at most, and 24 u covers the
+    weights' parts, merge and division.  Weights below 2^-110 of the largest may be
+    lost whole.  Every term is a share of that channel's own sum of p |v|."""
+    n, H, D = q.shape
+    g = H // k.shape[0]
+    out, bound = np.zeros((n, H, D)), np.zeros((n, H, D))
+    for h in range(H):
+        kk, vv = k[h // g], v[h // g]
+        for i in range(n):
+            at = np.flatnonzero(seen[i])
+            if not len(at):
+                continue
+            qi = q[i, h].astype(np.float64)
+            s = kk[at] @ qi * scale
+            e = np.abs(kk[at]) @ np.abs(qi) * (6 * D + 16) * abs(scale) * U
+            if softcap > 0:
+                s = softcap * np.tanh(s / softcap)
+                e = e + 8 * U * np.abs(s)
+            if slopes is not None:
+                away = slopes[h] * np.abs(w[i] - at)
+                s = s - away
+                e = e + 8 * U * (np.abs(away) + np.abs(s))
+            e = e + 4 * U * np.abs(s).max()
+            p = np.exp(s - s.max())
+            p = p / p.sum()
+            va = np.abs(vv[at])
+            off = e + p @ e + (6 * len(at) + 24) * U
+            out[i, h] = p @ vv[at]
+            bound[i, h] = (p * off) @ va + 2.0 ** -110 * va.sum(0)
+    return out, bound
