@@ -477,10 +477,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
     if (narrow && !p.rope_cos && t < t1 && (t + (t1 - 1 - t) / tstep * tstep + 1) * TILE > base) narrow_tree();
   }
 
-  // The weights are taken relative to m, which follows the scores' maximum only
-  // when they pass it by 2^kSlack, and then to 2^kHead below it: the outputs are
-  // seldom rescaled.
-  constexpr float kSlack = 15.f, kHead = 7.f;
+  // The weights are taken relative to m, which follows the scores' maximum only when
+  // they pass it, and then to 2^kRoom above it: the outputs are seldom rescaled, and no
+  // weight is above 1, so that sums over a whole window of values of 1e30 stay in
+  // range.  (A weight below 2^-118 of the largest may be lost.)
+  constexpr float kRoom = 8.f;
   float m[R], l[R];
   f32x4 o[R][NX];
 #pragma unroll
@@ -565,12 +566,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void window_kernel(const WindowPara
       for (int kt = 0; kt < K; ++kt)
         x = fmaxf(x, fmaxf(fmaxf(s[rt][kt][0], s[rt][kt][1]), fmaxf(s[rt][kt][2], s[rt][kt][3])));
       top[rt] = max_xor32(max_xor16(x));
-      passed |= top[rt] > m[rt] + kSlack;
+      passed |= top[rt] > m[rt];
     }
     if (__any(passed)) {
 #pragma unroll
       for (int rt = 0; rt < R; ++rt) {
-        const float now = fmaxf(m[rt], top[rt] - kHead), alpha = exp2_hw(m[rt] - now);
+        const float now = top[rt] > m[rt] ? top[rt] + kRoom : m[rt], alpha = exp2_hw(m[rt] - now);
         m[rt] = now;
         l[rt] *= alpha;
 #pragma unroll

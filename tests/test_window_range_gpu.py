@@ -149,3 +149,39 @@ def test_tiles_that_are_not_finite_between_others(gpu, poison, dtype):
                                     scale_for(D))
     assert np.isfinite(got[even]).all()
     assert (np.abs(got[even][:, HEADS] - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [4, 20])
+def test_many_rows_of_the_largest_values(gpu, T, dtype):
+    """60000 rows of values near 1e30 whose scores lie above those of every wave's
+    first tile, by e^5.47 = 2^7.9: the sums stay in f32's range on the way."""
+    import sts_attn
+    D, n = 8, 60000
+    at = np.arange(n)
+    x = np.where(at < 128, 0.0, 5.46875).astype(np.float32)  # exact in bf16
+    k1 = torch.zeros((n, D))
+    k1[:, 0] = torch.from_numpy(x)
+    v1 = torch.from_numpy((1e30 * (0.9 + 0.1 * at / n)).astype(np.float32))[:, None].expand(n, D)
+    k = k1.to(dtype).cuda()[None, None].expand(1, KH, n, D).contiguous()
+    v = v1.to(dtype).cuda()[None, None].expand(1, KH, n, D).contiguous()
+    q = torch.zeros((1, T, KH, D), device="cuda")
+    q[..., 0] = 1
+    lens, starts = (torch.tensor([y], dtype=torch.int32, device="cuda") for y in (n, 0))
+    parents = torch.full((1, T), -1, dtype=torch.int32, device="cuda")
+    q64, k64, v64 = np.zeros((T, 1, D)), k1.double().numpy()[None], v1.to(dtype).double().numpy()[None]
+    q64[..., 0] = 1
+    causal = at[None, :] <= np.arange(n - T, n)[:, None]
+    runs = [(tree_seen(np.full(T, -1), T, n), sts_attn.tree_attention(q, k, v, parents, lens, starts, 1.0)),
+            (causal, sts_attn.masked_attention(q, k, v, lens, starts, 1.0))]
+    for seen, got in runs:
+        want, bound = attend64_channels(q64, k64, v64, seen, 1.0)
+        got = got[0].cpu().numpy()
+        assert np.isfinite(got).all()
+        assert (np.abs(got - want) <= bound).all()
+    acc = torch.zeros((1, KH, n), device="cuda")
+    pair = torch.zeros((1, 2 * KH, D), device="cuda")
+    pair[..., 0] = 1
+    got = sts_attn.decode_ring_weights(pair, k, v, acc, lens, starts, 1.0)[0].cpu().numpy()
+    want, bound = attend64_channels(q64[:1], k64, v64, np.ones((1, n), bool), 1.0)
+    assert np.isfinite(got).all() and (np.abs(got - want[0]) <= bound[0]).all()
