@@ -315,16 +315,18 @@ def _arg(t: Optional[torch.Tensor], name: str, dtype, shape, device) -> Optional
     raise ValueError(f"{name} must be contiguous")
 
 
-def _made_for(stream, *tensors) -> None:
-    """Tensors allocated here on the current stream and used on `stream`: their
-    memory is not reused before that stream is done with them."""
-    if stream is None:
-        return
-    handle = _stream(stream)
-    if handle != _stream(None):
-        s = torch.cuda.ExternalStream(handle) if isinstance(stream, int) else stream
-        for t in tensors:
-            t.record_stream(s)
+def _empty(shape, dtype, device, stream) -> torch.Tensor:
+    """A new tensor for work on `stream`.  Its memory is taken from that stream's
+    pool, so that what held it before is done with it there, and not reused before
+    the current stream, on which the caller may go on with it, is done with it too."""
+    if stream is not None:
+        handle = _stream(stream)
+        if handle != _stream(None):
+            with torch.cuda.stream(torch.cuda.ExternalStream(handle) if isinstance(stream, int) else stream):
+                t = torch.empty(shape, dtype=dtype, device=device)
+            t.record_stream(torch.cuda.current_stream())
+            return t
+    return torch.empty(shape, dtype=dtype, device=device)
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -342,8 +344,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     T, H = shape[1], shape[2]
     qp = _arg(q, "q", _f32t, shape, dev)
     if out is None:
-        out = torch.empty_like(q)
-        _made_for(stream, out)
+        out = _empty(shape, _f32t, dev, stream)
         op = out.data_ptr()
     else:
         op = _arg(out, "out", _f32t, shape, dev)
@@ -391,8 +392,7 @@ def masked_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     S, H = shape[1], shape[2]
     qp = _arg(q, "q", _f32t, shape, dev)
     if out is None:
-        out = torch.empty_like(q)
-        _made_for(stream, out)
+        out = _empty(shape, _f32t, dev, stream)
         op = out.data_ptr()
     else:
         op = _arg(out, "out", _f32t, shape, dev)
@@ -421,14 +421,12 @@ def decode_ring_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     qp = _arg(q, "q", _f32t, shape, dev)
     # sts_decode_ring_weights_scratch floats: whole tiles of 16 scores and two
     # statistics for each head of each stream.
-    scratch = torch.empty(B * H * ((M + 15) // 16 * 16 + 2), dtype=_f32t, device=dev)
+    scratch = _empty(B * H * ((M + 15) // 16 * 16 + 2), _f32t, dev, stream)
     if out is None:
-        out = torch.empty_like(q)
-        _made_for(stream, out)
+        out = _empty(shape, _f32t, dev, stream)
         op = out.data_ptr()
     else:
         op = _arg(out, "out", _f32t, shape, dev)
-    _made_for(stream, scratch)
     one = (B,)
     _check(load().sts_decode_ring_weights(
         qp, k_cache.data_ptr(), v_cache.data_ptr(), op, _arg(weights, "weights", _f32t, (B, KH, M), dev),
@@ -450,8 +448,7 @@ def evict_ring(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tens
         raise StsError(STS_ERR_INVALID, f"need 1 <= keep ({keep}) <= max_len ({M}) and "
                        f"0 <= recent ({recent}) <= keep")
     if kept is None:
-        kept = torch.empty((B, KH, keep), dtype=torch.int32, device=dev)
-        _made_for(stream, kept)
+        kept = _empty((B, KH, keep), torch.int32, dev, stream)
     i32 = torch.int32
     _check(load().sts_evict_ring(
         k_cache.data_ptr(), v_cache.data_ptr(), _arg(weights, "weights", torch.float32, (B, KH, M), dev),
@@ -689,8 +686,7 @@ class KVCache:
         qs, ks = (T, self.n_heads, self.head_dim), (T, self.n_kv_heads, self.head_dim)
         qp = _arg(q, "q", torch.float32, qs, dev)
         if out is None:
-            out = torch.empty_like(q)
-            _made_for(stream, out)
+            out = _empty(qs, _f32t, dev, stream)
         _check(load().sts_kv_tree_step(
             self._h, rope.handle if rope is not None else None, qp,
             _arg(k_new, "k_new", torch.float32, ks, dev), _arg(v_new, "v_new", torch.float32, ks, dev),

@@ -1,0 +1,69 @@
+"""Drafts, masks, kept weights and eviction on streams other than the current one."""
+import numpy as np
+import pytest
+import torch
+
+import sts_attn
+from test_window_gpu import i32
+from windows import Window, queries, random_tree
+
+pytestmark = pytest.mark.gpu
+
+SLEEP = 20_000_000  # clocks: some milliseconds at least, a fraction of a second at most
+
+
+@pytest.mark.parametrize("as_handle", [False, True])
+@pytest.mark.parametrize("what", ["tree", "masked", "weights", "scratch", "evict", "step"])
+def test_new_memory_is_not_the_current_streams(gpu, what, as_handle):
+    """A block that the current stream has freed, but is still working on, is not
+    taken for the results or the scratch of a call on another stream."""
+    B, H, M, D, T = 2, 4, 1000, 64, 8
+    w = Window(41, B, H, M, D, [M, 700])
+    w.k, w.v = w.k.nan_to_num(0.0), w.v.nan_to_num(0.0)
+    k, v, dl, ds = w.dev("k", "v", "lens", "starts")
+    q = torch.from_numpy(queries(w.rng, B, T, H, D)).cuda()
+    parents = i32(np.stack([random_tree(w.rng, T, T) for _ in range(B)]))
+    acc = torch.rand((B, H, M), device="cuda")
+    side = torch.cuda.Stream()
+    s = side.cuda_stream if as_handle else side
+    cache = sts_attn.KVCache(M, H, D)
+    q1, o1 = q[:, 0].contiguous(), torch.zeros((B, H, D), device="cuda")
+    scratch = sts_attn.load().sts_decode_ring_weights_scratch(B, H, M)
+    run, words = {
+        "tree": (lambda: sts_attn.tree_attention(q, k, v, parents, dl, ds, 0.125, stream=s), q.numel()),
+        "masked": (lambda: sts_attn.masked_attention(q, k, v, dl, ds, 0.125, stream=s), q.numel()),
+        "weights": (lambda: sts_attn.decode_ring_weights(q1, k, v, acc, dl, ds, 0.125, stream=s), q1.numel()),
+        "scratch": (lambda: sts_attn.decode_ring_weights(q1, k, v, acc, dl, ds, 0.125, out=o1, stream=s), scratch),
+        "evict": (lambda: sts_attn.evict_ring(k, v, acc, dl, ds, 300, 20, stream=s), B * H * 300),
+        "step": (lambda: cache.tree_step(q[0], q[0], q[0], parents[0], 0.125, stream=s), q[0].numel()),
+    }[what]
+    run()  # the workspaces
+    torch.cuda.synchronize()
+    block = torch.full((words,), 7.0, device="cuda")
+    torch.cuda._sleep(SLEEP)
+    copy = block.clone()
+    del block
+    run()
+    torch.cuda.synchronize()
+    assert (copy == 7.0).all()
+
+
+def test_results_of_another_stream_outlive_it(gpu):
+    """A result that the current stream still reads is not overwritten by the next
+    call on the stream that made it."""
+    w = Window(42, 2, 4, 500, 64, [500, 400])
+    k, v, dl, ds = w.dev("k", "v", "lens", "starts")
+    q = torch.from_numpy(queries(w.rng, 2, 8, 4, 64)).cuda()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    want, other = sts_attn.masked_attention(q, k, v, dl, ds, 0.125), q * 2
+    torch.cuda.synchronize()
+    got = sts_attn.masked_attention(q, k, v, dl, ds, 0.125, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda._sleep(SLEEP)
+    copy = got.clone()
+    del got
+    for _ in range(3):
+        sts_attn.masked_attention(other, k, v, dl, ds, 0.125, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(copy, want)
