@@ -185,3 +185,48 @@ def test_many_rows_of_the_largest_values(gpu, T, dtype):
     got = sts_attn.decode_ring_weights(pair, k, v, acc, lens, starts, 1.0)[0].cpu().numpy()
     want, bound = attend64_channels(q64[:1], k64, v64, np.ones((1, n), bool), 1.0)
     assert np.isfinite(got).all() and (np.abs(got - want[0]) <= bound[0]).all()
+
+
+def test_every_row_counts_past_32_bits(gpu):
+    """33 streams whose windows hold more than 2^32 rows together (69 GB), two query
+    heads a K/V head.  Some thousand rows of each, the window's ends, the ring's seam
+    and others, share the whole weight, and each has values of its own: a row that is
+    missed or met twice shows in the mean."""
+    import sts_attn
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GB")
+    B, M = 33, 0x7FFFFFF0 // 16
+    assert B * M > 2 ** 32
+    rng = np.random.default_rng(44)
+    t = torch.zeros((B, 1, M, 4), device="cuda")  # K and V: dim 0 makes the scores, all four are values
+    lens = np.full(B, M, np.int32)
+    lens[1], lens[2] = M - 12345, 1000
+    starts = rng.integers(0, M, B).astype(np.int32)
+    lo = np.where(np.arange(B) % 3 == 0, lens // 3, 0).astype(np.int32)
+    marked = []
+    for b in range(B):
+        n, first = int(lens[b]), int(lo[b])
+        seam = (M - int(starts[b])) % M
+        at = np.unique(np.concatenate([[first, first + 1, first - 1, n - 1, n - 2, seam, seam - 1],
+                                       rng.integers(0, n, 1000)]))
+        at = at[(at >= 0) & (at < n)]
+        x = rng.uniform(-100, 100, (len(at), 4)).astype(np.float32)
+        x[:, 0] = 80  # score 40: a row of zeros gets e^-40 of a marked one's weight
+        slots = torch.from_numpy((int(starts[b]) + at) % M).cuda()
+        t[b, 0, slots] = torch.from_numpy(x).cuda()
+        marked.append((at, x.astype(np.float64)))
+    q = torch.zeros((B, 1, 2, 4), device="cuda")
+    q[..., 0] = 1
+    dl, ds, dlo = (torch.from_numpy(x).cuda() for x in (lens, starts, lo[:, None].copy()))
+    parents = torch.full((B, 1), -1, dtype=torch.int32, device="cuda")
+    got = [sts_attn.tree_attention(q, t, t, parents, dl, ds, 0.5), sts_attn.masked_attention(q, t, t, dl, ds, 0.5, lo=dlo)]
+    got = [x.cpu().numpy()[:, 0] for x in got]
+    del t
+    torch.cuda.empty_cache()
+    for b in range(B):
+        at, x = marked[b]
+        for y, seen in ((got[0][b], at >= 0), (got[1][b], at >= lo[b])):
+            # Equal weights: only the sums of the marked rows are rounded, and the
+            # zero rows' weights, M e^-40 = 6e-10 of one row's, lost or kept.
+            tol = (seen.sum() + 16) * 2.0 ** -24 * np.abs(x[seen]).mean(0) + 1e-6
+            assert (np.abs(y - x[seen].mean(0)) <= tol).all(), b

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import sts_attn
-from test_window_gpu import i32
+from test_window_gpu import calls, i32
 from windows import Window, queries, random_tree
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +67,29 @@ def test_results_of_another_stream_outlive_it(gpu):
         sts_attn.masked_attention(other, k, v, dl, ds, 0.125, stream=side)
     torch.cuda.synchronize()
     assert torch.equal(copy, want)
+
+
+def test_results_made_at_the_same_time(gpu):
+    """All four calls on two streams at once, what each wrote while the other ran kept
+    on its own stream and compared with what it writes alone."""
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    work = [calls(43 + i, s) for i, s in enumerate(sides)]
+    torch.cuda.synchronize()
+
+    def once(i):
+        fns, restore = work[i]
+        with torch.cuda.stream(sides[i]):
+            restore()
+            return [t.clone() for f in fns for t in f()]
+
+    alone = []
+    for i in range(2):
+        alone.append(once(i))
+        torch.cuda.synchronize()
+    rounds = [[once(i) for i in range(2)] for _ in range(12)]
+    torch.cuda.synchronize()
+    for got in rounds:
+        for i in range(2):
+            assert len(got[i]) == len(alone[i]) == 8
+            assert all(torch.equal(a, b) for a, b in zip(got[i], alone[i]))
+    assert not torch.equal(alone[0][0], alone[1][0])
