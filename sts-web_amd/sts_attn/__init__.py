@@ -697,6 +697,8 @@ class KVCache:
     def tree_commit(self, nodes: int, path: Sequence[int], stream=None) -> None:
         """Ends a draft of `nodes` rows: the rows of the accepted path (node indices,
         ascending) stay as the window's last ones, the others are rolled back."""
+        if any(x >> 32 for x in path):  # (the C array would take it modulo 2^32)
+            raise StsError(STS_ERR_INVALID, f"path must name nodes below {nodes} in ascending order")
         host = (_u32 * max(len(path), 1))(*path)
         _check(load().sts_kv_tree_commit(self._h, nodes, host, len(path), _stream(stream)))
 

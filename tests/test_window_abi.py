@@ -195,3 +195,13 @@ def test_tensors_of_the_wrong_place_type_or_shape():
         sts_attn._arg(q.transpose(0, 1), "q", torch.float32, (3, 2, 8, 64), q.device)
     with pytest.raises(ValueError, match="must be on"):
         sts_attn._arg(q, "q", torch.float32, q.shape, torch.device("meta"))
+
+
+def test_values_that_c_types_would_change():
+    """A path entry past 32 bits is refused, not taken modulo 2^32."""
+    c = sts_attn.KVCache(64, 4, 128)
+    c.advance(20)
+    for path in ([2 ** 32], [0, 2 ** 32 + 1], [-1], [-(2 ** 32)]):
+        with pytest.raises(sts_attn.StsError, match="ascending"):
+            c.tree_commit(3, path)
+    assert (c.offset(), c.seq_len()) == (20, 20)
