@@ -710,9 +710,10 @@ class KVCache:
         s = self.state()
         kp = None
         if kept is not None:
-            kp = _arg(kept, "kept", torch.int32, (s.batch, s.heads, keep), kept.device)
-            if kept.device.type != "cuda":
-                raise ValueError("kept must be on the GPU")
+            dev = kept.device
+            if dev.type != "cuda" or dev.index != torch.cuda.current_device():
+                raise ValueError(f"kept must be on the current GPU, got {dev}")
+            kp = _arg(kept, "kept", torch.int32, (s.batch, s.heads, keep), dev)
         _check(load().sts_kv_evict(self._h, keep, recent, kp, _stream(stream)))
 
     def close(self):

@@ -205,3 +205,23 @@ def test_values_that_c_types_would_change():
         with pytest.raises(sts_attn.StsError, match="ascending"):
             c.tree_commit(3, path)
     assert (c.offset(), c.seq_len()) == (20, 20)
+
+
+@pytest.mark.parametrize("index", [None, 1])
+def test_kept_rows_on_another_device(monkeypatch, index):
+    """Only a tensor on the current GPU may receive the kept rows."""
+    c = sts_attn.KVCache(16, 2, 64, keep_weights=True)
+
+    class Kept:
+        dtype, shape = torch.int32, (0, 2, 4)
+        device = torch.device("cpu") if index is None else torch.device("cuda", index)
+
+        def is_contiguous(self):
+            return True
+
+        def data_ptr(self):
+            raise AssertionError("its address is not taken")
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(ValueError, match="current GPU"):
+        c.evict(4, 2, kept=Kept())
