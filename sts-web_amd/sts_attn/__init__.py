@@ -390,6 +390,8 @@ def masked_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if len(shape) != 4 or shape[0] != B or shape[3] != D:
         raise ValueError(f"q must be [{B}, S, H, {D}], got {tuple(shape)}")
     S, H = shape[1], shape[2]
+    if softcap and not _f32(softcap).value:
+        raise ValueError(f"softcap {softcap} is zero in float32")
     qp = _arg(q, "q", _f32t, shape, dev)
     if out is None:
         out = _empty(shape, _f32t, dev, stream)

@@ -93,3 +93,14 @@ def test_results_made_at_the_same_time(gpu):
             assert len(got[i]) == len(alone[i]) == 8
             assert all(torch.equal(a, b) for a, b in zip(got[i], alone[i]))
     assert not torch.equal(alone[0][0], alone[1][0])
+
+
+def test_a_cap_that_is_zero_in_float32(gpu):
+    """Not taken for no cap."""
+    w = Window(45, 1, 1, 20, 64, [20])
+    k, v, dl, ds = w.dev("k", "v", "lens", "starts")
+    q = torch.zeros((1, 3, 1, 64), device="cuda")
+    with pytest.raises(ValueError, match="softcap"):
+        sts_attn.masked_attention(q, k, v, dl, ds, 0.125, softcap=1e-50)
+    with pytest.raises(sts_attn.StsError, match="softcap"):
+        sts_attn.masked_attention(q, k, v, dl, ds, 0.125, softcap=-1e-50 * 1e20)
