@@ -29,6 +29,8 @@ int fail(int code, const char* fmt, ...) {
   vsnprintf(buf, sizeof buf, fmt, ap);
   va_end(ap);
   g_last_error = buf;
+  // Reported here: HIP keeps it too, and a later launch's check would take it for its own.
+  if (code == STS_ERR_NOMEM || code == STS_ERR_HIP) (void)hipGetLastError();
   return code;
 }
 

@@ -104,3 +104,18 @@ def test_a_cap_that_is_zero_in_float32(gpu):
         sts_attn.masked_attention(q, k, v, dl, ds, 0.125, softcap=1e-50)
     with pytest.raises(sts_attn.StsError, match="softcap"):
         sts_attn.masked_attention(q, k, v, dl, ds, 0.125, softcap=-1e-50 * 1e20)
+
+
+@pytest.mark.parametrize("keep_weights", [False, True])
+def test_a_refused_allocation_is_reported_once(gpu, keep_weights):
+    """A cache too large for any memory is refused (no memory is taken); the calls
+    after it are not refused for it."""
+    big = sts_attn.KVCache(2 ** 31 - 1, 65535, 128, keep_weights=keep_weights)
+    x = torch.ones((1, 3, 2, 64), device="cuda")
+    c = sts_attn.KVCache(16, 2, 64, keep_weights=keep_weights)
+    for _ in range(2):
+        with pytest.raises(sts_attn.StsError, match="allocation"):
+            sts_attn._check(sts_attn.load().sts_kv_ensure_allocated(big.handle, 1, None, None, None, None))
+        c.update(x, x)
+        assert c.attend(x[:, 0].contiguous(), 0.125).eq(1).all()
+    assert big.state().allocated == 0 and c.seq_len() == 6
