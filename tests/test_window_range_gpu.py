@@ -230,3 +230,30 @@ def test_every_row_counts_past_32_bits(gpu):
             # zero rows' weights, M e^-40 = 6e-10 of one row's, lost or kept.
             tol = (seen.sum() + 16) * 2.0 ** -24 * np.abs(x[seen]).mean(0) + 1e-6
             assert (np.abs(y - x[seen].mean(0)) <= tol).all(), b
+
+
+def test_scores_are_short_sums(gpu):
+    """Up to 16 query rows over f32 rows: the outputs' error in the norm.
+
+    A score of standard deviation 3 is the sum of 128 products of variance
+    9 (log2 e)^2 / 128 = v.  An addition in f32 that reaches x is off by a variance of
+    (u x)^2 / 3 at most, and x^2 after k products is k v: one sum of all is off by
+    u sqrt(8256 v / 3) = 20 u, four sums of 32 and their sums by
+    u sqrt((4 * 528 + 256) v / 3) = 10.7 u, and q's rounding adds 2.5 u.  The weights,
+    and with them the outputs, are off by ln 2 times that: 8.3e-7 and 4.5e-7."""
+    import sts_attn
+    B, G, D, n = 4, 8, 128, 1000
+    w = Window(36, B, 4, n, D, [n, 800, 600, 400])
+    k, v, dl, ds = w.dev("k", "v", "lens", "starts")
+    q = 3 * w.rng.standard_normal((B, 1, 4 * G, D)).astype(np.float32)
+    dq = torch.from_numpy(q).cuda()
+    acc = torch.zeros((B, 4, n), device="cuda")
+    parents = torch.full((B, 1), -1, dtype=torch.int32, device="cuda")
+    got = {"tree": sts_attn.tree_attention(dq, k, v, parents, dl, ds, scale_for(D)),
+           "masked": sts_attn.masked_attention(dq, k, v, dl, ds, scale_for(D)),
+           "weights": sts_attn.decode_ring_weights(dq[:, 0].contiguous(), k, v, acc, dl, ds, scale_for(D))[:, None]}
+    want = np.stack([attend64_channels(q[b], w.rows(b, w.k), w.rows(b, w.v), np.ones((1, int(w.lens[b])), bool),
+                                       scale_for(D))[0] for b in range(B)])
+    for name, x in got.items():
+        err = np.linalg.norm(x.cpu().numpy() - want) / np.linalg.norm(want)
+        assert err <= 6e-7, f"{name}: {err:.2e}"
