@@ -232,12 +232,15 @@ int sts_prefill_attention_bf16kv(const float* q, const uint16_t* k16, const uint
  *   starts[b]    slot of its oldest row, 0..max_len-1      (device int32)
  *   row r of stream b lives in slot (starts[b] + r) % max_len
  * with values outside their ranges clamped on the device as there.  Query head
- * h reads K/V head h / (heads / kv_heads); q and out are f32, and so is the
- * arithmetic for either row type.  One head's rows take less than 2 GiB.  What
- * a query does not see has no influence on it beyond the rounding of f32, whatever
- * values are there.  Queries, K and V of up to 1e30 in magnitude are served; where
- * a query sees an infinity or NaN its outputs follow f32 arithmetic over f32 rows and
- * are undefined over bf16 rows.
+ * h reads K/V head h / (heads / kv_heads); q and out are f32, and the arithmetic is
+ * of f32's grade for either row type, every output channel held by its own values:
+ * f32 products, or products of bf16 parts that add up to the f32 values.  One head's
+ * rows take less than 2 GiB.  What a query does not see has no influence on it beyond
+ * the rounding of f32, whatever values are there.  Queries, K and V of up to 1e30 in
+ * magnitude whose scores are finite in f32 are served; elements below 2^-110 may be
+ * rounded to multiples of 2^-133, and weights below 2^-110 of a query's largest be
+ * lost.  Where a query sees an infinity or NaN its outputs follow f32 arithmetic over
+ * f32 rows and are undefined over bf16 rows.
  * Splits use the per-(device, stream) workspace as sts_decode_ring does.
  */
 enum sts_row_type {
@@ -399,10 +402,14 @@ int sts_kv_create(uint64_t max_len, uint64_t heads, uint64_t head_dim, sts_kv_ca
  * A mirrored cache needs 16-byte aligned inputs in sts_kv_update.
  * STS_KV_WEIGHTS: the handle keeps, for every slot and K/V head, the attention
  * weight its row was given by sts_kv_attend and sts_kv_decode_step (summed over
- * the heads of the group, as sts_decode_ring_weights does), for sts_kv_evict.  A row appended through
- * the handle starts at zero; the attention of sts_kv_prefill and
- * sts_kv_tree_step is not counted, and rows entered by sts_kv_advance keep what
- * their slots had.  Query heads are set before the first use.
+ * the heads of the group, as sts_decode_ring_weights does), for sts_kv_evict.  A
+ * row appended through the handle starts at zero; the attention of sts_kv_prefill
+ * and sts_kv_tree_step is not counted, and rows entered by sts_kv_advance keep what
+ * their slots had.  Query heads are set before the first use.  With it
+ * sts_kv_attend, sts_kv_decode_step and sts_kv_evict write the handle's weights and
+ * one scratch of its own: their work on one handle must not overlap in time (calls
+ * on one stream do not), sts_kv_attend's, which only reads such handles as keep no
+ * weights, included.
  */
 int sts_kv_create_ex(uint64_t max_len, uint64_t heads, uint64_t head_dim, uint32_t flags,
                      sts_kv_cache** out);

@@ -764,8 +764,8 @@ int launch_decode(DecodeParams p, uint32_t batch, uint32_t head_dim, uint32_t ma
   DecodePlan pl = plan_decode(units, max_rows);
   // Ranges are often far shorter than max_rows, and splits without rows cost their
   // launch: with a workgroup for each CU without splitting, splits twice as long (64
-  // tokens of 32 heads over 300 rows of 3000 95 us for 121; 9 tokens over 700 rows 35
-  // for 40, over up to 2777 rows 78 for 74).
+  // tokens of 32 heads over 300 rows of 3000 99 us for 127; 9 tokens over up to 700
+  // rows 33 for 39.5, over up to 2777 rows 74 for 73).
   if (p.masked && units >= (uint64_t)device_cu_count()) {
     pl.chunk *= 2;
     pl.nsplit = (max_rows + pl.chunk - 1) / pl.chunk;

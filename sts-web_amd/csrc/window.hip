@@ -79,8 +79,8 @@ WindowPlan plan_window(const WindowParams& p, WindowMode mode, uint32_t batch, b
   // One row tile is bound by the reads: as many workgroups as keep 64 KB of rows
   // requested on each CU (f32 rows of 128 one, bf16 rows of 64 four; at 7 streams of
   // 20011 such rows 52 us against 102 with one).  Two are bound by their products:
-  // two workgroups, what a CU holds at once (a draft of 60 over 3000 rows 34 us, with
-  // four 49).
+  // two workgroups, what a CU holds at once (a draft of 60 over 3000 rows 37 us, with
+  // four 54; 24 drafts of 40 nodes 202 and 200).
   const uint32_t tile = pl.row_tiles > 1 || bf16 ? 32 : 16;
   const uint32_t wide = p.dh <= 64 ? 64 : 128;
   const uint32_t tile_bytes = 2 * tile * wide * (bf16 ? 2 : 4) * window::kWaves;
@@ -94,7 +94,7 @@ WindowPlan plan_window(const WindowParams& p, WindowMode mode, uint32_t batch, b
     // Streams of different ages: splits of about equal length whatever their stream,
     // not more than fit at once where one round can hold them (rounding up gives each
     // window half a split more).  Products in several rounds end more evenly with
-    // splits of half the length (24 streams of 900 to 3000 rows 178 us for 183), reads
+    // splits of half the length (24 streams of 900 to 3000 rows 202 us for 213), reads
     // do not (9 tokens over 700 rows 40 us, with half 49).
     const uint64_t rounds = pl.row_tiles > 1 ? 2 : 1;
     const uint64_t fit = 2 * units <= target ? target - units / 2 : rounds * target;

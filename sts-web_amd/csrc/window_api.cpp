@@ -64,10 +64,10 @@ namespace kv {
 
 // One token a stream, with the scores kept or under a range: where every head has K
 // and V rows of its own, in f32, the decode kernel, which has no matrix tile to leave
-// 15/16 empty (kept, 32 heads of 3000 rows 17.5 us against 22, 64 such streams 550
-// against 577, and on a handle it also rotates and appends the token's rows, a launch
-// less; under a range, 2777 rows 18 us against 24, 64 streams over 300 rows each 93
-// against 113); else the window kernel, which reads the rows of a group of heads, or
+// 15/16 empty (kept, the account included, 32 heads of 3000 rows 22 us against 27, 64
+// streams of 128 to 3000 rows 559 against 592, and on a handle it also rotates and
+// appends the token's rows, a launch less; under a range, 2777 rows 17.5 us against
+// 22.5, 64 streams over 300 rows of 3000 99 against 112); else the window kernel, which reads the rows of a group of heads, or
 // bf16 rows, once.
 static bool by_decode(const WindowParams& p, bool bf16) { return p.group == 1 && !bf16; }
 
