@@ -67,8 +67,8 @@ namespace kv {
 // 15/16 empty (kept, the account included, 32 heads of 3000 rows 22 us against 27, 64
 // streams of 128 to 3000 rows 559 against 592, and on a handle it also rotates and
 // appends the token's rows, a launch less; under a range, 2777 rows 17.5 us against
-// 22.5, 64 streams over 300 rows of 3000 99 against 112); else the window kernel, which reads the rows of a group of heads, or
-// bf16 rows, once.
+// 22.5, 64 streams over 300 rows of 3000 99 against 112); else the window kernel,
+// which reads the rows of a group of heads, or bf16 rows, once.
 static bool by_decode(const WindowParams& p, bool bf16) { return p.group == 1 && !bf16; }
 
 static DecodeParams decode_params(const WindowParams& p) {

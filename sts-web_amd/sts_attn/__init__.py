@@ -322,7 +322,10 @@ def _empty(shape, dtype, device, stream) -> torch.Tensor:
     if stream is not None:
         handle = _stream(stream)
         if handle != _stream(None):
-            with torch.cuda.stream(torch.cuda.ExternalStream(handle) if isinstance(stream, int) else stream):
+            s = stream
+            if isinstance(stream, int):  # (an ExternalStream of 0 would be a new stream)
+                s = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+            with torch.cuda.stream(s):
                 t = torch.empty(shape, dtype=dtype, device=device)
             t.record_stream(torch.cuda.current_stream())
             return t

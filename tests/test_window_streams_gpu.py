@@ -48,6 +48,31 @@ def test_new_memory_is_not_the_current_streams(gpu, what, as_handle):
     assert (copy == 7.0).all()
 
 
+def test_new_memory_for_the_null_stream(gpu):
+    """The same with another stream current and the null stream's handle given."""
+    w = Window(46, 1, 4, 900, 64, [900])
+    w.k, w.v = w.k.nan_to_num(0.0), w.v.nan_to_num(0.0)
+    k, v, dl, ds = w.dev("k", "v", "lens", "starts")
+    q = torch.from_numpy(queries(w.rng, 1, 4, 64)).cuda()
+    out = torch.zeros_like(q)
+    acc = [torch.zeros((1, 4, 900), device="cuda") for _ in range(2)]
+    words = sts_attn.load().sts_decode_ring_weights_scratch(1, 4, 900)
+    sts_attn.decode_ring_weights(q, k, v, acc[0], dl, ds, 0.125, out=out)  # allocates, and frees, on the null stream
+    torch.cuda.synchronize()
+    block = torch.full((words,), 7.0, device="cuda")
+    where = block.data_ptr()
+    torch.cuda.synchronize()
+    del block  # free for work on the null stream, and for it alone
+    seen = []
+    real = sts_attn._empty
+    with pytest.MonkeyPatch.context() as m, torch.cuda.stream(torch.cuda.Stream()):
+        m.setattr(sts_attn, "_empty", lambda *a: seen.append(real(*a)) or seen[-1])
+        sts_attn.decode_ring_weights(q, k, v, acc[1], dl, ds, 0.125, out=out, stream=0)
+        assert [t.data_ptr() for t in seen] == [where]
+    torch.cuda.synchronize()
+    assert torch.equal(acc[0], acc[1])
+
+
 def test_results_of_another_stream_outlive_it(gpu):
     """A result that the current stream still reads is not overwritten by the next
     call on the stream that made it."""
