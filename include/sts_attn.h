@@ -94,6 +94,9 @@ enum sts_precision {
                                  within 1e-4 far beyond).  Prefill only.         */
 };
 
+/* The RoPE tables' handle (sts_rope_create). */
+typedef struct sts_rope sts_rope;
+
 /* Message for the calling thread's most recent failed call ("" if none). */
 const char* sts_last_error(void);
 
@@ -334,10 +337,131 @@ int sts_evict_ring(void* k_cache, void* v_cache, float* weights, int32_t* kept, 
                    uint32_t max_len, uint32_t keep, uint32_t recent, int row_type, void* stream);
 
 /* ------------------------------------------------------------------------ */
-/* RoPE (model.rs:38-122)                                                     */
+/* K/V rows in pages                                                         */
 /* ------------------------------------------------------------------------ */
 
-typedef struct sts_rope sts_rope;
+/*
+ * The calls of this section have no counterpart in the reference.  Streams keep their
+ * rows in pages of one pool, in f32, in bf16 or in 8 bits:
+ *   k, v           [pages][kv_heads][page_rows][head_dim] of row_type (device memory,
+ *                  16-byte aligned); page_rows a power of two in 16..4096; head_dim at
+ *                  most 128, a multiple of 4 (f32), 8 (bf16) or 16 (int8)
+ *   k_scale, v_scale  [pages][kv_heads][page_rows] f32 (int8 rows only, 16-byte aligned)
+ *   table          [batch][max_pages] (device int32): row r of stream b is row
+ *                  r % page_rows of page table[b][r / page_rows].  Streams may share
+ *                  pages that they only read.
+ *   lens[b]        rows of stream b (device int32), those to be appended included;
+ *                  taken as 0 below that and as max_rows above
+ *   max_rows       what no stream's rows exceed, at most max_pages * page_rows; the
+ *                  work is planned for it
+ * A table entry outside 0..pages-1 is no page: its rows are not written, read back as
+ * zeros and have no part in the attention.
+ *
+ * 8-bit rows: a row of a head is kept as whole numbers c of -127..127 and a scale s, and
+ * stands for c s: s = max|x| / 127 rounded to f32, c the whole number nearest to x / s
+ * (the even one of two).  A row whose largest value is below 2^-64 is kept as zeros, a
+ * row with an infinity or NaN as NaN (codes 0 under a scale of NaN).
+ */
+enum sts_page_type {
+  STS_PAGES_F32 = 0,
+  STS_PAGES_BF16 = 1,
+  STS_PAGES_INT8 = 2
+};
+
+typedef struct sts_pages {
+  void* k;
+  void* v;
+  float* k_scale; /* NULL unless row_type is STS_PAGES_INT8 */
+  float* v_scale;
+  uint32_t pages;
+  uint32_t page_rows;
+  uint32_t kv_heads;
+  uint32_t head_dim;
+  int32_t row_type; /* sts_page_type */
+} sts_pages;
+
+/*
+ * Writes each stream's newest counts[b] rows (device int32; NULL: `seq`; at most `seq`
+ * and lens[b]), rows lens[b] - counts[b] and on, rounding them to the pages' type (bf16:
+ * nearest even).  Token i of stream b is at k_new, v_new + (b * seq + i) * new_stride, its
+ * kv_heads rows of head_dim floats in turn (new_stride a multiple of 4: a packed qkv's
+ * row, for one).  With `rope`, K rows are rotated first, each at its row index; max_rows
+ * within the table.
+ */
+int sts_paged_append(const sts_pages* pages, const sts_rope* rope, const float* k_new,
+                     const float* v_new, uint64_t new_stride, const int32_t* table,
+                     const int32_t* counts, const int32_t* lens, uint32_t batch, uint32_t seq,
+                     uint32_t max_pages, uint32_t max_rows, void* stream);
+
+/*
+ * Attention of one query a stream over all of its rows (sts_decode_ring's, over pages):
+ * out_h = softmax(scale * q_h . k) v, query head h reading K/V head h / (heads /
+ * kv_heads).  Stream b's query is at q + b * q_stride (heads rows of head_dim floats;
+ * q_stride a multiple of 4), out is [batch][heads][head_dim]; a stream without rows gets
+ * zeros.  With k_new and v_new (both or neither) each stream's newest row is appended
+ * first, as sts_paged_append does with seq 1.  With `rope` the query is rotated at the
+ * newest row's index, and k_new with it.  The arithmetic is of f32's grade on the values
+ * that the rows stand for: f32 products, or products of bf16 parts that add up to the f32
+ * values.  Queries and values of up to 1e30 in magnitude are served; elements below
+ * 2^-110, and weights below 2^-110 of the largest, may be lost (2^-39 over 8-bit rows
+ * whose values are near 2^-64).
+ * Where an infinity or NaN is seen, outputs follow f32 arithmetic over f32 rows and are
+ * undefined over bf16 rows.  Splits use the per-(device, stream) workspace as
+ * sts_decode_ring does.
+ */
+int sts_paged_decode(const sts_pages* pages, const sts_rope* rope, const float* q,
+                     uint64_t q_stride, const float* k_new, const float* v_new,
+                     uint64_t new_stride, float* out, const int32_t* table, const int32_t* lens,
+                     uint32_t batch, uint32_t heads, uint32_t max_pages, uint32_t max_rows,
+                     float scale, void* stream);
+
+/*
+ * Reads rows back: row first[b] + i (device int32, NULL: 0) of stream b becomes row i of
+ * k_out, v_out [batch][kv_heads][max_len][head_dim], for all i < max_len that it has; the
+ * rows behind are left as they were.  out_type: STS_ROWS_F32 or STS_ROWS_BF16 (rounded to
+ * nearest even).  The caches are then rings with starts 0, for the calls above.
+ */
+int sts_paged_gather(const sts_pages* pages, void* k_out, void* v_out, const int32_t* table,
+                     const int32_t* first, const int32_t* lens, uint32_t batch,
+                     uint32_t max_pages, uint32_t max_rows, uint32_t max_len, int out_type,
+                     void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* The verdict on a draft                                                    */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Speculative sampling down a tree of drafted tokens (no counterpart in the reference):
+ * between sts_tree_attention, on whose nodes the target model gave its probabilities, and
+ * sts_tree_commit, which takes `path` and `accepted` as they are.  Node 0 is the last
+ * token, already decided, and always kept; every other hangs below it, parents before
+ * children.  At a kept node let p = target, q = draft there, r = p and m = 1; its children
+ * in turn, of token x:
+ *   kept if rand[child] * q(x) * m < r(x): the walk goes on at the child;
+ *   else r <- max(0, r / m - q), m <- sum r (as they were where that sum is zero)
+ * and where none is kept, the next token is the first at which the running sum of r
+ * passes rand[node 0] * sum r.  Children drawn from q then leave tokens distributed as the
+ * target's.  draft NULL: children chosen without chance, q = 1 at the child's own token:
+ * r(x) <- 0, m <- sum r instead.
+ *   target, draft   [batch][nodes][vocab] probabilities after each node (f32; negative
+ *                   ones and NaN count as 0)
+ *   tokens, parents [batch][nodes] (device int32); a node whose parent is no earlier one
+ *                   is never kept, nor one whose token is outside 0..vocab-1
+ *   counts          [batch] nodes of each stream, or NULL (device int32)
+ *   rand            [batch][nodes] in [0, 1)
+ *   path            [batch][nodes] the kept nodes, then -1;  accepted [batch] how many
+ *   next            [batch] the token after them (-1 where all of p is 0, or no node is)
+ * Sums and comparisons are in 64 bits: path, accepted and next are those of exact
+ * arithmetic unless a number of `rand` lies within 2^-45 of a border.
+ */
+int sts_verify_draft(const float* target, const float* draft, const int32_t* tokens,
+                     const int32_t* parents, const int32_t* counts, const float* rand,
+                     int32_t* path, int32_t* accepted, int32_t* next, uint32_t batch,
+                     uint32_t nodes, uint32_t vocab, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* RoPE (model.rs:38-122)                                                     */
+/* ------------------------------------------------------------------------ */
 
 /*
  * Builds the cos/sin tables [max_seq_len][head_dim/2] of RoPE::new

@@ -1,0 +1,50 @@
+// page_rows.hpp -- device code shared by the kernels over paged K/V rows.
+#pragma once
+
+#include <cfloat>
+
+#include "pages.hpp"
+#include "sts_attn.h"
+
+namespace sts {
+
+// Rows of stream b.
+__device__ __forceinline__ uint32_t paged_len(const PagedRows& p, uint32_t b) {
+  const int32_t n = p.lens[b];
+  return n <= 0 ? 0u : min((uint32_t)n, p.max_rows);
+}
+
+// Row r of stream b, head j as a row index into k, v and their scales; false where no
+// page holds it.
+__device__ __forceinline__ bool paged_row(const PagedRows& p, uint32_t b, uint32_t j, uint32_t r, uint64_t& at) {
+  const uint32_t page = (uint32_t)p.table[(uint64_t)b * p.max_pages + (r >> p.shift)];
+  at = (((uint64_t)page * p.KH + j) << p.shift) + (r & ((1u << p.shift) - 1));
+  return page < p.pages;
+}
+
+// 8-bit rows.  A row is kept as codes c in -127..127 and one f32 scale s, the value
+// being c s: s = max|x| / 127 rounded to f32, c the whole number nearest to x / s (of
+// two, the even one).
+//
+// The row's scale; rows whose largest value is below 2^-64 are kept as zeros (their scale
+// times an attention weight would lose bits to f32's lower end), rows with an infinity or
+// NaN as NaN.
+__device__ __forceinline__ float row_scale(float top) {
+  if (!(top <= FLT_MAX)) return __builtin_nanf("");
+  return top < 0x1p-64f ? 0.f : top / 127.f;
+}
+
+// The code of x under scale s (by = 1 / s, rounded): x by, rounded, is at most one
+// step off; what it leaves of x is exact in f32 (x itself below s / 2, else a
+// difference of multiples of a unit of s, or of x between s / 2 and s) and says whether
+// the next code is nearer.
+__device__ __forceinline__ int row_code(float x, float s, float by) {
+  const float c = rintf(x * by);
+  const float left = fmaf(-c, s, x), half = 0.5f * s;
+  int code = (int)c;
+  if (left > half || (left == half && (code & 1))) ++code;
+  else if (left < -half || (left == -half && (code & 1))) --code;
+  return min(max(code, -127), 127);
+}
+
+}  // namespace sts

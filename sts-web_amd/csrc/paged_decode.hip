@@ -1,0 +1,621 @@
+// paged_decode.hip -- attention of one query a stream over K/V rows in pages (gfx950).
+// No counterpart in the reference, whose decode reads one ring a stream
+// (crates/sts-wasm/src/model.rs:598-668).
+//
+// For query head h over the rows r of its stream
+//   out_h = sum_r 2^(x_r - m) v_r / sum_r 2^(x_r - m),  x_r = scale log2(e) q_h.k_r
+// in one pass with a running maximum m and sum in f32.
+//
+// A workgroup takes up to 16 query heads of one (stream, K/V head) and one split of
+// the stream's rows; its four waves deal the split's tiles among themselves.  A tile is
+// 16 rows of f32, 32 of bf16, 64 of int8: at a head dim of 128 16 KB of K and V, which
+// a wave has requested while it works on the last.  Sixteen rows lie in one page, so
+// that each has a buffer resource of its own, ending with the stream's rows or empty
+// where no page holds them: a lane's offsets are the same for all tiles, rows that are
+// not there read as zeros, and pools may pass 4 GB.
+//   S^T = K Q^T     A = K: lane (m, g) = (lane & 15, lane >> 4) holds row m; B = Q
+//   O^T += V^T P^T  A = V^T: the lane holds of rows 4g + i the dims (16 c + m) VW + e;
+//                   B = the weights as the first product leaves them in the lane
+// f32 rows multiply in f32 (16x16x4).  bf16 rows are operands as they stand, against Q
+// and the weights as three bf16 parts each, which add up to the f32 values; int8 codes
+// are whole numbers that bf16 holds, and their rows' scales go into the scores and the
+// weights.  Every product is therefore of f32's grade.
+#include <algorithm>
+
+#include "coherent.hpp"
+#include "common.hpp"
+#include "lane.hpp"
+#include "page_rows.hpp"
+#include "rope.hpp"
+#include "score.hpp"
+
+namespace sts {
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kNt = 2;  // cache policy: nontemporal, each row is read once
+constexpr uint32_t kOutside = 0x80000000u;  // past every buffer resource: loads zeros
+constexpr int kMaxSplits = 128;
+constexpr int kParts = 3;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+template <int WORDS>
+struct Words {
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t off) {
+    if constexpr (WORDS == 4) {
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, kNt);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = x[i];
+    } else if constexpr (WORDS == 2) {
+      const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, kNt);
+      w[0] = x[0];
+      w[1] = x[1];
+    } else {
+      w[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, kNt);
+    }
+  }
+};
+
+// x[8] as three operands of bf16 values, each the nearest to what the ones before
+// leave: their sum is x to 2^-26 of it (bf16 has f32's exponents).
+__device__ __forceinline__ void parts_of(const float* x, bf16x8 (&y)[kParts]) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  u32x4 w[kParts];
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    float a = x[e], z = x[e + 1];
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) {
+      w[n][e / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, z}, b2));
+      a -= __uint_as_float(w[n][e / 2] << 16);
+      z -= __uint_as_float(w[n][e / 2] & 0xffff0000u);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < kParts; ++n) y[n] = __builtin_bit_cast(bf16x8, w[n]);
+}
+
+// The code in byte B of w as a float; whole numbers up to 127 are bf16 values, the
+// upper half of the float's bits.
+template <int B>
+__device__ __forceinline__ uint32_t code_bits(uint32_t w) {
+  return __float_as_uint((float)(int)(int8_t)(w >> (8 * B)));
+}
+__device__ __forceinline__ uint32_t pair_up(uint32_t hi, uint32_t lo) {
+  return __builtin_amdgcn_perm(hi, lo, 0x07060302);
+}
+
+template <int D, int TYPE, bool PAD>
+__global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const PagedDecode p) {
+  constexpr bool F32 = TYPE == STS_PAGES_F32, I8 = TYPE == STS_PAGES_INT8;
+  constexpr int ES = F32 ? 4 : I8 ? 1 : 2;
+  constexpr int CW = 16 / ES;                     // dims of K a lane loads at once
+  constexpr int NC = D / (4 * CW);                // loads per K row
+  constexpr int VW = CW < D / 16 ? CW : D / 16;   // dims of V a lane loads at once
+  constexpr int NV = D / (16 * VW);               // loads per V row
+  constexpr int KT = F32 ? 1 : I8 ? 4 : 2;        // 16-row tiles a wave takes at once
+  constexpr int TILE = 16 * KT;
+  constexpr int NX = NV * VW;                     // 16-dim tiles of the output
+  constexpr int NP = D / 32;                      // 32-dim steps of K Q^T
+  constexpr int LDO = D + 4;                      // LDS row of a partial output
+  constexpr int C4 = D / 4;
+
+  constexpr int kPartBytes = F32 ? 0 : NP * kParts * 64 * 16;
+  constexpr int kOutBytes = kWaves * 16 * LDO * 4;
+  constexpr int kMergeBytes = 2 * kMaxSplits * 16 * 4 + kWaves * 64 * 16;
+  constexpr int kMostBytes = kPartBytes > kOutBytes ? kPartBytes : kOutBytes;
+  __shared__ __align__(16) char s_mem[kMostBytes > kMergeBytes ? kMostBytes : kMergeBytes];
+  auto& s_q = *reinterpret_cast<bf16x8(*)[NP][kParts][64]>(s_mem);
+  auto& s_o = *reinterpret_cast<float(*)[kWaves][16][LDO]>(s_mem);
+  __shared__ float s_ml[kWaves][16][2];
+  __shared__ uint32_t s_last;
+
+  const PagedRows& rows = p.rows;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m16 = lane & 15, g = lane >> 4;
+  const uint32_t rb = blockIdx.x % p.rblocks, share = blockIdx.x / p.rblocks;
+  uint32_t b, kvh, split, splits;
+  uint32_t first;  // splits of the streams before, each counted once for all heads
+  uint32_t len;
+  if (p.rows_factor > 0.f) {
+    // Streams of different lengths are cut into splits of about the same length: lane
+    // x looks at stream x, and the share's stream is the last whose streams before take
+    // no more shares.
+    const uint32_t mine_len = lane < (int)p.batch ? paged_len(rows, lane) : 0u;
+    float total = (float)mine_len;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x, 64);
+    const uint32_t chunk = max((uint32_t)min(total * p.rows_factor, 0x1p31f) + 1, (uint32_t)(kWaves * TILE));
+    const uint32_t mine = lane < (int)p.batch ? min(max((mine_len + chunk - 1) / chunk, 1u), p.nsplit) : 0;
+    uint32_t before = mine;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) {
+      const uint32_t y = (uint32_t)__shfl_up((int)before, x, 64);
+      before += lane >= x ? y : 0;
+    }
+    if (share >= (uint32_t)__builtin_amdgcn_readlane((int)before, 63) * rows.KH) return;
+    before -= mine;
+    b = 63 - __builtin_clzll(__ballot(lane < (int)p.batch && before * rows.KH <= share));
+    splits = (uint32_t)__builtin_amdgcn_readlane((int)mine, b);
+    first = (uint32_t)__builtin_amdgcn_readlane((int)before, b);
+    const uint32_t at = share - first * rows.KH;
+    kvh = at % rows.KH;
+    split = at / rows.KH;
+    len = (uint32_t)__builtin_amdgcn_readlane((int)mine_len, b);
+  } else {
+    splits = p.nsplit;
+    split = share % splits;
+    kvh = share / splits % rows.KH;
+    b = share / splits / rows.KH;
+    first = b * splits;
+    len = __builtin_amdgcn_readfirstlane(paged_len(rows, b));
+  }
+  const uint32_t dh = PAD ? rows.dh : (uint32_t)D;
+  const uint32_t h0 = kvh * p.group + rb * 16;           // the block's first query head
+  const uint32_t live = min(p.group - rb * 16, 16u);     // its heads
+  float* out = p.out + ((uint64_t)b * p.H + h0) * dh;
+  if (len == 0) {
+    if (split == 0)
+      for (uint32_t t = tid; t < live * dh; t += kWaves * 64) out[t] = 0.f;
+    return;
+  }
+  // Tiles of TILE rows, dealt to the splits and waves in turn; a split gets at least a
+  // tile for each wave.
+  const uint32_t tiles = (len + TILE - 1) / TILE;
+  const uint32_t nsplit = min(splits, (tiles + kWaves - 1) / kWaves);
+  if (split >= nsplit) return;
+  const uint32_t tstep = nsplit * kWaves;
+  uint32_t t = split + nsplit * wave;
+
+  // The pages of a tile: lane x of each four asks for sixteen rows x of the tile.
+  const __amdgpu_buffer_rsrc_t trs =
+      coherent_rsrc(rows.table + (uint64_t)b * rows.max_pages, rows.max_pages * 4);
+  auto ask_pages = [&](uint32_t t) {
+    const uint32_t r = t * TILE + (lane & (KT - 1)) * 16;
+    return __builtin_amdgcn_raw_buffer_load_b32(trs, r < len ? (r >> rows.shift) * 4 : kOutside, 0, 0);
+  };
+  // Where the tile's rows are.  Uniform.
+  struct Where {
+    uint64_t at;    // row index of the first
+    uint32_t rows;  // how many there are
+  };
+  auto find = [&](uint32_t t, uint32_t asked, Where (&w)[KT]) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)asked, kt);
+      const uint32_t r0 = t * TILE + kt * 16;
+      w[kt].at = (((uint64_t)page * rows.KH + kvh) << rows.shift) + (r0 & ((1u << rows.shift) - 1));
+      w[kt].rows = r0 < len && page < rows.pages ? min(len - r0, 16u) : 0u;
+      if (w[kt].rows == 0) w[kt].at = 0;
+    }
+  };
+  typedef Words<CW * ES / 4> KRow[NC];
+  typedef Words<VW * ES / 4> VRow[4][NV];
+  KRow kk[KT];
+  VRow vv[KT];
+  f32x4 ks[I8 ? KT : 1], vs[I8 ? KT : 1];
+  const uint32_t rowb = dh * ES;
+  const uint32_t koff = m16 * rowb + g * (CW * ES);
+  auto load_k = [&](const Where (&w)[KT]) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const __amdgpu_buffer_rsrc_t rs =
+          coherent_rsrc(static_cast<const char*>(rows.k) + w[kt].at * rowb, w[kt].rows * rowb);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        kk[kt][c].load(rs, !PAD || (uint32_t)(c * 4 + g) * CW < dh ? koff + c * (4 * CW * ES) : kOutside);
+      if constexpr (I8) {
+        const __amdgpu_buffer_rsrc_t ss = coherent_rsrc(rows.ks + w[kt].at, w[kt].rows * 4);
+        ks[kt] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ss, g * 16, 0, kNt));
+      }
+    }
+  };
+  auto load_v = [&](const Where (&w)[KT]) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const __amdgpu_buffer_rsrc_t rs =
+          coherent_rsrc(static_cast<const char*>(rows.v) + w[kt].at * rowb, w[kt].rows * rowb);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+          vv[kt][i][c].load(rs, !PAD || (uint32_t)(c * 16 + m16) * VW < dh
+                                    ? (4 * g + i) * rowb + m16 * (VW * ES) + c * (16 * VW * ES) : kOutside);
+      if constexpr (I8) {
+        const __amdgpu_buffer_rsrc_t ss = coherent_rsrc(rows.vs + w[kt].at, w[kt].rows * 4);
+        vs[kt] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ss, g * 16, 0, kNt));
+      }
+    }
+  };
+
+  // The pages are asked for two tiles ahead, so that no rows wait for them but the
+  // first, and the queries, wanted by then, first of all.
+  const bool mine = (uint32_t)m16 < live;  // this lane's column is a query head
+  const float* qsrc = p.q + b * p.q_stride + (uint64_t)(h0 + (mine ? m16 : 0)) * dh;
+  // Dims of the lane's elements in 32-dim step c (f32: of its 4-dim load c).
+  auto q_dim = [&](int c) {
+    return F32 ? (c * 4 + g) * 4 : I8 ? c / 2 * 64 + g * 16 + c % 2 * 8 : (c * 4 + g) * 8;
+  };
+  auto get_q = [&](uint32_t d) {  // four of them, rotated and scaled
+    if (!mine || (PAD && d >= dh)) return make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 y = *reinterpret_cast<const float4*>(qsrc + d);
+    if (rows.rope_cos) {
+      const uint64_t ro = (uint64_t)(len - 1) * (dh / 2) + d / 2;
+      y = rope4(y, *reinterpret_cast<const float2*>(rows.rope_cos + ro),
+                *reinterpret_cast<const float2*>(rows.rope_sin + ro));
+    }
+    return make_float4(y.x * p.qscale, y.y * p.qscale, y.z * p.qscale, y.w * p.qscale);
+  };
+  uint32_t asked = ask_pages(t);
+  uint32_t asked_next = ask_pages(t + tstep);
+  Where now[KT];
+  find(t, asked, now);
+  load_k(now);
+  load_v(now);
+  float qf[F32 ? NC : 1][4];
+  if constexpr (F32) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const float4 y = get_q(q_dim(c));
+      qf[c][0] = y.x;
+      qf[c][1] = y.y;
+      qf[c][2] = y.z;
+      qf[c][3] = y.w;
+    }
+  } else {
+    for (int c = wave; c < NP; c += kWaves) {
+      const float4 y = get_q(q_dim(c)), z = get_q(q_dim(c) + 4);
+      const float x[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+      bf16x8 f[kParts];
+      parts_of(x, f);
+#pragma unroll
+      for (int n = 0; n < kParts; ++n) s_q[c][n][lane] = f[n];
+    }
+    __syncthreads();
+  }
+
+  // The weights are relative to m, which follows the scores' maximum only when they
+  // pass it, and then to 2^kRoom above it: the outputs are seldom rescaled.  (A weight
+  // below 2^-118 of the largest may be lost.)
+  constexpr float kRoom = 8.f;
+  float m = -FLT_MAX, l = 0.f;
+  f32x4 o[NX];
+#pragma unroll
+  for (int x = 0; x < NX; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (; t < tiles; t += tstep) {
+    f32x4 s[KT];
+    if constexpr (F32) {
+      // Four sums of the dims in turn: shorter sums round less.
+      f32x4 sum[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) sum[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          sum[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk[0][c].w[e]), qf[c][e], sum[e], 0, 0, 0);
+      s[0] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    } else {
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NP; ++c) {
+        bf16x8 kf[KT];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          if constexpr (I8) {
+            u32x4 y;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t w = kk[kt][c / 2].w[c % 2 * 2 + i];
+              y[i * 2] = pair_up(code_bits<1>(w), code_bits<0>(w));
+              y[i * 2 + 1] = pair_up(code_bits<3>(w), code_bits<2>(w));
+            }
+            kf[kt] = __builtin_bit_cast(bf16x8, y);
+          } else {
+            kf[kt] = __builtin_bit_cast(bf16x8, kk[kt][c]);
+          }
+        }
+#pragma unroll
+        for (int n = kParts - 1; n >= 0; --n) {
+          const bf16x8 q = s_q[c][n][lane];
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kt], q, s[kt], 0, 0, 0);
+        }
+      }
+      if constexpr (I8) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) s[kt] *= ks[kt];
+      }
+    }
+    // Rows that are not there.
+    uint32_t there = 0;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) there += now[kt].rows;
+    const bool partly = there < TILE;
+    if (partly) {
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((uint32_t)(4 * g + i) >= now[kt].rows) s[kt][i] = -INFINITY;
+    }
+    // The next tile's K, now that this one's is used up.
+    Where next[KT];
+    find(t + tstep, asked_next, next);
+    asked_next = ask_pages(t + 2 * tstep);
+    load_k(next);
+
+    float top = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) top = fmaxf(top, fmaxf(fmaxf(s[kt][0], s[kt][1]), fmaxf(s[kt][2], s[kt][3])));
+    top = max_xor32(max_xor16(top));
+    if (__any(top > m)) {
+      const float to = top > m ? top + kRoom : m, alpha = exp2_hw(m - to);
+      m = to;
+      l *= alpha;
+#pragma unroll
+      for (int x = 0; x < NX; ++x) o[x] *= alpha;
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[kt][i] = exp2_hw(s[kt][i] - m);
+      l += (s[kt][0] + s[kt][1]) + (s[kt][2] + s[kt][3]);
+    }
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int x = 0; x < NX; ++x)
+          o[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vv[0][i][x / VW].w[x % VW]), s[0][i], o[x], 0, 0, 0);
+    } else {
+      if constexpr (I8) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)  // (what lies behind the rows may not be a number)
+            s[kt][i] *= partly && (uint32_t)(4 * g + i) >= now[kt].rows ? 0.f : vs[kt][i];
+      }
+#pragma unroll
+      for (int k2 = 0; k2 < KT; k2 += 2) {
+        bf16x8 pp[kParts];
+        const float w[8] = {s[k2][0], s[k2][1], s[k2][2], s[k2][3],
+                            s[k2 + 1][0], s[k2 + 1][1], s[k2 + 1][2], s[k2 + 1][3]};
+        parts_of(w, pp);
+#pragma unroll
+        for (int x = 0; x < NX; ++x) {
+          u32x4 y;  // the rows' values of dim x, paired along the rows
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t a = vv[k2 + k / 2][k % 2 * 2][x / VW].w[x % VW * ES / 4];
+            const uint32_t z = vv[k2 + k / 2][k % 2 * 2 + 1][x / VW].w[x % VW * ES / 4];
+            if constexpr (I8) {
+              const int sh = x % 4 * 8;
+              y[k] = pair_up(__float_as_uint((float)(int)(int8_t)(z >> sh)), __float_as_uint((float)(int)(int8_t)(a >> sh)));
+            } else {
+              y[k] = __builtin_amdgcn_perm(z, a, x & 1 ? 0x07060302 : 0x05040100);
+            }
+          }
+          const bf16x8 vf = __builtin_bit_cast(bf16x8, y);
+#pragma unroll
+          for (int n = kParts - 1; n >= 0; --n) o[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pp[n], o[x], 0, 0, 0);
+        }
+      }
+    }
+    load_v(next);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) now[kt] = next[kt];
+  }
+  if constexpr (!F32) __syncthreads();  // every wave is done with the queries' parts
+
+  // The waves' states merged through LDS.
+  l = sum_xor32(sum_xor16(l));
+  if (g == 0) {
+    s_ml[wave][m16][0] = m;
+    s_ml[wave][m16][1] = l;
+  }
+  if (mine) {
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < VW; e += 4)
+          *reinterpret_cast<f32x4*>(&s_o[wave][m16][(c * 16 + 4 * g + i) * VW + e]) =
+              f32x4{o[c * VW + e][i], o[c * VW + e + 1][i], o[c * VW + e + 2][i], o[c * VW + e + 3][i]};
+  }
+  __syncthreads();
+  const uint32_t slots = live * C4;  // float4 columns of the block's outputs
+  auto finish = [&](uint32_t x, float4 a, float lt) {
+    const uint32_t row = x / C4, col = x % C4;
+    const float f = lt > 0.f || lt != lt ? 1.f / lt : 0.f;  // nothing seen: zeros
+    if (!PAD || col * 4 < dh)
+      *reinterpret_cast<float4*>(out + (uint64_t)row * dh + col * 4) = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
+  };
+  const uint32_t REC = p.record;  // floats of a split's record: O, then (m, l)
+  const uint64_t unit = ((uint64_t)b * rows.KH + kvh) * p.rblocks + rb;
+  const __amdgpu_buffer_rsrc_t prs =
+      coherent_rsrc(p.part + (((uint64_t)first * rows.KH + kvh * splits) * p.rblocks + rb * splits) * REC,
+                    nsplit > 1 ? splits * REC * 4 : 0);
+  for (uint32_t x = tid; x < slots; x += kWaves * 64) {
+    const uint32_t row = x / C4, col = x % C4;
+    float mt = s_ml[0][row][0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) mt = fmaxf(mt, s_ml[w][row][0]);
+    float lt = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = exp2_hw(s_ml[w][row][0] - mt);
+      lt += f * s_ml[w][row][1];
+      const float4 y = *reinterpret_cast<const float4*>(&s_o[w][row][col * 4]);
+      a.x += f * y.x;
+      a.y += f * y.y;
+      a.z += f * y.z;
+      a.w += f * y.w;
+    }
+    if (nsplit == 1) {
+      finish(x, a, lt);
+    } else {
+      st_coherent4(prs, (split * REC + x * 4) * 4, coh_f4{a.x, a.y, a.z, a.w});
+      if (col == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(mt), __float_as_uint(lt)}, prs,
+                                              (split * REC + live * D + row * 2) * 4, 0, kSc1);
+    }
+  }
+  if (nsplit == 1) return;
+
+  // Every thread's records are acknowledged before the workgroup takes its arrival
+  // ticket; the last one merges the splits, always in the same order.
+  __builtin_amdgcn_s_waitcnt(0);
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+  __syncthreads();
+  if (tid == 0) {
+    const uint32_t ticket = atomicAdd(p.counters + unit, 1u);
+    s_last = ticket == nsplit - 1;
+    if (ticket == nsplit - 1) atomicExch(p.counters + unit, 0u);
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+  // The splits' (m, l) of every head; m gives way to the split's factor 2^(m_s - m).
+  auto& s_f = *reinterpret_cast<float(*)[kMaxSplits][16]>(s_mem);
+  auto& s_l = *reinterpret_cast<float(*)[kMaxSplits][16]>(s_mem + kMaxSplits * 16 * 4);
+  auto& s_sum = *reinterpret_cast<f32x4(*)[kWaves * 64]>(s_mem + 2 * kMaxSplits * 16 * 4);
+  for (uint32_t x = tid; x < nsplit * live; x += kWaves * 64) {
+    const uint32_t sp = x / live, row = x % live;
+    const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(prs, (sp * REC + live * D + row * 2) * 4, 0, kSc1);
+    s_f[sp][row] = __uint_as_float(y[0]);
+    s_l[sp][row] = __uint_as_float(y[1]);
+  }
+  __syncthreads();
+  if (tid < (int)live) {
+    float mt = -FLT_MAX, lt = 0.f;
+    for (uint32_t sp = 0; sp < nsplit; ++sp) mt = fmaxf(mt, s_f[sp][tid]);
+    for (uint32_t sp = 0; sp < nsplit; ++sp) {
+      const float f = exp2_hw(s_f[sp][tid] - mt);
+      s_f[sp][tid] = f;
+      lt += f * s_l[sp][tid];
+    }
+    s_ml[0][tid][1] = lt;
+  }
+  __syncthreads();
+  // Groups of threads, one for each column, take the splits in turn.
+  constexpr int AT = 8;
+  for (uint32_t x0 = 0; x0 < slots; x0 += kWaves * 64) {
+    const uint32_t n = min(slots - x0, (uint32_t)(kWaves * 64)), groups = kWaves * 64 / n;
+    const uint32_t x = x0 + tid % n, grp = tid / n;
+    f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (grp < groups) {
+      for (uint32_t sp = grp; sp < nsplit; sp += AT * groups) {
+        coh_f4 y[AT];
+#pragma unroll
+        for (int u = 0; u < AT; ++u)
+          y[u] = ld_coherent4(prs, sp + u * groups < nsplit ? ((sp + u * groups) * REC + x * 4) * 4 : kOutside);
+#pragma unroll
+        for (int u = 0; u < AT; ++u)
+          if (sp + u * groups < nsplit) a += y[u] * s_f[sp + u * groups][x / C4];
+      }
+    }
+    __syncthreads();
+    s_sum[tid] = a;
+    __syncthreads();
+    if (grp == 0) {
+      for (uint32_t u = 1; u < groups; ++u) a += s_sum[tid + u * n];
+      finish(x, make_float4(a[0], a[1], a[2], a[3]), s_ml[0][x / C4][1]);
+    }
+  }
+}
+
+struct PagedPlan {
+  uint32_t rblocks = 1, nsplit = 1, shares = 0, record = 0;
+  float rows_factor = 0.f;
+};
+
+PagedPlan plan_paged(const PagedDecode& p, uint32_t batch) {
+  PagedPlan pl;
+  const PagedRows& rows = p.rows;
+  pl.rblocks = (p.group + 15) / 16;
+  const uint64_t units = (uint64_t)batch * rows.KH * pl.rblocks;
+  const uint64_t target = (uint64_t)device_cu_count() * 2;
+  // A split is worth its record from a tile for each of its waves on.
+  const uint32_t tile = (rows.type == STS_PAGES_F32 ? 16 : rows.type == STS_PAGES_BF16 ? 32 : 64) * kWaves;
+  const uint64_t most = std::min<uint64_t>((rows.max_rows + tile - 1) / tile, kMaxSplits);
+  if (batch > 1 && batch <= 64) {
+    // Streams of different ages: splits of about equal length whatever their stream,
+    // not more than fit at once where one round can hold them (rounding up gives each
+    // stream half a split more).
+    const uint64_t heads = (uint64_t)rows.KH * pl.rblocks;
+    const uint64_t fit = 2 * units <= target ? target - units / 2 : target;
+    pl.rows_factor = (float)heads / (float)fit;
+    pl.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(fit / heads + 1, most));
+    pl.shares = (uint32_t)(rows.KH * (fit / heads + batch + 1));
+  } else {
+    const uint64_t want = std::max<uint64_t>(1, (target + units - 1) / units);
+    pl.nsplit = (uint32_t)std::max<uint64_t>(1, std::min(want, most));
+    pl.shares = batch * rows.KH * pl.nsplit;
+  }
+  const uint32_t live = std::min(p.group, 16u), wide = rows.dh <= 64 ? 64 : 128;
+  pl.record = live * wide + (2 * live + 3) / 4 * 4;
+  return pl;
+}
+
+int paged_workspace(const PagedDecode& p, const PagedPlan& pl, uint32_t batch, hipStream_t stream, Workspace** out) {
+  *out = nullptr;
+  if (pl.nsplit <= 1) return STS_OK;
+  return get_workspace(stream, (size_t)pl.shares * pl.rblocks * pl.record,
+                       (size_t)batch * p.rows.KH * pl.rblocks, out);
+}
+
+template <int TYPE>
+void launch_type(const PagedDecode& p, dim3 grid, hipStream_t stream) {
+  const dim3 block(kWaves * 64);
+  if (p.rows.dh == 128)
+    hipLaunchKernelGGL((paged_decode_kernel<128, TYPE, false>), grid, block, 0, stream, p);
+  else if (p.rows.dh == 64)
+    hipLaunchKernelGGL((paged_decode_kernel<64, TYPE, false>), grid, block, 0, stream, p);
+  else if (p.rows.dh > 64)
+    hipLaunchKernelGGL((paged_decode_kernel<128, TYPE, true>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((paged_decode_kernel<64, TYPE, true>), grid, block, 0, stream, p);
+}
+
+}  // namespace
+
+int reserve_paged_decode(const PagedDecode& p, uint32_t batch, hipStream_t stream) {
+  Workspace* ws = nullptr;
+  return paged_workspace(p, plan_paged(p, batch), batch, stream, &ws);
+}
+
+int launch_paged_decode(PagedDecode p, uint32_t batch, hipStream_t stream) {
+  const PagedPlan pl = plan_paged(p, batch);
+  Workspace* ws = nullptr;
+  if (int rc = paged_workspace(p, pl, batch, stream, &ws)) return rc;
+  if (ws) {
+    p.part = ws->part;
+    p.counters = ws->counters;
+  }
+  p.rblocks = pl.rblocks;
+  p.nsplit = pl.nsplit;
+  p.shares = pl.shares;
+  p.batch = batch;
+  p.rows_factor = pl.rows_factor;
+  p.record = pl.record;
+  const dim3 grid(pl.shares * pl.rblocks);
+  if (p.rows.type == STS_PAGES_F32) launch_type<STS_PAGES_F32>(p, grid, stream);
+  else if (p.rows.type == STS_PAGES_BF16) launch_type<STS_PAGES_BF16>(p, grid, stream);
+  else launch_type<STS_PAGES_INT8>(p, grid, stream);
+  STS_HIP(hipGetLastError());
+  return STS_OK;
+}
+
+}  // namespace sts

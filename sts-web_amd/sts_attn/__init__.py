@@ -42,6 +42,9 @@ KV_WEIGHTS = 2
 ROWS_F32 = 0
 ROWS_BF16 = 1
 TREE_MAX_NODES = 256
+PAGES_F32 = 0
+PAGES_BF16 = 1
+PAGES_INT8 = 2
 
 _vp = ctypes.c_void_p
 _u32 = ctypes.c_uint32
@@ -60,6 +63,12 @@ class KvState(ctypes.Structure):
     _fields_ = [("offset", _u64), ("len", _u64), ("write_pos", _u64), ("max_len", _u64),
                 ("heads", _u64), ("head_dim", _u64), ("batch", _u64), ("allocated", ctypes.c_int32),
                 ("flags", ctypes.c_int32), ("q_heads", _u64)]
+
+
+class Pages(ctypes.Structure):
+    """sts_pages."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _u32),
+                ("page_rows", _u32), ("kv_heads", _u32), ("head_dim", _u32), ("row_type", ctypes.c_int32)]
 
 
 # name -> (restype, argtypes); the exported set of include/sts_attn.h.
@@ -81,6 +90,10 @@ SIGNATURES = {
     "sts_decode_ring_weights": (_int, [_vp] * 8 + [_u32] * 5 + [_f32, _int, _vp]),
     "sts_decode_ring_weights_scratch": (_u64, [_u32, _u32, _u32]),
     "sts_evict_ring": (_int, [_vp] * 6 + [_u32] * 6 + [_int, _vp]),
+    "sts_paged_append": (_int, [_vp] * 4 + [_u64] + [_vp] * 3 + [_u32] * 4 + [_vp]),
+    "sts_paged_decode": (_int, [_vp] * 3 + [_u64, _vp, _vp, _u64] + [_vp] * 3 + [_u32] * 4 + [_f32, _vp]),
+    "sts_paged_gather": (_int, [_vp] * 6 + [_u32] * 4 + [_int, _vp]),
+    "sts_verify_draft": (_int, [_vp] * 9 + [_u32] * 3 + [_vp]),
     "sts_rope_create": (_int, [_u32, _u32, _f32, ctypes.POINTER(_vp)]),
     "sts_rope_destroy": (_int, [_vp]),
     "sts_rope_apply": (_int, [_vp, _vp, _u32, _u32, _u32, _u32, _vp]),
@@ -460,6 +473,180 @@ def evict_ring(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tens
         _arg(kept, "kept", i32, (B, KH, keep), dev), _arg(lens, "lens", i32, (B,), dev),
         _arg(starts, "starts", i32, (B,), dev), B, KH, D, M, keep, recent, rows, _stream(stream)))
     return kept
+
+
+# ---------------------------------------------------------------------------
+# K/V rows in pages, and the verdict on a draft
+# ---------------------------------------------------------------------------
+
+_PAGE_TYPES = {torch.float32: PAGES_F32, torch.bfloat16: PAGES_BF16, torch.int8: PAGES_INT8}
+
+
+def _heads_stride(t: torch.Tensor, name: str, lead, heads: Optional[int], D: int, device):
+    """(address, stride between tokens in elements) of float32 rows [*lead, heads, D] whose
+    last two dimensions are contiguous and whose tokens are equally far apart."""
+    shape = t.shape
+    if t.dtype is not _f32t:
+        raise TypeError(f"{name} must be {_f32t}, got {t.dtype}")
+    if len(shape) != len(lead) + 2 or shape[-1] != D or tuple(shape[:-2]) != lead or (heads and shape[-2] != heads):
+        want = ", ".join(str(x) for x in (*lead, heads or "heads", D))
+        raise ValueError(f"{name} must be [{want}], got {tuple(shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    st = t.stride()
+    step = st[-3] if shape[-3] > 1 else 0
+    if len(lead) == 2 and shape[0] > 1:
+        # One distance for all tokens: from stream to stream too.
+        if shape[1] == 1:
+            step = st[0]
+        elif st[0] != step * shape[1]:
+            raise ValueError(f"{name}'s tokens must be equally far apart")
+    if (D > 1 and st[-1] != 1) or (shape[-2] > 1 and st[-2] != D):
+        raise ValueError(f"{name}'s heads must be contiguous")
+    return t.data_ptr(), step or shape[-2] * D
+
+
+class PagedKV:
+    """A pool of pages of K/V rows that streams share by page tables.
+
+    k, v [pages, KVH, page_rows, D] float32, bfloat16 or int8, and for int8 k_scale, v_scale
+    [pages, KVH, page_rows] float32: row r of stream b is row r % page_rows of page
+    table[b, r // page_rows] (table [B, P] int32; an entry that is no page holds no rows).
+    lens [B] int32 counts a stream's rows, those to be appended included.  max_rows bounds
+    them (default: what the table can hold)."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+                 v_scale: Optional[torch.Tensor] = None):
+        if k.dtype not in _PAGE_TYPES or v.dtype is not k.dtype:
+            raise TypeError(f"pages must both be float32, bfloat16 or int8, got {k.dtype}, {v.dtype}")
+        if k.dim() != 4 or v.shape != k.shape:
+            raise ValueError(f"pages must both be [pages, KVH, page_rows, D], got {tuple(k.shape)}, {tuple(v.shape)}")
+        if v.device != k.device or not k.is_contiguous() or not v.is_contiguous():
+            raise ValueError("pages must be contiguous and on one device")
+        int8 = k.dtype is torch.int8
+        if int8 and (k_scale is None or v_scale is None):
+            raise ValueError("8-bit pages need k_scale and v_scale")
+        if not int8 and (k_scale is not None or v_scale is not None):
+            raise ValueError(f"{k.dtype} pages have no scales")
+        n, KH, R, D = k.shape
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.n_kv_heads, self.page_rows, self.head_dim, self.device = n, KH, R, D, k.device
+        self._c = Pages(k.data_ptr(), v.data_ptr(), _arg(k_scale, "k_scale", _f32t, (n, KH, R), k.device),
+                        _arg(v_scale, "v_scale", _f32t, (n, KH, R), k.device), n, R, KH, D, _PAGE_TYPES[k.dtype])
+        self._at = ctypes.addressof(self._c)
+
+    @classmethod
+    def empty(cls, pages: int, page_rows: int, n_kv_heads: int, head_dim: int,
+              dtype: torch.dtype = torch.float32, device="cuda") -> "PagedKV":
+        """A pool of zeros."""
+        shape = (pages, n_kv_heads, page_rows, head_dim)
+        k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        if dtype is not torch.int8:
+            return cls(k, v)
+        return cls(k, v, *(torch.zeros(shape[:3], dtype=_f32t, device=device) for _ in range(2)))
+
+    def _streams(self, table: torch.Tensor, lens: torch.Tensor, max_rows: Optional[int]):
+        """(B, P, max_rows, addresses of table and lens), after their checks."""
+        dev = self.device
+        if dev.type != "cuda" or dev.index != torch._C._cuda_getDevice():
+            raise ValueError(f"pages must be on the current GPU, got {dev}")
+        if table.dim() != 2:
+            raise ValueError(f"table must be [B, P], got {tuple(table.shape)}")
+        B, P = table.shape
+        most = P * self.page_rows if max_rows is None else max_rows
+        if most < 0 or most >> 32:
+            raise StsError(STS_ERR_INVALID, f"max_rows {most} out of range")
+        return (B, P, most, _arg(table, "table", _i32, (B, P), dev), _arg(lens, "lens", _i32, (B,), dev))
+
+    def append(self, k_new: torch.Tensor, v_new: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+               counts: Optional[torch.Tensor] = None, rope: Optional["RoPE"] = None,
+               max_rows: Optional[int] = None, stream=None) -> None:
+        """Writes the newest counts[b] rows (default all T) of each stream, in the pages'
+        type: k_new, v_new [B, T, KVH, D] float32, whose tokens may lie apart (a packed
+        qkv's).  With `rope`, K rows are rotated at their row index."""
+        B, P, most, tp, lp = self._streams(table, lens, max_rows)
+        if k_new.dim() != 4:
+            raise ValueError(f"k_new must be [B, T, KVH, D], got {tuple(k_new.shape)}")
+        T, dev = k_new.shape[1], self.device
+        kp, ks = _heads_stride(k_new, "k_new", (B, T), self.n_kv_heads, self.head_dim, dev)
+        vp, vs = _heads_stride(v_new, "v_new", (B, T), self.n_kv_heads, self.head_dim, dev)
+        if ks != vs:
+            raise ValueError("k_new's and v_new's tokens must be equally far apart")
+        _check(load().sts_paged_append(
+            self._at, rope.handle if rope is not None else None, kp, vp, ks, tp,
+            _arg(counts, "counts", _i32, (B,), dev), lp, B, T, P, most, _stream(stream)))
+
+    def decode(self, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float,
+               k_new: Optional[torch.Tensor] = None, v_new: Optional[torch.Tensor] = None,
+               rope: Optional["RoPE"] = None, max_rows: Optional[int] = None,
+               out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """Attention of one query a stream, q [B, H, D] float32, over all of its rows; with
+        k_new, v_new [B, KVH, D] its newest row is appended first.  With `rope`, q and k_new
+        are rotated at the newest row's index.  Streams may lie apart in q, k_new, v_new."""
+        B, P, most, tp, lp = self._streams(table, lens, max_rows)
+        D, dev = self.head_dim, self.device
+        qp, qs = _heads_stride(q, "q", (B,), None, D, dev)
+        H = q.shape[1]
+        kp = vp = None
+        ns = 0
+        if k_new is not None or v_new is not None:
+            if k_new is None or v_new is None:
+                raise ValueError("k_new and v_new must both be given")
+            kp, ns = _heads_stride(k_new, "k_new", (B,), self.n_kv_heads, D, dev)
+            vp, vs = _heads_stride(v_new, "v_new", (B,), self.n_kv_heads, D, dev)
+            if ns != vs:
+                raise ValueError("k_new's and v_new's streams must be equally far apart")
+        if out is None:
+            out = _empty((B, H, D), _f32t, dev, stream)
+            op = out.data_ptr()
+        else:
+            op = _arg(out, "out", _f32t, (B, H, D), dev)
+        _check(load().sts_paged_decode(
+            self._at, rope.handle if rope is not None else None, qp, qs, kp, vp, ns, op, tp, lp, B, H, P,
+            most, scale, _stream(stream)))
+        return out
+
+    def gather(self, table: torch.Tensor, lens: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor,
+               first: Optional[torch.Tensor] = None, max_rows: Optional[int] = None, stream=None) -> None:
+        """Reads rows first[b] (default 0) and on of each stream into rows 0 and on of
+        k_out, v_out [B, KVH, M, D] float32 or bfloat16; the rows behind stay as they were."""
+        B, P, most, tp, lp = self._streams(table, lens, max_rows)
+        dev = self.device
+        if k_out.dtype not in _ROW_TYPES:
+            raise TypeError(f"k_out must be float32 or bfloat16, got {k_out.dtype}")
+        if k_out.dim() != 4:
+            raise ValueError(f"k_out must be [B, KVH, M, D], got {tuple(k_out.shape)}")
+        M = k_out.shape[2]
+        shape = (B, self.n_kv_heads, M, self.head_dim)
+        _check(load().sts_paged_gather(
+            self._at, _arg(k_out, "k_out", k_out.dtype, shape, dev), _arg(v_out, "v_out", k_out.dtype, shape, dev),
+            tp, _arg(first, "first", _i32, (B,), dev), lp, B, P, most, M, _ROW_TYPES[k_out.dtype],
+            _stream(stream)))
+
+
+def verify_draft(target: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, rand: torch.Tensor,
+                 draft: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+                 stream=None):
+    """How far each stream's draft, a tree of T tokens below node 0 (the last token, always
+    kept), holds against the target's probabilities after each node, target [B,T,V] float32:
+    draft [B,T,V] the probabilities that a node's children were drawn from (None: they were
+    chosen without chance), tokens/parents [B,T] and counts [B] int32, rand [B,T] float32
+    in [0, 1): entry i decides node i, entry 0 draws the token that follows.  Returns (path
+    [B,T], accepted [B], next [B]) int32; path and accepted are tree_commit's."""
+    shape, dev = target.shape, target.device
+    if len(shape) != 3:
+        raise ValueError(f"target must be [B, T, V], got {tuple(shape)}")
+    if dev.type != "cuda" or dev.index != torch._C._cuda_getDevice():
+        raise ValueError(f"target must be on the current GPU, got {dev}")
+    B, T, V = shape
+    each, one = (B, T), (B,)
+    args = [_arg(target, "target", _f32t, shape, dev), _arg(draft, "draft", _f32t, shape, dev),
+            _arg(tokens, "tokens", _i32, each, dev), _arg(parents, "parents", _i32, each, dev),
+            _arg(counts, "counts", _i32, one, dev), _arg(rand, "rand", _f32t, each, dev)]
+    path, accepted, following = (_empty(s, _i32, dev, stream) for s in (each, one, one))
+    _check(load().sts_verify_draft(*args, path.data_ptr(), accepted.data_ptr(), following.data_ptr(), B, T, V,
+                                   _stream(stream)))
+    return path, accepted, following
 
 
 # ---------------------------------------------------------------------------

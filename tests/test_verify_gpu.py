@@ -1,0 +1,212 @@
+"""The verdict on a draft on the GPU, against exact fractions."""
+import numpy as np
+import pytest
+import torch
+
+import sts_attn
+from conftest import scale_for
+from pages import verdict
+from windows import Window, attend64_channels, queries, tree_seen
+
+pytestmark = pytest.mark.gpu
+
+
+def soft(x):
+    e = np.exp(x - x.max(-1, keepdims=True))
+    return (e / e.sum(-1, keepdims=True)).astype(np.float32)
+
+
+def tree(rng, T):
+    parents = np.full(T, -1, np.int32)
+    for i in range(1, T):
+        parents[i] = i - 1 if rng.random() < 0.3 else rng.integers(0, i)
+    return parents
+
+
+def check(target, draft, tokens, parents, rand, counts=None):
+    B, T, V = target.shape
+    dev = [None if x is None else torch.from_numpy(np.ascontiguousarray(x)).cuda()
+           for x in (target, tokens.astype(np.int32), parents.astype(np.int32), rand.astype(np.float32), draft,
+                     None if counts is None else np.asarray(counts, np.int32))]
+    path, accepted, following = (x.cpu().numpy() for x in sts_attn.verify_draft(*dev[:4], draft=dev[4], counts=dev[5]))
+    taken = 0
+    for b in range(B):
+        n = T if counts is None else min(max(int(counts[b]), 0), T)
+        want, word = verdict(target[b], None if draft is None else draft[b], tokens[b], parents[b], n, rand[b])
+        assert list(path[b][:len(want)]) == want and (path[b][len(want):] == -1).all(), (b, path[b], want)
+        assert accepted[b] == len(want) and following[b] == word, (b, following[b], word)
+        taken += max(len(want) - 1, 0)
+    return taken
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("V", [1, 2, 3, 5, 255, 257, 1000, 4097])
+def test_trees(gpu, V, drawn):
+    """Random trees, some nodes kept and some not, some streams with fewer nodes."""
+    rng = np.random.default_rng(V + drawn)
+    B, T = 12, 14
+    x = rng.standard_normal((B, T, V)) * 2
+    target, draft = soft(x), soft(0.7 * x + 0.5 * rng.standard_normal((B, T, V)))
+    parents = np.stack([tree(rng, T) for _ in range(B)])
+    tokens = np.zeros((B, T), np.int32)
+    for b in range(B):
+        for i in range(1, T):
+            q = draft[b, parents[b, i]].astype(np.float64)
+            tokens[b, i] = rng.choice(V, p=q / q.sum()) if drawn else np.argsort(-q)[min(i % 3, V - 1)]
+    counts = rng.integers(0, T + 2, B)
+    taken = check(target, draft if drawn else None, tokens, parents, rng.random((B, T), np.float32), counts)
+    assert taken > 0 or V > 1000  # (of thousands of words none is likely)
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+def test_large_vocabulary(gpu, drawn):
+    rng = np.random.default_rng(30)
+    B, T, V = 2, 5, 70001
+    x = rng.standard_normal((B, T, V)) * 3
+    target, draft = soft(x), soft(x + 0.8 * rng.standard_normal((B, T, V)))
+    parents = np.array([[-1, 0, 0, 0, 1], [-1, 0, 1, 2, 3]])
+    tokens = rng.integers(0, V, (B, T))
+    tokens[1, 1] = target[1, 0].argmax()
+    check(target, draft if drawn else None, tokens, parents, rng.random((B, T), np.float32))
+
+
+def test_most_nodes(gpu):
+    rng = np.random.default_rng(31)
+    B, T, V = 2, 256, 40
+    target = soft(rng.standard_normal((B, T, V)))
+    parents = np.stack([tree(rng, T), np.r_[-1, np.zeros(T - 1, int)]])  # a tree, and 255 children of one node
+    check(target, None, rng.integers(0, V, (B, T)), parents, rng.random((B, T), np.float32))
+    check(target, soft(rng.standard_normal((B, T, V))), rng.integers(0, V, (B, T)), parents,
+          rng.random((B, T), np.float32))
+
+
+def test_chosen_cases(gpu):
+    """Dyadic probabilities, whose sums are exact: borders, siblings of one token, nothing left."""
+    p = np.array([0.5, 0.25, 0.125, 0.125], np.float32)
+    one = np.array([0, 1, 0, 0], np.float32)
+    half = np.array([0.5, 0.5, 0, 0], np.float32)
+    none = np.zeros(4, np.float32)
+
+    def run(target, tokens, parents, rand, draft=None):
+        T = len(tokens)
+        check(np.broadcast_to(target, (1, T, 4)) if target.ndim == 1 else target[None], draft if draft is None else
+              np.broadcast_to(draft, (1, T, 4)), np.array([tokens]), np.array([parents]), np.array([rand], np.float32))
+
+    for u in (0.0, 0.25, 0.5, 0.75, 0.874, 0.875, 0.999):
+        run(p, [0], [-1], [u])
+        for w in (0.0, 0.249, 0.25, 0.5, 0.75):
+            run(p, [0, 1], [-1, 0], [u, w])
+            run(p, [0, 1], [-1, 0], [u, w], draft=half)
+            run(p, [0, 1, 1, 2], [-1, 0, 0, 0], [u, w, w, w])           # two siblings of one token
+            run(p, [0, 0, 1, 2, 3], [-1, 0, 0, 0, 0], [u, .9, .9, .9, .9])  # every word tried
+            run(p, [0, 1, 0], [-1, 0, 0], [u, w, w], draft=p)            # r = 0 once it is cut: stays as it was
+            run(one, [0, 1, 0], [-1, 0, 0], [u, w, w])
+            run(one, [0, 0, 1], [-1, 0, 0], [u, w, w], draft=half)
+            run(p, [0, 3, 3], [-1, 0, 1], [u, w, w], draft=one)          # a token its draft could not give
+    run(none, [0, 1, 2], [-1, 0, 0], [0.3, 0.0, 0.0])
+    run(none, [0], [-1], [0.0], draft=half)
+    # Tokens and parents that are none.
+    run(p, [0, -1, 4, 2 ** 31 - 1, 1], [-1, 0, 0, 0, 0], [0.6, 0.0, 0.0, 0.0, 0.1])
+    run(p, [0, -7, 0], [-1, 0, 0], [0.6, 0.0, 0.3], draft=half)
+    run(p, [0, 0, 0, 0], [0, 1, 3, -2], [0.6, 0.0, 0.0, 0.0])
+    # Negative probabilities and NaN count as nothing.
+    odd = np.array([np.nan, -0.5, 0.25, 0.75], np.float32)
+    run(odd, [0, 0, 1, 2], [-1, 0, 0, 0], [0.9, 0.0, 0.0, 0.7])
+    run(odd, [0, 2, 3], [-1, 0, 0], [0.9, 0.8, 0.9], draft=np.array([np.nan, 0.25, 0.5, -1], np.float32))
+
+
+def test_tokens_follow_the_target(gpu):
+    """The first token after node 0, kept or drawn, comes as often as the target says: within five
+    standard deviations of a binomial count."""
+    rng = np.random.default_rng(33)
+    B, V = 60000, 5
+    p, q = soft(rng.standard_normal(V)), soft(rng.standard_normal(V))
+    tokens = np.zeros((B, 3), np.int32)
+    tokens[:, 1:] = rng.choice(V, (B, 2), p=q.astype(np.float64) / q.astype(np.float64).sum())
+    target = np.broadcast_to(p, (B, 3, V)).copy()
+    draft = np.broadcast_to(q, (B, 3, V)).copy()
+    parents = np.tile(np.array([-1, 0, 0], np.int32), (B, 1))
+    args = [torch.from_numpy(x).cuda() for x in (target, tokens, parents, rng.random((B, 3), np.float32), draft)]
+    path, accepted, following = (x.cpu().numpy() for x in sts_attn.verify_draft(*args[:4], draft=args[4]))
+    first = np.where(accepted > 1, tokens[np.arange(B), np.maximum(path[:, 1], 0)], following)
+    assert (accepted > 1).mean() > 0.3
+    for v in range(V):
+        want = float(p[v])
+        assert abs((first == v).mean() - want) < 5 * np.sqrt(want * (1 - want) / B), v
+
+
+def test_refusals(gpu):
+    p = torch.zeros((2, 3, 5), device="cuda")
+    i = torch.zeros((2, 3), dtype=torch.int32, device="cuda")
+    u = torch.zeros((2, 3), device="cuda")
+    with pytest.raises(ValueError, match="target"):
+        sts_attn.verify_draft(p[0], i, i, u)
+    with pytest.raises(ValueError, match="tokens"):
+        sts_attn.verify_draft(p, i[:, :2].contiguous(), i, u)
+    with pytest.raises(TypeError, match="tokens"):
+        sts_attn.verify_draft(p, i.long(), i, u)
+    with pytest.raises(ValueError, match="draft"):
+        sts_attn.verify_draft(p, i, i, u, draft=p[:, :2].contiguous())
+    with pytest.raises(ValueError, match="contiguous"):
+        sts_attn.verify_draft(p.transpose(0, 1).contiguous().transpose(0, 1), i, i, u)
+
+
+def test_in_a_graph(gpu):
+    rng = np.random.default_rng(34)
+    B, T, V = 4, 6, 3001
+    target = torch.from_numpy(soft(rng.standard_normal((B, T, V)))).cuda()
+    parents = torch.from_numpy(np.stack([tree(rng, T) for _ in range(B)])).cuda()
+    tokens = target.argmax(-1).int()
+    rand = torch.rand((B, T), device="cuda")
+    sts_attn.verify_draft(target, tokens, parents, rand)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = sts_attn.verify_draft(target, tokens, parents, rand)
+    for _ in range(4):
+        rand.copy_(torch.rand_like(rand) ** 3)
+        tokens.copy_(torch.randint(0, 9, tokens.shape, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, sts_attn.verify_draft(target, tokens, parents, rand)):
+            assert torch.equal(a, b)
+
+
+def test_draft_attended_judged_committed(gpu):
+    """A draft's round as a server runs it: its attention, the verdict, the commit, and the next
+    token's attention over the rows that stayed, against 64 bits."""
+    B, H, KH, M, D, T, V = 5, 4, 2, 90, 64, 8, 300
+    scale = scale_for(D)
+    lens = [60, 33, 89, 8, 20]
+    w = Window(35, B, KH, M, D, lens)
+    parents = np.stack([tree(w.rng, T) for _ in range(B)])
+    counts = np.array([8, 5, 8, 8, 1], np.int32)
+    k, v, lens_, starts = w.dev("k", "v", "lens", "starts")
+    par, cnt = torch.from_numpy(parents).cuda(), torch.from_numpy(counts).cuda()
+    q = queries(w.rng, B, T, H, D)
+    hidden = sts_attn.tree_attention(torch.from_numpy(q).cuda(), k, v, par, lens_, starts, scale, counts=cnt)
+    for b in range(B):
+        n = counts[b]
+        out, bound = attend64_channels(q[b, :n], w.rows(b, w.k), w.rows(b, w.v), tree_seen(parents[b], n, lens[b]), scale)
+        assert (np.abs(hidden[b, :n].cpu().numpy() - out) <= bound).all()
+    # Probabilities after each node, from its hidden state.
+    head = torch.randn((H * D, V), generator=torch.Generator().manual_seed(1)).cuda()
+    target = torch.softmax(hidden.reshape(B, T, H * D) @ head, -1)
+    tokens = target.argmax(-1).int()
+    at = par.clamp_min(0).long()
+    tokens = torch.gather(tokens, 1, at).int()  # each child its parent's likeliest word
+    rand = torch.rand((B, T), generator=torch.Generator().manual_seed(2)).cuda()
+    path, accepted, following = sts_attn.verify_draft(target, tokens, par, rand, counts=cnt)
+    for b in range(B):
+        want, word = verdict(target[b].cpu().numpy(), None, tokens[b].cpu().numpy(), parents[b], counts[b],
+                             rand[b].cpu().numpy())
+        assert path[b, :len(want)].tolist() == want and int(accepted[b]) == len(want) and int(following[b]) == word
+    assert int(accepted.max()) > 1
+    sts_attn.tree_commit(k, v, path, accepted, lens_, starts, counts=cnt)
+    left = lens_ - cnt + accepted
+    q1 = queries(w.rng, B, H, D)
+    got = sts_attn.masked_attention(torch.from_numpy(q1[:, None]).cuda(), k, v, left, starts, scale).cpu().numpy()
+    for b in range(B):
+        rows = np.r_[np.arange(lens[b] - counts[b]), lens[b] - counts[b] + path[b, :int(accepted[b])].cpu().numpy()]
+        kk, vv = (w.rows(b, x)[:, rows] for x in (w.k, w.v))
+        out, bound = attend64_channels(q1[b:b + 1], kk, vv, np.ones((1, len(rows)), bool), scale)
+        assert (np.abs(got[b] - out) <= bound).all()
