@@ -47,4 +47,24 @@ __device__ __forceinline__ int row_code(float x, float s, float by) {
   return min(max(code, -127), 127);
 }
 
+// Four codes, the first in the low byte; zeros for a row without a scale.
+__device__ __forceinline__ uint32_t row_codes(float4 x, float s) {
+  if (!(s > 0.f)) return 0u;
+  const float by = 1.f / s;
+  return ((uint32_t)row_code(x.x, s, by) & 255u) | ((uint32_t)row_code(x.y, s, by) & 255u) << 8 |
+         ((uint32_t)row_code(x.z, s, by) & 255u) << 16 | (uint32_t)row_code(x.w, s, by) << 24;
+}
+
+__device__ __forceinline__ uint2 bf16x4(float4 x) {
+  typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+  const b4 y = {(__bf16)x.x, (__bf16)x.y, (__bf16)x.z, (__bf16)x.w};
+  return __builtin_bit_cast(uint2, y);
+}
+
+// The largest magnitude; a NaN stays (fmaxf would drop it).
+__device__ __forceinline__ float largest(float4 x) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(fabsf(x.x), fabsf(x.y)),
+                                       __builtin_elementwise_maximum(fabsf(x.z), fabsf(x.w)));
+}
+
 }  // namespace sts

@@ -22,45 +22,16 @@
 // weights.  Every product is therefore of f32's grade.
 #include <algorithm>
 
-#include "coherent.hpp"
-#include "common.hpp"
-#include "lane.hpp"
-#include "page_rows.hpp"
-#include "rope.hpp"
-#include "score.hpp"
+#include "page_attend.hpp"
 
 namespace sts {
 
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kNt = 2;  // cache policy: nontemporal, each row is read once
-constexpr uint32_t kOutside = 0x80000000u;  // past every buffer resource: loads zeros
-constexpr int kMaxSplits = 128;
+using namespace paged;
+
 constexpr int kParts = 3;
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-
-template <int WORDS>
-struct Words {
-  uint32_t w[WORDS];
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t off) {
-    if constexpr (WORDS == 4) {
-      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, kNt);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = x[i];
-    } else if constexpr (WORDS == 2) {
-      const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, kNt);
-      w[0] = x[0];
-      w[1] = x[1];
-    } else {
-      w[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, kNt);
-    }
-  }
-};
 
 // x[8] as three operands of bf16 values, each the nearest to what the ones before
 // leave: their sum is x to 2^-26 of it (bf16 has f32's exponents).
@@ -109,7 +80,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
 
   constexpr int kPartBytes = F32 ? 0 : NP * kParts * 64 * 16;
   constexpr int kOutBytes = kWaves * 16 * LDO * 4;
-  constexpr int kMergeBytes = 2 * kMaxSplits * 16 * 4 + kWaves * 64 * 16;
   constexpr int kMostBytes = kPartBytes > kOutBytes ? kPartBytes : kOutBytes;
   __shared__ __align__(16) char s_mem[kMostBytes > kMergeBytes ? kMostBytes : kMergeBytes];
   auto& s_q = *reinterpret_cast<bf16x8(*)[NP][kParts][64]>(s_mem);
@@ -121,42 +91,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m16 = lane & 15, g = lane >> 4;
   const uint32_t rb = blockIdx.x % p.rblocks, share = blockIdx.x / p.rblocks;
-  uint32_t b, kvh, split, splits;
-  uint32_t first;  // splits of the streams before, each counted once for all heads
-  uint32_t len;
-  if (p.rows_factor > 0.f) {
-    // Streams of different lengths are cut into splits of about the same length: lane
-    // x looks at stream x, and the share's stream is the last whose streams before take
-    // no more shares.
-    const uint32_t mine_len = lane < (int)p.batch ? paged_len(rows, lane) : 0u;
-    float total = (float)mine_len;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x, 64);
-    const uint32_t chunk = max((uint32_t)min(total * p.rows_factor, 0x1p31f) + 1, (uint32_t)(kWaves * TILE));
-    const uint32_t mine = lane < (int)p.batch ? min(max((mine_len + chunk - 1) / chunk, 1u), p.nsplit) : 0;
-    uint32_t before = mine;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) {
-      const uint32_t y = (uint32_t)__shfl_up((int)before, x, 64);
-      before += lane >= x ? y : 0;
-    }
-    if (share >= (uint32_t)__builtin_amdgcn_readlane((int)before, 63) * rows.KH) return;
-    before -= mine;
-    b = 63 - __builtin_clzll(__ballot(lane < (int)p.batch && before * rows.KH <= share));
-    splits = (uint32_t)__builtin_amdgcn_readlane((int)mine, b);
-    first = (uint32_t)__builtin_amdgcn_readlane((int)before, b);
-    const uint32_t at = share - first * rows.KH;
-    kvh = at % rows.KH;
-    split = at / rows.KH;
-    len = (uint32_t)__builtin_amdgcn_readlane((int)mine_len, b);
-  } else {
-    splits = p.nsplit;
-    split = share % splits;
-    kvh = share / splits % rows.KH;
-    b = share / splits / rows.KH;
-    first = b * splits;
-    len = __builtin_amdgcn_readfirstlane(paged_len(rows, b));
-  }
+  Share at;
+  if (!find_share(p, share, kWaves * TILE, at)) return;
+  const uint32_t b = at.b, kvh = at.kvh, split = at.split, splits = at.splits, first = at.first, len = at.len;
   const uint32_t dh = PAD ? rows.dh : (uint32_t)D;
   const uint32_t h0 = kvh * p.group + rb * 16;           // the block's first query head
   const uint32_t live = min(p.group - rb * 16, 16u);     // its heads
@@ -473,67 +410,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
     }
   }
   if (nsplit == 1) return;
-
-  // Every thread's records are acknowledged before the workgroup takes its arrival
-  // ticket; the last one merges the splits, always in the same order.
-  __builtin_amdgcn_s_waitcnt(0);
-  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
-  __syncthreads();
-  if (tid == 0) {
-    const uint32_t ticket = atomicAdd(p.counters + unit, 1u);
-    s_last = ticket == nsplit - 1;
-    if (ticket == nsplit - 1) atomicExch(p.counters + unit, 0u);
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
-  // The splits' (m, l) of every head; m gives way to the split's factor 2^(m_s - m).
-  auto& s_f = *reinterpret_cast<float(*)[kMaxSplits][16]>(s_mem);
-  auto& s_l = *reinterpret_cast<float(*)[kMaxSplits][16]>(s_mem + kMaxSplits * 16 * 4);
-  auto& s_sum = *reinterpret_cast<f32x4(*)[kWaves * 64]>(s_mem + 2 * kMaxSplits * 16 * 4);
-  for (uint32_t x = tid; x < nsplit * live; x += kWaves * 64) {
-    const uint32_t sp = x / live, row = x % live;
-    const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(prs, (sp * REC + live * D + row * 2) * 4, 0, kSc1);
-    s_f[sp][row] = __uint_as_float(y[0]);
-    s_l[sp][row] = __uint_as_float(y[1]);
-  }
-  __syncthreads();
-  if (tid < (int)live) {
-    float mt = -FLT_MAX, lt = 0.f;
-    for (uint32_t sp = 0; sp < nsplit; ++sp) mt = fmaxf(mt, s_f[sp][tid]);
-    for (uint32_t sp = 0; sp < nsplit; ++sp) {
-      const float f = exp2_hw(s_f[sp][tid] - mt);
-      s_f[sp][tid] = f;
-      lt += f * s_l[sp][tid];
-    }
-    s_ml[0][tid][1] = lt;
-  }
-  __syncthreads();
-  // Groups of threads, one for each column, take the splits in turn.
-  constexpr int AT = 8;
-  for (uint32_t x0 = 0; x0 < slots; x0 += kWaves * 64) {
-    const uint32_t n = min(slots - x0, (uint32_t)(kWaves * 64)), groups = kWaves * 64 / n;
-    const uint32_t x = x0 + tid % n, grp = tid / n;
-    f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (grp < groups) {
-      for (uint32_t sp = grp; sp < nsplit; sp += AT * groups) {
-        coh_f4 y[AT];
-#pragma unroll
-        for (int u = 0; u < AT; ++u)
-          y[u] = ld_coherent4(prs, sp + u * groups < nsplit ? ((sp + u * groups) * REC + x * 4) * 4 : kOutside);
-#pragma unroll
-        for (int u = 0; u < AT; ++u)
-          if (sp + u * groups < nsplit) a += y[u] * s_f[sp + u * groups][x / C4];
-      }
-    }
-    __syncthreads();
-    s_sum[tid] = a;
-    __syncthreads();
-    if (grp == 0) {
-      for (uint32_t u = 1; u < groups; ++u) a += s_sum[tid + u * n];
-      finish(x, make_float4(a[0], a[1], a[2], a[3]), s_ml[0][x / C4][1]);
-    }
-  }
+  merge_splits<D, PAD>(p, prs, s_mem, s_ml[0], s_last, live, nsplit, unit, finish);
 }
 
 struct PagedPlan {
@@ -611,6 +488,7 @@ int launch_paged_decode(PagedDecode p, uint32_t batch, hipStream_t stream) {
   p.rows_factor = pl.rows_factor;
   p.record = pl.record;
   const dim3 grid(pl.shares * pl.rblocks);
+  if (p.group == 1) return launch_paged_lone(p, grid, stream);
   if (p.rows.type == STS_PAGES_F32) launch_type<STS_PAGES_F32>(p, grid, stream);
   else if (p.rows.type == STS_PAGES_BF16) launch_type<STS_PAGES_BF16>(p, grid, stream);
   else launch_type<STS_PAGES_INT8>(p, grid, stream);

@@ -10,18 +10,6 @@ namespace sts {
 
 namespace {
 
-__device__ __forceinline__ uint2 bf16x4(float4 x) {
-  typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-  const b4 y = {(__bf16)x.x, (__bf16)x.y, (__bf16)x.z, (__bf16)x.w};
-  return __builtin_bit_cast(uint2, y);
-}
-
-__device__ __forceinline__ float largest(float4 x) {
-  // (maximum, unlike fmaxf, keeps a NaN.)
-  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(fabsf(x.x), fabsf(x.y)),
-                                       __builtin_elementwise_maximum(fabsf(x.z), fabsf(x.w)));
-}
-
 // Four values of a row, of which lane c of G holds dims 4c .. 4c+3, to row `at`.
 template <int TYPE, int G>
 __device__ __forceinline__ void store_row(void* rows, float* scales, uint64_t at, uint32_t dh, int c, float4 x,
@@ -36,12 +24,7 @@ __device__ __forceinline__ void store_row(void* rows, float* scales, uint64_t at
 #pragma unroll
     for (int d = 1; d < G; d *= 2) top = __builtin_elementwise_maximum(top, __shfl_xor(top, d, G));
     const float s = row_scale(top);
-    uint32_t codes = 0;
-    if (s > 0.f) {
-      const float by = 1.f / s;
-      codes = ((uint32_t)row_code(x.x, s, by) & 255u) | ((uint32_t)row_code(x.y, s, by) & 255u) << 8 |
-              ((uint32_t)row_code(x.z, s, by) & 255u) << 16 | (uint32_t)row_code(x.w, s, by) << 24;
-    }
+    const uint32_t codes = row_codes(x, s);
     if (on) *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(rows) + to) = codes;
     if (on && c == 0) scales[at] = s;
   }

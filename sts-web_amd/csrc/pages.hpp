@@ -54,6 +54,11 @@ struct PagedDecode {
   PagedRows rows;
   const float* q = nullptr;  // stream b, head h at q + b*q_stride + h*dh
   uint64_t q_stride = 0;
+  // The newest row of stream b, written first: K/V head j at k_new + b*new_stride + j*dh;
+  // or null.
+  const float* k_new = nullptr;
+  const float* v_new = nullptr;
+  uint64_t new_stride = 0;
   float* out = nullptr;      // [B][H][dh]
   uint32_t H = 0, group = 1;
   float qscale = 0.f;        // scale * log2(e)
