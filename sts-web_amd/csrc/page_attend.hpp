@@ -87,78 +87,135 @@ __device__ __forceinline__ bool find_share(const PagedDecode& p, uint32_t share,
   return true;
 }
 
-// The splits of a block of `live` query heads merged by the last of its workgroups to
-// arrive, always in the same order: record sp of prs holds O [live][D], then (m, l)
-// [live].  mem: kMergeBytes of LDS that every thread is done with; sums [16][2];
-// finish(x, a, l) gets float4 column x of the unnormalised outputs and its head's l.
+// ---- merge of the splits ------------------------------------------------------
+//
+// Record sp of a block of `live` query heads holds its split's O [live][D], then (m, l)
+// [live]; a workgroup that has published its own takes a ticket, and the last to arrive
+// merges them, always in the same order.  A thread has kAhead columns of records
+// requested at once.  Where that would be more than two round trips (one workgroup of 128
+// splits of 8 heads: 17 us), clusters of about the root of their number are merged first,
+// each by its own last, and the clusters' records after that.
+constexpr int kAhead = 8;
+constexpr int kClusters = 16;  // at most: of kMaxSplits, 11
+constexpr uint32_t kCounters = 1 + kClusters;  // arrival counters of a block
 constexpr int kMergeBytes = 2 * kMaxSplits * 16 * 4 + kWaves * 64 * 16;
-template <int D, bool PAD, class Finish>
-__device__ __forceinline__ void merge_splits(const PagedDecode& p, __amdgpu_buffer_rsrc_t prs, char* mem,
-                                             float (*sums)[2], uint32_t& s_last, uint32_t live, uint32_t nsplit,
-                                             uint64_t unit, Finish finish) {
-  constexpr int C4 = D / 4;
-  const int tid = threadIdx.x;
-  const uint32_t REC = p.record, slots = live * C4;
-  // Every thread's records are acknowledged before the workgroup takes its arrival
-  // ticket; the last one merges the splits, always in the same order.
+
+struct Records {
+  __amdgpu_buffer_rsrc_t rs;
+  uint32_t size;  // floats of a record
+  uint32_t live;
+};
+
+// Whether this workgroup, whose stores it waits for, is the last of n to get here.
+__device__ __forceinline__ bool last_of(uint32_t* counter, uint32_t n, uint32_t& s_last) {
   __builtin_amdgcn_s_waitcnt(0);
   __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
   __syncthreads();
-  if (tid == 0) {
-    const uint32_t ticket = atomicAdd(p.counters + unit, 1u);
-    s_last = ticket == nsplit - 1;
-    if (ticket == nsplit - 1) atomicExch(p.counters + unit, 0u);
+  if (threadIdx.x == 0) {
+    const uint32_t ticket = atomicAdd(counter, 1u);
+    s_last = ticket == n - 1;
+    if (ticket == n - 1) atomicExch(counter, 0u);
   }
   __syncthreads();
-  if (!s_last) return;
+  const bool last = s_last;
   __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
-  // The splits' (m, l) of every head; m gives way to the split's factor 2^(m_s - m).
+  return last;
+}
+
+// Records from, from + step, ... (n of them): put(x, a, m, l) gets float4 column x of
+// their merged O and its head's m and l.  mem: kMergeBytes of LDS that every thread is
+// done with.
+template <int D, class Put>
+__device__ __forceinline__ void merge_records(const Records& r, uint32_t from, uint32_t step, uint32_t n, char* mem,
+                                              Put put) {
+  constexpr int C4 = D / 4;
+  const int tid = threadIdx.x;
+  const uint32_t live = r.live, slots = live * C4;
   auto& s_f = *reinterpret_cast<float(*)[kMaxSplits][16]>(mem);
   auto& s_l = *reinterpret_cast<float(*)[kMaxSplits][16]>(mem + kMaxSplits * 16 * 4);
   auto& s_sum = *reinterpret_cast<f32x4(*)[kWaves * 64]>(mem + 2 * kMaxSplits * 16 * 4);
-  for (uint32_t x = tid; x < nsplit * live; x += kWaves * 64) {
+  coh_f4 y[kAhead];
+  // Groups of threads, one for each column, take the records in turn.
+  auto request = [&](uint32_t sp, uint32_t groups, uint32_t x) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      y[u] = ld_coherent4(r.rs, sp + u * groups < n ? ((from + (sp + u * groups) * step) * r.size + x * 4) * 4 : kOutside);
+  };
+  const uint32_t n0 = min(slots, (uint32_t)(kWaves * 64)), g0 = kWaves * 64 / n0;
+  if (tid / n0 < g0) request(tid / n0, g0, tid % n0);
+  for (uint32_t x = tid; x < n * live; x += kWaves * 64) {
     const uint32_t sp = x / live, row = x % live;
-    const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(prs, (sp * REC + live * D + row * 2) * 4, 0, kSc1);
-    s_f[sp][row] = __uint_as_float(y[0]);
-    s_l[sp][row] = __uint_as_float(y[1]);
+    const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(
+        r.rs, ((from + sp * step) * r.size + live * D + row * 2) * 4, 0, kSc1);
+    s_f[sp][row] = __uint_as_float(ml[0]);
+    s_l[sp][row] = __uint_as_float(ml[1]);
   }
   __syncthreads();
+  // m gives way to the record's factor 2^(m_s - m); the block's m and l take the place
+  // behind the last record's.
   if (tid < (int)live) {
     float mt = -FLT_MAX, lt = 0.f;
-    for (uint32_t sp = 0; sp < nsplit; ++sp) mt = fmaxf(mt, s_f[sp][tid]);
-    for (uint32_t sp = 0; sp < nsplit; ++sp) {
+    for (uint32_t sp = 0; sp < n; ++sp) mt = fmaxf(mt, s_f[sp][tid]);
+    for (uint32_t sp = 0; sp < n; ++sp) {
       const float f = exp2_hw(s_f[sp][tid] - mt);
       s_f[sp][tid] = f;
       lt += f * s_l[sp][tid];
     }
-    sums[tid][1] = lt;
+    s_l[0][tid] = lt;
+    s_l[1][tid] = mt;
   }
   __syncthreads();
-  // Groups of threads, one for each column, take the splits in turn.
-  constexpr int AT = 8;
   for (uint32_t x0 = 0; x0 < slots; x0 += kWaves * 64) {
-    const uint32_t n = min(slots - x0, (uint32_t)(kWaves * 64)), groups = kWaves * 64 / n;
-    const uint32_t x = x0 + tid % n, grp = tid / n;
+    const uint32_t cols = min(slots - x0, (uint32_t)(kWaves * 64)), groups = kWaves * 64 / cols;
+    const uint32_t x = x0 + tid % cols, grp = tid / cols;
     f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
     if (grp < groups) {
-      for (uint32_t sp = grp; sp < nsplit; sp += AT * groups) {
-        coh_f4 y[AT];
+      for (uint32_t sp = grp; sp < n; sp += kAhead * groups) {
+        if (x0 > 0 || sp != grp) request(sp, groups, x);
 #pragma unroll
-        for (int u = 0; u < AT; ++u)
-          y[u] = ld_coherent4(prs, sp + u * groups < nsplit ? ((sp + u * groups) * REC + x * 4) * 4 : kOutside);
-#pragma unroll
-        for (int u = 0; u < AT; ++u)
-          if (sp + u * groups < nsplit) a += y[u] * s_f[sp + u * groups][x / C4];
+        for (int u = 0; u < kAhead; ++u)
+          if (sp + u * groups < n) a += y[u] * s_f[sp + u * groups][x / C4];
       }
     }
-    __syncthreads();
-    s_sum[tid] = a;
-    __syncthreads();
-    if (grp == 0) {
-      for (uint32_t u = 1; u < groups; ++u) a += s_sum[tid + u * n];
-      finish(x, make_float4(a[0], a[1], a[2], a[3]), sums[x / C4][1]);
+    if (groups > 1) {
+      s_sum[tid] = a;
+      __syncthreads();
+      if (grp == 0)
+        for (uint32_t u = 1; u < groups; ++u) a += s_sum[tid + u * cols];
     }
+    if (grp == 0) put(x, make_float4(a[0], a[1], a[2], a[3]), s_l[1][x / C4], s_l[0][x / C4]);
   }
+}
+
+// Column x of a record, and its head's (m, l).
+template <int D>
+__device__ __forceinline__ void put_record(const Records& r, uint32_t sp, uint32_t x, float4 a, float m, float l) {
+  constexpr int C4 = D / 4;
+  st_coherent4(r.rs, (sp * r.size + x * 4) * 4, coh_f4{a.x, a.y, a.z, a.w});
+  if (x % C4 == 0)
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, r.rs,
+                                          (sp * r.size + r.live * D + x / C4 * 2) * 4, 0, kSc1);
+}
+
+// What follows a split's put_record: its part in the merge, whose outcome goes to put.
+template <int D, class Put>
+__device__ __forceinline__ void merge_splits(const Records& r, uint32_t* counters, uint32_t split, uint32_t nsplit,
+                                             char* mem, uint32_t& s_last, Put put) {
+  const uint32_t slots = r.live * (D / 4), at_once = slots <= kWaves * 64 ? kWaves * 64 / slots * kAhead : kAhead / 2;
+  uint32_t from = 0, step = 1, n = nsplit;
+  if (nsplit > 2 * at_once) {
+    uint32_t size = 1;
+    while (size * size < nsplit) ++size;
+    const uint32_t cluster = split / size, first = cluster * size, some = min(size, nsplit - first);
+    if (!last_of(counters + 1 + cluster, some, s_last)) return;
+    // (A column's first record is read by the thread that then writes it.)
+    merge_records<D>(r, first, 1, some, mem,
+                     [&](uint32_t x, float4 a, float m, float l) { put_record<D>(r, first, x, a, m, l); });
+    step = size;
+    n = (nsplit + size - 1) / size;
+  }
+  if (!last_of(counters, n, s_last)) return;
+  merge_records<D>(r, from, step, n, mem, put);
 }
 
 }  // namespace paged

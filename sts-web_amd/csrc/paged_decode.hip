@@ -8,11 +8,10 @@
 //
 // A workgroup takes up to 16 query heads of one (stream, K/V head) and one split of
 // the stream's rows; its four waves deal the split's tiles among themselves.  A tile is
-// 16 rows of f32, 32 of bf16, 64 of int8: at a head dim of 128 16 KB of K and V, which
-// a wave has requested while it works on the last.  Sixteen rows lie in one page, so
-// that each has a buffer resource of its own, ending with the stream's rows or empty
-// where no page holds them: a lane's offsets are the same for all tiles, rows that are
-// not there read as zeros, and pools may pass 4 GB.
+// 16 rows of f32, 32 of the others, requested while the last is worked on.  A tile, or
+// each sixteen of its rows, lies in one page and has a buffer resource of its own, ending
+// with the stream's rows or empty where no page holds them: a lane's offsets are the same
+// for all tiles, rows that are not there read as zeros, and pools may pass 4 GB.
 //   S^T = K Q^T     A = K: lane (m, g) = (lane & 15, lane >> 4) holds row m; B = Q
 //   O^T += V^T P^T  A = V^T: the lane holds of rows 4g + i the dims (16 c + m) VW + e;
 //                   B = the weights as the first product leaves them in the lane
@@ -63,7 +62,8 @@ __device__ __forceinline__ uint32_t pair_up(uint32_t hi, uint32_t lo) {
   return __builtin_amdgcn_perm(hi, lo, 0x07060302);
 }
 
-template <int D, int TYPE, bool PAD>
+// WHOLE: a tile never passes the end of a page.
+template <int D, int TYPE, bool PAD, bool WHOLE>
 __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const PagedDecode p) {
   constexpr bool F32 = TYPE == STS_PAGES_F32, I8 = TYPE == STS_PAGES_INT8;
   constexpr int ES = F32 ? 4 : I8 ? 1 : 2;
@@ -71,8 +71,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
   constexpr int NC = D / (4 * CW);                // loads per K row
   constexpr int VW = CW < D / 16 ? CW : D / 16;   // dims of V a lane loads at once
   constexpr int NV = D / (16 * VW);               // loads per V row
-  constexpr int KT = F32 ? 1 : I8 ? 4 : 2;        // 16-row tiles a wave takes at once
+  constexpr int KT = F32 ? 1 : 2;                 // 16-row tiles a wave takes at once
   constexpr int TILE = 16 * KT;
+  constexpr int NS = WHOLE ? 1 : KT;              // pieces of a tile that lie in one page
+  constexpr int PIECE = TILE / NS;
   constexpr int NX = NV * VW;                     // 16-dim tiles of the output
   constexpr int NP = D / 32;                      // 32-dim steps of K Q^T
   constexpr int LDO = D + 4;                      // LDS row of a partial output
@@ -111,26 +113,27 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
   const uint32_t tstep = nsplit * kWaves;
   uint32_t t = split + nsplit * wave;
 
-  // The pages of a tile: lane x of each four asks for sixteen rows x of the tile.
+  // The pages of a tile: lane x asks for piece x.
   const __amdgpu_buffer_rsrc_t trs =
       coherent_rsrc(rows.table + (uint64_t)b * rows.max_pages, rows.max_pages * 4);
   auto ask_pages = [&](uint32_t t) {
-    const uint32_t r = t * TILE + (lane & (KT - 1)) * 16;
+    const uint32_t r = t * TILE + (lane & (NS - 1)) * PIECE;
     return __builtin_amdgcn_raw_buffer_load_b32(trs, r < len ? (r >> rows.shift) * 4 : kOutside, 0, 0);
   };
-  // Where the tile's rows are.  Uniform.
+  // Where the rows of a tile's pieces are.  Uniform.
   struct Where {
-    uint64_t at;    // row index of the first
-    uint32_t rows;  // how many there are
+    uint64_t at[NS];    // row index of the first
+    uint32_t rows[NS];  // how many there are
   };
-  auto find = [&](uint32_t t, uint32_t asked, Where (&w)[KT]) {
+  const uint32_t in_page = (1u << rows.shift) - 1, page_heads = rows.KH << rows.shift, head = kvh << rows.shift;
+  auto find = [&](uint32_t t, uint32_t asked, Where& w) {
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)asked, kt);
-      const uint32_t r0 = t * TILE + kt * 16;
-      w[kt].at = (((uint64_t)page * rows.KH + kvh) << rows.shift) + (r0 & ((1u << rows.shift) - 1));
-      w[kt].rows = r0 < len && page < rows.pages ? min(len - r0, 16u) : 0u;
-      if (w[kt].rows == 0) w[kt].at = 0;
+    for (int n = 0; n < NS; ++n) {
+      const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)asked, n);
+      const uint32_t r0 = t * TILE + n * PIECE;
+      const bool there = r0 < len && page < rows.pages;
+      w.at[n] = there ? (uint64_t)page * page_heads + (head + (r0 & in_page)) : 0;
+      w.rows[n] = there ? min(len - r0, (uint32_t)PIECE) : 0u;
     }
   };
   typedef Words<CW * ES / 4> KRow[NC];
@@ -140,36 +143,47 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
   f32x4 ks[I8 ? KT : 1], vs[I8 ? KT : 1];
   const uint32_t rowb = dh * ES;
   const uint32_t koff = m16 * rowb + g * (CW * ES);
-  auto load_k = [&](const Where (&w)[KT]) {
+  // rows of 16-row tile kt, which begin at row `from` of its piece's resource
+  auto scales = [&](const float* s, const Where& w, f32x4 (&x)[I8 ? KT : 1]) {
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      const __amdgpu_buffer_rsrc_t rs =
-          coherent_rsrc(static_cast<const char*>(rows.k) + w[kt].at * rowb, w[kt].rows * rowb);
+    for (int n = 0; n < NS; ++n) {
+      const __amdgpu_buffer_rsrc_t rs = coherent_rsrc(s + w.at[n], w.rows[n] * 4);
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        kk[kt][c].load(rs, !PAD || (uint32_t)(c * 4 + g) * CW < dh ? koff + c * (4 * CW * ES) : kOutside);
-      if constexpr (I8) {
-        const __amdgpu_buffer_rsrc_t ss = coherent_rsrc(rows.ks + w[kt].at, w[kt].rows * 4);
-        ks[kt] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ss, g * 16, 0, kNt));
-      }
+      for (int k = 0; k < KT / NS; ++k)
+        x[n * (KT / NS) + k] =
+            __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, g * 16 + k * 64, 0, kNt));
     }
   };
-  auto load_v = [&](const Where (&w)[KT]) {
+  auto load_k = [&](const Where& w) {
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
+    for (int n = 0; n < NS; ++n) {
       const __amdgpu_buffer_rsrc_t rs =
-          coherent_rsrc(static_cast<const char*>(rows.v) + w[kt].at * rowb, w[kt].rows * rowb);
+          coherent_rsrc(static_cast<const char*>(rows.k) + w.at[n] * rowb, w.rows[n] * rowb);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int k = 0; k < KT / NS; ++k)
 #pragma unroll
-        for (int c = 0; c < NV; ++c)
-          vv[kt][i][c].load(rs, !PAD || (uint32_t)(c * 16 + m16) * VW < dh
-                                    ? (4 * g + i) * rowb + m16 * (VW * ES) + c * (16 * VW * ES) : kOutside);
-      if constexpr (I8) {
-        const __amdgpu_buffer_rsrc_t ss = coherent_rsrc(rows.vs + w[kt].at, w[kt].rows * 4);
-        vs[kt] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ss, g * 16, 0, kNt));
-      }
+        for (int c = 0; c < NC; ++c)
+          kk[n * (KT / NS) + k][c].load(rs, !PAD || (uint32_t)(c * 4 + g) * CW < dh
+                                                ? koff + k * 16 * rowb + c * (4 * CW * ES) : kOutside);
     }
+    if constexpr (I8) scales(rows.ks, w, ks);
+  };
+  auto load_v = [&](const Where& w) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      const __amdgpu_buffer_rsrc_t rs =
+          coherent_rsrc(static_cast<const char*>(rows.v) + w.at[n] * rowb, w.rows[n] * rowb);
+#pragma unroll
+      for (int k = 0; k < KT / NS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int c = 0; c < NV; ++c)
+            vv[n * (KT / NS) + k][i][c].load(
+                rs, !PAD || (uint32_t)(c * 16 + m16) * VW < dh
+                        ? (k * 16 + 4 * g + i) * rowb + m16 * (VW * ES) + c * (16 * VW * ES) : kOutside);
+    }
+    if constexpr (I8) scales(rows.vs, w, vs);
   };
 
   // The pages are asked for two tiles ahead, so that no rows wait for them but the
@@ -192,7 +206,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
   };
   uint32_t asked = ask_pages(t);
   uint32_t asked_next = ask_pages(t + tstep);
-  Where now[KT];
+  Where now;
   find(t, asked, now);
   load_k(now);
   load_v(now);
@@ -276,17 +290,19 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
     // Rows that are not there.
     uint32_t there = 0;
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) there += now[kt].rows;
-    const bool partly = there < TILE;
-    if (partly) {
+    for (int n = 0; n < NS; ++n) there += now.rows[n];
+    if (there < TILE) {
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if ((uint32_t)(4 * g + i) >= now[kt].rows) s[kt][i] = -INFINITY;
+          if ((uint32_t)(kt % (KT / NS) * 16 + 4 * g + i) >= now.rows[kt / (KT / NS)]) {
+            s[kt][i] = -INFINITY;
+            if constexpr (I8) vs[kt][i] = 0.f;  // (what lies behind the rows may not be a number)
+          }
     }
     // The next tile's K, now that this one's is used up.
-    Where next[KT];
+    Where next;
     find(t + tstep, asked_next, next);
     asked_next = ask_pages(t + 2 * tstep);
     load_k(next);
@@ -317,10 +333,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
     } else {
       if constexpr (I8) {
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)  // (what lies behind the rows may not be a number)
-            s[kt][i] *= partly && (uint32_t)(4 * g + i) >= now[kt].rows ? 0.f : vs[kt][i];
+        for (int kt = 0; kt < KT; ++kt) s[kt] *= vs[kt];
       }
 #pragma unroll
       for (int k2 = 0; k2 < KT; k2 += 2) {
@@ -349,8 +362,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
       }
     }
     load_v(next);
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) now[kt] = next[kt];
+    now = next;
   }
   if constexpr (!F32) __syncthreads();  // every wave is done with the queries' parts
 
@@ -372,17 +384,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
   }
   __syncthreads();
   const uint32_t slots = live * C4;  // float4 columns of the block's outputs
-  auto finish = [&](uint32_t x, float4 a, float lt) {
+  auto finish = [&](uint32_t x, float4 a, float, float lt) {
     const uint32_t row = x / C4, col = x % C4;
     const float f = lt > 0.f || lt != lt ? 1.f / lt : 0.f;  // nothing seen: zeros
     if (!PAD || col * 4 < dh)
       *reinterpret_cast<float4*>(out + (uint64_t)row * dh + col * 4) = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
   };
-  const uint32_t REC = p.record;  // floats of a split's record: O, then (m, l)
-  const uint64_t unit = ((uint64_t)b * rows.KH + kvh) * p.rblocks + rb;
-  const __amdgpu_buffer_rsrc_t prs =
-      coherent_rsrc(p.part + (((uint64_t)first * rows.KH + kvh * splits) * p.rblocks + rb * splits) * REC,
-                    nsplit > 1 ? splits * REC * 4 : 0);
+  const Records rec{coherent_rsrc(p.part + (((uint64_t)first * rows.KH + kvh * splits) * p.rblocks + rb * splits) * p.record,
+                                  nsplit > 1 ? splits * p.record * 4 : 0),
+                    p.record, live};
   for (uint32_t x = tid; x < slots; x += kWaves * 64) {
     const uint32_t row = x / C4, col = x % C4;
     float mt = s_ml[0][row][0];
@@ -400,17 +410,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
       a.z += f * y.z;
       a.w += f * y.w;
     }
-    if (nsplit == 1) {
-      finish(x, a, lt);
-    } else {
-      st_coherent4(prs, (split * REC + x * 4) * 4, coh_f4{a.x, a.y, a.z, a.w});
-      if (col == 0)
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(mt), __float_as_uint(lt)}, prs,
-                                              (split * REC + live * D + row * 2) * 4, 0, kSc1);
-    }
+    if (nsplit == 1) finish(x, a, mt, lt);
+    else put_record<D>(rec, split, x, a, mt, lt);
   }
   if (nsplit == 1) return;
-  merge_splits<D, PAD>(p, prs, s_mem, s_ml[0], s_last, live, nsplit, unit, finish);
+  const uint64_t unit = ((uint64_t)b * rows.KH + kvh) * p.rblocks + rb;
+  merge_splits<D>(rec, p.counters + unit * kCounters, split, nsplit, s_mem, s_last, finish);
 }
 
 struct PagedPlan {
@@ -425,7 +430,7 @@ PagedPlan plan_paged(const PagedDecode& p, uint32_t batch) {
   const uint64_t units = (uint64_t)batch * rows.KH * pl.rblocks;
   const uint64_t target = (uint64_t)device_cu_count() * 2;
   // A split is worth its record from a tile for each of its waves on.
-  const uint32_t tile = (rows.type == STS_PAGES_F32 ? 16 : rows.type == STS_PAGES_BF16 ? 32 : 64) * kWaves;
+  const uint32_t tile = (rows.type == STS_PAGES_F32 ? 16 : 32) * kWaves;
   const uint64_t most = std::min<uint64_t>((rows.max_rows + tile - 1) / tile, kMaxSplits);
   if (batch > 1 && batch <= 64) {
     // Streams of different ages: splits of about equal length whatever their stream,
@@ -450,20 +455,20 @@ int paged_workspace(const PagedDecode& p, const PagedPlan& pl, uint32_t batch, h
   *out = nullptr;
   if (pl.nsplit <= 1) return STS_OK;
   return get_workspace(stream, (size_t)pl.shares * pl.rblocks * pl.record,
-                       (size_t)batch * p.rows.KH * pl.rblocks, out);
+                       (size_t)batch * p.rows.KH * pl.rblocks * kCounters, out);
 }
 
-template <int TYPE>
+template <int TYPE, bool WHOLE>
 void launch_type(const PagedDecode& p, dim3 grid, hipStream_t stream) {
   const dim3 block(kWaves * 64);
   if (p.rows.dh == 128)
-    hipLaunchKernelGGL((paged_decode_kernel<128, TYPE, false>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((paged_decode_kernel<128, TYPE, false, WHOLE>), grid, block, 0, stream, p);
   else if (p.rows.dh == 64)
-    hipLaunchKernelGGL((paged_decode_kernel<64, TYPE, false>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((paged_decode_kernel<64, TYPE, false, WHOLE>), grid, block, 0, stream, p);
   else if (p.rows.dh > 64)
-    hipLaunchKernelGGL((paged_decode_kernel<128, TYPE, true>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((paged_decode_kernel<128, TYPE, true, WHOLE>), grid, block, 0, stream, p);
   else
-    hipLaunchKernelGGL((paged_decode_kernel<64, TYPE, true>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((paged_decode_kernel<64, TYPE, true, WHOLE>), grid, block, 0, stream, p);
 }
 
 }  // namespace
@@ -489,9 +494,12 @@ int launch_paged_decode(PagedDecode p, uint32_t batch, hipStream_t stream) {
   p.record = pl.record;
   const dim3 grid(pl.shares * pl.rblocks);
   if (p.group == 1) return launch_paged_lone(p, grid, stream);
-  if (p.rows.type == STS_PAGES_F32) launch_type<STS_PAGES_F32>(p, grid, stream);
-  else if (p.rows.type == STS_PAGES_BF16) launch_type<STS_PAGES_BF16>(p, grid, stream);
-  else launch_type<STS_PAGES_INT8>(p, grid, stream);
+  const bool whole = p.rows.shift > 4;  // pages of 32 rows or more hold whole tiles
+  if (p.rows.type == STS_PAGES_F32) launch_type<STS_PAGES_F32, true>(p, grid, stream);
+  else if (p.rows.type == STS_PAGES_BF16)
+    whole ? launch_type<STS_PAGES_BF16, true>(p, grid, stream) : launch_type<STS_PAGES_BF16, false>(p, grid, stream);
+  else
+    whole ? launch_type<STS_PAGES_INT8, true>(p, grid, stream) : launch_type<STS_PAGES_INT8, false>(p, grid, stream);
   STS_HIP(hipGetLastError());
   return STS_OK;
 }

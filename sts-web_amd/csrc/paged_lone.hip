@@ -80,7 +80,7 @@ __global__ __launch_bounds__(kWaves * 64) void paged_lone_kernel(const PagedDeco
   __shared__ __align__(16) float s_p[kWaves][UNIT];
   __shared__ float s_ml[NST][2];
   __shared__ f32x4 s_part[kWaves * 64];
-  __shared__ float s_sums[16][2];
+  __shared__ float s_sums[kWaves * 64 / C4];
   __shared__ uint32_t s_last;
 
   const PagedRows& rows = p.rows;
@@ -334,34 +334,30 @@ __global__ __launch_bounds__(kWaves * 64) void paged_lone_kernel(const PagedDeco
     a += *reinterpret_cast<const f32x4*>(&s_acc[x + part][col * 4]) * f;
   }
   s_part[tid] = a;
-  if (col == 0) s_sums[part][0] = lt;
+  if (col == 0) s_sums[part] = lt;
   __syncthreads();
-  const uint64_t unit = (uint64_t)b * rows.KH + h;
-  const __amdgpu_buffer_rsrc_t prs = coherent_rsrc(
-      p.part + ((uint64_t)at.first * rows.KH + h * at.splits) * p.record, nsplit > 1 ? at.splits * p.record * 4 : 0);
-  auto finish = [&](uint32_t x, float4 a, float lt) {
+  auto finish = [&](uint32_t x, float4 a, float, float lt) {
     const float f = lt > 0.f || lt != lt ? 1.f / lt : 0.f;  // nothing seen: zeros
     if (!PAD || x * 4 < dh)
       *reinterpret_cast<float4*>(out + x * 4) = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
   };
+  const Records rec{coherent_rsrc(p.part + ((uint64_t)at.first * rows.KH + h * at.splits) * p.record,
+                                  nsplit > 1 ? at.splits * p.record * 4 : 0),
+                    p.record, 1};
   if (tid < C4) {
     lt = 0.f;
     a = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < PARTS; ++x) {
       a += s_part[x * C4 + tid];
-      lt += s_sums[x][0];
+      lt += s_sums[x];
     }
-    if (nsplit == 1) {
-      finish(tid, make_float4(a[0], a[1], a[2], a[3]), lt);
-    } else {
-      st_coherent4(prs, (at.split * p.record + tid * 4) * 4, a);
-      if (tid == 0)
-        st_coherent4(prs, (at.split * p.record + D) * 4, coh_f4{mt, lt, 0.f, 0.f});
-    }
+    const float4 y = make_float4(a[0], a[1], a[2], a[3]);
+    if (nsplit == 1) finish(tid, y, mt, lt);
+    else put_record<D>(rec, at.split, tid, y, mt, lt);
   }
   if (nsplit == 1) return;
-  merge_splits<D, PAD>(p, prs, s_mem, s_sums, s_last, 1, nsplit, unit, finish);
+  merge_splits<D>(rec, p.counters + ((uint64_t)b * rows.KH + h) * kCounters, at.split, nsplit, s_mem, s_last, finish);
 }
 
 template <int TYPE>
