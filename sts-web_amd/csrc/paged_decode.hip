@@ -30,6 +30,7 @@ namespace {
 using namespace paged;
 
 constexpr int kParts = 3;
+constexpr uint32_t kSplitRows = 128;  // rows that a split is worth its record from
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // x[8] as three operands of bf16 values, each the nearest to what the ones before
@@ -64,7 +65,7 @@ __device__ __forceinline__ uint32_t pair_up(uint32_t hi, uint32_t lo) {
 
 // WHOLE: a tile never passes the end of a page.
 template <int D, int TYPE, bool PAD, bool WHOLE>
-__global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const PagedDecode p) {
+__global__ __launch_bounds__(kWaves * 64, 3) void paged_decode_kernel(const PagedDecode p) {
   constexpr bool F32 = TYPE == STS_PAGES_F32, I8 = TYPE == STS_PAGES_INT8;
   constexpr int ES = F32 ? 4 : I8 ? 1 : 2;
   constexpr int CW = 16 / ES;                     // dims of K a lane loads at once
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
   const int m16 = lane & 15, g = lane >> 4;
   const uint32_t rb = blockIdx.x % p.rblocks, share = blockIdx.x / p.rblocks;
   Share at;
-  if (!find_share(p, share, kWaves * TILE, at)) return;
+  if (!find_share(p, share, kSplitRows, at)) return;
   const uint32_t b = at.b, kvh = at.kvh, split = at.split, splits = at.splits, first = at.first, len = at.len;
   const uint32_t dh = PAD ? rows.dh : (uint32_t)D;
   const uint32_t h0 = kvh * p.group + rb * 16;           // the block's first query head
@@ -105,10 +106,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
       for (uint32_t t = tid; t < live * dh; t += kWaves * 64) out[t] = 0.f;
     return;
   }
-  // Tiles of TILE rows, dealt to the splits and waves in turn; a split gets at least a
-  // tile for each wave.
+  // Tiles of TILE rows, dealt to the splits and waves in turn.
   const uint32_t tiles = (len + TILE - 1) / TILE;
-  const uint32_t nsplit = min(splits, (tiles + kWaves - 1) / kWaves);
+  const uint32_t nsplit = min(splits, (len + kSplitRows - 1) / kSplitRows);
   if (split >= nsplit) return;
   const uint32_t tstep = nsplit * kWaves;
   uint32_t t = split + nsplit * wave;
@@ -243,6 +243,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
 
   for (; t < tiles; t += tstep) {
     f32x4 s[KT];
+    // The queries' parts are read anew for every tile: kept in registers (the compiler
+    // lifts the loads out of the loop) they would take a third workgroup's.
+    int at_lane = lane;
+    asm volatile("" : "+v"(at_lane));
     if constexpr (F32) {
       // Four sums of the dims in turn: shorter sums round less.
       f32x4 sum[4];
@@ -277,7 +281,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_decode_kernel(const Page
         }
 #pragma unroll
         for (int n = kParts - 1; n >= 0; --n) {
-          const bf16x8 q = s_q[c][n][lane];
+          const bf16x8 q = s_q[c][n][at_lane];
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kt], q, s[kt], 0, 0, 0);
         }
@@ -428,10 +432,17 @@ PagedPlan plan_paged(const PagedDecode& p, uint32_t batch) {
   const PagedRows& rows = p.rows;
   pl.rblocks = (p.group + 15) / 16;
   const uint64_t units = (uint64_t)batch * rows.KH * pl.rblocks;
-  const uint64_t target = (uint64_t)device_cu_count() * 2;
-  // A split is worth its record from a tile for each of its waves on.
-  const uint32_t tile = (rows.type == STS_PAGES_F32 ? 16 : 32) * kWaves;
-  const uint64_t most = std::min<uint64_t>((rows.max_rows + tile - 1) / tile, kMaxSplits);
+  // Two workgroups a CU, which between them even out what streams of different lengths
+  // leave uneven (24 streams of 900 to 4099 bf16 rows of 8 heads 47 us, with one a CU 59;
+  // 9 of 31 to 2777 f32 rows 72 and 74.6); one for a single stream, whose splits are alike
+  // and whose merge is then shorter (3000 8-bit rows of 32 heads 10.8 us for 12.6, 30000 of
+  // 4 heads 15.8 for 18.5).
+  const uint64_t target = (uint64_t)device_cu_count() * (batch > 1 ? 2 : 1);
+  // A split is worth its record from 128 rows of a group's head on (30 streams of 20 to 500
+  // f32 rows of 6 heads 16 us, from 64 on 20, from 256 on 18.6), of a lone head from a unit
+  // for each of its waves on.
+  const uint32_t least = p.group == 1 ? 64 : kSplitRows;
+  const uint64_t most = std::min<uint64_t>((rows.max_rows + least - 1) / least, kMaxSplits);
   if (batch > 1 && batch <= 64) {
     // Streams of different ages: splits of about equal length whatever their stream,
     // not more than fit at once where one round can hold them (rounding up gives each
