@@ -21,6 +21,7 @@
 // a stretch of the words, so that the draw finds its wave from sixteen sums.  What bounds
 // it is the latency of these steps, not the bytes.
 #include "common.hpp"
+#include "lane.hpp"
 #include "verify.hpp"
 #include "window.hpp"
 
@@ -32,20 +33,56 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBatch = 8;
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // rows start anywhere
 
-__device__ __forceinline__ double wave_total(double x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d, 64);
+constexpr int kPieces = 64;  // sums that a wave keeps of its stretch of the words
+
+// The value of the lane whose index differs in bit LEVEL (and, for 2 and 3, in the bits
+// below).
+template <int LEVEL>
+__device__ __forceinline__ double xchg64(double x) {
+  const uint2 y = __builtin_bit_cast(uint2, x);
+  float lo = __uint_as_float(y.x), hi = __uint_as_float(y.y);
+  if constexpr (LEVEL == 5) {
+    lo = xor32(lo);
+    hi = xor32(hi);
+  } else {
+    lo = xchg<LEVEL>(lo);
+    hi = xchg<LEVEL>(hi);
+  }
+  return __builtin_bit_cast(double, make_uint2(__float_as_uint(lo), __float_as_uint(hi)));
+}
+template <int LEVELS = 6>
+__device__ __forceinline__ double lanes_total(double x) {
+  if constexpr (LEVELS > 0) {
+    x += xchg64<LEVELS - 1>(x);
+    return lanes_total<LEVELS - 1>(x);
+  }
   return x;
 }
+// kBatch values summed over the lanes: the lane ends with value lane / 8.
+template <int N = kBatch, int LEVEL = 5>
+__device__ __forceinline__ double batch_totals(double* x, int lane) {
+  if constexpr (N > 1) {
+    const bool up = (lane >> LEVEL) & 1;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const double keep = up ? x[i + N / 2] : x[i], give = up ? x[i] : x[i + N / 2];
+      x[i] = keep + xchg64<LEVEL>(give);
+    }
+    return batch_totals<N / 2, LEVEL - 1>(x, lane);
+  }
+  return lanes_total<LEVEL + 1>(x[0]);
+}
+static_assert(kBatch == 8, "eight values leave three levels of single ones");
 
 // CH: 64 nodes each.
 template <bool DRAWN, int CH>
 __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
   __shared__ int32_t s_token[CH * 64], s_parent[CH * 64];
   __shared__ float s_rand[CH * 64], s_p[CH * 64], s_q[CH * 64];
-  __shared__ double s_mass[DRAWN ? CH * 64 : 1];  // the masses that rejections divided by
+  __shared__ double s_mass[kWaves][DRAWN ? CH * 64 : 1][2];  // each wave's copy of the masses that rejections divided by, and 1 / them
   __shared__ int32_t s_out[DRAWN ? 1 : CH * 64];  // the words that a sum leaves out
-  __shared__ double s_sum[kWaves];
+  __shared__ double s_sum[2][kWaves];             // the waves' sums of r, by turns
+  __shared__ double s_piece[kWaves][kPieces];     // and those of their pieces
   __shared__ int32_t s_last[kWaves];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -92,8 +129,9 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     path[c] = -1;
   }
 
-  // The wave's stretch of the words: whole steps of 256.
+  // The wave's stretch of the words: steps of 256, in at most kPieces pieces of `rounds`.
   const uint32_t steps = ((V + 255) / 256 + kWaves - 1) / kWaves;
+  const uint32_t rounds = (steps + kPieces - 1) / kPieces;  // a piece's steps
   const uint32_t from = wave * steps * 256 + lane * 4;
   auto word4 = [&](const float* row, uint32_t x) {  // words x .. x+3 of a row, zeros past its end
     f4 y = {0.f, 0.f, 0.f, 0.f};
@@ -106,79 +144,113 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     }
     return y;
   };
-  // The words of steps step .. step + kBatch - 1 of place cur, requested together.
+  // The words of steps step, step + stride, ... (kBatch of them) of place cur, requested
+  // together.
   struct Batch {
     f4 p[kBatch], q[DRAWN ? kBatch : 1];
   };
-  auto load = [&](int cur, uint32_t step, Batch& x) {
+  auto load = [&](int cur, uint32_t step, uint32_t stride, Batch& x) {
     const float* row = p.target + (base + cur) * V;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) x.p[i] = word4(row, step + i < steps ? from + (step + i) * 256 : V);
+    for (int i = 0; i < kBatch; ++i) x.p[i] = word4(row, step + i * stride < steps ? from + (step + i * stride) * 256 : V);
     if constexpr (DRAWN) {
       row = p.draft + (base + cur) * V;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) x.q[i] = word4(row, step + i < steps ? from + (step + i) * 256 : V);
+      for (int i = 0; i < kBatch; ++i) x.q[i] = word4(row, step + i * stride < steps ? from + (step + i * stride) * 256 : V);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  // What is left of N words after k rejections.
-  auto left_of = [&](const float* at_p, const float* at_q, int k, auto& r) {
-    constexpr int N = sizeof(r) / sizeof(double);
+  // Takes the k words of s_out out of a batch (without draft).
+  auto take_out = [&](uint32_t step, uint32_t stride, int k, Batch& x) {
+    uint32_t out = 0;  // bit 4 i + e: word e of the lane's four of step i
+    for (int j = 0; j < k; ++j) {
+      const uint32_t rel = __builtin_amdgcn_readfirstlane((uint32_t)s_out[j] - wave * steps * 256);
 #pragma unroll
-    for (int e = 0; e < N; ++e) r[e] = at_p[e] > 0.f ? (double)at_p[e] : 0.0;
-    if constexpr (DRAWN) {
-      if (k > 0) {
+      for (int i = 0; i < kBatch; ++i)
+        if (rel >> 8 == step + i * stride && (rel & 255) >> 2 == (uint32_t)lane) out |= 1u << (4 * i + (rel & 3));
+    }
+    if (__any(out)) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) r[e] = fmax(r[e] - (at_q[e] > 0.f ? (double)at_q[e] : 0.0), 0.0);
+      for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.p[i][e] = out >> (4 * i + e) & 1 ? 0.f : x.p[i][e];
+    }
+  };
+  // What is left of a word after k rejections.  max(p, q) - q is max(0, p - q), exactly;
+  // a quotient is the product with the inverse and one correction, which rounds it right.
+  auto left_of = [&](float at_p, float at_q, int k) {
+    const float p0 = fmaxf(at_p, 0.f);  // (of NaN, too)
+    if constexpr (!DRAWN) return (double)p0;
+    if (k == 0) return (double)p0;
+    const float q0 = fmaxf(at_q, 0.f);
+    const double q = (double)q0;
+    double r = (double)fmaxf(p0, q0) - q;
 #pragma unroll 1
-        for (int j = 1; j < k; ++j) {
-          const double m = s_mass[j];
+    for (int j = 1; j < k; ++j) {
+      const double m = s_mass[wave][j][0], by = s_mass[wave][j][1];
+      const double t = r * by, d = fma(fma(-t, m, r), by, t) - q;
+      r = d > 0.0 ? d : 0.0;
+    }
+    return r;
+  };
+  // Words of step i of a batch.
+  auto left4 = [&](const Batch& y, int i, int k, double (&r)[4]) {
+    if constexpr (DRAWN) {
+      // (As above, the loop over the rejections outside.)
+      float q0[4];
 #pragma unroll
-          for (int e = 0; e < N; ++e) r[e] = fmax(r[e] / m - (at_q[e] > 0.f ? (double)at_q[e] : 0.0), 0.0);
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = fmaxf(y.p[i][e], 0.f);
+        q0[e] = k > 0 ? fmaxf(y.q[i][e], 0.f) : 0.f;
+        r[e] = (double)fmaxf(p0, q0[e]) - (double)q0[e];
+      }
+#pragma unroll 1
+      for (int j = 1; j < k; ++j) {
+        const double m = s_mass[wave][j][0], by = s_mass[wave][j][1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const double t = r[e] * by, d = fma(fma(-t, m, r[e]), by, t) - (double)q0[e];
+          r[e] = d > 0.0 ? d : 0.0;
         }
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = (double)fmaxf(y.p[i][e], 0.f);
     }
   };
-  // The same of words x .. x+3 of step i of a batch (without draft: without the k words of
-  // s_out).
-  auto left4 = [&](const Batch& y, int i, uint32_t x, int k, double (&r)[4]) {
-    const float at_p[4] = {y.p[i][0], y.p[i][1], y.p[i][2], y.p[i][3]};
-    float at_q[4] = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (DRAWN) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) at_q[e] = y.q[i][e];
-    }
-    left_of(at_p, at_q, k, r);
-    if constexpr (!DRAWN) {
-      for (int j = 0; j < k; ++j) {
-        const uint32_t d = (uint32_t)s_out[j] - x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (d == (uint32_t)e) r[e] = 0.0;
-      }
-    }
-  };
-  // Its sum over all words, the waves' sums in s_sum.
+  // Its sum over all words; the waves' sums in s_sum[turn], and of their pieces in s_piece.
+  int turn = 0;
   auto sum_left = [&](int cur, int k) {
     double sum = 0.0;
 #pragma unroll 1
-    for (uint32_t step = 0; step < steps; step += kBatch) {
-      Batch y;
-      load(cur, step, y);
+    for (uint32_t piece = 0; piece * rounds < steps; piece += kBatch) {
+      double part[kBatch];
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        double r[4];
-        left4(y, i, from + (step + i) * 256, k, r);
-        sum += (r[0] + r[1]) + (r[2] + r[3]);
-        __builtin_amdgcn_sched_barrier(0);  // (registers)
+      for (int i = 0; i < kBatch; ++i) part[i] = 0.0;
+#pragma unroll 1
+      for (uint32_t round = 0; round < rounds; ++round) {
+        Batch y;
+        load(cur, piece * rounds + round, rounds, y);
+        if constexpr (!DRAWN) take_out(piece * rounds + round, rounds, k, y);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          double r[4];
+          left4(y, i, k, r);
+          part[i] += (r[0] + r[1]) + (r[2] + r[3]);
+          __builtin_amdgcn_sched_barrier(0);  // (registers)
+        }
       }
+      const double mine = batch_totals(part, lane);
+      if ((lane & 7) == 0) s_piece[wave][piece + lane / 8] = mine;
+      sum += (lane & 7) == 0 ? mine : 0.0;
     }
-    sum = wave_total(sum);
-    __syncthreads();
-    if (lane == 0) s_sum[wave] = sum;
+    sum = lanes_total(sum);
+    turn ^= 1;
+    if (lane == 0) s_sum[turn][wave] = sum;
     __syncthreads();
     double total = 0.0;
-    for (int w = 0; w < kWaves; ++w) total += s_sum[w];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += s_sum[turn][w];
     return total;
   };
 
@@ -217,9 +289,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
   };
   if (lane == 0) path[0] = 0;
   for (int i = next_child(0); i < n; i = next_child(i)) {
-    double left[1];
-    left_of(&s_p[i], &s_q[i], k, left);
-    double r = left[0];
+    double r = left_of(s_p[i], s_q[i], k);
     const int word = s_token[i];
     if constexpr (!DRAWN) {
 #pragma unroll
@@ -240,9 +310,10 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
       continue;
     }
     if constexpr (DRAWN) {
-      __syncthreads();
-      if (tid == 0) s_mass[k] = mass;
-      __syncthreads();
+      if (lane < 2) s_mass[wave][k][lane] = lane ? 1.0 / mass : mass;
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       const double total = sum_left(cur, k + 1);
       summed = total > 0.0;
       if (summed) {
@@ -271,7 +342,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
         more |= __any(counts[c]);
       }
       double total = others;
-      if (more) total += wave_total(behind);
+      if (more) total += lanes_total(behind);
       summed = total > 0.0 && !more;
       if (total > 0.0) {
         mass = total;
@@ -285,72 +356,90 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     total = sum_left(cur, k);
   }
 
-  // The draw: the first word at which the running sum passes its share of the whole.
+  // The draw: the first word at which the running sum passes its share of the whole.  The
+  // wave, then its piece, then the word; where rounding leaves none, the last with anything
+  // left.
   const double point = (double)s_rand[0] * total;
-  int at = -1;  // the wave
-  double below = 0.0;
-  for (int w = 0; w < kWaves && at < 0; ++w) {
-    if (below + s_sum[w] > point) at = w;
-    else below += s_sum[w];
-  }
   if (wave == 0) {
 #pragma unroll
     for (int c = 0; c < CH; ++c)
       if (c * 64 + lane < (int)p.T) p.path[base + c * 64 + lane] = path[c];
     if (lane == 0) p.accepted[b] = len;
   }
-  // Of the wave's stretch, the first word whose running sum from `below` passes the point,
-  // or else (rounding) the last of which anything is left.
-  auto search = [&](double below, double point) {
-    int found = -1, some = -1;
-#pragma unroll 1
-    for (uint32_t step = 0; step < steps && found < 0; step += kBatch) {
-      Batch y;
-      load(cur, step, y);
+  int at = -1;
+  double below = 0.0;
+  for (int w = 0; w < kWaves && at < 0; ++w) {
+    const double sum = s_sum[turn][w];
+    if (below + sum > point) at = w;
+    else below += sum;
+  }
+  // Running sums over the lanes, from `below` on.
+  auto running = [&](double x) {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        __builtin_amdgcn_sched_barrier(0);
-        if (found >= 0) continue;
-        const uint32_t x = from + (step + i) * 256;
-        double r[4];
-        left4(y, i, x, k, r);
-        const double four = (r[0] + r[1]) + (r[2] + r[3]);
-        double upto = four;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const double y = __shfl_up(upto, d, 64);
-          if (lane >= d) upto += y;
-        }
-        double run = below + (upto - four);
-        int mine = -1;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          run += r[e];
-          if (r[e] > 0.0) {
-            some = (int)(x + e);
-            if (mine < 0 && run > point) mine = (int)(x + e);
-          }
-        }
-        const uint64_t who = __ballot(mine >= 0);
-        if (who) found = __shfl(mine, __builtin_ctzll(who), 64);
-        below += __shfl(upto, 63, 64);
-      }
+    for (int d = 1; d < 64; d *= 2) {
+      const double y = __shfl_up(x, d, 64);
+      if (lane >= d) x += y;
     }
-    if (found >= 0) return found;
+    return below + x;
+  };
+  // The first word of piece `piece` of this wave whose running sum passes `point`, or -1;
+  // `some`: the last with anything left.
+  int some = -1;
+  auto search = [&](uint32_t piece, double point) {
+    int found = -1;
+#pragma unroll 1
+    for (uint32_t step = piece * rounds; step < min((piece + 1) * rounds, steps) && found < 0; ++step) {
+      Batch y;
+      const uint32_t x = from + step * 256;
+      y.p[0] = word4(p.target + (base + cur) * V, x);
+      if constexpr (DRAWN) y.q[0] = word4(p.draft + (base + cur) * V, x);
+      if constexpr (!DRAWN) {
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) some = max(some, __shfl_xor(some, d, 64));
-    return some;
+        for (int i = 1; i < kBatch; ++i) y.p[i] = f4{0.f, 0.f, 0.f, 0.f};
+        take_out(step, 1, k, y);
+      }
+      double r[4];
+      left4(y, 0, k, r);
+      const double four = (r[0] + r[1]) + (r[2] + r[3]), upto = running(four);
+      double run = upto - four;
+      int mine = -1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        run += r[e];
+        if (r[e] > 0.0) {
+          some = (int)(x + e);
+          if (mine < 0 && run > point) mine = (int)(x + e);
+        }
+      }
+      const uint64_t who = __ballot(mine >= 0);
+      if (who) found = __shfl(mine, __builtin_ctzll(who), 64);
+      below = __shfl(upto, 63, 64);
+    }
+    return found;
   };
   if (at >= 0) {
-    if (wave == at) {
-      const int word = search(below, point);
-      if (lane == 0) p.next[b] = word;
+    if (wave != at) return;
+    const uint32_t pieces = (steps + rounds - 1) / rounds;
+    const double mine = (uint32_t)lane < pieces ? s_piece[wave][lane] : 0.0, upto = running(mine);
+    const uint64_t who = __ballot((uint32_t)lane < pieces && mine > 0.0 && upto > point);
+    // (Rounding: the last piece with anything left.)
+    const uint64_t any = __ballot((uint32_t)lane < pieces && mine > 0.0);
+    const int piece = who ? __builtin_ctzll(who) : 63 - __builtin_clzll(any);
+    below = __shfl(upto - mine, piece, 64);
+    int word = search(piece, point);
+    if (word < 0) {
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) some = max(some, __shfl_xor(some, d, 64));
+      word = some;
     }
+    if (lane == 0) p.next[b] = word;
     return;
   }
-  // Rounding, or nothing left anywhere (-1): the last word of which anything is.
-  const int word = search(0.0, __builtin_inf());
-  if (lane == 0) s_last[wave] = word;
+  // Nothing passes the point: the last word of all with anything left, -1 if there is none.
+  for (uint32_t piece = 0; piece * rounds < steps; ++piece) search(piece, __builtin_inf());
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) some = max(some, __shfl_xor(some, d, 64));
+  if (lane == 0) s_last[wave] = some;
   __syncthreads();
   if (tid == 0) {
     int last = -1;

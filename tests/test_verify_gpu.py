@@ -115,6 +115,21 @@ def test_chosen_cases(gpu):
     run(odd, [0, 2, 3], [-1, 0, 0], [0.9, 0.8, 0.9], draft=np.array([np.nan, 0.25, 0.5, -1], np.float32))
 
 
+@pytest.mark.parametrize("V", [3, 700, 5000, 270001])
+def test_the_end_of_the_vocabulary(gpu, V):
+    """A share of all that is left (a number past the range, as rounding may give) takes the last
+    word with anything left; no share the first."""
+    p = np.zeros((2, 2, V), np.float32)
+    first, last = V // 3, V - 1 - V // 4
+    p[:, :, first:last + 1:2] = 2.0 ** -20
+    last -= (last - first) % 2
+    i = torch.zeros((2, 2), dtype=torch.int32, device="cuda")
+    rand = torch.tensor([[1.0, 0.5], [0.0, 0.5]], device="cuda")
+    path, accepted, following = sts_attn.verify_draft(torch.from_numpy(p).cuda(), i, i - 1, rand)
+    assert path.tolist() == [[0, -1], [0, -1]] and accepted.tolist() == [1, 1]
+    assert following.tolist() == [last, first]
+
+
 def test_tokens_follow_the_target(gpu):
     """The first token after node 0, kept or drawn, comes as often as the target says: within five
     standard deviations of a binomial count."""
