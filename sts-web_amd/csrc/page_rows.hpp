@@ -67,4 +67,13 @@ __device__ __forceinline__ float largest(float4 x) {
                                        __builtin_elementwise_maximum(fabsf(x.z), fabsf(x.w)));
 }
 
+// The largest magnitude of the G lanes' values (G consecutive lanes, a power of two).
+template <int G>
+__device__ __forceinline__ float lanes_largest(float4 x) {
+  float top = largest(x);
+#pragma unroll
+  for (int d = 1; d < G; d *= 2) top = __builtin_elementwise_maximum(top, __shfl_xor(top, d, G));
+  return top;
+}
+
 }  // namespace sts

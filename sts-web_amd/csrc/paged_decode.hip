@@ -65,7 +65,7 @@ __device__ __forceinline__ uint32_t pair_up(uint32_t hi, uint32_t lo) {
 
 // WHOLE: a tile never passes the end of a page.
 template <int D, int TYPE, bool PAD, bool WHOLE>
-__global__ __launch_bounds__(kWaves * 64, 3) void paged_decode_kernel(const PagedDecode p) {
+__global__ __launch_bounds__(kWaves * 64, TYPE == STS_PAGES_F32 ? 2 : 3) void paged_decode_kernel(const PagedDecode p) {
   constexpr bool F32 = TYPE == STS_PAGES_F32, I8 = TYPE == STS_PAGES_INT8;
   constexpr int ES = F32 ? 4 : I8 ? 1 : 2;
   constexpr int CW = 16 / ES;                     // dims of K a lane loads at once
@@ -88,6 +88,8 @@ __global__ __launch_bounds__(kWaves * 64, 3) void paged_decode_kernel(const Page
   auto& s_q = *reinterpret_cast<bf16x8(*)[NP][kParts][64]>(s_mem);
   auto& s_o = *reinterpret_cast<float(*)[kWaves][16][LDO]>(s_mem);
   __shared__ float s_ml[kWaves][16][2];
+  __shared__ __align__(16) char s_new[2][D * ES];  // the appended row, K and V, as the page holds it
+  __shared__ float s_scale[2];
   __shared__ uint32_t s_last;
 
   const PagedRows& rows = p.rows;
@@ -232,6 +234,60 @@ __global__ __launch_bounds__(kWaves * 64, 3) void paged_decode_kernel(const Page
     __syncthreads();
   }
 
+  // A row to append is made by the wave that comes to its tile, K by the first D / 4 lanes
+  // and V by the next: rotated, rounded, stored (by the first block of the group's heads)
+  // and left in LDS, from where it takes its place among the loaded rows.
+  const uint32_t new_row = len - 1, new_tile = new_row / TILE;
+  bool appended = false;
+  if (p.k_new && new_tile % nsplit == split && new_tile / nsplit % kWaves == (uint32_t)wave) {
+    const uint32_t page = (uint32_t)rows.table[(uint64_t)b * rows.max_pages + (new_row >> rows.shift)];
+    appended = page < rows.pages;
+    constexpr int G = D / 4;
+    const int which = lane / G;
+    const uint32_t d = lane % G * 4;
+    const bool on = which < 2 && (!PAD || d < dh);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on) {
+      x = *reinterpret_cast<const float4*>((which ? p.v_new : p.k_new) + b * p.new_stride + (uint64_t)kvh * dh + d);
+      if (rows.rope_cos && !which) {
+        const uint64_t ro = (uint64_t)new_row * (dh / 2) + d / 2;
+        x = rope4(x, *reinterpret_cast<const float2*>(rows.rope_cos + ro),
+                  *reinterpret_cast<const float2*>(rows.rope_sin + ro));
+      }
+    }
+    float scale = 1.f;
+    if constexpr (I8) scale = row_scale(lanes_largest<G>(x));
+    uint32_t words[ES];  // four values of ES bytes
+    if constexpr (I8) {
+      words[0] = row_codes(x, scale);
+    } else if constexpr (F32) {
+      words[0] = __float_as_uint(x.x);
+      words[1] = __float_as_uint(x.y);
+      words[2] = __float_as_uint(x.z);
+      words[3] = __float_as_uint(x.w);
+    } else {
+      const uint2 y = bf16x4(x);
+      words[0] = y.x;
+      words[1] = y.y;
+    }
+    if (on) {
+      uint32_t* to = reinterpret_cast<uint32_t*>(&s_new[which][d * ES]);
+#pragma unroll
+      for (int i = 0; i < ES; ++i) to[i] = words[i];
+      if (I8 && d == 0) s_scale[which] = scale;
+      if (appended && rb == 0) {
+        const uint64_t at = (uint64_t)page * page_heads + (head + (new_row & in_page));
+        to = reinterpret_cast<uint32_t*>(static_cast<char*>(which ? rows.v : rows.k) + at * rowb + d * ES);
+#pragma unroll
+        for (int i = 0; i < ES; ++i) to[i] = words[i];
+        if (I8 && d == 0) (which ? rows.vs : rows.ks)[at] = scale;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+
   // The weights are relative to m, which follows the scores' maximum only when they
   // pass it, and then to 2^kRoom above it: the outputs are seldom rescaled.  (A weight
   // below 2^-118 of the largest may be lost.)
@@ -242,6 +298,28 @@ __global__ __launch_bounds__(kWaves * 64, 3) void paged_decode_kernel(const Page
   for (int x = 0; x < NX; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   for (; t < tiles; t += tstep) {
+    if (appended && t == new_tile) {
+      const uint32_t r = new_row % TILE;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          if (r == (uint32_t)(kt * 16 + m16) && (!PAD || (uint32_t)(c * 4 + g) * CW < dh))
+            kk[kt][c] = *reinterpret_cast<const Words<CW * ES / 4>*>(&s_new[0][(c * 4 + g) * (CW * ES)]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (r == (uint32_t)(kt * 16 + 4 * g + i)) {
+#pragma unroll
+            for (int c = 0; c < NV; ++c)
+              if (!PAD || (uint32_t)(c * 16 + m16) * VW < dh)
+                vv[kt][i][c] = *reinterpret_cast<const Words<VW * ES / 4>*>(&s_new[1][(c * 16 + m16) * (VW * ES)]);
+            if constexpr (I8) {
+              ks[kt][i] = s_scale[0];
+              vs[kt][i] = s_scale[1];
+            }
+          }
+      }
+    }
     f32x4 s[KT];
     // The queries' parts are read anew for every tile: kept in registers (the compiler
     // lifts the loads out of the loop) they would take a third workgroup's.
@@ -483,11 +561,6 @@ void launch_type(const PagedDecode& p, dim3 grid, hipStream_t stream) {
 }
 
 }  // namespace
-
-int reserve_paged_decode(const PagedDecode& p, uint32_t batch, hipStream_t stream) {
-  Workspace* ws = nullptr;
-  return paged_workspace(p, plan_paged(p, batch), batch, stream, &ws);
-}
 
 int launch_paged_decode(PagedDecode p, uint32_t batch, hipStream_t stream) {
   const PagedPlan pl = plan_paged(p, batch);

@@ -23,10 +23,7 @@ __device__ __forceinline__ void store_row(void* rows, float* scales, uint64_t at
   } else if constexpr (TYPE == STS_PAGES_BF16) {
     if (on) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(rows) + to) = bf16x4(x);
   } else {
-    float top = largest(x);
-#pragma unroll
-    for (int d = 1; d < G; d *= 2) top = __builtin_elementwise_maximum(top, __shfl_xor(top, d, G));
-    const float s = row_scale(top);
+    const float s = row_scale(lanes_largest<G>(x));
     const uint32_t codes = row_codes(x, s);
     if (on) *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(rows) + to) = codes;
     if (on && c == 0) scales[at] = s;

@@ -71,7 +71,4 @@ struct PagedDecode {
 };
 int launch_paged_decode(PagedDecode p, uint32_t batch, hipStream_t stream);
 
-// Makes sure that the split workspace launch_paged_decode needs exists.
-int reserve_paged_decode(const PagedDecode& p, uint32_t batch, hipStream_t stream);
-
 }  // namespace sts

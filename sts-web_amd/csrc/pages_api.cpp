@@ -127,15 +127,9 @@ int sts_paged_decode(const sts_pages* pages, const sts_rope* rope, const float* 
     a.stride = new_stride;
     a.T = 1;
     if (int rc = check_append(a, batch)) return rc;
-    if (d.group == 1) {
-      d.k_new = k_new;
-      d.v_new = v_new;
-      d.new_stride = new_stride;
-    } else {
-      // A rejected call leaves the pages as they were.
-      if (int rc = sts::reserve_paged_decode(d, batch, as_stream(stream))) return rc;
-      if (int rc = sts::launch_paged_append(a, batch, as_stream(stream))) return rc;
-    }
+    d.k_new = k_new;
+    d.v_new = v_new;
+    d.new_stride = new_stride;
   }
   return sts::launch_paged_decode(d, batch, as_stream(stream));
 }
