@@ -163,7 +163,7 @@ int sts_verify_draft(const float* target, const float* draft, const int32_t* tok
   STS_CHECK(target && tokens && parents && rand && path && accepted && next, "null pointer argument");
   STS_CHECK(nodes >= 1 && nodes <= STS_TREE_MAX_NODES, "nodes %u must be in 1..%u", nodes, STS_TREE_MAX_NODES);
   STS_CHECK(batch >= 1 && vocab >= 1, "empty shape");
-  STS_CHECK(batch <= 65535 && vocab <= (1u << 30), "batch (%u) must be <= 65535 and vocab (%u) <= 2^30", batch,
+  STS_CHECK(batch <= 65535 && vocab <= (1u << 28), "batch (%u) must be <= 65535 and vocab (%u) <= 2^28", batch,
             vocab);
   sts::VerifyDraft v;
   v.target = target;

@@ -20,6 +20,7 @@
 // together; whole rows only where something is rejected and for the last draw, each wave
 // a stretch of the words, so that the draw finds its wave from sixteen sums.  What bounds
 // it is the latency of these steps, not the bytes.
+#include "coherent.hpp"
 #include "common.hpp"
 #include "lane.hpp"
 #include "verify.hpp"
@@ -31,7 +32,8 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBatch = 8;
-typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // rows start anywhere
+constexpr uint32_t kOutside = 0x80000000u;  // past every row: loads zeros
+typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPieces = 64;  // sums that a wave keeps of its stretch of the words
 
@@ -133,30 +135,25 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
   const uint32_t steps = ((V + 255) / 256 + kWaves - 1) / kWaves;
   const uint32_t rounds = (steps + kPieces - 1) / kPieces;  // a piece's steps
   const uint32_t from = wave * steps * 256 + lane * 4;
-  auto word4 = [&](const float* row, uint32_t x) {  // words x .. x+3 of a row, zeros past its end
-    f4 y = {0.f, 0.f, 0.f, 0.f};
-    if (x + 4 <= V) {
-      y = *reinterpret_cast<const f4*>(row + x);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (x + e < V) y[e] = row[x + e];
-    }
-    return y;
-  };
   // The words of steps step, step + stride, ... (kBatch of them) of place cur, requested
   // together.
   struct Batch {
     f4 p[kBatch], q[DRAWN ? kBatch : 1];
   };
+  // (Buffer loads: words past the row's end are zeros, without a branch.)
+  auto row_of = [&](const float* x, int cur) { return coherent_rsrc(x + (base + cur) * V, V * 4); };
+  auto word4 = [&](__amdgpu_buffer_rsrc_t row, uint32_t step) {
+    return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(
+                                      row, step < steps ? (from + step * 256) * 4 : kOutside, 0, 0));
+  };
   auto load = [&](int cur, uint32_t step, uint32_t stride, Batch& x) {
-    const float* row = p.target + (base + cur) * V;
+    const __amdgpu_buffer_rsrc_t target = row_of(p.target, cur);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) x.p[i] = word4(row, step + i * stride < steps ? from + (step + i * stride) * 256 : V);
+    for (int i = 0; i < kBatch; ++i) x.p[i] = word4(target, step + i * stride);
     if constexpr (DRAWN) {
-      row = p.draft + (base + cur) * V;
+      const __amdgpu_buffer_rsrc_t draft = row_of(p.draft, cur);
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) x.q[i] = word4(row, step + i * stride < steps ? from + (step + i * stride) * 256 : V);
+      for (int i = 0; i < kBatch; ++i) x.q[i] = word4(draft, step + i * stride);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -391,8 +388,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     for (uint32_t step = piece * rounds; step < min((piece + 1) * rounds, steps) && found < 0; ++step) {
       Batch y;
       const uint32_t x = from + step * 256;
-      y.p[0] = word4(p.target + (base + cur) * V, x);
-      if constexpr (DRAWN) y.q[0] = word4(p.draft + (base + cur) * V, x);
+      y.p[0] = word4(row_of(p.target, cur), step);
+      if constexpr (DRAWN) y.q[0] = word4(row_of(p.draft, cur), step);
       if constexpr (!DRAWN) {
 #pragma unroll
         for (int i = 1; i < kBatch; ++i) y.p[i] = f4{0.f, 0.f, 0.f, 0.f};

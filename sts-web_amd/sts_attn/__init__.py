@@ -491,6 +491,9 @@ def _heads_stride(t: torch.Tensor, name: str, lead, heads: Optional[int], D: int
     """(address, stride between tokens in elements) of float32 rows [*lead, heads, D] whose
     last two dimensions are contiguous and whose tokens are equally far apart."""
     shape = t.shape
+    if (t.is_contiguous() and t.dtype is _f32t and shape[:-2] == lead and shape[-1] == D
+            and (heads is None or shape[-2] == heads) and t.device == device):
+        return t.data_ptr(), shape[-2] * D
     if t.dtype is not _f32t:
         raise TypeError(f"{name} must be {_f32t}, got {t.dtype}")
     if len(shape) != len(lead) + 2 or shape[-1] != D or tuple(shape[:-2]) != lead or (heads and shape[-2] != heads):

@@ -116,7 +116,7 @@ def test_verify_refusals():
     assert "empty" in _err(verify(batch=0))
     assert "empty" in _err(verify(vocab=0))
     assert "65535" in _err(verify(batch=65536))
-    assert "vocab" in _err(verify(vocab=(1 << 30) + 1))
+    assert "vocab" in _err(verify(vocab=(1 << 28) + 1))
 
 
 def test_pages_layout_matches_header():
