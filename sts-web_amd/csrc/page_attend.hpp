@@ -98,7 +98,23 @@ __device__ __forceinline__ bool find_share(const PagedDecode& p, uint32_t share,
 constexpr int kAhead = 8;
 constexpr int kClusters = 16;  // at most: of kMaxSplits, 11
 constexpr uint32_t kCounters = 1 + kClusters;  // arrival counters of a block
-constexpr int kMergeBytes = 2 * kMaxSplits * 16 * 4 + kWaves * 64 * 16;
+constexpr int kMergeBytes = kMaxSplits * 16 * 4 + 128 + kWaves * 64 * 16;
+
+// Over all 64 lanes.
+__device__ __forceinline__ float lanes_max(float x) {
+  x = fmaxf(x, xchg<0>(x));
+  x = fmaxf(x, xchg<1>(x));
+  x = fmaxf(x, xchg<2>(x));
+  x = fmaxf(x, xchg<3>(x));
+  return max_xor32(max_xor16(x));
+}
+__device__ __forceinline__ float lanes_sum(float x) {
+  x += xchg<0>(x);
+  x += xchg<1>(x);
+  x += xchg<2>(x);
+  x += xchg<3>(x);
+  return sum_xor32(sum_xor16(x));
+}
 
 struct Records {
   __amdgpu_buffer_rsrc_t rs;
@@ -131,9 +147,9 @@ __device__ __forceinline__ void merge_records(const Records& r, uint32_t from, u
   constexpr int C4 = D / 4;
   const int tid = threadIdx.x;
   const uint32_t live = r.live, slots = live * C4;
-  auto& s_f = *reinterpret_cast<float(*)[kMaxSplits][16]>(mem);
-  auto& s_l = *reinterpret_cast<float(*)[kMaxSplits][16]>(mem + kMaxSplits * 16 * 4);
-  auto& s_sum = *reinterpret_cast<f32x4(*)[kWaves * 64]>(mem + 2 * kMaxSplits * 16 * 4);
+  auto& s_f = *reinterpret_cast<float(*)[kMaxSplits][16]>(mem);  // the records' factors 2^(m_s - m)
+  auto& s_ml = *reinterpret_cast<float(*)[2][16]>(mem + kMaxSplits * 16 * 4);
+  auto& s_sum = *reinterpret_cast<f32x4(*)[kWaves * 64]>(mem + kMaxSplits * 16 * 4 + 128);
   coh_f4 y[kAhead];
   // Groups of threads, one for each column, take the records in turn.
   auto request = [&](uint32_t sp, uint32_t groups, uint32_t x) {
@@ -142,27 +158,41 @@ __device__ __forceinline__ void merge_records(const Records& r, uint32_t from, u
       y[u] = ld_coherent4(r.rs, sp + u * groups < n ? ((from + (sp + u * groups) * step) * r.size + x * 4) * 4 : kOutside);
   };
   const uint32_t n0 = min(slots, (uint32_t)(kWaves * 64)), g0 = kWaves * 64 / n0;
-  if (tid / n0 < g0) request(tid / n0, g0, tid % n0);
-  for (uint32_t x = tid; x < n * live; x += kWaves * 64) {
-    const uint32_t sp = x / live, row = x % live;
-    const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(
-        r.rs, ((from + sp * step) * r.size + live * D + row * 2) * 4, 0, kSc1);
-    s_f[sp][row] = __uint_as_float(ml[0]);
-    s_l[sp][row] = __uint_as_float(ml[1]);
-  }
-  __syncthreads();
-  // m gives way to the record's factor 2^(m_s - m); the block's m and l take the place
-  // behind the last record's.
-  if (tid < (int)live) {
-    float mt = -FLT_MAX, lt = 0.f;
-    for (uint32_t sp = 0; sp < n; ++sp) mt = fmaxf(mt, s_f[sp][tid]);
-    for (uint32_t sp = 0; sp < n; ++sp) {
-      const float f = exp2_hw(s_f[sp][tid] - mt);
-      s_f[sp][tid] = f;
-      lt += f * s_l[sp][tid];
+  // A wave looks after every fourth head, its lanes after two records each.
+  const uint32_t lane = tid & 63, wave = tid >> 6;
+  u32x2 ml[16 / kWaves][2];
+#pragma unroll
+  for (int i = 0; i < 16 / kWaves; ++i)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t sp = lane + 64 * u, row = wave + kWaves * i;
+      ml[i][u] = __builtin_amdgcn_raw_buffer_load_b64(
+          r.rs, sp < n && row < live ? ((from + sp * step) * r.size + live * D + row * 2) * 4 : kOutside, 0, kSc1);
     }
-    s_l[0][tid] = lt;
-    s_l[1][tid] = mt;
+  if (tid / n0 < g0) request(tid / n0, g0, tid % n0);
+#pragma unroll
+  for (int i = 0; i < 16 / kWaves; ++i) {
+    const uint32_t row = wave + kWaves * i;
+    if (row >= live) break;
+    float m[2], mt = -FLT_MAX;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      m[u] = lane + 64 * u < n ? __uint_as_float(ml[i][u][0]) : -FLT_MAX;
+      mt = fmaxf(mt, m[u]);
+    }
+    mt = lanes_max(mt);
+    float lt = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float f = exp2_hw(m[u] - mt);
+      if (lane + 64 * u < n) s_f[lane + 64 * u][row] = f;
+      lt += f * __uint_as_float(ml[i][u][1]);  // (0 past the records)
+    }
+    lt = lanes_sum(lt);
+    if (lane == 0) {
+      s_ml[0][row] = mt;
+      s_ml[1][row] = lt;
+    }
   }
   __syncthreads();
   for (uint32_t x0 = 0; x0 < slots; x0 += kWaves * 64) {
@@ -183,7 +213,7 @@ __device__ __forceinline__ void merge_records(const Records& r, uint32_t from, u
       if (grp == 0)
         for (uint32_t u = 1; u < groups; ++u) a += s_sum[tid + u * cols];
     }
-    if (grp == 0) put(x, make_float4(a[0], a[1], a[2], a[3]), s_l[1][x / C4], s_l[0][x / C4]);
+    if (grp == 0) put(x, make_float4(a[0], a[1], a[2], a[3]), s_ml[0][x / C4], s_ml[1][x / C4]);
   }
 }
 

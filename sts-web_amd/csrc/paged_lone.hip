@@ -8,8 +8,7 @@
 // requested while it works on the last.  The dot products are summed over the G lanes by
 // a butterfly that leaves each lane one row's score, so that scales, masks and
 // exponentials are done once a row, and the weights go to the row's lanes through LDS.
-// Each row group of a wave keeps its own running maximum and sum; they are merged at the
-// end.  Sixteen rows lie in one page and have a buffer resource of their own, as there.
+// Sixteen rows lie in one page and have a buffer resource of their own, as there.
 //
 // A row to be appended is made by the wave that comes to its unit: rotated, rounded,
 // stored, and used from registers.
@@ -52,6 +51,27 @@ __device__ __forceinline__ float fold_all(float* s, int c) {
   }
   return s[0];
 }
+// The same over lanes whose index differs in bits FROM .. FROM + log2 N - 1 alone: N
+// values in, of which each lane ends with N / M (those from (lane >> FROM) N / M on), M the
+// number of lanes.
+template <int LEVEL>
+__device__ __forceinline__ float xor_lane(float x) {
+  if constexpr (LEVEL == 5) return xor32(x);
+  else return __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(x), 0x1F | 1 << (LEVEL + 10)));
+}
+template <int FROM, int LEVEL, int N>
+__device__ __forceinline__ void fold_groups(float* s, int lane) {
+  if constexpr (LEVEL >= FROM) {
+    static_assert(N > 1, "a value for each lane at least");
+    const bool hi = (lane >> LEVEL) & 1;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float a = s[i], z = s[i + N / 2];
+      s[i] = (hi ? z : a) + xor_lane<LEVEL>(hi ? a : z);
+    }
+    fold_groups<FROM, LEVEL - 1, N / 2>(s, lane);
+  }
+}
 // An operation over lanes whose index differs in bits FROM .. TO-1.
 template <int FROM, int TO, class Op>
 __device__ __forceinline__ float over(float x, Op op) {
@@ -70,17 +90,14 @@ __global__ __launch_bounds__(kWaves * 64) void paged_lone_kernel(const PagedDeco
   constexpr int RPG = G < 8 ? G : 8, LR = log2_of(RPG);  // loads of a unit
   constexpr int UNIT = NG * RPG;
   constexpr int NSUB = UNIT / 16;
-  constexpr int NST = kWaves * NG;
   constexpr int C4 = D / 4;
   static_assert(UNIT >= 16, "whole sixteens");
 
-  constexpr int kAccBytes = NST * D * 4;
+  constexpr int kAccBytes = kWaves * D * 4;
   __shared__ __align__(16) char s_mem[kAccBytes > kMergeBytes ? kAccBytes : kMergeBytes];
-  auto& s_acc = *reinterpret_cast<float(*)[NST][D]>(s_mem);
+  auto& s_acc = *reinterpret_cast<float(*)[kWaves][D]>(s_mem);
   __shared__ __align__(16) float s_p[kWaves][UNIT];
-  __shared__ float s_ml[NST][2];
-  __shared__ f32x4 s_part[kWaves * 64];
-  __shared__ float s_sums[kWaves * 64 / C4];
+  __shared__ float s_ml[kWaves][2];
   __shared__ uint32_t s_last;
 
   const PagedRows& rows = p.rows;
@@ -270,7 +287,9 @@ __global__ __launch_bounds__(kWaves * 64) void paged_lone_kernel(const PagedDeco
     float sc = fold_all<LG, RPG>(s, c);
     if constexpr (I8) sc *= ks;
     sc = now.seen ? sc : -INFINITY;
-    const float top = over<LG - LR, LG>(sc, [](float a, float z) { return fmaxf(a, z); });
+    // (One maximum for the wave, so that its rows' sums add up without factors.)
+    float top = over<LG - LR, 4>(sc, [](float a, float z) { return fmaxf(a, z); });
+    top = max_xor32(max_xor16(top));
     if (__any(top > m)) {
       const float to = top > m ? top + kRoom : m, alpha = exp2_hw(m - to);
       m = to;
@@ -309,32 +328,17 @@ __global__ __launch_bounds__(kWaves * 64) void paged_lone_kernel(const PagedDeco
     u += step;
   }
 
-  // The row groups' states merged through LDS: rows are in the 2^(LG - LR) lanes that
-  // share them, a group's sum is over the others.
-  l = over<LG - LR, LG>(l, [](float a, float z) { return a + z; });
+  // The row groups' sums added up, and the waves' states merged through LDS.  (A row's weight
+  // is in the 2^(LG - LR) lanes that share it.)
+  l = sum_xor32(sum_xor16(over<LG - LR, 4>(l, [](float a, float z) { return a + z; })));
+  fold_groups<LG, 5, CW>(acc, lane);
+  constexpr int PER = CW / NG;
 #pragma unroll
-  for (int e = 0; e < CW; e += 4)
-    *reinterpret_cast<f32x4*>(&s_acc[wave * NG + g][c * CW + e]) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
-  if (c == 0) {
-    s_ml[wave * NG + g][0] = m;
-    s_ml[wave * NG + g][1] = l;
+  for (int e = 0; e < PER; ++e) s_acc[wave][c * CW + g * PER + e] = acc[e];
+  if (lane == 0) {
+    s_ml[wave][0] = m;
+    s_ml[wave][1] = l;
   }
-  __syncthreads();
-  float mt = s_ml[0][0];
-#pragma unroll
-  for (int x = 1; x < NST; ++x) mt = fmaxf(mt, s_ml[x][0]);
-  constexpr int PARTS = kWaves * 64 / C4;
-  const int col = tid % C4, part = tid / C4;
-  f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
-  float lt = 0.f;
-#pragma unroll
-  for (int x = 0; x < NST; x += PARTS) {
-    const float f = exp2_hw(s_ml[x + part][0] - mt);
-    lt = fmaf(f, s_ml[x + part][1], lt);
-    a += *reinterpret_cast<const f32x4*>(&s_acc[x + part][col * 4]) * f;
-  }
-  s_part[tid] = a;
-  if (col == 0) s_sums[part] = lt;
   __syncthreads();
   auto finish = [&](uint32_t x, float4 a, float, float lt) {
     const float f = lt > 0.f || lt != lt ? 1.f / lt : 0.f;  // nothing seen: zeros
@@ -345,12 +349,15 @@ __global__ __launch_bounds__(kWaves * 64) void paged_lone_kernel(const PagedDeco
                                   nsplit > 1 ? at.splits * p.record * 4 : 0),
                     p.record, 1};
   if (tid < C4) {
-    lt = 0.f;
-    a = f32x4{0.f, 0.f, 0.f, 0.f};
+    float mt = s_ml[0][0], lt = 0.f;
 #pragma unroll
-    for (int x = 0; x < PARTS; ++x) {
-      a += s_part[x * C4 + tid];
-      lt += s_sums[x];
+    for (int w = 1; w < kWaves; ++w) mt = fmaxf(mt, s_ml[w][0]);
+    f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = exp2_hw(s_ml[w][0] - mt);
+      lt = fmaf(f, s_ml[w][1], lt);
+      a += *reinterpret_cast<const f32x4*>(&s_acc[w][tid * 4]) * f;
     }
     const float4 y = make_float4(a[0], a[1], a[2], a[3]);
     if (nsplit == 1) finish(tid, y, mt, lt);
