@@ -81,7 +81,9 @@ template <bool DRAWN, int CH>
 __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
   __shared__ int32_t s_token[CH * 64], s_parent[CH * 64];
   __shared__ float s_rand[CH * 64], s_p[CH * 64], s_q[CH * 64];
-  __shared__ double s_mass[kWaves][DRAWN ? CH * 64 : 1][2];  // each wave's copy of the masses that rejections divided by, and 1 / them
+  // The masses that a place's second and later rejections divide by, and 1 / them.  Every wave
+  // writes the same; an entry changes only behind a barrier of the place's first sum.
+  __shared__ double s_mass[DRAWN ? CH * 64 : 1][2];
   __shared__ int32_t s_out[DRAWN ? 1 : CH * 64];  // the words that a sum leaves out
   __shared__ double s_sum[2][kWaves];             // the waves' sums of r, by turns
   __shared__ double s_piece[kWaves][kPieces];     // and those of their pieces
@@ -184,7 +186,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     double r = (double)fmaxf(p0, q0) - q;
 #pragma unroll 1
     for (int j = 1; j < k; ++j) {
-      const double m = s_mass[wave][j][0], by = s_mass[wave][j][1];
+      const double m = s_mass[j][0], by = s_mass[j][1];
       const double t = r * by, d = fma(fma(-t, m, r), by, t) - q;
       r = d > 0.0 ? d : 0.0;
     }
@@ -203,7 +205,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
       }
 #pragma unroll 1
       for (int j = 1; j < k; ++j) {
-        const double m = s_mass[wave][j][0], by = s_mass[wave][j][1];
+        const double m = s_mass[j][0], by = s_mass[j][1];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const double t = r[e] * by, d = fma(fma(-t, m, r[e]), by, t) - (double)q0[e];
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
       continue;
     }
     if constexpr (DRAWN) {
-      if (lane < 2) s_mass[wave][k][lane] = lane ? 1.0 / mass : mass;
+      if (k > 0 && lane < 2) s_mass[k][lane] = lane ? 1.0 / mass : mass;
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");

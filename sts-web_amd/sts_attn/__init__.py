@@ -19,6 +19,7 @@ counterpart of the reference's `.expect(...)` panics.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from typing import Optional, Sequence
 
@@ -501,17 +502,15 @@ def _heads_stride(t: torch.Tensor, name: str, lead, heads: Optional[int], D: int
         raise ValueError(f"{name} must be [{want}], got {tuple(shape)}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
-    st = t.stride()
-    step = st[-3] if shape[-3] > 1 else 0
-    if len(lead) == 2 and shape[0] > 1:
-        # One distance for all tokens: from stream to stream too.
-        if shape[1] == 1:
-            step = st[0]
-        elif st[0] != step * shape[1]:
-            raise ValueError(f"{name}'s tokens must be equally far apart")
+    st, row = t.stride(), shape[-2] * D
     if (D > 1 and st[-1] != 1) or (shape[-2] > 1 and st[-2] != D):
         raise ValueError(f"{name}'s heads must be contiguous")
-    return t.data_ptr(), step or shape[-2] * D
+    # One distance for all tokens, from stream to stream too, and no token over another.
+    steps = {st[i] // math.prod(shape[i + 1:-2]) if st[i] % math.prod(shape[i + 1:-2]) == 0 else 0
+             for i in range(len(lead)) if shape[i] > 1}
+    if len(steps) > 1 or any(x < row for x in steps):
+        raise ValueError(f"{name}'s tokens must be equally far apart and not overlap")
+    return t.data_ptr(), steps.pop() if steps else row
 
 
 class PagedKV:

@@ -166,9 +166,15 @@ def test_strides_of_new_rows():
     assert at(qkv[:1, :, 2:4], (1, 5)) == 48
     assert at(qkv[0, :, 2:4], (5,)) == 48
     assert at(qkv[:1, :1, 2:4], (1, 1)) == 16
-    for wrong in (qkv[:, :4, 2:4], qkv.transpose(0, 1)[:, :, 2:4]):
+    one = torch.zeros((1, 1, 2, 8))
+    for wrong in (qkv[:, :4, 2:4], qkv.transpose(0, 1)[:, :, 2:4], one.expand(3, 1, 2, 8), one.expand(1, 5, 2, 8),
+                  one.expand(3, 5, 2, 8), qkv[:1, :, 2:4].expand(3, 5, 2, 8), qkv.as_strided((3, 5, 2, 8), (60, 12, 8, 1))):
         with pytest.raises(ValueError, match="equally far"):
             at(wrong, tuple(wrong.shape[:2]))
+    for wrong in (one[0].expand(3, 2, 8), qkv.as_strided((3, 2, 8), (8, 8, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            at(wrong, (3,))
+    assert at(one.expand(3, 5, 2, 8)[:1, :1], (1, 1)) == 16
     with pytest.raises(ValueError, match="heads must be contiguous"):
         at(qkv[:, :, ::3], (3, 5))
     with pytest.raises(TypeError, match="float32"):

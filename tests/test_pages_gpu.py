@@ -216,6 +216,13 @@ def test_decode_many_streams(gpu, rows):
     check_decode(Pool(12, lens, 2, 64, 16, rows), 4)
 
 
+@pytest.mark.parametrize("rows,H", [("f32", 1), ("bf16", 2), ("int8", 3), ("int8", 1)])
+def test_decode_many_streams_in_splits(gpu, rows, H):
+    """More streams than a wave looks at, with few heads, so that each is split."""
+    lens = np.r_[np.random.default_rng(24).integers(0, 700, 68), 900, 1]
+    check_decode(Pool(25, lens, 1, 64, 32, rows), H)
+
+
 @pytest.mark.parametrize("rows", ["f32", "bf16", "int8"])
 def test_decode_missing_pages(gpu, rows):
     """Rows of an entry that is no page have no part: in the middle, first, last, all of them."""
@@ -379,6 +386,25 @@ def test_calls_on_another_stream(gpu):
     for o in outs:
         assert torch.equal(o, want)
     assert torch.equal(k, k2) and torch.equal(v, v2)
+
+
+def test_two_streams_at_once(gpu):
+    """Split decodes that run side by side on two streams keep to their own workspaces."""
+    pools = [Pool(26 + i, [3000 - 500 * i, 800], 2, 128, 32, rows) for i, rows in enumerate(("int8", "f32"))]
+    calls = []
+    for pool, H in zip(pools, (2, 6)):
+        cache, table, lens = pool.gpu()
+        calls.append((cache, torch.from_numpy(queries(pool.rng, 2, H, 128)).cuda(), table, lens))
+    want = [c.decode(q, t, n, 0.1) for c, q, t, n in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[] for _ in calls]
+    for _ in range(20):
+        for i, (c, q, t, n) in enumerate(calls):
+            got[i].append(c.decode(q, t, n, 0.1, stream=streams[i]))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, w) for x in g)
 
 
 @pytest.mark.parametrize("rows", ["f32", "bf16", "int8"])
