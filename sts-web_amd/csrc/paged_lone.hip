@@ -80,8 +80,14 @@ __device__ __forceinline__ float over(float x, Op op) {
 }
 constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
 
+// (Of 8-bit rows two workgroups a CU, not the three that its registers would allow: 64
+// streams 134.7 us for 139.  The others have four: 9 streams' f32 step 71.3 us, with two 72.9.)
+template <int TYPE>
+constexpr int kMostWaves = TYPE == STS_PAGES_INT8 ? 2 : 8;
+
 template <int D, int TYPE, bool PAD>
-__global__ __launch_bounds__(kWaves * 64) void paged_lone_kernel(const PagedDecode p) {
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, kMostWaves<TYPE>)))
+void paged_lone_kernel(const PagedDecode p) {
   constexpr bool I8 = TYPE == STS_PAGES_INT8;
   constexpr int ES = TYPE == STS_PAGES_F32 ? 4 : I8 ? 1 : 2;
   constexpr int CW = 16 / ES;                // a lane's dims

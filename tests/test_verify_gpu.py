@@ -25,7 +25,7 @@ def tree(rng, T):
 
 def check(target, draft, tokens, parents, rand, counts=None):
     B, T, V = target.shape
-    dev = [None if x is None else torch.from_numpy(np.ascontiguousarray(x)).cuda()
+    dev = [None if x is None else torch.from_numpy(np.array(x, order="C")).cuda()
            for x in (target, tokens.astype(np.int32), parents.astype(np.int32), rand.astype(np.float32), draft,
                      None if counts is None else np.asarray(counts, np.int32))]
     path, accepted, following = (x.cpu().numpy() for x in sts_attn.verify_draft(*dev[:4], draft=dev[4], counts=dev[5]))
