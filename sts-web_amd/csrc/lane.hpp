@@ -8,6 +8,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstdint>
+
 namespace sts {
 
 // GFX9 DPP control encodings.
@@ -61,6 +63,30 @@ __device__ __forceinline__ float sum_xor16(float x) {
 __device__ __forceinline__ float sum_xor32(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The sum of x over the lanes up to this one, by the row shifts and row broadcasts of DPP
+// (six steps on the vector unit, where a shuffle is a trip through the LDS unit).
+// lane_from<CTRL, ROWS>: the value of the lane that CTRL names, for the rows of ROWS; 0 where
+// there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lane_from(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double lane_from(double x) {
+  const uint2 y = __builtin_bit_cast(uint2, x);
+  return __builtin_bit_cast(double, make_uint2(lane_from<CTRL, ROWS>(y.x), lane_from<CTRL, ROWS>(y.y)));
+}
+template <class T>
+__device__ __forceinline__ T lanes_upto(T x) {
+  x += lane_from<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
+  x += lane_from<0x112, 0xF>(x);
+  x += lane_from<0x114, 0xF>(x);
+  x += lane_from<0x118, 0xF>(x);
+  x += lane_from<0x142, 0xA>(x);  // row_bcast 15: rows 1 and 3 take the row before's sum
+  x += lane_from<0x143, 0xC>(x);  // row_bcast 31: rows 2 and 3 the first half's
+  return x;
 }
 
 }  // namespace sts

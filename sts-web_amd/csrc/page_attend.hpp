@@ -39,6 +39,22 @@ struct Words {
   }
 };
 
+// Over all 64 lanes.
+__device__ __forceinline__ float lanes_max(float x) {
+  x = fmaxf(x, xchg<0>(x));
+  x = fmaxf(x, xchg<1>(x));
+  x = fmaxf(x, xchg<2>(x));
+  x = fmaxf(x, xchg<3>(x));
+  return max_xor32(max_xor16(x));
+}
+__device__ __forceinline__ float lanes_sum(float x) {
+  x += xchg<0>(x);
+  x += xchg<1>(x);
+  x += xchg<2>(x);
+  x += xchg<3>(x);
+  return sum_xor32(sum_xor16(x));
+}
+
 // What a workgroup has to do: one split of one stream and K/V head.
 struct Share {
   uint32_t b, kvh, split, splits;
@@ -56,17 +72,10 @@ __device__ __forceinline__ bool find_share(const PagedDecode& p, uint32_t share,
     // no more shares.
     const int lane = threadIdx.x & 63;
     const uint32_t mine_len = lane < (int)p.batch ? paged_len(rows, lane) : 0u;
-    float total = (float)mine_len;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x, 64);
+    const float total = lanes_sum((float)mine_len);
     const uint32_t chunk = max((uint32_t)min(total * p.rows_factor, 0x1p31f) + 1, unit);
     const uint32_t mine = lane < (int)p.batch ? min(max((mine_len + chunk - 1) / chunk, 1u), p.nsplit) : 0;
-    uint32_t before = mine;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) {
-      const uint32_t y = (uint32_t)__shfl_up((int)before, x, 64);
-      before += lane >= x ? y : 0;
-    }
+    uint32_t before = lanes_upto(mine);
     if (share >= (uint32_t)__builtin_amdgcn_readlane((int)before, 63) * rows.KH) return false;
     before -= mine;
     s.b = 63 - __builtin_clzll(__ballot(lane < (int)p.batch && before * rows.KH <= share));
@@ -99,22 +108,6 @@ constexpr int kAhead = 8;
 constexpr int kClusters = 16;  // at most: of kMaxSplits, 11
 constexpr uint32_t kCounters = 1 + kClusters;  // arrival counters of a block
 constexpr int kMergeBytes = kMaxSplits * 16 * 4 + 128 + kWaves * 64 * 16;
-
-// Over all 64 lanes.
-__device__ __forceinline__ float lanes_max(float x) {
-  x = fmaxf(x, xchg<0>(x));
-  x = fmaxf(x, xchg<1>(x));
-  x = fmaxf(x, xchg<2>(x));
-  x = fmaxf(x, xchg<3>(x));
-  return max_xor32(max_xor16(x));
-}
-__device__ __forceinline__ float lanes_sum(float x) {
-  x += xchg<0>(x);
-  x += xchg<1>(x);
-  x += xchg<2>(x);
-  x += xchg<3>(x);
-  return sum_xor32(sum_xor16(x));
-}
 
 struct Records {
   __amdgpu_buffer_rsrc_t rs;

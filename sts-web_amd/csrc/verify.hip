@@ -373,14 +373,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     else below += sum;
   }
   // Running sums over the lanes, from `below` on.
-  auto running = [&](double x) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const double y = __shfl_up(x, d, 64);
-      if (lane >= d) x += y;
-    }
-    return below + x;
-  };
+  auto running = [&](double x) { return below + lanes_upto(x); };
   // The first word of piece `piece` of this wave whose running sum passes `point`, or -1;
   // `some`: the last with anything left.
   int some = -1;

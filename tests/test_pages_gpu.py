@@ -185,7 +185,7 @@ def check_decode(pool, H, q=None, scale=None, got=None, **kw):
 SHAPES = [("f32", 128, 4, 4, 16), ("f32", 64, 8, 2, 64), ("f32", 20, 3, 3, 16), ("f32", 100, 6, 2, 32),
           ("bf16", 128, 4, 4, 16), ("bf16", 64, 12, 4, 128), ("bf16", 8, 2, 2, 16), ("bf16", 72, 10, 2, 32),
           ("int8", 128, 4, 4, 16), ("int8", 64, 9, 3, 256), ("int8", 16, 2, 1, 16), ("int8", 80, 5, 1, 32),
-          ("int8", 48, 4, 2, 64)]
+          ("int8", 48, 4, 2, 64), ("f32", 4, 2, 2, 16), ("f32", 4, 6, 2, 16)]
 
 
 @pytest.mark.parametrize("rows,D,H,KH,R", SHAPES)
