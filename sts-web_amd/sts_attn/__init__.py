@@ -492,9 +492,8 @@ def _heads_stride(t: torch.Tensor, name: str, lead, heads: Optional[int], D: int
     """(address, stride between tokens in elements) of float32 rows [*lead, heads, D] whose
     last two dimensions are contiguous and whose tokens are equally far apart."""
     shape = t.shape
-    if (t.is_contiguous() and t.dtype is _f32t and shape[:-2] == lead and shape[-1] == D
-            and (heads is None or shape[-2] == heads) and t.device == device):
-        return t.data_ptr(), shape[-2] * D
+    if heads and t.dtype is _f32t and shape == (*lead, heads, D) and t.device == device and t.is_contiguous():
+        return t.data_ptr(), heads * D
     if t.dtype is not _f32t:
         raise TypeError(f"{name} must be {_f32t}, got {t.dtype}")
     if len(shape) != len(lead) + 2 or shape[-1] != D or tuple(shape[:-2]) != lead or (heads and shape[-2] != heads):
@@ -541,6 +540,7 @@ class PagedKV:
         self._c = Pages(k.data_ptr(), v.data_ptr(), _arg(k_scale, "k_scale", _f32t, (n, KH, R), k.device),
                         _arg(v_scale, "v_scale", _f32t, (n, KH, R), k.device), n, R, KH, D, _PAGE_TYPES[k.dtype])
         self._at = ctypes.addressof(self._c)
+        self._index = k.device.index if k.device.type == "cuda" else None
 
     @classmethod
     def empty(cls, pages: int, page_rows: int, n_kv_heads: int, head_dim: int,
@@ -555,15 +555,16 @@ class PagedKV:
     def _streams(self, table: torch.Tensor, lens: torch.Tensor, max_rows: Optional[int]):
         """(B, P, max_rows, addresses of table and lens), after their checks."""
         dev = self.device
-        if dev.type != "cuda" or dev.index != torch._C._cuda_getDevice():
+        if self._index is None or self._index != torch._C._cuda_getDevice():
             raise ValueError(f"pages must be on the current GPU, got {dev}")
-        if table.dim() != 2:
-            raise ValueError(f"table must be [B, P], got {tuple(table.shape)}")
-        B, P = table.shape
+        shape = table.shape
+        if len(shape) != 2:
+            raise ValueError(f"table must be [B, P], got {tuple(shape)}")
+        B, P = shape
         most = P * self.page_rows if max_rows is None else max_rows
         if most < 0 or most >> 32:
             raise StsError(STS_ERR_INVALID, f"max_rows {most} out of range")
-        return (B, P, most, _arg(table, "table", _i32, (B, P), dev), _arg(lens, "lens", _i32, (B,), dev))
+        return B, P, most, _arg(table, "table", _i32, shape, dev), _arg(lens, "lens", _i32, (B,), dev)
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
                counts: Optional[torch.Tensor] = None, rope: Optional["RoPE"] = None,
@@ -592,8 +593,8 @@ class PagedKV:
         are rotated at the newest row's index.  Streams may lie apart in q, k_new, v_new."""
         B, P, most, tp, lp = self._streams(table, lens, max_rows)
         D, dev = self.head_dim, self.device
-        qp, qs = _heads_stride(q, "q", (B,), None, D, dev)
-        H = q.shape[1]
+        H = q.shape[1] if q.dim() == 3 else None
+        qp, qs = _heads_stride(q, "q", (B,), H, D, dev)
         kp = vp = None
         ns = 0
         if k_new is not None or v_new is not None:
