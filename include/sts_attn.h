@@ -383,10 +383,10 @@ typedef struct sts_pages {
 /*
  * Writes each stream's newest counts[b] rows (device int32; NULL: `seq`; at most `seq`
  * and lens[b]), rows lens[b] - counts[b] and on, rounding them to the pages' type (bf16:
- * nearest even).  Token i of stream b is at k_new, v_new + (b * seq + i) * new_stride, its
- * kv_heads rows of head_dim floats in turn (new_stride a multiple of 4: a packed qkv's
- * row, for one).  With `rope`, K rows are rotated first, each at its row index; max_rows
- * within the table.
+ * nearest even); seq is at most max_rows.  Token i of stream b is at
+ * k_new, v_new + (b * seq + i) * new_stride, its kv_heads rows of head_dim floats in turn
+ * (new_stride a multiple of 4: a packed qkv's row, for one).  With `rope`, K rows are
+ * rotated first, each at its row index; max_rows within the table.
  */
 int sts_paged_append(const sts_pages* pages, const sts_rope* rope, const float* k_new,
                      const float* v_new, uint64_t new_stride, const int32_t* table,
@@ -405,8 +405,8 @@ int sts_paged_append(const sts_pages* pages, const sts_rope* rope, const float* 
  * values.  Queries and values of up to 1e30 in magnitude are served; elements below
  * 2^-110, and weights below 2^-110 of the largest, may be lost (2^-39 over 8-bit rows
  * whose values are near 2^-64).
- * Where an infinity or NaN is seen, outputs follow f32 arithmetic over f32 rows and are
- * undefined over bf16 rows.  Splits use the per-(device, stream) workspace as
+ * Where an infinity or NaN is seen, outputs follow f32 arithmetic over f32 rows (zeros
+ * where every score is -infinity) and are undefined over bf16 rows.  Splits use the per-(device, stream) workspace as
  * sts_decode_ring does.
  */
 int sts_paged_decode(const sts_pages* pages, const sts_rope* rope, const float* q,
@@ -444,7 +444,7 @@ int sts_paged_gather(const sts_pages* pages, void* k_out, void* v_out, const int
  * target's.  draft NULL: children chosen without chance, q = 1 at the child's own token:
  * r(x) <- 0, m <- sum r instead.
  *   target, draft   [batch][nodes][vocab] probabilities after each node (f32; negative
- *                   ones and NaN count as 0)
+ *                   ones and NaN count as 0); at most 256 nodes and 2^28 words
  *   tokens, parents [batch][nodes] (device int32); a node whose parent is no earlier one
  *                   is never kept, nor one whose token is outside 0..vocab-1
  *   counts          [batch] nodes of each stream, or NULL (device int32)

@@ -512,12 +512,12 @@ PagedPlan plan_paged(const PagedDecode& p, uint32_t batch) {
   const uint64_t units = (uint64_t)batch * rows.KH * pl.rblocks;
   // Two workgroups a CU, which between them even out what streams of different lengths
   // leave uneven (24 streams of 900 to 4099 bf16 rows of 8 heads 47 us, with one a CU 59;
-  // 9 of 31 to 2777 f32 rows 72 and 74.6); one for a single stream, whose splits are alike
-  // and whose merge is then shorter (3000 8-bit rows of 32 heads 10.8 us for 12.6, 30000 of
-  // 4 heads 15.8 for 18.5).
+  // 9 of 31 to 2777 f32 rows 70.1 and 73.1); one for a single stream, whose splits are
+  // alike and whose merge is then shorter (3000 8-bit rows of 32 heads 10.7 us for 11.8,
+  // 30000 of 4 heads 16.3 for 18.7).
   const uint64_t target = (uint64_t)device_cu_count() * (batch > 1 ? 2 : 1);
   // A split is worth its record from 128 rows of a group's head on (30 streams of 20 to 500
-  // f32 rows of 6 heads 16 us, from 64 on 20, from 256 on 18.6), of a lone head from a unit
+  // f32 rows of 6 heads 15.7 us, from 64 on 19.7, from 256 on 18.4), of a lone head from a unit
   // for each of its waves on.
   const uint32_t least = p.group == 1 ? 64 : kSplitRows;
   const uint64_t most = std::min<uint64_t>((rows.max_rows + least - 1) / least, kMaxSplits);

@@ -273,6 +273,27 @@ def test_decode_not_a_number(gpu):
         assert torch.isfinite(out[0, :2]).all() and torch.isfinite(out[1]).all()
 
 
+@pytest.mark.parametrize("H", [2, 6])
+def test_decode_infinite_scores(gpu, H):
+    """Rows whose score is -infinity have no part, and a stream of such rows alone gets zeros."""
+    pool = Pool(18, [40, 5, 300], 2, 64, 16)
+    cache, table, lens = pool.gpu()
+    q = queries(pool.rng, 3, H, 64)
+    q[:, :, 3] = np.abs(q[:, :, 3]) + 0.5
+    seen = [np.ones(n, bool) for n in (40, 5, 300)]
+    seen[0][[7, 39]] = False
+    seen[1][:] = False
+    seen[2][64:] = False
+    for b, on in enumerate(seen):
+        for r in np.flatnonzero(~on):
+            cache.k[int(pool.table[b, r // 16]), :, r % 16, 3] = float("-inf")
+    got = cache.decode(torch.from_numpy(q).cuda(), table, lens, 0.1).cpu().numpy()
+    for b in (0, 2):
+        out, bound = attend64_channels(q[b:b + 1], pool.stream(b, "k")[0], pool.stream(b, "v")[0], seen[b][None], 0.1)
+        assert (np.abs(got[b] - out[0]) <= bound[0]).all()
+    assert (got[1] == 0).all()
+
+
 @pytest.mark.parametrize("rows,D,H,KH", [("f32", 128, 4, 4), ("bf16", 64, 6, 2), ("int8", 128, 4, 4), ("int8", 32, 40, 2),
                                          ("f32", 36, 34, 2), ("bf16", 128, 8, 8)])
 @pytest.mark.parametrize("rope", [False, True])
