@@ -3,6 +3,7 @@
 
 #include <cfloat>
 
+#include "lane.hpp"
 #include "pages.hpp"
 #include "sts_attn.h"
 
@@ -28,31 +29,47 @@ __device__ __forceinline__ bool paged_row(const PagedRows& p, uint32_t b, uint32
 //
 // The row's scale; rows whose largest value is below 2^-64 are kept as zeros (their scale
 // times an attention weight would lose bits to f32's lower end), rows with an infinity or
-// NaN as NaN.
+// NaN as NaN.  The quotient is the product with 1 / 127, half an ulp and a sixteenth off at
+// most, and one correction by what it leaves, which rounds it right (Markstein 1990).
 __device__ __forceinline__ float row_scale(float top) {
+  constexpr float by = 1.f / 127.f;
+  const float s = top * by, right = fmaf(fmaf(-s, 127.f, top), by, s);
   if (!(top <= FLT_MAX)) return __builtin_nanf("");
-  return top < 0x1p-64f ? 0.f : top / 127.f;
+  return top < 0x1p-64f ? 0.f : right;
 }
 
-// The code of x under scale s (by = 1 / s, rounded): x by, rounded, is at most one
-// step off; what it leaves of x is exact in f32 (x itself below s / 2, else a
-// difference of multiples of a unit of s, or of x between s / 2 and s) and says whether
-// the next code is nearer.
-__device__ __forceinline__ int row_code(float x, float s, float by) {
-  const float c = rintf(x * by);
-  const float left = fmaf(-c, s, x), half = 0.5f * s;
-  int code = (int)c;
-  if (left > half || (left == half && (code & 1))) ++code;
-  else if (left < -half || (left == -half && (code & 1))) --code;
-  return min(max(code, -127), 127);
+// The code of x under scale s: c is at most one step off; what it leaves of x is exact in
+// f32 (x itself below s / 2, else a difference of multiples of a unit of s, or of x between
+// s / 2 and s) and says whether the next code is nearer.
+__device__ __forceinline__ int nearer_code(float x, float s, int c) {
+  const float left = fmaf(-(float)c, s, x), half = 0.5f * s;
+  if (left > half || (left == half && (c & 1))) ++c;
+  else if (left < -half || (left == -half && (c & 1))) --c;
+  return min(max(c, -127), 127);
 }
 
-// Four codes, the first in the low byte; zeros for a row without a scale.
+// Four codes, the first in the low byte; zeros for a row without a scale.  Adding 1.5 2^23
+// leaves the whole number in the float's low bits; where it leaves less than half a step of
+// x, as nearly always, it is the code.
 __device__ __forceinline__ uint32_t row_codes(float4 x, float s) {
   if (!(s > 0.f)) return 0u;
-  const float by = 1.f / s;
-  return ((uint32_t)row_code(x.x, s, by) & 255u) | ((uint32_t)row_code(x.y, s, by) & 255u) << 8 |
-         ((uint32_t)row_code(x.z, s, by) & 255u) << 16 | (uint32_t)row_code(x.w, s, by) << 24;
+  const float by = __builtin_amdgcn_rcpf(s), half = 0.5f * s;
+  const float in[4] = {x.x, x.y, x.z, x.w};
+  uint32_t c[4];
+  bool sure = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float y = fmaf(in[i], by, 0x1.8p23f);
+    sure &= fabsf(fmaf(0x1.8p23f - y, s, in[i])) < half;
+    c[i] = __float_as_uint(y);
+  }
+  if (!sure) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      c[i] = (uint32_t)nearer_code(in[i], s, (int)(__uint_as_float(c[i]) - 0x1.8p23f));
+  }
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400),
+                               __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400), 0x05040100);
 }
 
 __device__ __forceinline__ uint2 bf16x4(float4 x) {
@@ -67,12 +84,11 @@ __device__ __forceinline__ float largest(float4 x) {
                                        __builtin_elementwise_maximum(fabsf(x.z), fabsf(x.w)));
 }
 
-// The largest magnitude of the G lanes' values (G consecutive lanes, a power of two).
-template <int G>
-__device__ __forceinline__ float lanes_largest(float4 x) {
-  float top = largest(x);
-#pragma unroll
-  for (int d = 1; d < G; d *= 2) top = __builtin_elementwise_maximum(top, __shfl_xor(top, d, G));
+// The largest of the G lanes' magnitudes (G consecutive lanes, a power of two up to 32).
+template <int G, int LEVEL = 0>
+__device__ __forceinline__ float lanes_largest(float top) {
+  if constexpr ((1 << LEVEL) < G)
+    return lanes_largest<G, LEVEL + 1>(__builtin_elementwise_maximum(top, xchg<LEVEL>(top)));
   return top;
 }
 

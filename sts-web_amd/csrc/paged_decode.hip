@@ -256,7 +256,7 @@ __global__ __launch_bounds__(kWaves * 64, TYPE == STS_PAGES_F32 ? 2 : 3) void pa
       }
     }
     float scale = 1.f;
-    if constexpr (I8) scale = row_scale(lanes_largest<G>(x));
+    if constexpr (I8) scale = row_scale(lanes_largest<G>(largest(x)));
     uint32_t words[ES];  // four values of ES bytes
     if constexpr (I8) {
       words[0] = row_codes(x, scale);

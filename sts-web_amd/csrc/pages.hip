@@ -23,15 +23,17 @@ __device__ __forceinline__ void store_row(void* rows, float* scales, uint64_t at
   } else if constexpr (TYPE == STS_PAGES_BF16) {
     if (on) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(rows) + to) = bf16x4(x);
   } else {
-    const float s = row_scale(lanes_largest<G>(x));
+    const float s = row_scale(lanes_largest<G>(largest(x)));
     const uint32_t codes = row_codes(x, s);
     if (on) *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(rows) + to) = codes;
     if (on && c == 0) scales[at] = s;
   }
 }
 
-// G lanes a row (K and V of it), 256 / G rows a workgroup.  (Two or four rows for a group of
-// lanes, requested together, measured slower: 512 8-bit rows of 32 heads 8.7 us, 9.6, 12.5.)
+// G lanes a row (K and V of it), 256 / G rows a workgroup.  The 8-bit rows' instructions
+// count: with the codes' corrections behind a test 512 rows of 32 heads take 7.5 us (9.7
+// without).  (Measured slower: two or four rows for a group of lanes; half the lanes with
+// eight values each, 2048 f32 rows of 32 heads 26.0 us for 23.3.)
 template <int TYPE, int G>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppend p, uint32_t total) {
   const PagedRows& rows = p.rows;
