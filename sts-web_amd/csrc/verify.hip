@@ -79,8 +79,11 @@ static_assert(kBatch == 8, "eight values leave three levels of single ones");
 // CH: 64 nodes each.
 template <bool DRAWN, int CH>
 __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
-  __shared__ int32_t s_token[CH * 64], s_parent[CH * 64];
-  __shared__ float s_rand[CH * 64], s_p[CH * 64], s_q[CH * 64];
+  // What the first wave asks the others for: the place, the words out, whether to sum, whether
+  // to draw then; and the mass of r, where it has that.
+  __shared__ int32_t s_ask[4];
+  __shared__ double s_mass_of;
+  __shared__ float s_rand[CH * 64], s_p[CH * 64], s_q[DRAWN ? CH * 64 : 1];
   // The masses that a place's second and later rejections divide by, and 1 / them.  Every wave
   // writes the same; an entry changes only behind a barrier of the place's first sum.
   __shared__ double s_mass[DRAWN ? CH * 64 : 1][2];
@@ -92,29 +95,28 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t b = blockIdx.x, V = p.V;
   const uint64_t base = (uint64_t)b * p.T;
-  int count_at = (int)p.T;
-  if (p.counts) count_at = p.counts[b];
-  if (tid < CH * 64) {
-    int token_at = -1, parent_at = -1;
-    float u_at = 0.f, at_p = 0.f, at_q = DRAWN ? 0.f : 1.f;
-    if (tid < (int)p.T) {
-      token_at = p.tokens[base + tid];
-      parent_at = p.parents[base + tid];
-      u_at = p.rand[base + tid];
+  int count = (int)p.T;
+  if (p.counts) count = p.counts[b];
+  // A wave that walks keeps the nodes in its lanes, node c*64 + lane in element c; the numbers
+  // at their tokens are the first wave's to fetch.
+  const bool walks = DRAWN || wave == 0;
+  int token[CH], parent[CH], path[CH];
+  bool fresh[CH];  // without draft: no earlier child of the place has the word
+  float u[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = c * 64 + lane;
+    token[c] = parent[c] = -1;
+    u[c] = 0.f;
+    if (walks && i < (int)p.T) {
+      parent[c] = p.parents[base + i];
+      if (wave == 0) {
+        token[c] = p.tokens[base + i];
+        u[c] = p.rand[base + i];
+      }
     }
-    parent_at = tid < count_at && parent_at >= 0 && parent_at < tid ? parent_at : -1;
-    token_at = (uint32_t)token_at < V ? token_at : -1;
-    if (parent_at >= 0 && token_at >= 0) {
-      at_p = p.target[(base + parent_at) * V + token_at];
-      if constexpr (DRAWN) at_q = p.draft[(base + parent_at) * V + token_at];
-    }
-    s_token[tid] = token_at;
-    s_parent[tid] = parent_at;
-    s_rand[tid] = u_at;
-    s_p[tid] = at_p > 0.f ? at_p : 0.f;
-    s_q[tid] = at_q > 0.f ? at_q : 0.f;
   }
-  const int n = min(max(count_at, 0), (int)p.T);
+  const int n = min(max(count, 0), (int)p.T);
   if (n == 0) {
     if (tid < (int)p.T) p.path[base + tid] = -1;
     if (tid == 0) {
@@ -123,14 +125,38 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     }
     return;
   }
-  __syncthreads();
-  // Every wave keeps the nodes in its lanes, node c*64 + lane in element c.
-  int token[CH], parent[CH], path[CH];
+  if (walks) {
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    token[c] = s_token[c * 64 + lane];
-    parent[c] = s_parent[c * 64 + lane];
-    path[c] = -1;
+    for (int c = 0; c < CH; ++c) {
+      const int i = c * 64 + lane;
+      if (i >= n || parent[c] >= i || parent[c] < 0) parent[c] = -1;
+      path[c] = i == 0 ? 0 : -1;
+    }
+    if (wave == 0) {
+      float at_p[CH], at_q[CH];
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        at_p[c] = at_q[c] = 0.f;
+        if ((uint32_t)token[c] >= V) token[c] = -1;
+        if (parent[c] >= 0 && token[c] >= 0) {
+          at_p[c] = p.target[(base + parent[c]) * V + token[c]];
+          if constexpr (DRAWN) at_q[c] = p.draft[(base + parent[c]) * V + token[c]];
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        s_rand[c * 64 + lane] = u[c];
+        s_p[c * 64 + lane] = fmaxf(at_p[c], 0.f);  // (of NaN, too)
+        if constexpr (DRAWN) s_q[c * 64 + lane] = fmaxf(at_q[c], 0.f);
+      }
+    }
+    if constexpr (DRAWN) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
   }
 
   // The wave's stretch of the words: steps of 256, in at most kPieces pieces of `rounds`.
@@ -164,6 +190,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     uint32_t out = 0;  // bit 4 i + e: word e of the lane's four of step i
     for (int j = 0; j < k; ++j) {
       const uint32_t rel = __builtin_amdgcn_readfirstlane((uint32_t)s_out[j] - wave * steps * 256);
+      if (rel >= steps * 256) continue;  // another wave's
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
         if (rel >> 8 == step + i * stride && (rel & 255) >> 2 == (uint32_t)lane) out |= 1u << (4 * i + (rel & 3));
@@ -253,8 +280,11 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     return total;
   };
 
-  // The walk, the same on every wave: a node's children come after it, and once one is
-  // kept its own come next.
+  // The walk: a node's children come after it, and once one is kept its own come next.
+  // Without draft the first wave walks and the others wait for rows to sum: 64 streams' trees
+  // with two places of rejections 13.9 us, 16.5 where every wave walks, for whose instructions
+  // the four waves of a SIMD wait in turn.  With draft each rejection needs a sum, and telling
+  // the others costs what it saves (20.7 and 19.9 us for three).
   int cur = 0, k = 0, len = 1;
   double mass = 1.0;
   bool summed = false;  // s_sum holds the sums of r as it is
@@ -262,6 +292,14 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
   // -1); the words out are those of the children up to node `cut`.
   double others = -1.0;
   int cut = 0;
+  // Node i's element of x.
+  auto of_node = [&](const int (&x)[CH], int i) {
+    int y = __builtin_amdgcn_readlane(x[0], i & 63);
+#pragma unroll
+    for (int c = 1; c < CH; ++c)
+      if (i >> 6 == c) y = __builtin_amdgcn_readlane(x[c], i & 63);
+    return y;
+  };
   // The first child of cur behind node i, or n.
   auto next_child = [&](int i) {
     int found = n;
@@ -274,85 +312,147 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
   };
   // Lists the words that are out, of the children up to node `last`, and counts them.
   auto list_out = [&](int last) {
-    __syncthreads();  // (every thread is past its last look at them)
     int count = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const bool out = parent[c] == cur && c * 64 + lane <= last && token[c] >= 0;
       const uint64_t m = __ballot(out);
-      if (out && wave == 0) s_out[count + __builtin_popcountll(m & ((1ull << lane) - 1))] = token[c];
+      if (out) s_out[count + __builtin_popcountll(m & ((1ull << lane) - 1))] = token[c];
       count += __builtin_popcountll(m);
     }
-    __syncthreads();
     return count;
   };
-  if (lane == 0) path[0] = 0;
-  for (int i = next_child(0); i < n; i = next_child(i)) {
-    double r = left_of(s_p[i], s_q[i], k);
-    const int word = s_token[i];
-    if constexpr (!DRAWN) {
+  // Without draft: child i is rejected, `others` known.
+  auto reject = [&](int i) {
+    // The words of the children behind, each once, but those of children before.
+    double behind = 0.0;
+    bool more = false;
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
-        if (__any(parent[c] == cur && c * 64 + lane <= cut && token[c] == word)) r = 0.0;
+    for (int c = 0; c < CH; ++c) {
+      const bool counts = fresh[c] && c * 64 + lane > i;
+      behind += counts ? (double)s_p[c * 64 + lane] : 0.0;
+      more |= __any(counts);
     }
-    if ((double)s_rand[i] * (double)s_q[i] * mass < r) {
-      cur = i;
-      k = 0;
+    double total = others;
+    if (more) total += lanes_total(behind);
+    summed = total > 0.0 && !more;
+    if (total > 0.0) {
+      mass = total;
       cut = i;
-      mass = 1.0;
-      others = -1.0;
-      summed = false;
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-        if (c * 64 + lane == len) path[c] = i;
-      ++len;
-      continue;
     }
-    if constexpr (DRAWN) {
-      if (k > 0 && lane < 2) s_mass[k][lane] = lane ? 1.0 / mass : mass;
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      const double total = sum_left(cur, k + 1);
-      summed = total > 0.0;
-      if (summed) {
-        mass = total;
-        ++k;
-      }
-    } else {
-      if (others < 0.0) {
-        k = list_out(n - 1);
-        others = sum_left(cur, k);
-      }
-      // And the words of the children behind, each once, but those of children before.
-      bool counts[CH];
+  };
+  auto keep = [&](int i) {
+    cur = i;
+    k = 0;
+    cut = i;
+    mass = 1.0;
+    others = -1.0;
+    summed = false;
 #pragma unroll
-      for (int c = 0; c < CH; ++c) counts[c] = parent[c] == cur && c * 64 + lane > i && token[c] >= 0;
-      for (int j = next_child(cur); j < n; j = next_child(j)) {
-        const int word = s_token[j];
+    for (int c = 0; c < CH; ++c)
+      if (c * 64 + lane == len) path[c] = i;
+    ++len;
+  };
+  // Without draft: all the children behind i at once, `others` known and more than nothing.
+  // The mass that a child divides by is that of the words which no child before it has: the
+  // others and, summed from the last child on, its own and those behind.  Returns the child
+  // that is kept, or n.
+  auto decide = [&](int i) {
+    double behind = 0.0;
+    int found = n;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) counts[c] &= c * 64 + lane <= j || token[c] != word;
+    for (int c = CH - 1; c >= 0; --c) {
+      const int at = 63 - lane;  // the lanes in reverse
+      const bool on = __ballot(fresh[c] && c * 64 + lane > i) >> at & 1;
+      const double p_at = on ? (double)s_p[c * 64 + at] : 0.0, upto = behind + lanes_upto(p_at);
+      const uint64_t kept = __ballot(on && (double)s_rand[c * 64 + at] * (others + upto) < p_at);
+      if (kept) found = c * 64 + __builtin_clzll(kept);
+      behind = __shfl(upto, 63, 64);
+    }
+    return found;
+  };
+  int i = 0;          // the last node looked at
+  bool asked = false; // for a sum that i's rejection needs
+  double total = 0.0; // of the last row summed
+  for (;;) {
+    if (walks) {
+      if (asked) {
+        if constexpr (DRAWN) {
+          summed = total > 0.0;
+          if (summed) {
+            mass = total;
+            ++k;
+          }
+        } else {
+          others = total;
+          if (others > 0.0) {
+            i = decide(i);
+            if (i < n) {
+              keep(i);
+            } else {
+              mass = others;
+              summed = true;
+            }
+          } else {
+            reject(i);
+          }
+        }
+        asked = false;
       }
-      double behind = 0.0;
-      bool more = false;
+      while (!asked && (i = next_child(i)) < n) {
+        const double p_at = (double)s_p[i];
+        double r = p_at, q_at = 1.0;
+        if constexpr (DRAWN) {
+          q_at = (double)s_q[i];
+          r = left_of(s_p[i], s_q[i], k);
+        } else {
+          const int word = of_node(token, i);
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        behind += counts[c] ? (double)s_p[c * 64 + lane] : 0.0;
-        more |= __any(counts[c]);
+          for (int c = 0; c < CH; ++c)
+            if (__any(parent[c] == cur && c * 64 + lane <= cut && token[c] == word)) r = 0.0;
+        }
+        if ((double)s_rand[i] * q_at * mass < r) {
+          keep(i);
+        } else if constexpr (DRAWN) {
+          if (k > 0 && lane < 2) s_mass[k][lane] = lane ? 1.0 / mass : mass;
+          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+          asked = true;
+        } else if (others < 0.0) {
+#pragma unroll
+          for (int c = 0; c < CH; ++c) fresh[c] = parent[c] == cur && token[c] >= 0;
+          for (int j = next_child(cur); j < n; j = next_child(j)) {
+            const int word = of_node(token, j);
+#pragma unroll
+            for (int c = 0; c < CH; ++c) fresh[c] &= c * 64 + lane <= j || token[c] != word;
+          }
+          k = list_out(n - 1);
+          asked = true;
+        } else {
+          reject(i);
+        }
       }
-      double total = others;
-      if (more) total += lanes_total(behind);
-      summed = total > 0.0 && !more;
-      if (total > 0.0) {
-        mass = total;
-        cut = i;
+      if (!DRAWN && !asked && !summed) k = list_out(cut);
+      if (!DRAWN && lane == 0) {
+        s_ask[0] = cur;
+        s_ask[1] = k;
+        s_ask[2] = asked || !summed;
+        s_ask[3] = !asked;
+        s_mass_of = mass;
       }
     }
-  }
-  double total = mass;
-  if (!summed) {
-    if constexpr (!DRAWN) k = list_out(cut);
-    total = sum_left(cur, k);
+    bool sums = asked || !summed, last = !asked;
+    if constexpr (!DRAWN) {
+      __syncthreads();
+      cur = __builtin_amdgcn_readfirstlane(s_ask[0]);
+      k = __builtin_amdgcn_readfirstlane(s_ask[1]);
+      sums = __builtin_amdgcn_readfirstlane(s_ask[2]);
+      last = __builtin_amdgcn_readfirstlane(s_ask[3]);
+      mass = s_mass_of;
+    }
+    total = sums ? sum_left(cur, DRAWN && asked ? k + 1 : k) : mass;
+    if (last) break;
   }
 
   // The draw: the first word at which the running sum passes its share of the whole.  The

@@ -80,6 +80,20 @@ def test_most_nodes(gpu):
           rng.random((B, T), np.float32))
 
 
+@pytest.mark.parametrize("drawn", [False, True])
+def test_many_children(gpu, drawn):
+    """Hundreds of children of one node, words among them more than once."""
+    rng = np.random.default_rng(11)
+    B, T, V = 6, 200, 300
+    x = rng.standard_normal((B, T, V)) * 0.3
+    target, draft = soft(x), soft(x + 0.1 * rng.standard_normal((B, T, V)))
+    parents = np.zeros((B, T), np.int32)
+    parents[:, 0] = -1
+    parents[3:, 150:] = 70  # (below one that few streams keep)
+    tokens = rng.integers(0, V // 2, (B, T))
+    check(target, draft if drawn else None, tokens, parents, rng.random((B, T), np.float32))
+
+
 def test_chosen_cases(gpu):
     """Dyadic probabilities, whose sums are exact: borders, siblings of one token, nothing left."""
     p = np.array([0.5, 0.25, 0.125, 0.125], np.float32)
