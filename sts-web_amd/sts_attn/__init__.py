@@ -652,7 +652,7 @@ def verify_draft(target: torch.Tensor, tokens: torch.Tensor, parents: torch.Tens
             _arg(tokens, "tokens", _i32, each, dev), _arg(parents, "parents", _i32, each, dev),
             _arg(counts, "counts", _i32, one, dev), _arg(rand, "rand", _f32t, each, dev)]
     path = _empty_like(tokens, stream)
-    accepted = _empty_like(counts, stream) if counts is not None else _empty(one, _i32, dev, stream)
+    accepted = tokens.new_empty(one) if stream is None else _empty(one, _i32, dev, stream)
     following = _empty_like(accepted, stream)
     _check(load().sts_verify_draft(*args, path.data_ptr(), accepted.data_ptr(), following.data_ptr(), B, T, V,
                                    _stream(stream)))
