@@ -174,12 +174,13 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(
                                       row, step < steps ? (from + step * 256) * 4 : kOutside, 0, 0));
   };
-  auto load = [&](int cur, uint32_t step, uint32_t stride, Batch& x) {
+  auto load = [&](int cur, int k, uint32_t step, uint32_t stride, Batch& x) {
     const __amdgpu_buffer_rsrc_t target = row_of(p.target, cur);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) x.p[i] = word4(target, step + i * stride);
     if constexpr (DRAWN) {
-      const __amdgpu_buffer_rsrc_t draft = row_of(p.draft, cur);
+      // (Without rejections none are wanted: an empty row.)
+      const __amdgpu_buffer_rsrc_t draft = coherent_rsrc(p.draft + (base + cur) * V, k > 0 ? V * 4 : 0);
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) x.q[i] = word4(draft, step + i * stride);
     }
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
 #pragma unroll 1
       for (uint32_t round = 0; round < rounds; ++round) {
         Batch y;
-        load(cur, piece * rounds + round, rounds, y);
+        load(cur, k, piece * rounds + round, rounds, y);
         if constexpr (!DRAWN) take_out(piece * rounds + round, rounds, k, y);
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
