@@ -91,6 +91,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
   __shared__ double s_sum[2][kWaves];             // the waves' sums of r, by turns
   __shared__ double s_piece[kWaves][kPieces];     // and those of their pieces
   __shared__ int32_t s_last[kWaves];
+  __shared__ int32_t s_path[CH * 64];  // the kept nodes (a barrier of the sum behind the last is before they are read)
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t b = blockIdx.x, V = p.V;
@@ -100,7 +101,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
   // A wave that walks keeps the nodes in its lanes, node c*64 + lane in element c; the numbers
   // at their tokens are the first wave's to fetch.
   const bool walks = DRAWN || wave == 0;
-  int token[CH], parent[CH], path[CH];
+  int token[CH], parent[CH];
   bool fresh[CH];  // without draft: no earlier child of the place has the word
   float u[CH];
 #pragma unroll
@@ -130,8 +131,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     for (int c = 0; c < CH; ++c) {
       const int i = c * 64 + lane;
       if (i >= n || parent[c] >= i || parent[c] < 0) parent[c] = -1;
-      path[c] = i == 0 ? 0 : -1;
     }
+    if (tid == 0) s_path[0] = 0;
     if (wave == 0) {
       float at_p[CH], at_q[CH];
 #pragma unroll
@@ -174,13 +175,12 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(
                                       row, step < steps ? (from + step * 256) * 4 : kOutside, 0, 0));
   };
-  auto load = [&](int cur, int k, uint32_t step, uint32_t stride, Batch& x) {
+  auto load = [&](auto many, int cur, uint32_t step, uint32_t stride, Batch& x) {
     const __amdgpu_buffer_rsrc_t target = row_of(p.target, cur);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) x.p[i] = word4(target, step + i * stride);
-    if constexpr (DRAWN) {
-      // (Without rejections none are wanted: an empty row.)
-      const __amdgpu_buffer_rsrc_t draft = coherent_rsrc(p.draft + (base + cur) * V, k > 0 ? V * 4 : 0);
+    if constexpr (DRAWN && decltype(many)::value > 0) {
+      const __amdgpu_buffer_rsrc_t draft = row_of(p.draft, cur);
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) x.q[i] = word4(draft, step + i * stride);
     }
@@ -220,24 +220,26 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     }
     return r;
   };
-  // Words of step i of a batch.
-  auto left4 = [&](const Batch& y, int i, int k, double (&r)[4]) {
-    if constexpr (DRAWN) {
-      // (As above, the loop over the rejections outside.)
+  // Words of step i of a batch, after no rejection (MANY 0), one (1) or k of them (2).
+  auto left4 = [&](auto many, const Batch& y, int i, int k, double (&r)[4]) {
+    constexpr int MANY = decltype(many)::value;
+    if constexpr (DRAWN && MANY > 0) {
       float q0[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float p0 = fmaxf(y.p[i][e], 0.f);
-        q0[e] = k > 0 ? fmaxf(y.q[i][e], 0.f) : 0.f;
-        r[e] = (double)fmaxf(p0, q0[e]) - (double)q0[e];
+        q0[e] = MANY == 1 || k > 0 ? fmaxf(y.q[i][e], 0.f) : 0.f;
+        r[e] = (double)fmaxf(fmaxf(y.p[i][e], 0.f), q0[e]) - (double)q0[e];
       }
+      if constexpr (MANY > 1) {
+        // (left_of's loop over the rejections outside.)
 #pragma unroll 1
-      for (int j = 1; j < k; ++j) {
-        const double m = s_mass[j][0], by = s_mass[j][1];
+        for (int j = 1; j < k; ++j) {
+          const double m = s_mass[j][0], by = s_mass[j][1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const double t = r[e] * by, d = fma(fma(-t, m, r[e]), by, t) - (double)q0[e];
-          r[e] = d > 0.0 ? d : 0.0;
+          for (int e = 0; e < 4; ++e) {
+            const double t = r[e] * by, d = fma(fma(-t, m, r[e]), by, t) - (double)q0[e];
+            r[e] = d > 0.0 ? d : 0.0;
+          }
         }
       }
     } else {
@@ -249,28 +251,35 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
   int turn = 0;
   auto sum_left = [&](int cur, int k) {
     double sum = 0.0;
+    auto words = [&](auto many) {
 #pragma unroll 1
-    for (uint32_t piece = 0; piece * rounds < steps; piece += kBatch) {
-      double part[kBatch];
+      for (uint32_t piece = 0; piece * rounds < steps; piece += kBatch) {
+        double part[kBatch];
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) part[i] = 0.0;
+        for (int i = 0; i < kBatch; ++i) part[i] = 0.0;
 #pragma unroll 1
-      for (uint32_t round = 0; round < rounds; ++round) {
-        Batch y;
-        load(cur, k, piece * rounds + round, rounds, y);
-        if constexpr (!DRAWN) take_out(piece * rounds + round, rounds, k, y);
+        for (uint32_t round = 0; round < rounds; ++round) {
+          Batch y;
+          load(many, cur, piece * rounds + round, rounds, y);
+          if constexpr (!DRAWN) take_out(piece * rounds + round, rounds, k, y);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          double r[4];
-          left4(y, i, k, r);
-          part[i] += (r[0] + r[1]) + (r[2] + r[3]);
-          __builtin_amdgcn_sched_barrier(0);  // (registers)
+          for (int i = 0; i < kBatch; ++i) {
+            double r[4];
+            left4(many, y, i, k, r);
+            part[i] += (r[0] + r[1]) + (r[2] + r[3]);
+            __builtin_amdgcn_sched_barrier(0);  // (registers)
+          }
         }
+        const double mine = batch_totals(part, lane);
+        if ((lane & 7) == 0) s_piece[wave][piece + lane / 8] = mine;
+        sum += (lane & 7) == 0 ? mine : 0.0;
       }
-      const double mine = batch_totals(part, lane);
-      if ((lane & 7) == 0) s_piece[wave][piece + lane / 8] = mine;
-      sum += (lane & 7) == 0 ? mine : 0.0;
-    }
+    };
+    // (Loops of their own: one for all costs the place without rejections a microsecond, and
+    // branches inside it the registers.)
+    if (!DRAWN || k == 0) words(std::integral_constant<int, 0>{});
+    else if (k == 1) words(std::integral_constant<int, 1>{});
+    else words(std::integral_constant<int, 2>{});
     sum = lanes_total(sum);
     turn ^= 1;
     if (lane == 0) s_sum[turn][wave] = sum;
@@ -349,9 +358,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     mass = 1.0;
     others = -1.0;
     summed = false;
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-      if (c * 64 + lane == len) path[c] = i;
+    if (tid == 0) s_path[len] = i;
     ++len;
   };
   // Without draft: all the children behind i at once, `others` known and more than nothing.
@@ -463,7 +470,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
   if (wave == 0) {
 #pragma unroll
     for (int c = 0; c < CH; ++c)
-      if (c * 64 + lane < (int)p.T) p.path[base + c * 64 + lane] = path[c];
+      if (c * 64 + lane < (int)p.T) p.path[base + c * 64 + lane] = c * 64 + lane < len ? s_path[c * 64 + lane] : -1;
     if (lane == 0) p.accepted[b] = len;
   }
   int at = -1;
@@ -492,7 +499,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
         take_out(step, 1, k, y);
       }
       double r[4];
-      left4(y, 0, k, r);
+      left4(std::integral_constant<int, 2>{}, y, 0, k, r);
       const double four = (r[0] + r[1]) + (r[2] + r[3]), upto = running(four);
       double run = upto - four;
       int mine = -1;
