@@ -332,23 +332,25 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyDraft p) {
     }
     return count;
   };
-  // Without draft: child i is rejected, `others` known.
+  // Without draft: child i is rejected, and no words but the children's have anything left: what
+  // is left are the words of the children past `cut`, each counted where it comes first.  Where
+  // only the child's own has, it stays, with the mass as it was, and the cut, which would take
+  // it out, goes no further.
   auto reject = [&](int i) {
-    // The words of the children behind, each once, but those of children before.
-    double behind = 0.0;
-    bool more = false;
+    const int word = of_node(token, i);
+    double rest = 0.0;
+    bool before = false;  // a word that stayed
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const bool counts = fresh[c] && c * 64 + lane > i;
-      behind += counts ? (double)s_p[c * 64 + lane] : 0.0;
-      more |= __any(counts);
+      const int at = c * 64 + lane;
+      const double x = fresh[c] && at > cut && token[c] != word ? (double)s_p[at] : 0.0;
+      rest += x;
+      before |= __any(x > 0.0 && at < i);
     }
-    double total = others;
-    if (more) total += lanes_total(behind);
-    summed = total > 0.0 && !more;
-    if (total > 0.0) {
-      mass = total;
-      cut = i;
+    rest = lanes_total(rest);
+    if (rest > 0.0) {
+      mass = rest;
+      if (!before) cut = i;
     }
   };
   auto keep = [&](int i) {

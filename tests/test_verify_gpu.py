@@ -129,6 +129,38 @@ def test_chosen_cases(gpu):
     run(odd, [0, 2, 3], [-1, 0, 0], [0.9, 0.8, 0.9], draft=np.array([np.nan, 0.25, 0.5, -1], np.float32))
 
 
+def test_rows_that_do_not_sum_to_one(gpu):
+    """Rows cut to a few words and not normalised, dyadic so that every sum is exact: where the first
+    rejected child has all that is left of its row, it stays, and later rejections take its mass."""
+    def run(target, tokens, rand):
+        T = len(tokens)
+        check(np.broadcast_to(np.float32(target), (1, T, 4)), None, np.array([tokens]),
+              np.array([[-1] + [0] * (T - 1)]), np.array([rand], np.float32))
+
+    half = [0, 0.5, 0, 0]
+    run(half, [0, 1, 2, 1], [0.3, 0.9, 0.9, 0.9])        # kept at last: 0.9 * 0.5 < 0.5
+    run(half, [0, 1, 2], [0.3, 0.9, 0.9])                # no child kept: the word is drawn
+    run(half, [0, 1, -1, 1], [0.3, 0.9, 0.9, 0.9])       # the second child's token is none
+    run(half, [0, 2, 1, 1], [0.3, 0.9, 0.9, 0.9])        # a word without mass goes first
+    run(half, [0, -1, 1], [0.3, 0.9, 0.9])
+    run(half, [0, 1, 1, 2, 3, 1], [0.3, 0.9, 0.9, 0.9, 0.9, 0.9])
+    run([0.25, 0.25, 0, 0], [0, 0, 1], [0.3, 0.9, 0.9])  # the second word takes all that is left
+    run([0.25, 0.25, 0, 0], [0, 0, 0, 2, 1], [0.3, 0.9, 0.9, 0.9, 0.9])
+    run([0, 0, 0, 0], [0, 1, 2, 1], [0.3, 0.9, 0.9, 0.9])
+
+    rng = np.random.default_rng(40)
+    for V, T, B in ((2, 7, 300), (4, 9, 300), (6, 80, 100)):
+        target = np.zeros((B, T, V), np.float32)
+        for _ in range(2):
+            at = rng.integers(0, V, (B, T, 1))
+            np.put_along_axis(target, at, (rng.integers(0, 12, (B, T, 1)) / 16).astype(np.float32), 2)
+        tokens = rng.integers(-1, V + 1, (B, T))
+        parents = np.where(rng.random((B, T)) < 0.8, 0, np.stack([tree(rng, T) for _ in range(B)]))
+        parents[:, 0] = -1
+        rand = ((rng.integers(8, 16, (B, T)) * 2 + 1) / 32).astype(np.float32)
+        check(target, None, tokens, parents, rand)
+
+
 @pytest.mark.parametrize("V", [3, 700, 5000, 270001])
 def test_the_end_of_the_vocabulary(gpu, V):
     """A share of all that is left (a number past the range, as rounding may give) takes the last
