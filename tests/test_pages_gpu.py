@@ -203,6 +203,42 @@ def test_decode_groups(gpu, rows, group):
 
 
 @pytest.mark.parametrize("rows", ["f32", "bf16", "int8"])
+@pytest.mark.parametrize("D", [80, 128])
+@pytest.mark.parametrize("group", [9, 11, 12, 13, 16, 17, 33])
+def test_decode_wide_groups(gpu, rows, D, group):
+    """Groups whose outputs are more columns than a workgroup has threads, in splits that are merged
+    at once and, for the longer streams, in clusters."""
+    check_decode(Pool(27, [301, 1500, 5], 2, D, 32, rows), 2 * group)
+    check_decode(Pool(28, [3003], 1, D, 64, rows), group)
+
+
+@pytest.mark.parametrize("rows", ["f32", "bf16", "int8"])
+@pytest.mark.parametrize("H,KH", [(12, 1), (16, 1), (29, 1), (80, 4)])
+def test_decode_wide_groups_long(gpu, rows, H, KH):
+    """The most splits there are, of up to sixteen heads a block."""
+    check_decode(Pool(29, [18001], KH, 128, 256, rows), H)
+    check_decode(Pool(30, [9000, 700, 0, 2001], KH, 128, 16, rows), H)
+
+
+@pytest.mark.parametrize("rows", ["f32", "bf16", "int8"])
+def test_decode_wide_groups_that_append(gpu, rows):
+    """Blocks of sixteen heads all see the row that the first of them stores."""
+    B, H, KH, D = 4, 50, 2, 128
+    lens = [2000, 1, 33, 700]
+    pool = Pool(31, lens, KH, D, 16, rows)
+    qkv = torch.from_numpy(queries(pool.rng, B, H + 2 * KH, D)).cuda()
+    q, k_new, v_new = qkv[:, :H], qkv[:, H:H + KH], qkv[:, H + KH:]
+    one, table, lens_ = pool.gpu()
+    got = one.decode(q, table, lens_, scale_for(D), k_new=k_new, v_new=v_new).cpu().numpy()
+    want = appended(pool, k_new[:, None].cpu().numpy(), v_new[:, None].cpu().numpy(), [1] * B)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        if want[name] is not None:
+            assert torch.equal(bits(getattr(one, name).cpu()), bits(want[name])), name
+    pool.data = want
+    check_decode(pool, H, q=q.cpu().numpy(), got=got)
+
+
+@pytest.mark.parametrize("rows", ["f32", "bf16", "int8"])
 def test_decode_long(gpu, rows):
     """One stream whose splits are merged many at once, and one head of many rows."""
     check_decode(Pool(9, [20011], 1, 64, 256, rows), 3)
@@ -357,6 +393,51 @@ def test_pool_past_4_gb(gpu):
         assert torch.equal(k[b, :, :n].cpu(), rows.float()) and torch.equal(v[b, :, :n].cpu(), rows.float())
         out, bound = attend64_channels(q[b:b + 1], rows.numpy(), rows.numpy(), np.ones((1, n), bool), scale_for(D))
         assert (np.abs(got[b] - out[0]) <= bound[0]).all()
+
+
+@pytest.mark.parametrize("H", [1, 3])
+def test_rows_past_2_32(gpu, H):
+    """Row numbers past 2^32, of codes and of scales, in and out.  (K and V are one memory, to which
+    append gives the same rows twice: 86 GB instead of 172.)"""
+    KH, R, D = 1, 4096, 16
+    pages = 2 ** 32 // R + 3
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 100 GB of GPU memory")
+    x = torch.empty((pages, KH, R, D), dtype=torch.int8, device="cuda")
+    s = torch.empty((pages, KH, R), device="cuda")
+    cache = sts_attn.PagedKV(x, x, s, s)
+    half = 2 ** 31 // R
+    t = np.array([[pages - 1, half - 1, pages - 2], [0, half, pages - 3]], np.int32)
+    table = torch.from_numpy(t).cuda()
+    n = [2 * R + 70, 2 * R + 9]
+    lens = torch.tensor(n, dtype=torch.int32, device="cuda")
+    rng = np.random.default_rng(32)
+    new = rng.standard_normal((2, n[0], KH, D)).astype(np.float32)
+    dev = torch.from_numpy(new).cuda()
+    cache.append(dev, dev, table, lens, counts=lens)
+    k, v = (torch.zeros((2, KH, n[0], D), device="cuda") for _ in range(2))
+    cache.gather(table, lens, k, v)
+    q = queries(rng, 2, H, D)
+    got = cache.decode(torch.from_numpy(q).cuda(), table, lens, scale_for(D)).cpu().numpy()
+    row = torch.from_numpy(queries(rng, 2, KH, D)).cuda()
+    step = cache.decode(torch.from_numpy(q).cuda(), table, lens, scale_for(D), k_new=row, v_new=row).cpu().numpy()
+    for b in range(2):
+        codes, scales = stored(new[b, :n[b]], "int8")
+        for i in range(3):  # where the definition puts them
+            at = slice(i * R, min((i + 1) * R, n[b]))
+            m = min(R, n[b] - i * R) - (i == 2)  # (the step has written over the last)
+            assert torch.equal(x[t[b, i], 0, :m].cpu(), codes[at][:m, 0])
+            assert torch.equal(s[t[b, i], 0, :m].cpu(), scales[at][:m, 0])
+        rows = value64(codes, scales).transpose(0, 1)
+        assert torch.equal(k[b, :, :n[b]].cpu(), rows.float()) and torch.equal(v[b], k[b])
+        last = value64(*stored(row[b].cpu().numpy(), "int8"))
+        other = rows.clone()
+        other[:, -1] = last
+        for out, r in ((got[b], rows), (step[b], other)):
+            want, bound = attend64_channels(q[b:b + 1], r.numpy(), r.numpy(), np.ones((1, n[b]), bool), scale_for(D))
+            assert (np.abs(out - want[0]) <= bound[0]).all()
+    del cache, x, s
+    torch.cuda.empty_cache()
 
 
 # ---------------------------------------------------------------------------
