@@ -452,7 +452,10 @@ int sts_paged_gather(const sts_pages* pages, void* k_out, void* v_out, const int
  *   path            [batch][nodes] the kept nodes, then -1;  accepted [batch] how many
  *   next            [batch] the token after them (-1 where all of p is 0, or no node is)
  * Sums and comparisons are in 64 bits: path, accepted and next are those of exact
- * arithmetic unless a number of `rand` lies within 2^-45 of a border.
+ * arithmetic unless a number of `rand` lies within 2^-45 of a border (2^-41 in rows of
+ * more than 2^23 words).  With draft, every rejection at a place after the first makes that
+ * distance up to 4 / m times as large, m being the mass that it leaves (r is then a
+ * difference of r / m and q, which may nearly agree).
  */
 int sts_verify_draft(const float* target, const float* draft, const int32_t* tokens,
                      const int32_t* parents, const int32_t* counts, const float* rand,

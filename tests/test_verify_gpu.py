@@ -1,4 +1,6 @@
 """The verdict on a draft on the GPU, against exact fractions."""
+from fractions import Fraction
+
 import numpy as np
 import pytest
 import torch
@@ -159,6 +161,71 @@ def test_rows_that_do_not_sum_to_one(gpu):
         parents[:, 0] = -1
         rand = ((rng.integers(8, 16, (B, T)) * 2 + 1) / 32).astype(np.float32)
         check(target, None, tokens, parents, rand)
+
+
+def cut_to(p, share):
+    """p's likeliest words, `share` of it together, as probabilities."""
+    by = np.argsort(-p)
+    few = by[:int(np.searchsorted(np.cumsum(p[by].astype(np.float64)), share)) + 1]
+    y = np.zeros_like(p)
+    y[few] = p[few]
+    return (y / y.sum(dtype=np.float64)).astype(np.float32)
+
+
+def left_after(p, q, k):
+    """What k rejections leave of p, exactly: (whole numbers, one for each word, in proportion; the
+    distance from a border within which a verdict is open)."""
+    one = 2 ** 160
+    p, q = ([int(Fraction(float(x)) * one) for x in a] for a in (p, q))
+    r, unit, near = p, one, Fraction(1, 2 ** 45)  # r[x] / unit is what q[x] is taken off
+    for j in range(k):
+        r = [max(0, a * one - unit * b) for a, b in zip(r, q)]
+        if j > 0:
+            near *= 4 / Fraction(sum(r), unit * one)
+        unit = sum(r)
+    return r, near
+
+
+def beside(border, near):
+    """The float32 numbers next to a border on both sides that are `near` away at least."""
+    lo = np.float32(float(border - near))
+    while Fraction(float(lo)) > border - near:
+        lo = np.nextafter(lo, np.float32(-1))
+    hi = np.float32(float(border + near))
+    while Fraction(float(hi)) < border + near:
+        hi = np.nextafter(hi, np.float32(2))
+    return lo, hi
+
+
+@pytest.mark.parametrize("noise", [0.02, 0.3, 1.0])
+@pytest.mark.parametrize("k", [1, 2, 3, 4])
+def test_next_to_borders(gpu, k, noise):
+    """After k rejections at one place, of words that the target's row leaves out, random numbers as
+    near to a child's border and to those of the draw as the verdict is exact there."""
+    rng = np.random.default_rng(41 + k)
+    V, T = 150, k + 2
+    trees = []  # (p, q, tokens, rand, nodes, whether the last child is kept)
+    while len(trees) < 48:
+        x = rng.standard_normal(V) * 2
+        q, p = soft(x), cut_to(soft(x + noise * rng.standard_normal(V)), 0.999)
+        r, near = left_after(p, q, k)
+        total = sum(r)
+        out = np.flatnonzero(p == 0)
+        below, child, draw = 0, [], []  # (distance, word, number, whether it is below the border)
+        for x in range(V):
+            below += r[x]
+            for sides, border in ((child, Fraction(r[x], total) / Fraction(float(q[x]))), (draw, Fraction(below, total))):
+                if r[x] and near < border < 1 - near:
+                    sides += [(abs(Fraction(float(u)) - border), x, u, u < border) for u in beside(border, near)]
+        for _, x, u, kept in sorted(child)[:2]:
+            trees.append((p, q, np.r_[0, rng.choice(out, k), x], np.r_[0.5, np.ones(k) * 0.5, u], T, kept))
+        for _, x, u, _ in sorted(draw)[:2]:
+            trees.append((p, q, np.r_[0, rng.choice(out, k), 0], np.r_[u, np.ones(k) * 0.5, 0.5], T - 1, False))
+    p, q, tokens, rand, n, kept = (np.array(x) for x in zip(*trees))
+    B = len(n)
+    parents = np.tile(np.r_[-1, np.zeros(T - 1, int)], (B, 1))
+    rows = [np.repeat(x[:, None], T, 1) for x in (p, q)]
+    assert check(rows[0], rows[1], tokens, parents, rand, counts=n) == kept.sum() > 0
 
 
 @pytest.mark.parametrize("V", [3, 700, 5000, 270001])
