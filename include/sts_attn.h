@@ -440,9 +440,11 @@ int sts_paged_gather(const sts_pages* pages, void* k_out, void* v_out, const int
  *   kept if rand[child] * q(x) * m < r(x): the walk goes on at the child;
  *   else r <- max(0, r / m - q), m <- sum r (as they were where that sum is zero)
  * and where none is kept, the next token is the first at which the running sum of r
- * passes rand[node 0] * sum r.  Children drawn from q then leave tokens distributed as the
- * target's.  draft NULL: children chosen without chance, q = 1 at the child's own token:
- * r(x) <- 0, m <- sum r instead.
+ * passes rand[node 0] * sum r.  Where rows sum to 1, children that are each drawn from the
+ * whole of q, independently of one another (one word may come twice), then leave tokens
+ * distributed as the target's; children drawn without replacement do not.  draft NULL:
+ * children chosen without chance (or drawn in any other way that `rand` has no part in),
+ * q = 1 at the child's own token: r(x) <- 0, m <- sum r instead.
  *   target, draft   [batch][nodes][vocab] probabilities after each node (f32; negative
  *                   ones and NaN count as 0); at most 256 nodes and 2^28 words
  *   tokens, parents [batch][nodes] (device int32); a node whose parent is no earlier one

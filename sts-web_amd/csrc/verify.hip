@@ -7,7 +7,8 @@
 //   kept      if u q(x) m < r(x): the walk goes on at the child
 //   rejected  otherwise: r <- max(0, r / m - q), m <- sum r (unless that is zero)
 // and where no child is kept a token is drawn from r / m.  The tokens are then distributed
-// as the target's.  Children taken without chance (no q) stand for q = 1 at their own
+// as the target's if each child was drawn from q independently of the others (with
+// replacement).  Children taken without chance (no q) stand for q = 1 at their own
 // token: r(x) <- 0 instead, m <- sum r.
 //
 // r is never stored: a word's r follows from p, q and the masses of the rejections

@@ -637,10 +637,11 @@ def verify_draft(target: torch.Tensor, tokens: torch.Tensor, parents: torch.Tens
                  stream=None):
     """How far each stream's draft, a tree of T tokens below node 0 (the last token, always
     kept), holds against the target's probabilities after each node, target [B,T,V] float32:
-    draft [B,T,V] the probabilities that a node's children were drawn from (None: they were
-    chosen without chance), tokens/parents [B,T] and counts [B] int32, rand [B,T] float32
-    in [0, 1): entry i decides node i, entry 0 draws the token that follows.  Returns (path
-    [B,T], accepted [B], next [B]) int32; path and accepted are tree_commit's."""
+    draft [B,T,V] the probabilities that a node's children were drawn from, each independently
+    of the others (None: they were chosen without chance), tokens/parents [B,T] and counts [B]
+    int32, rand [B,T] float32 in [0, 1): entry i decides node i, entry 0 draws the token that
+    follows.  Returns (path [B,T], accepted [B], next [B]) int32; path and accepted are
+    tree_commit's."""
     shape, dev = target.shape, target.device
     if len(shape) != 3:
         raise ValueError(f"target must be [B, T, V], got {tuple(shape)}")

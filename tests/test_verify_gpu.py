@@ -263,6 +263,25 @@ def test_tokens_follow_the_target(gpu):
         assert abs((first == v).mean() - want) < 5 * np.sqrt(want * (1 - want) / B), v
 
 
+def test_siblings_drawn_without_replacement(gpu):
+    """Children drawn one from what the other leaves, judged as chosen without chance: the first token
+    comes as often as the target says (with their probabilities it would not: .4, .4, .2 for
+    .5, .3, .2 under .2, .2, .6), within five standard deviations of a binomial count."""
+    rng = np.random.default_rng(35)
+    B, V = 60000, 3
+    p, q = np.float32([0.5, 0.3, 0.2]), np.array([0.2, 0.2, 0.6])
+    tokens = np.zeros((B, 3), np.int32)
+    tokens[:, 1:] = np.argsort(-(np.log(q) + rng.gumbel(size=(B, V))), 1)[:, :2]
+    target = np.broadcast_to(p, (B, 3, V)).copy()
+    parents = np.tile(np.array([-1, 0, 0], np.int32), (B, 1))
+    args = [torch.from_numpy(x).cuda() for x in (target, tokens, parents, rng.random((B, 3), np.float32))]
+    path, accepted, following = (x.cpu().numpy() for x in sts_attn.verify_draft(*args))
+    first = np.where(accepted > 1, tokens[np.arange(B), np.maximum(path[:, 1], 0)], following)
+    for v in range(V):
+        want = float(p[v])
+        assert abs((first == v).mean() - want) < 5 * np.sqrt(want * (1 - want) / B), v
+
+
 def test_refusals(gpu):
     p = torch.zeros((2, 3, 5), device="cuda")
     i = torch.zeros((2, 3), dtype=torch.int32, device="cuda")
