@@ -220,22 +220,29 @@ __device__ __forceinline__ void put_record(const Records& r, uint32_t sp, uint32
                                           (sp * r.size + r.live * D + x / C4 * 2) * 4, 0, kSc1);
 }
 
+// Records of `slots` columns that are read in one round trip.
+__host__ __device__ constexpr uint32_t read_at_once(uint32_t slots) {
+  return slots <= kWaves * 64 ? kWaves * 64 / slots * kAhead : kAhead / 2;
+}
+
 // What follows a split's put_record: its part in the merge, whose outcome goes to put.
-template <int D, class Put>
+// HEADS: a block's at most (of one head no splits are too many for one merge).
+template <int D, int HEADS, class Put>
 __device__ __forceinline__ void merge_splits(const Records& r, uint32_t* counters, uint32_t split, uint32_t nsplit,
                                              char* mem, uint32_t& s_last, Put put) {
-  const uint32_t slots = r.live * (D / 4), at_once = slots <= kWaves * 64 ? kWaves * 64 / slots * kAhead : kAhead / 2;
   uint32_t from = 0, step = 1, n = nsplit;
-  if (nsplit > 2 * at_once) {
-    uint32_t size = 1;
-    while (size * size < nsplit) ++size;
-    const uint32_t cluster = split / size, first = cluster * size, some = min(size, nsplit - first);
-    if (!last_of(counters + 1 + cluster, some, s_last)) return;
-    // (A column's first record is read by the thread that then writes it.)
-    merge_records<D>(r, first, 1, some, mem,
-                     [&](uint32_t x, float4 a, float m, float l) { put_record<D>(r, first, x, a, m, l); });
-    step = size;
-    n = (nsplit + size - 1) / size;
+  if constexpr (kMaxSplits > 2 * read_at_once(HEADS * (D / 4))) {
+    if (nsplit > 2 * read_at_once(r.live * (D / 4))) {
+      uint32_t size = 1;
+      while (size * size < nsplit) ++size;
+      const uint32_t cluster = split / size, first = cluster * size, some = min(size, nsplit - first);
+      if (!last_of(counters + 1 + cluster, some, s_last)) return;
+      // (A column's first record is read by the thread that then writes it.)
+      merge_records<D>(r, first, 1, some, mem,
+                       [&](uint32_t x, float4 a, float m, float l) { put_record<D>(r, first, x, a, m, l); });
+      step = size;
+      n = (nsplit + size - 1) / size;
+    }
   }
   if (!last_of(counters, n, s_last)) return;
   merge_records<D>(r, from, step, n, mem, put);
@@ -243,7 +250,7 @@ __device__ __forceinline__ void merge_splits(const Records& r, uint32_t* counter
 
 }  // namespace paged
 
-// The kernels' launches: p is planned, nsplit and shares set.
+// The kernels' launches: p is planned.
 int launch_paged_lone(const PagedDecode& p, dim3 grid, hipStream_t stream);
 
 }  // namespace sts

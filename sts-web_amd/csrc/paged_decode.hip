@@ -497,7 +497,7 @@ __global__ __launch_bounds__(kWaves * 64, TYPE == STS_PAGES_F32 ? 2 : 3) void pa
   }
   if (nsplit == 1) return;
   const uint64_t unit = ((uint64_t)b * rows.KH + kvh) * p.rblocks + rb;
-  merge_splits<D>(rec, p.counters + unit * kCounters, split, nsplit, s_mem, s_last, finish);
+  merge_splits<D, 16>(rec, p.counters + unit * kCounters, split, nsplit, s_mem, s_last, finish);
 }
 
 struct PagedPlan {
@@ -572,7 +572,6 @@ int launch_paged_decode(PagedDecode p, uint32_t batch, hipStream_t stream) {
   }
   p.rblocks = pl.rblocks;
   p.nsplit = pl.nsplit;
-  p.shares = pl.shares;
   p.batch = batch;
   p.rows_factor = pl.rows_factor;
   p.record = pl.record;

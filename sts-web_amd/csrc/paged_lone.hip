@@ -370,7 +370,7 @@ void paged_lone_kernel(const PagedDecode p) {
     else put_record<D>(rec, at.split, tid, y, mt, lt);
   }
   if (nsplit == 1) return;
-  merge_splits<D>(rec, p.counters + ((uint64_t)b * rows.KH + h) * kCounters, at.split, nsplit, s_mem, s_last, finish);
+  merge_splits<D, 1>(rec, p.counters + ((uint64_t)b * rows.KH + h) * kCounters, at.split, nsplit, s_mem, s_last, finish);
 }
 
 template <int TYPE>

@@ -63,7 +63,7 @@ struct PagedDecode {
   uint32_t H = 0, group = 1;
   float qscale = 0.f;        // scale * log2(e)
   // Set by launch_paged_decode.
-  uint32_t rblocks = 1, nsplit = 1, shares = 0, batch = 0;
+  uint32_t rblocks = 1, nsplit = 1, batch = 0;
   float rows_factor = 0.f;   // rows of a split for each row there is; 0: nsplit for every stream
   uint32_t record = 0;       // floats of a split's record
   float* part = nullptr;
