@@ -535,12 +535,18 @@ class PagedKV:
         if not int8 and (k_scale is not None or v_scale is not None):
             raise ValueError(f"{k.dtype} pages have no scales")
         n, KH, R, D = k.shape
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._held = k, v, k_scale, v_scale
         self.pages, self.n_kv_heads, self.page_rows, self.head_dim, self.device = n, KH, R, D, k.device
         self._c = Pages(k.data_ptr(), v.data_ptr(), _arg(k_scale, "k_scale", _f32t, (n, KH, R), k.device),
                         _arg(v_scale, "v_scale", _f32t, (n, KH, R), k.device), n, R, KH, D, _PAGE_TYPES[k.dtype])
         self._at = ctypes.addressof(self._c)
         self._index = k.device.index if k.device.type == "cuda" else None
+
+    # Read only: the calls go by the addresses that the pool was made with.
+    k = property(lambda self: self._held[0])
+    v = property(lambda self: self._held[1])
+    k_scale = property(lambda self: self._held[2])
+    v_scale = property(lambda self: self._held[3])
 
     @classmethod
     def empty(cls, pages: int, page_rows: int, n_kv_heads: int, head_dim: int,

@@ -181,3 +181,14 @@ def test_strides_of_new_rows():
         at(qkv.double()[:, :, :2], (3, 5))
     with pytest.raises(ValueError, match="must be"):
         at(qkv[:, :, :3], (3, 5))
+
+
+def test_a_pool_keeps_its_tensors():
+    """Another tensor in their place would leave the calls with the old ones' addresses, freed perhaps."""
+    k, s = torch.zeros((3, 2, 16, 64), dtype=torch.int8), torch.zeros((3, 2, 16))
+    pool = sts_attn.PagedKV(k, k.clone(), s, s.clone())
+    for name in ("k", "v", "k_scale", "v_scale"):
+        t = getattr(pool, name)
+        with pytest.raises(AttributeError):
+            setattr(pool, name, t.clone())
+        assert getattr(pool, name) is t and getattr(pool._c, name) == t.data_ptr()
