@@ -80,13 +80,8 @@ __device__ __forceinline__ float over(float x, Op op) {
 }
 constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
 
-// (Of 8-bit rows two workgroups a CU, not the three that its registers would allow: 64
-// streams 134.7 us for 139.  The others have four: 9 streams' f32 step 71.3 us, with two 72.9.)
-template <int TYPE>
-constexpr int kMostWaves = TYPE == STS_PAGES_INT8 ? 2 : 8;
-
 template <int D, int TYPE, bool PAD>
-__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, kMostWaves<TYPE>)))
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 8)))
 void paged_lone_kernel(const PagedDecode p) {
   constexpr bool I8 = TYPE == STS_PAGES_INT8;
   constexpr int ES = TYPE == STS_PAGES_F32 ? 4 : I8 ? 1 : 2;
@@ -373,17 +368,32 @@ void paged_lone_kernel(const PagedDecode p) {
   merge_splits<D, 1>(rec, p.counters + ((uint64_t)b * rows.KH + h) * kCounters, at.split, nsplit, s_mem, s_last, finish);
 }
 
+// Of 8-bit rows a CU holds three or four workgroups, by their registers, or two, by LDS that
+// the launch asks for and nobody uses.  Four heads a CU or more, over long rows, gain by two
+// (64 streams of 32 heads of 128 to 3000 rows of 128 dims 134 us for 138, 100 of 150 to 3000
+// rows of 64 dims 105 for 110); fewer or shorter ones lose (100 streams of 8 heads of 150 to
+// 3000 rows of 128 dims 64 for 60, 64 of 32 heads of 25 to 500 rows 32 for 29, 100 of 64 dims
+// 33 for 25).
+constexpr uint32_t kTwoACu = 48 * 1024;
+uint32_t spare_lds(const PagedDecode& p) {
+  if (p.rows.type != STS_PAGES_INT8) return 0;
+  const bool many = (uint64_t)p.batch * p.rows.KH >= 4ull * device_cu_count();
+  const bool longs = (uint64_t)p.rows.max_rows * p.rows.dh >= 128 * 1024;
+  return many && longs ? kTwoACu : 0;
+}
+
 template <int TYPE>
 void launch_type(const PagedDecode& p, dim3 grid, hipStream_t stream) {
   const dim3 block(kWaves * 64);
+  const uint32_t lds = spare_lds(p);
   if (p.rows.dh == 128)
-    hipLaunchKernelGGL((paged_lone_kernel<128, TYPE, false>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((paged_lone_kernel<128, TYPE, false>), grid, block, lds, stream, p);
   else if (p.rows.dh == 64)
-    hipLaunchKernelGGL((paged_lone_kernel<64, TYPE, false>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((paged_lone_kernel<64, TYPE, false>), grid, block, lds, stream, p);
   else if (p.rows.dh > 64)
-    hipLaunchKernelGGL((paged_lone_kernel<128, TYPE, true>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((paged_lone_kernel<128, TYPE, true>), grid, block, lds, stream, p);
   else
-    hipLaunchKernelGGL((paged_lone_kernel<64, TYPE, true>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((paged_lone_kernel<64, TYPE, true>), grid, block, lds, stream, p);
 }
 
 }  // namespace

@@ -259,6 +259,13 @@ def test_decode_many_streams_in_splits(gpu, rows, H):
     check_decode(Pool(25, lens, 1, 64, 32, rows), H)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_decode_many_heads_over_long_rows(gpu, D):
+    """8-bit rows of more than a thousand heads, one stream long: fewer workgroups a CU."""
+    lens = np.r_[np.random.default_rng(36).integers(0, 40, 65), 2050]
+    check_decode(Pool(37, lens, 16, D, 64, "int8"), 16)
+
+
 @pytest.mark.parametrize("rows", ["f32", "bf16", "int8"])
 def test_decode_missing_pages(gpu, rows):
     """Rows of an entry that is no page have no part: in the middle, first, last, all of them."""
