@@ -353,7 +353,8 @@ int sts_evict_ring(void* k_cache, void* v_cache, float* weights, int32_t* kept, 
  *   lens[b]        rows of stream b (device int32), those to be appended included;
  *                  taken as 0 below that and as max_rows above
  *   max_rows       what no stream's rows exceed, at most max_pages * page_rows; the
- *                  work is planned for it
+ *                  work is planned for it (up to 64 streams are dealt out by their
+ *                  lengths, more of them as if all were of this one)
  * A table entry outside 0..pages-1 is no page: its rows are not written, read back as
  * zeros and have no part in the attention.
  *
@@ -406,8 +407,8 @@ int sts_paged_append(const sts_pages* pages, const sts_rope* rope, const float* 
  * 2^-110, and weights below 2^-110 of the largest, may be lost (2^-39 over 8-bit rows
  * whose values are near 2^-64).
  * Where an infinity or NaN is seen, outputs follow f32 arithmetic over f32 rows (zeros
- * where every score is -infinity) and are undefined over bf16 rows.  Splits use the per-(device, stream) workspace as
- * sts_decode_ring does.
+ * where every score is -infinity) and are undefined over bf16 rows.  Splits use the
+ * per-(device, stream) workspace as sts_decode_ring does.
  */
 int sts_paged_decode(const sts_pages* pages, const sts_rope* rope, const float* q,
                      uint64_t q_stride, const float* k_new, const float* v_new,
