@@ -15,8 +15,8 @@
 // before.  Without q, one sum over the words that are no child's token serves all of a
 // place's rejections: the children's own are added to it.  Sums and comparisons are in
 // f64, so that the verdict is that of exact arithmetic but where a random number lies
-// within 2^-45 of a border (rows of up to 2^23 words, whose sums pass through 160
-// roundings at most; 2^-41 up to 2^28 words).  With q a place's second and later
+// within 2^-45 of a border (rows of up to 2^23 words, whose running sum and total pass
+// through 180 roundings at most; 2^-41 up to 2^28 words, 3200).  With q a place's second and later
 // rejections each make that distance up to 4 / m times as large: the errors of r and of m
 // before, relative to what was left, come to twice themselves and a rounding in r / m,
 // and are then relative to the smaller m that max(0, r / m - q) leaves.
